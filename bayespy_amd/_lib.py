@@ -97,6 +97,13 @@ SIGNATURES = {
                             _vp, _i64, _vp]),
     "dme_solve_cpt": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _f64, _int, _vp,
                              _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "dme_log_loss_workspace_bytes": (_i64, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _vp, _int]),
+    "dme_log_loss": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _vp, _i64, _vp]),
+    "dme_log_loss_gradient": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _vp, _vp,
+                                     _vp, _vp, _vp, _i64, _vp]),
+    "dme_orthogonal_step_workspace_bytes": (_i64, [_int, _i64, _i64, _i64]),
+    "dme_orthogonal_step": (_int, [_vp, _i64, _i64, _i64, _int, _i64, _i64, _i64, _int, _f64, _f64, _f64, _vp, _vp,
+                                   _i64, _vp]),
     "dme_synth_scratch_bytes": (_i64, [_i64]),
     "dme_synth_dirmult": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _u64, _i64, _vp, _i64, _vp]),
 }
@@ -106,6 +113,12 @@ SIGNATURES = {
 class Ragged(ctypes.Structure):
     """dme_ragged_t (include/dme_hip.h): a host struct of device pointers."""
     _fields_ = [("offU", _vp), ("slotoff", _vp), ("slotcol", _vp), ("nslots", _i64), ("total", _i64)]
+
+
+class CountRowsArg(ctypes.Structure):
+    """dme_count_rows_t (include/dme_hip.h): a host struct of device pointers."""
+    _fields_ = [("kind", ctypes.c_int32), ("elem", ctypes.c_int32), ("labels", _vp), ("rowptr", _vp),
+                ("colidx", _vp), ("vals", _vp), ("nnz", _i64), ("X", _vp), ("ld", _i64)]
 
 
 SEGMENT_TERMS = 256  # DME_SEGMENT_TERMS

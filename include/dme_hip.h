@@ -568,6 +568,77 @@ int dme_synth_dirmult(void* X /*[dev]*/, int elem_bytes, int64_t N, int64_t K, i
                       const double* cdf /*[dev][K]*/, uint64_t seed, int64_t row_offset,
                       void* scratch, int64_t scratch_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Count rows under a linear predictor: z_ik = sum_d H[i][d] W[k][d] + bias[k].  The likelihoods that
+ * DE/dme.py:16-48 evaluates at one parameter vector, here with one of its own for every row
+ * (no counterpart of this path in the reference's Python; its DirichletRegression/ starts from
+ * findDirichletPriors, dirichletRegression.py:137-141, as bias = log(priors) does here).
+ * With T = sum_k x_k, l = log sum_k exp(z_k):
+ *   multinomial   loss = T l - sum_k x_k z_k                          (softmax; the multinomial coefficient left out)
+ *   Dirichlet     loss = lgamma(e^l + T) - lgamma(e^l) - sum_k [lgamma(e^z_k + x_k) - lgamma(e^z_k)]
+ * z is never stored whole: the loss takes one pass over the columns, the gradient makes z again in pieces of the
+ * columns (1 GB of scratch at most beside the rows' own).
+ *
+ *   H [dev][N][ldh], W [dev][K][ldw]: bf16 or fp32 (type), values contiguous within a row, any pitch
+ *     and alignment (rows that are not whole 16-byte groups cost a copy of the operand).
+ *   bias [dev][K] fp32 or NULL.  -inf takes a column out: its probability is 0, a count in it costs +inf.
+ *   rows: what the counts are (a host struct of device pointers), see below.
+ *   row_weights [dev][N] fp32 or NULL (ones): the gradient is that of sum_i row_weights[i] loss[i].
+ *   loss [dev][N] fp32, unweighted.  A row without counts has loss 0 and gradient 0.
+ *   dH [dev][N][D], dW [dev][K][D] in H's type, dbias [dev][K] fp32 or NULL: overwritten, aligned to 16 bytes.
+ * Sums, l and the row terms are held in 32 bits or more; d loss / d z is rounded once to H's type
+ * before its products with W and H (dbias is summed before that rounding).  Results do not depend on timing:
+ * the same call gives the same bits.
+ * Rows: DME_ROWS_LABELS  labels int64 [N]: one count in column labels[i]; negative: no count.
+ *       DME_ROWS_CSR     rowptr int64 [N+1], colidx int32 [nnz] strictly ascending within a row, vals int32 [nnz] >= 0.
+ *       DME_ROWS_DENSE   X [N][ld], uint16 (elem 2) or int32 >= 0 (elem 4).
+ * A row that breaks its format (a column out of range or out of order, a negative count, a label >= K,
+ * a rowptr that runs backwards or beyond nnz) has loss NaN and makes the gradient NaN; nothing out of range is read.
+ * ------------------------------------------------------------------------------------------- */
+#define DME_TYPE_F32 0
+#define DME_TYPE_BF16 1
+#define DME_ROWS_LABELS 0
+#define DME_ROWS_CSR 1
+#define DME_ROWS_DENSE 2
+#define DME_LIKELIHOOD_MULTINOMIAL 0
+#define DME_LIKELIHOOD_DIRICHLET 1
+
+typedef struct {
+    int32_t kind;          /* DME_ROWS_* */
+    int32_t elem;          /* dense: bytes of a count, 2 (uint16) or 4 (int32) */
+    const int64_t* labels; /* [dev][N] */
+    const int64_t* rowptr; /* [dev][N+1] */
+    const int32_t* colidx; /* [dev][nnz] */
+    const int32_t* vals;   /* [dev][nnz] */
+    int64_t nnz;
+    const void* X;         /* [dev][N][ld] */
+    int64_t ld;
+} dme_count_rows_t;
+
+int64_t dme_log_loss_workspace_bytes(const void* H /*[dev]*/, int64_t ldh, const void* W /*[dev]*/, int64_t ldw, int type, int64_t N,
+                                     int64_t K, int64_t D, const dme_count_rows_t* rows /*[host]*/, int gradient);
+int dme_log_loss(const void* H /*[dev]*/, int64_t ldh, const void* W /*[dev]*/, int64_t ldw, const float* bias /*[dev][K] or NULL*/,
+                 int type, int64_t N, int64_t K, int64_t D, const dme_count_rows_t* rows /*[host]*/, int likelihood,
+                 float* loss /*[dev][N]*/, void* ws, int64_t ws_bytes, void* stream);
+int dme_log_loss_gradient(const void* H /*[dev]*/, int64_t ldh, const void* W /*[dev]*/, int64_t ldw,
+                          const float* bias /*[dev][K] or NULL*/, int type, int64_t N, int64_t K, int64_t D,
+                          const dme_count_rows_t* rows /*[host]*/, int likelihood, const float* row_weights /*[dev][N] or NULL*/,
+                          float* loss /*[dev][N]*/, void* dH /*[dev][N][D]*/, void* dW /*[dev][K][D]*/,
+                          float* dbias /*[dev][K] or NULL*/, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The orthogonalised step: `batch` matrices G (rows x cols, any strides, in elements) become
+ * X = G / |G|_F, then `steps` times X <- a X + b X X'X + c X X'X X'X (products over the smaller side);
+ * out [dev][batch][rows][cols], contiguous, in G's type.  A zero matrix stays zero.  bf16 matrices go through
+ * fp16 products with 32-bit sums and a 32-bit X, fp32 matrices through fp32 products.  The coefficients
+ * must keep singular values that begin in [0, 1] below 3.  The step that dme_predicted_step takes from a Hessian is taken
+ * here from the gradient alone: log-sum-exp losses are smooth in the spectral norm.
+ * ------------------------------------------------------------------------------------------- */
+int64_t dme_orthogonal_step_workspace_bytes(int type, int64_t batch, int64_t rows, int64_t cols);
+int dme_orthogonal_step(const void* G /*[dev]*/, int64_t batch_stride, int64_t row_stride, int64_t col_stride, int type,
+                        int64_t batch, int64_t rows, int64_t cols, int steps, double a, double b, double c, void* out /*[dev]*/,
+                        void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
