@@ -3,10 +3,13 @@
 // leaves its singular vectors alone (Carlson et al. 2015 take this step's limit as the steepest descent of log-sum-exp
 // losses; the quintic iteration is Bjorck and Bowie's, 1971).
 //
-// X is kept m x n with m <= n (G transposed where it is tall), so S is the smaller square.  Operands of the products are
-// fp16 for bf16 matrices, scaled by powers of two, and X itself stays in 32 bits beside them: what fp16 drops of X then
-// only passes through (b S + c S S), which is small where X's singular values are, instead of being amplified by a at every
-// step.  For fp32 matrices everything is fp32.
+// S is the square of the smaller side: X X' for a wide X, X' X for a tall one (then X <- a X + X (b S + c S S)); X keeps G's
+// orientation.  Operands of the products are fp16 for bf16 matrices, scaled by powers of two, and X itself stays in 32 bits
+// beside them: what fp16 drops of X then only passes through b S + c S S, which is small where X's singular values are, instead
+// of being amplified by a at every step.  The diagonals of S and of b S + c S S are kept out of the operands and applied in 32 bits:
+// where singular values are alike the diagonal is nearly one number, and its rounding would not average out (50000 x 256 of
+// near-flat spectrum, five steps: 3.7e-3 of the result with the diagonal in fp16, below 1e-3 without).  For fp32 matrices everything
+// is fp32.
 #include <math.h>
 
 #include <atomic>
@@ -26,18 +29,37 @@ struct Scale<_Float16> {
     static constexpr float X = 4096.f, S = 4096.f, B = 1024.f;
 };
 
-constexpr int NORM_BLOCKS = 64;
+constexpr int NORM_BLOCKS = 256;
 
+// Sums of squares of the workgroups' shares, in 64 bits.  lines x length values, those of a line `step` apart.  Also clears the
+// 16 bytes that products read in place of what lies outside an operand.
 template <class T>
-__global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, long long rs, long long cs, long long m, long long n, double* part) {
+__global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, long long line, long long step, long long lines, long long length, double* part,
+                                                   u32* zeros) {
     __shared__ double sums[4];
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) zeros[threadIdx.x] = 0;
     const T* g = G + blockIdx.y * sb;
     double s = 0.0;
-    const long long total = m * n;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / n, c = i - r * n;
-        const double v = (double)(float)g[r * rs + c * cs];
-        s += v * v;
+    constexpr int VEC = 16 / sizeof(T);
+    typedef T tv __attribute__((ext_vector_type(VEC)));
+    if (lines == 1 && step == 1 && (uintptr_t)g % 16 == 0) {  // contiguous: 16 bytes a lane
+        const long long n = length / VEC;
+        const tv* v = (const tv*)g;
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += NORM_BLOCKS * 256) {
+            const tv x = v[i];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) s += (double)(float)x[q] * (double)(float)x[q];
+        }
+        const long long i = n * VEC + threadIdx.x;
+        if (blockIdx.x == 0 && i < length) s += (double)(float)g[i] * (double)(float)g[i];
+    } else {  // a workgroup's lines one after the other, or pieces of a single one
+        const long long l0 = lines > 1 ? blockIdx.x : 0, ls = lines > 1 ? NORM_BLOCKS : 1;
+        const long long i0 = lines > 1 ? threadIdx.x : (long long)blockIdx.x * 256 + threadIdx.x, is = lines > 1 ? 256 : NORM_BLOCKS * 256;
+        for (long long l = l0; l < lines; l += ls)
+            for (long long i = i0; i < length; i += is) {
+                const double x = (double)(float)g[l * line + i * step];
+                s += x * x;
+            }
     }
     s = dme_wave_sum_f64(s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
@@ -47,141 +69,237 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, lon
 
 template <class W>
 struct Matrices {
-    float* X;      // [m][ldn] in 32 bits; for fp32 matrices also the operand
-    W* Xw;         // [m][ldn]
-    W* Xt[2];      // [n][ldm]
-    float* S;      // [m][ldm]
-    W* Sw;         // [m][ldm]
-    W* Bw;         // [m][ldm]
-    long long stride_x, stride_t, stride_s;  // from matrix to matrix
-    long long m, n, ldm, ldn;
+    float* X;      // [rows][ldx]; not used for fp32 matrices
+    W* Xw[2];      // [rows][ldx]: the operand, read and written in turn
+    float* S;      // [m][lds]
+    W* Sw;         // [m][lds]: S without its diagonal
+    W* Bw;         // [m][lds]: b S + c S S without its diagonal
+    float* Sd;     // [m]: the diagonals
+    float* Bd;
+    float* part;   // [split][m][lds]: pieces of S
+    long long stride_x, stride_s, stride_part;  // from matrix to matrix
+    long long rows, cols, ldx, m, lds;
 };
 
-// X = G / |G| and its transpose, zero in the padding of their pitches.
+// X = G / |G|, zero in the padding of its pitch.
 template <class T, class W>
 __global__ __launch_bounds__(256) void begin_kernel(const T* G, long long sb, long long rs, long long cs, const double* part, Matrices<W> a) {
     __shared__ float tile[64][65];
-    double s = 0.0;
-    for (int i = 0; i < NORM_BLOCKS; ++i) s += part[blockIdx.y * NORM_BLOCKS + i];
+    __shared__ double sums[4];
+    double s = dme_wave_sum_f64(part[blockIdx.y * NORM_BLOCKS + threadIdx.x]);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     const double scale = s > 0.0 || s != s ? 1.0 / sqrt(s) : 0.0;
     const T* g = G + blockIdx.y * sb;
-    const long long xo = blockIdx.y * a.stride_x, to = blockIdx.y * a.stride_t;
+    const long long xo = blockIdx.y * a.stride_x;
     const int lo = threadIdx.x & 63, hi = threadIdx.x >> 6;
-    const bool along = cs == 1;  // neighbouring lanes read neighbouring values
-    const long long tiles_c = (a.ldn + 63) / 64, tiles_r = (a.ldm + 63) / 64;
+    const bool along = cs == 1 || a.cols == 1;  // neighbouring values are neighbours in G too; otherwise tiles are turned in LDS
+    const long long tiles_c = (a.ldx + 63) / 64, tiles_r = (a.rows + 63) / 64;
     for (long long t = blockIdx.x; t < tiles_c * tiles_r; t += gridDim.x) {
         const long long r0 = t / tiles_c * 64, c0 = t % tiles_c * 64;
-        for (int q = hi; q < 64; q += 4) {
-            const int y = along ? q : lo, x = along ? lo : q;
-            const long long r = r0 + y, c = c0 + x;
-            tile[y][x] = r < a.m && c < a.n ? (float)((double)(float)g[r * rs + c * cs] * scale) : 0.f;
+        if (!along) {
+            __syncthreads();
+            for (int q = hi; q < 64; q += 4) {
+                const long long r = r0 + lo, c = c0 + q;
+                if (r < a.rows && c < a.cols) tile[lo][q] = (float)g[r * rs + c * cs];
+            }
+            __syncthreads();
         }
-        __syncthreads();
         for (int q = hi; q < 64; q += 4) {
             const long long r = r0 + q, c = c0 + lo;
-            if (r < a.m && c < a.ldn) {
-                a.X[xo + r * a.ldn + c] = tile[q][lo];
-                if ((void*)a.Xw != (void*)a.X) a.Xw[xo + r * a.ldn + c] = (W)(tile[q][lo] * Scale<W>::X);
-            }
-            const long long rr = r0 + lo, cc = c0 + q;
-            if (cc < a.n && rr < a.ldm) a.Xt[0][to + cc * a.ldm + rr] = (W)(tile[lo][q] * Scale<W>::X);
+            if (r >= a.rows || c >= a.ldx) continue;
+            float v = 0.f;
+            if (c < a.cols) v = (float)((double)(along ? (float)g[r * rs + c * cs] : tile[q][lo]) * scale);
+            if (sizeof(W) == 2) a.X[xo + r * a.ldx + c] = v;
+            a.Xw[0][xo + r * a.ldx + c] = (W)(v * Scale<W>::X);
         }
-        __syncthreads();
     }
 }
-
-enum { MAKE_S, MAKE_B, MAKE_X, MAKE_LAST };
 
 template <class T, class W>
 struct StepArgs {
     Matrices<W> mat;
     const char* zeros;
     float a, b, c;
-    int from;  // which of Xt is read
-    T* out;    // MAKE_LAST
-    long long out_batch, out_row, out_col;
-    long long tiles_r, tiles_c;
+    int from;  // which of Xw is read
+    T* out;    // the last step's result, or null
+    long long out_batch;
+    int vector;  // its rows are aligned to four values
+    long long tiles_r, tiles_c, batch;
+    int slices, per_split;
 };
 
-// One of a step's three products with what follows it: S = X X', B = b S + c S S, X = a X + B X.
-template <class T, class W, int MAKE>
-__global__ __launch_bounds__(256, 2) void step_kernel(StepArgs<T, W> a) {
+// Tile `t` of the lower triangle of a square of tiles, numbered along its rows; XCDs take eighths of them (dme_tile_of).
+__device__ __forceinline__ void triangle_tile(long long block, long long n, long long& tr, long long& tc) {
+    const long long all = n * (n + 1) / 2, per = all / 8, more = all % 8, x = block & 7, at = block >> 3;
+    const long long t = x * per + (x < more ? x : more) + at;
+    long long r = (long long)((sqrt(8.0 * (double)t + 1.0) - 1.0) * 0.5);
+    while (r * (r + 1) / 2 > t) --r;
+    while ((r + 1) * (r + 2) / 2 <= t) ++r;
+    tr = r;
+    tc = t - r * (r + 1) / 2;
+}
+
+// what becomes of S[r][c] = v
+template <class W>
+__device__ __forceinline__ void put_s(const Matrices<W>& x, long long so, long long mo, long long r, long long c, float v) {
+    x.S[so + r * x.lds + c] = v;
+    x.Sw[so + r * x.lds + c] = r == c ? (W)0.f : (W)(v * Scale<W>::S);
+    if (r == c) x.Sd[mo + r] = v;
+}
+
+// S = X X' (X' X for a tall X), the tiles on and below the diagonal; what lies above is their mirror image.  Where the tiles are
+// too few for the card, k is split and join_kernel adds the pieces.
+template <class T, class W, int SIDE, bool TALL>
+__global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void square_kernel(StepArgs<T, W> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeTile<W, 128, 128, 2, 2> Tile;
+    typedef DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2, TALL, TALL> Tile;
     const Matrices<W>& x = a.mat;
-    const long long xo = blockIdx.y * x.stride_x, to = blockIdx.y * x.stride_t, so = blockIdx.y * x.stride_s;
-    constexpr long long size = sizeof(W);
-    DmeOperands op;
-    if (MAKE == MAKE_S) {
-        const char* p = (const char*)(x.Xw + xo);
-        op = DmeOperands{p, p, x.ldn * size, x.ldn * size, x.m, x.m, x.ldn * size, a.zeros};
-    } else if (MAKE == MAKE_B) {
-        const char* p = (const char*)(x.Sw + so);
-        op = DmeOperands{p, p, x.ldm * size, x.ldm * size, x.m, x.m, x.ldm * size, a.zeros};
-    } else {
-        op = DmeOperands{(const char*)(x.Bw + so), (const char*)(x.Xt[a.from] + to), x.ldm * size, x.ldm * size, x.m, x.n, x.ldm * size, a.zeros};
-    }
+    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    const DmeOperand op{(const char*)(x.Xw[a.from] + blockIdx.y * x.stride_x), x.ldx * (long long)sizeof(W), x.m};
     long long tr, tc;
-    dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
+    triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
+    const int s0 = (int)blockIdx.z * a.per_split;
+    int s1 = s0 + a.per_split;
+    s1 = s1 < a.slices ? s1 : a.slices;
     Tile t;
-    t.run(op, lds, tr * 128, tc * 128, 0, (int)((op.kbytes + DME_SLICE - 1) / DME_SLICE));
-    typedef Scale<W> K;
-    const long long width = MAKE == MAKE_S || MAKE == MAKE_B ? x.m : x.n, pitch = MAKE == MAKE_S || MAKE == MAKE_B ? x.ldm : x.ldn;
+    t.run(op, op, TALL ? x.rows : x.cols, a.zeros, lds, tr * SIDE, tc * SIDE, s0, s1);
+    constexpr float UNIT = 1.f / (Scale<W>::X * Scale<W>::X);
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
-        const long long r = tr * 128 + Tile::row_of(j);
+        const long long r = tr * SIDE + Tile::row_of(j);
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) {
-            const long long c = tc * 128 + Tile::col_of(i);
-            if (c >= pitch) continue;
-            f32x4 v = t.acc[i][j];
-            if (MAKE == MAKE_S) {
-                if (r >= x.m) continue;
-                v *= 1.f / (K::X * K::X);
-            } else if (MAKE == MAKE_B) {
-                if (r >= x.m) continue;
-                const f32x4 s = *(const f32x4*)(x.S + so + r * pitch + c);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) v[q] = __builtin_fmaf(a.c, v[q] * (1.f / (K::S * K::S)), a.b * s[q]);
-            } else if (r < x.m) {
-                const f32x4 s = *(const f32x4*)(x.X + xo + r * pitch + c);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) v[q] = __builtin_fmaf(a.a, s[q], v[q] * (1.f / (K::B * K::X)));
+            const long long c = tc * SIDE + Tile::col_of(i);
+            if (r >= x.lds || c >= x.lds) continue;
+            const f32x4 v = t.acc[i][j] * UNIT;
+            if (gridDim.z > 1) {
+                if (r < x.m) *(f32x4*)(x.part + blockIdx.y * x.stride_part + blockIdx.z * x.stride_s + r * x.lds + c) = v;
+                continue;
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = r < x.m && c + q < width ? v[q] : 0.f;
-            if (MAKE == MAKE_S) {
-                *(f32x4*)(x.S + so + r * pitch + c) = v;
-                if ((void*)x.Sw != (void*)x.S) dme_store4(x.Sw + so + r * pitch + c, v * K::S);
-            } else if (MAKE == MAKE_B) {
-                dme_store4(x.Bw + so + r * pitch + c, v * K::B);
-            } else if (MAKE == MAKE_X) {
-                if (r < x.m) {
-                    *(f32x4*)(x.X + xo + r * pitch + c) = v;
-                    if ((void*)x.Xw != (void*)x.X) dme_store4(x.Xw + xo + r * pitch + c, v * K::X);
-                }
-                if (r < x.ldm) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (c + q < x.n) x.Xt[a.from ^ 1][to + (c + q) * x.ldm + r] = (W)(v[q] * K::X);
-                }
-            } else if (r < x.m) {
-                T* o = a.out + blockIdx.y * a.out_batch + r * a.out_row + c * a.out_col;
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (c + q < x.n) o[q * a.out_col] = (T)v[q];
+            for (int q = 0; q < 4; ++q) {  // the pitch's padding is zero, below the diagonal and above it
+                const bool in = r < x.m && c + q < x.m;
+                if (tr != tc && c + q < x.m) put_s(x, so, mo, c + q, r, in ? v[q] : 0.f);
+                if (r < x.m) put_s(x, so, mo, r, c + q, in ? v[q] : 0.f);
             }
         }
     }
 }
 
-__global__ void zeros_kernel(u32* p) { p[threadIdx.x] = 0; }
+template <class W>
+__global__ __launch_bounds__(256) void join_kernel(Matrices<W> x, int splits) {
+    const long long n = x.m * x.lds, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long r = i / x.lds, c = i - r * x.lds;
+        float v = 0.f;
+        if (c < x.m) {
+            const float* at = x.part + blockIdx.y * x.stride_part + (r > c ? r * x.lds + c : c * x.lds + r);
+            for (int s = 0; s < splits; ++s) v += at[s * x.stride_s];
+        }
+        put_s(x, so, mo, r, c, v);
+    }
+}
+
+// B = b S + c S S.  With S = d + O (diagonal, rest): (S S)[r][c] = (O O)[r][c] + (d_r + d_c) O[r][c], + d_r^2 where r = c.
+template <class T, class W, int SIDE>
+__global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void poly_kernel(StepArgs<T, W> a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    typedef DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2> Tile;
+    const Matrices<W>& x = a.mat;
+    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    const DmeOperand op{(const char*)(x.Sw + so), x.lds * (long long)sizeof(W), x.m};
+    long long tr, tc;
+    triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
+    Tile t;
+    t.run(op, op, x.m, a.zeros, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+    constexpr float UNIT = 1.f / (Scale<W>::S * Scale<W>::S);
+#pragma unroll
+    for (int j = 0; j < Tile::NJ; ++j) {
+        const long long r = tr * SIDE + Tile::row_of(j);
+        if (r >= x.lds) continue;
+        const bool real = r < x.m;  // the rows beyond are the padding above the diagonal
+        const float dr = real ? x.Sd[mo + r] : 0.f;
+#pragma unroll
+        for (int i = 0; i < Tile::NI; ++i) {
+            const long long c = tc * SIDE + Tile::col_of(i);
+            if (c >= x.lds) continue;
+            f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (real) s = *(const f32x4*)(x.S + so + r * x.lds + c);
+            f32x4 v;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const bool in = real && c + q < x.m, on = in && c + q == r;
+                const float dc = in ? x.Sd[mo + c + q] : 0.f;
+                const float ss = t.acc[i][j][q] * UNIT + (on ? dr * dr : (dr + dc) * s[q]);
+                const float poly = __builtin_fmaf(a.c, ss, a.b * s[q]);
+                if (on) x.Bd[mo + r] = poly;
+                v[q] = in && !on ? poly * Scale<W>::B : 0.f;
+                if (tr != tc && c + q < x.m) x.Bw[so + (c + q) * x.lds + r] = (W)v[q];
+            }
+            if (real) dme_store4(x.Bw + so + r * x.lds + c, v);
+        }
+    }
+}
+
+// X <- a X + B X (a X + X B for a tall X)
+template <class T, class W, int SIDE, bool TALL>
+__global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void update_kernel(StepArgs<T, W> a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    typedef DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2, false, !TALL> Tile;
+    const Matrices<W>& x = a.mat;
+    const long long xo = blockIdx.y * x.stride_x, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    constexpr long long size = sizeof(W);
+    const DmeOperand b{(const char*)(x.Bw + so), x.lds * size, x.m};
+    const DmeOperand y{(const char*)(x.Xw[a.from] + xo), x.ldx * size, TALL ? x.rows : x.cols};
+    long long tr, tc;
+    dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
+    Tile t;
+    t.run(TALL ? y : b, TALL ? b : y, x.m, a.zeros, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+    constexpr float UNIT = 1.f / (Scale<W>::B * Scale<W>::X);
+    W* to = x.Xw[a.from ^ 1] + xo;
+#pragma unroll
+    for (int j = 0; j < Tile::NJ; ++j) {
+        const long long r = tr * SIDE + Tile::row_of(j);
+        if (r >= x.rows) continue;
+        const float dr = TALL ? 0.f : a.a + x.Bd[mo + r];
+#pragma unroll
+        for (int i = 0; i < Tile::NI; ++i) {
+            const long long c = tc * SIDE + Tile::col_of(i);
+            if (c >= x.ldx) continue;
+            const long long at = r * x.ldx + c;
+            const f32x4 old = size == 2 ? *(const f32x4*)(x.X + xo + at) : *(const f32x4*)((const float*)(x.Xw[a.from] + xo) + at);
+            f32x4 v;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const bool in = c + q < x.cols;
+                const float d = TALL ? (in ? a.a + x.Bd[mo + c + q] : 0.f) : dr;
+                v[q] = in ? __builtin_fmaf(d, old[q], t.acc[i][j][q] * UNIT) : 0.f;
+            }
+            if (!a.out) {
+                if (size == 2) *(f32x4*)(x.X + xo + at) = v;
+                dme_store4(to + at, v * Scale<W>::X);
+            } else if (c < x.cols) {  // the result has no padding
+                T* o = a.out + blockIdx.y * a.out_batch + r * x.cols + c;
+                if (a.vector) {
+                    dme_store4(o, v);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (c + q < x.cols) o[q] = (T)v[q];
+                }
+            }
+        }
+    }
+}
 
 inline long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 struct StepPlan {
-    long long m, n, ldm, ldn;
-    long long zeros, norm, X, Xw, Xt[2], S, Sw, Bw, bytes;
+    long long m, n, ldx, lds;
+    DmeCut square, poly, update;
+    long long zeros, norm, X, Xw[2], S, Sw, Bw, Sd, Bd, part, bytes;
 };
 
 StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
@@ -190,8 +308,12 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     const long long size = half ? 2 : 4, per = 16 / size;
     p.m = rows < cols ? rows : cols;
     p.n = rows < cols ? cols : rows;
-    p.ldm = up(p.m, per);
-    p.ldn = up(p.n, per);
+    p.ldx = up(cols, per);
+    p.lds = up(p.m, per);
+    const auto slices = [&](long long k) { return (k * size + DME_SLICE - 1) / DME_SLICE; };
+    p.square = dme_cut(p.m, p.m, slices(p.n), (int)size, true, 0.0, true);
+    p.poly = dme_cut(p.m, p.m, slices(p.m), (int)size, false, 0.0, true);
+    p.update = dme_cut(rows, cols, slices(p.m), (int)size, false);
     long long at = 0;
     const auto take = [&](long long bytes) {
         const long long here = at;
@@ -200,74 +322,114 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     };
     p.zeros = take(256);
     p.norm = take(batch * NORM_BLOCKS * 8);
-    p.X = take(batch * p.m * p.ldn * 4);
-    p.Xw = half ? take(batch * p.m * p.ldn * 2) : p.X;
-    for (int i = 0; i < 2; ++i) p.Xt[i] = take(batch * p.n * p.ldm * size);
-    p.S = take(batch * p.m * p.ldm * 4);
-    p.Sw = half ? take(batch * p.m * p.ldm * 2) : p.S;
-    p.Bw = take(batch * p.m * p.ldm * size);
+    if (half) p.X = take(batch * rows * p.ldx * 4);
+    for (int i = 0; i < 2; ++i) p.Xw[i] = take(batch * rows * p.ldx * size);
+    p.S = take(batch * p.m * p.lds * 4);
+    p.Sw = take(batch * p.m * p.lds * size);
+    p.Bw = take(batch * p.m * p.lds * size);
+    p.Sd = take(batch * p.m * 4);
+    p.Bd = take(batch * p.m * 4);
+    if (p.square.splits > 1) p.part = take(batch * p.square.splits * p.m * p.lds * 4);
     p.bytes = at;
     return p;
 }
 
-template <class T, class W, int MAKE>
-int launch(StepArgs<T, W> a, long long batch, hipStream_t s) {
-    typedef DmeTile<W, 128, 128, 2, 2> Tile;
-    a.tiles_r = (a.mat.m + 127) / 128;
-    a.tiles_c = ((MAKE == MAKE_S || MAKE == MAKE_B ? a.mat.m : a.mat.n) + 127) / 128;
-    static std::atomic<bool> done[64];
+template <class W, int SIDE, class F, class A>
+int launch(F kernel, std::atomic<bool>* done, const A& a, long long tiles, int splits, hipStream_t s) {
+    constexpr int bytes = 2 * DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2>::STAGE;
     int dev = 0;
     DME_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
-        DME_HIP_CHECK(hipFuncSetAttribute((const void*)step_kernel<T, W, MAKE>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * Tile::STAGE));
+        DME_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
     }
-    hipLaunchKernelGGL((step_kernel<T, W, MAKE>), dim3((unsigned)(a.tiles_r * a.tiles_c), (unsigned)batch), dim3(256), 2 * Tile::STAGE, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)splits), dim3(SIDE == 256 ? 512 : 256), bytes, s, a);
     return DME_OK;
+}
+
+template <class T, class W, int SIDE, bool TALL>
+int square(StepArgs<T, W> a, const DmeCut& cut, hipStream_t s) {
+    static std::atomic<bool> done[64];
+    a.tiles_r = (a.mat.m + SIDE - 1) / SIDE;
+    a.slices = (int)(((TALL ? a.mat.rows : a.mat.cols) * (long long)sizeof(W) + DME_SLICE - 1) / DME_SLICE);
+    a.per_split = (a.slices + cut.splits - 1) / cut.splits;
+    return launch<W, SIDE>(square_kernel<T, W, SIDE, TALL>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, cut.splits, s);
+}
+
+template <class T, class W, int SIDE>
+int poly(StepArgs<T, W> a, hipStream_t s) {
+    static std::atomic<bool> done[64];
+    a.tiles_r = (a.mat.m + SIDE - 1) / SIDE;
+    a.slices = (int)((a.mat.m * (long long)sizeof(W) + DME_SLICE - 1) / DME_SLICE);
+    return launch<W, SIDE>(poly_kernel<T, W, SIDE>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, 1, s);
+}
+
+template <class T, class W, int SIDE, bool TALL>
+int update(StepArgs<T, W> a, hipStream_t s) {
+    static std::atomic<bool> done[64];
+    a.tiles_r = (a.mat.rows + SIDE - 1) / SIDE;
+    a.tiles_c = (a.mat.cols + SIDE - 1) / SIDE;
+    a.slices = (int)((a.mat.m * (long long)sizeof(W) + DME_SLICE - 1) / DME_SLICE);
+    return launch<W, SIDE>(update_kernel<T, W, SIDE, TALL>, done, a, a.tiles_r * a.tiles_c, 1, s);
+}
+
+template <class T, class W, bool TALL>
+int one_step(const StepArgs<T, W>& k, const StepPlan& p, hipStream_t s) {
+    int rc = p.square.side == 256   ? square<T, W, 256, TALL>(k, p.square, s)
+             : p.square.side == 128 ? square<T, W, 128, TALL>(k, p.square, s)
+                                    : square<T, W, 64, TALL>(k, p.square, s);
+    if (rc) return rc;
+    if (p.square.splits > 1)
+        hipLaunchKernelGGL(join_kernel<W>, dim3((unsigned)dme_blocks(p.m * p.lds, 256, 2048), (unsigned)k.batch), dim3(256), 0, s, k.mat, p.square.splits);
+    rc = p.poly.side == 256 ? poly<T, W, 256>(k, s) : p.poly.side == 128 ? poly<T, W, 128>(k, s) : poly<T, W, 64>(k, s);
+    if (rc) return rc;
+    return p.update.side == 256   ? update<T, W, 256, TALL>(k, s)
+           : p.update.side == 128 ? update<T, W, 128, TALL>(k, s)
+                                  : update<T, W, 64, TALL>(k, s);
 }
 
 template <class T, class W>
 int run(const T* G, long long sb, long long rs, long long cs, long long batch, long long rows, long long cols, int steps, double a, double b, double c,
         T* out, char* ws, const StepPlan& p, hipStream_t s) {
     const bool tall = rows > cols;
-    const long long row = tall ? cs : rs, col = tall ? rs : cs;  // of X
     StepArgs<T, W> k{};
     Matrices<W>& x = k.mat;
     x.X = (float*)(ws + p.X);
-    x.Xw = (W*)(ws + p.Xw);
-    for (int i = 0; i < 2; ++i) x.Xt[i] = (W*)(ws + p.Xt[i]);
+    for (int i = 0; i < 2; ++i) x.Xw[i] = (W*)(ws + p.Xw[i]);
     x.S = (float*)(ws + p.S);
     x.Sw = (W*)(ws + p.Sw);
     x.Bw = (W*)(ws + p.Bw);
+    x.Sd = (float*)(ws + p.Sd);
+    x.Bd = (float*)(ws + p.Bd);
+    x.part = (float*)(ws + p.part);
+    x.rows = rows;
+    x.cols = cols;
+    x.ldx = p.ldx;
     x.m = p.m;
-    x.n = p.n;
-    x.ldm = p.ldm;
-    x.ldn = p.ldn;
-    x.stride_x = p.m * p.ldn;
-    x.stride_t = p.n * p.ldm;
-    x.stride_s = p.m * p.ldm;
+    x.lds = p.lds;
+    x.stride_x = rows * p.ldx;
+    x.stride_s = p.m * p.lds;
+    x.stride_part = p.square.splits * p.m * p.lds;
     k.zeros = ws + p.zeros;
     k.a = (float)a;
     k.b = (float)b;
     k.c = (float)c;
-    k.out = out;
     k.out_batch = rows * cols;
-    k.out_row = tall ? 1 : cols;
-    k.out_col = tall ? cols : 1;
-    hipLaunchKernelGGL(zeros_kernel, dim3(1), dim3(64), 0, s, (u32*)(ws + p.zeros));
+    k.vector = cols % 4 == 0 && (uintptr_t)out % 16 == 0;
+    k.batch = batch;
     double* part = (double*)(ws + p.norm);
-    // the norm is read in G's own order
-    if (tall)
-        hipLaunchKernelGGL(norm_kernel<T>, dim3(NORM_BLOCKS, (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, rows, cols, part);
-    else
-        hipLaunchKernelGGL(norm_kernel<T>, dim3(NORM_BLOCKS, (unsigned)batch), dim3(256), 0, s, G, sb, row, col, p.m, p.n, part);
-    const long long tiles = (p.ldn + 63) / 64 * ((p.ldm + 63) / 64);
-    hipLaunchKernelGGL((begin_kernel<T, W>), dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, row, col, part, x);
+    // the norm is read along G's contiguous direction, as one line where G has no gaps
+    const bool turn = rs == 1 && cs != 1;
+    const long long line = turn ? cs : rs, step = turn ? rs : cs, lines = turn ? cols : rows, length = turn ? rows : cols;
+    const bool whole = step == 1 && line == length;
+    hipLaunchKernelGGL(norm_kernel<T>, dim3(NORM_BLOCKS, (unsigned)batch), dim3(256), 0, s, G, sb, line, step, whole ? 1 : lines,
+                       whole ? lines * length : length, part, (u32*)(ws + p.zeros));
+    const long long tiles = (p.ldx + 63) / 64 * ((rows + 63) / 64);
+    hipLaunchKernelGGL((begin_kernel<T, W>), dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, part, x);
     for (int i = 0; i < steps; ++i) {
         k.from = i & 1;
-        int rc = launch<T, W, MAKE_S>(k, batch, s);
-        if (!rc) rc = launch<T, W, MAKE_B>(k, batch, s);
-        if (!rc) rc = i + 1 < steps ? launch<T, W, MAKE_X>(k, batch, s) : launch<T, W, MAKE_LAST>(k, batch, s);
+        k.out = i + 1 < steps ? nullptr : out;
+        const int rc = tall ? one_step<T, W, true>(k, p, s) : one_step<T, W, false>(k, p, s);
         if (rc) return rc;
     }
     DME_HIP_CHECK(hipGetLastError());

@@ -42,65 +42,121 @@ __device__ __forceinline__ void dme_store4(T* to, f32x4 v) {
     *(t4*)to = o;
 }
 
-// Operands of one product.  Rows are clamped to the last real one (their outputs are not used), k beyond kbytes is read
-// from `zeros` (16 zero bytes); base pointers and pitches are multiples of 16 bytes (dme_pack_kernel sees to that).
-struct DmeOperands {
-    const char* P;
-    const char* Q;
-    long long ldp, ldq;  // pitches in bytes
-    long long R, C;      // rows of P, rows of Q
-    long long kbytes;    // bytes of k in a row, a multiple of 16
-    const char* zeros;
+// An operand of a product: `rows` rows of k values, either with k contiguous (ld: bytes from row to row; what follows the
+// row's k values up to a multiple of 16 bytes is zero), or "k-major", with the rows contiguous (ld: bytes from one k to the next;
+// what follows the rows up to a multiple of 16 bytes may be read and is not used).  Base and ld are multiples of 16 bytes.
+struct DmeOperand {
+    const char* at;
+    long long ld;
+    long long rows;
 };
 
 constexpr int DME_SLICE = 128;  // bytes of k in a slice
 
-template <class T, int TR, int TC, int WR, int WC>
+// The product of a TR x TC tile.  PK / QK: the operand is k-major.
+//
+// A k-major slice lies in LDS as it does in memory, one line of TR (TC) values for each k.  16-bit operands are turned by the
+// transposing LDS read (16 lanes read 4 lines of 16 values, each lane gets one row's 4 k), 32-bit ones by four reads of a
+// word.  The 16 lines that a wave reads at once begin in the same bank, so the 16-value groups of line k are stored at
+// group ^ f(k), f spreading them over the banks.
+template <class T, int TR, int TC, int WR, int WC, bool PK = false, bool QK = false>
 struct DmeTile {
     static constexpr int NW = WR * WC, NT = NW * 64;
     static constexpr int WTR = TR / WR, WTC = TC / WC;  // a wave's part
     static constexpr int NJ = WTR / 16, NI = WTC / 16;  // its 16 x 16 blocks
     static constexpr int STAGE = (TR + TC) * DME_SLICE;  // bytes of one buffer
-    static constexpr int COPIES = (TR + TC) * 8 / 64;    // wave copies (1 KB) of one slice
+    static constexpr int COPIES = (TR + TC) / 8;         // wave copies (1 KB) of one slice
     static constexpr int PER_WAVE = (COPIES + NW - 1) / NW;
+    static constexpr int SIZE = sizeof(T);
+    static constexpr int KS = DME_SLICE / SIZE;  // k of a slice
+    static constexpr int KH = KS / 2;            // k of one instruction round (64 bytes)
 
     f32x4 acc[NI][NJ];
 
-    // acc = the tile at (r0, c0) over the slices [s0, s1).  lds: 2 * STAGE bytes, free for the caller afterwards (a
-    // barrier has been passed).  Every thread of the workgroup calls this.
-    __device__ __forceinline__ void run(const DmeOperands& o, char* lds, long long r0, long long c0, int s0, int s1) {
+    // where line k of a k-major operand of TM rows keeps its groups of 16 values
+    template <int TM>
+    __device__ __forceinline__ static int spread(int k) {
+        if (SIZE == 4) return (k >> 2) & 3;
+        return TM == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;
+    }
+
+    // source of one lane's 16 bytes of piece `piece` (1 KB) of an operand, and in how many slices from the first on it lies
+    // inside the operand
+    template <int TM, bool KMAJOR>
+    __device__ __forceinline__ static void source(const DmeOperand& o, long long first, long long K, int piece, int lane, const char*& src, int& limit) {
+        if (!KMAJOR) {
+            const int chunk = (lane & 7) ^ (lane >> 3);  // piece * 8 rows do not change row & 7
+            long long r = first + piece * 8 + (lane >> 3);
+            r = r < o.rows ? r : o.rows - 1;  // rows beyond the last are not used: any will do
+            src = o.at + r * o.ld + chunk * 16;
+            const long long bytes = K * SIZE - chunk * 16;
+            limit = bytes > 0 ? (int)((bytes + DME_SLICE - 1) / DME_SLICE) : 0;
+        } else {
+            constexpr int LINE = TM * SIZE / 16;  // 16-byte chunks of a line
+            const int at = piece * 64 + lane, k = at / LINE, slot = at % LINE;
+            const int chunk = slot ^ (spread<TM>(k) * SIZE);  // a group is SIZE chunks
+            const long long r = first + chunk * (16 / SIZE);
+            src = o.at + k * o.ld + r * SIZE;
+            limit = r < o.rows && k < K ? (int)((K - k + KS - 1) / KS) : 0;
+        }
+    }
+
+    // block b (16 rows) of an operand's slice in LDS, round h: this lane's 16 bytes of k
+    template <int TM, bool KMAJOR>
+    __device__ __forceinline__ static u32q fragment(const char* at, int b, int h) {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+        if (!KMAJOR) return *(const u32q*)(at + (b * 16 + c) * DME_SLICE + ((h * 4 + g) ^ (lane & 7)) * 16);
+        constexpr int LINE = TM * SIZE;
+        if constexpr (SIZE == 2) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+            const int k = h * KH + 8 * g + (c >> 2);  // + 4: the same spread
+            const char* p = at + k * LINE + (b ^ spread<TM>(k)) * 32 + (c & 3) * 8;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * LINE));
+            return __builtin_bit_cast(u32q, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int k = h * KH + 4 * g;
+            const char* p = at + k * LINE + (b ^ spread<TM>(k)) * 64 + c * 4;
+            u32q v;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) v[s] = *(const u32*)(p + s * LINE);
+            return v;
+        }
+    }
+
+    // acc = the tile at (r0, c0) over the slices [s0, s1) of k < K.  lds: 2 * STAGE bytes, free for the caller afterwards (a
+    // barrier has been passed).  zeros: 16 zero bytes, read in place of what lies outside.  Every thread of the workgroup calls this.
+    __device__ __forceinline__ void run(const DmeOperand& P, const DmeOperand& Q, long long K, const char* zeros, char* lds, long long r0, long long c0,
+                                        int s0, int s1) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        const int chunk = (lane & 7) ^ (lane >> 3);  // the chunk of k this lane copies, whatever the row group
         const char* src[PER_WAVE];
+        int limit[PER_WAVE];
+        const long long pstep = PK ? KS * P.ld : DME_SLICE, qstep = QK ? KS * Q.ld : DME_SLICE;
 #pragma unroll
         for (int t = 0; t < PER_WAVE; ++t) {
-            const int row = (t * NW + wave) * 8 + (lane >> 3);
-            if (row < TR) {
-                long long r = r0 + row;
-                r = r < o.R ? r : o.R - 1;
-                src[t] = o.P + r * o.ldp + chunk * 16;
+            const int piece = t * NW + wave;
+            if (piece < TR / 8) {
+                source<TR, PK>(P, r0, K, piece, lane, src[t], limit[t]);
+                src[t] += s0 * pstep;
             } else {
-                long long c = c0 + (row - TR);
-                c = c < o.C ? c : o.C - 1;
-                src[t] = o.Q + c * o.ldq + chunk * 16;
+                source<TC, QK>(Q, c0, K, piece - TR / 8, lane, src[t], limit[t]);
+                src[t] += s0 * qstep;
             }
         }
         auto copy = [&](int s, int buf) {
-            const long long k = (long long)s * DME_SLICE;
-            const bool in = k + chunk * 16 < o.kbytes;
 #pragma unroll
             for (int t = 0; t < PER_WAVE; ++t) {
                 const int piece = t * NW + wave;
                 if (COPIES % NW == 0 || piece < COPIES) {
-                    const char* from = in ? src[t] + k : o.zeros;
+                    const char* from = s < limit[t] ? src[t] : zeros;
                     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                                      (__attribute__((address_space(3))) void*)(lds + buf * STAGE + piece * 1024), 16, 0, 0);
+                    src[t] += piece < TR / 8 ? pstep : qstep;
                 }
             }
         };
-        const int wr = wave / WC, wc = wave % WC;
-        const int swz = lane & 7, g = lane >> 4;
-        const int prow = (wr * WTR + (lane & 15)) * DME_SLICE, qrow = (TR + wc * WTC + (lane & 15)) * DME_SLICE;
+        const int wr = wave / WC * NJ, wc = wave % WC * NI;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -114,12 +170,11 @@ struct DmeTile {
             const char* at = lds + buf * STAGE;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int off = ((h * 4 + g) ^ swz) * 16;
                 u32q p[NJ], q[NI];
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) p[j] = *(const u32q*)(at + prow + j * 16 * DME_SLICE + off);
+                for (int j = 0; j < NJ; ++j) p[j] = fragment<TR, PK>(at, wr + j, h);
 #pragma unroll
-                for (int i = 0; i < NI; ++i) q[i] = *(const u32q*)(at + qrow + i * 16 * DME_SLICE + off);
+                for (int i = 0; i < NI; ++i) q[i] = fragment<TC, QK>(at + TR * DME_SLICE, wc + i, h);
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -165,28 +220,35 @@ __global__ void dme_pack_kernel(const T* src, long long lds_, long long rows, lo
     }
 }
 
-// dst [cols][ldd] = transpose of src [rows][cols], zero beyond rows (ldd >= rows, in elements).
-template <class T>
-__global__ void dme_transpose_kernel(const T* src, long long lds_, long long rows, long long cols, T* dst, long long ldd) {
-    __shared__ T tile[64][65];
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const long long tiles_c = (cols + 63) / 64, tiles_r = (ldd + 63) / 64;
-    for (long long t = blockIdx.x; t < tiles_c * tiles_r; t += gridDim.x) {
-        const long long r0 = t / tiles_c * 64, c0 = t % tiles_c * 64;
-        for (int y = ty; y < 64; y += 4) {
-            const long long r = r0 + y, c = c0 + tx;
-            tile[y][tx] = r < rows && c < cols ? src[r * lds_ + c] : (T)0.f;
-        }
-        __syncthreads();
-        for (int y = ty; y < 64; y += 4) {
-            const long long c = c0 + y, r = r0 + tx;
-            if (c < cols && r < ldd) dst[c * ldd + r] = tile[tx][y];
-        }
-        __syncthreads();
-    }
-}
-
 inline int dme_blocks(long long work, long long per, long long most) {
     long long b = (work + per - 1) / per;
     return (int)(b < 1 ? 1 : b > most ? most : b);
+}
+
+// How a product of R x C outputs over `slices` slices of k is cut: tiles of 256, 128 or 64 a side, and into how many pieces of
+// k.  A workgroup of 256 x 256 has a CU to itself and makes 1230 TFLOP/s in bf16 at 8192^3, 128 x 128 two to a CU 970,
+// 64 x 64 four to a CU about 700 (fp32: 141, 138, 128); small products are bound by how many CUs have a tile at all, and pieces of k
+// cost a pass over their 32-bit sums.
+struct DmeCut {
+    int side, splits;
+    double us;
+};
+inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool split, double extra_per_tile_us = 0.0, bool symmetric = false) {
+    DmeCut best{0, 1, 0.0};
+    for (int side = 256; side >= 64; side /= 2) {
+        const int per_cu = side == 256 ? 1 : side == 128 ? 2 : 4;
+        const double rate = size == 4 ? (side == 256 ? 141e6 : side == 128 ? 138e6 : 128e6) : (side == 256 ? 1230e6 : side == 128 ? 970e6 : 700e6);
+        const long long along = (R + side - 1) / side, slots = 256ll * per_cu;
+        const long long tiles = symmetric ? along * (along + 1) / 2 : along * ((C + side - 1) / side);
+        // one slice of one tile while the CU's other places are taken too
+        const double slice = (double)side * side * (DME_SLICE / size) * 2.0 * slots / rate;
+        for (int s = 1; s <= (split ? 64 : 1); s *= 2) {
+            if (s > 1 && slices / s < 2) break;
+            const double rounds = (double)((tiles * s + slots - 1) / slots);
+            double us = rounds * ((double)((slices + s - 1) / s + 2) * slice + extra_per_tile_us * side * side / 65536.0 * per_cu);
+            if (s > 1) us += 4.0 + (double)s * R * C * 8.0 / 4e6;
+            if (best.side == 0 || us < best.us) best = DmeCut{side, s, us};
+        }
+    }
+    return best;
 }
