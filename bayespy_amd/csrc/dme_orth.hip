@@ -31,13 +31,10 @@ struct Scale<_Float16> {
 
 constexpr int NORM_BLOCKS = 256;
 
-// Sums of squares of the workgroups' shares, in 64 bits.  lines x length values, those of a line `step` apart.  Also clears the
-// 16 bytes that products read in place of what lies outside an operand.
+// Sums of squares of the workgroups' shares, in 64 bits.  lines x length values, those of a line `step` apart.
 template <class T>
-__global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, long long line, long long step, long long lines, long long length, double* part,
-                                                   u32* zeros) {
+__global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, long long line, long long step, long long lines, long long length, double* part) {
     __shared__ double sums[4];
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) zeros[threadIdx.x] = 0;
     const T* g = G + blockIdx.y * sb;
     double s = 0.0;
     constexpr int VEC = 16 / sizeof(T);
@@ -120,7 +117,6 @@ __global__ __launch_bounds__(256) void begin_kernel(const T* G, long long sb, lo
 template <class T, class W>
 struct StepArgs {
     Matrices<W> mat;
-    const char* zeros;
     float a, b, c;
     int from;  // which of Xw is read
     T* out;    // the last step's result, or null
@@ -164,7 +160,7 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void square_kernel(StepArg
     int s1 = s0 + a.per_split;
     s1 = s1 < a.slices ? s1 : a.slices;
     Tile t;
-    t.run(op, op, TALL ? x.rows : x.cols, a.zeros, lds, tr * SIDE, tc * SIDE, s0, s1);
+    t.run(op, op, TALL ? x.rows : x.cols, lds, tr * SIDE, tc * SIDE, s0, s1);
     constexpr float UNIT = 1.f / (Scale<W>::X * Scale<W>::X);
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
@@ -213,7 +209,7 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void poly_kernel(StepArgs<
     long long tr, tc;
     triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
     Tile t;
-    t.run(op, op, x.m, a.zeros, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+    t.run(op, op, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
     constexpr float UNIT = 1.f / (Scale<W>::S * Scale<W>::S);
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
@@ -256,7 +252,7 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void update_kernel(StepArg
     long long tr, tc;
     dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
     Tile t;
-    t.run(TALL ? y : b, TALL ? b : y, x.m, a.zeros, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+    t.run(TALL ? y : b, TALL ? b : y, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
     constexpr float UNIT = 1.f / (Scale<W>::B * Scale<W>::X);
     W* to = x.Xw[a.from ^ 1] + xo;
 #pragma unroll
@@ -299,7 +295,7 @@ inline long long up(long long v, long long to) { return (v + to - 1) / to * to; 
 struct StepPlan {
     long long m, n, ldx, lds;
     DmeCut square, poly, update;
-    long long zeros, norm, X, Xw[2], S, Sw, Bw, Sd, Bd, part, bytes;
+    long long norm, X, Xw[2], S, Sw, Bw, Sd, Bd, part, bytes;
 };
 
 StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
@@ -320,7 +316,6 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
         at += up(bytes, 256);
         return here;
     };
-    p.zeros = take(256);
     p.norm = take(batch * NORM_BLOCKS * 8);
     if (half) p.X = take(batch * rows * p.ldx * 4);
     for (int i = 0; i < 2; ++i) p.Xw[i] = take(batch * rows * p.ldx * size);
@@ -410,7 +405,6 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
     x.stride_x = rows * p.ldx;
     x.stride_s = p.m * p.lds;
     x.stride_part = p.square.splits * p.m * p.lds;
-    k.zeros = ws + p.zeros;
     k.a = (float)a;
     k.b = (float)b;
     k.c = (float)c;
@@ -423,7 +417,7 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
     const long long line = turn ? cs : rs, step = turn ? rs : cs, lines = turn ? cols : rows, length = turn ? rows : cols;
     const bool whole = step == 1 && line == length;
     hipLaunchKernelGGL(norm_kernel<T>, dim3(NORM_BLOCKS, (unsigned)batch), dim3(256), 0, s, G, sb, line, step, whole ? 1 : lines,
-                       whole ? lines * length : length, part, (u32*)(ws + p.zeros));
+                       whole ? lines * length : length, part);
     const long long tiles = (p.ldx + 63) / 64 * ((rows + 63) / 64);
     hipLaunchKernelGGL((begin_kernel<T, W>), dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, part, x);
     for (int i = 0; i < steps; ++i) {

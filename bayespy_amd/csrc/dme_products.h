@@ -53,6 +53,9 @@ struct DmeOperand {
 
 constexpr int DME_SLICE = 128;  // bytes of k in a slice
 
+// What products read in place of what lies outside an operand.  Never written.
+static __device__ __attribute__((aligned(256))) u32 dme_zeros[64];
+
 // The product of a TR x TC tile.  PK / QK: the operand is k-major.
 //
 // A k-major slice lies in LDS as it does in memory, one line of TR (TC) values for each k.  16-bit operands are turned by the
@@ -126,9 +129,8 @@ struct DmeTile {
     }
 
     // acc = the tile at (r0, c0) over the slices [s0, s1) of k < K.  lds: 2 * STAGE bytes, free for the caller afterwards (a
-    // barrier has been passed).  zeros: 16 zero bytes, read in place of what lies outside.  Every thread of the workgroup calls this.
-    __device__ __forceinline__ void run(const DmeOperand& P, const DmeOperand& Q, long long K, const char* zeros, char* lds, long long r0, long long c0,
-                                        int s0, int s1) {
+    // barrier has been passed).  Every thread of the workgroup calls this.
+    __device__ __forceinline__ void run(const DmeOperand& P, const DmeOperand& Q, long long K, char* lds, long long r0, long long c0, int s0, int s1) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const char* src[PER_WAVE];
         int limit[PER_WAVE];
@@ -149,7 +151,7 @@ struct DmeTile {
             for (int t = 0; t < PER_WAVE; ++t) {
                 const int piece = t * NW + wave;
                 if (COPIES % NW == 0 || piece < COPIES) {
-                    const char* from = s < limit[t] ? src[t] : zeros;
+                    const char* from = s < limit[t] ? src[t] : (const char*)dme_zeros;
                     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                                      (__attribute__((address_space(3))) void*)(lds + buf * STAGE + piece * 1024), 16, 0, 0);
                     src[t] += piece < TR / 8 ? pstep : qstep;

@@ -75,6 +75,34 @@ __device__ __forceinline__ double g_of(int likelihood, double z, double x) {
     return likelihood == DME_LIKELIHOOD_DIRICHLET ? dirichlet_g(z, x) : x;
 }
 
+// e^z in 32 bits, good to a few last bits however large |z|: the exponent's rounding is made up for.
+__device__ __forceinline__ float exp_f32(float z) {
+    const float t = z * LOG2E, rest = __builtin_fmaf(z, LOG2E, -t) + z * 1.9259630e-8f;  // log2 e - LOG2E
+    const float e = __builtin_amdgcn_exp2f(t);
+    return z > -100.f ? __builtin_fmaf(e, rest * 0.69314718f, e) : 0.f;  // (-inf - -inf) kept out
+}
+
+// The counts that most cells of a dense matrix hold: 1 <= x <= 16, and e^z small enough for 32-bit products of the 15 terms
+// (64 + 15)^15 < 2^96.  F = z + log prod_{1 <= n < x} (e^z + n) with one logarithm, G = 1 + e^z sum 1 / (e^z + n) with one
+// reciprocal of the same product: 15 roundings of 2^-24 at most.  Others take the 64-bit functions above.
+__device__ __forceinline__ bool is_small(float z, int x) { return x <= 16 && z <= 4.1f; }
+__device__ __forceinline__ float small_f(float z, int x) {
+    const float a = exp_f32(z);
+    float prod = 1.f;
+    for (int n = 1; n < x; ++n) prod *= a + (float)n;
+    return __builtin_fmaf(__builtin_amdgcn_logf(prod), 0.69314718f, z);
+}
+__device__ __forceinline__ float small_g(float z, int x) {
+    const float a = exp_f32(z);
+    float den = 1.f, num = 0.f;
+    for (int n = 1; n < x; ++n) {
+        const float term = a + (float)n;
+        num = __builtin_fmaf(num, term, den);
+        den *= term;
+    }
+    return __builtin_fmaf(a * num, __builtin_amdgcn_rcpf(den), 1.f);
+}
+
 // Reductions over the 16 lanes that share a row.
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float v) {
@@ -123,7 +151,6 @@ __device__ __forceinline__ int count_at(const Rows& rows, long long r, long long
 struct TileArgs {
     DmeOperand h, w;
     long long D;
-    const char* zeros;
     long long tiles_r, tiles_c;
     int slices;
     const float* bias;
@@ -175,30 +202,120 @@ __device__ __forceinline__ float dot_step(const u32q& h, const u32q& w, float s,
     return s;
 }
 
-// z at a row's counts: a scalar product for each, 16 lanes an entry.  There are few of them beside the N K values of z that the
-// tiles make (and drop), so they are made once more here instead of being looked for in every tile.  `first` of every
-// `step` entries, by the caller's 16-lane group.
+// z at a row's counts: a scalar product for each, 16 lanes an entry, 16 entries of a wave in flight.  There are few of them beside
+// the N K values of z that the tiles make (and drop), so they are made once more here instead of being looked for in every tile.
+// One wave takes batches `first`, `first + step`, ... of 16 entries.
 template <class T, int KIND>
 __device__ __forceinline__ void entries_of(const TileArgs& a, long long r, int first, int step) {
-    const int sub = threadIdx.x & 15;
+    const int lane = threadIdx.x & 63, sub = lane & 15, group = lane >> 4;
     const int chunks = (int)((a.D * (long long)sizeof(T) + 15) / 16);
     const u32q* h = (const u32q*)(a.h.at + r * a.h.ld);
     const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
-    for (long long e = p0 + first; e < p1; e += step) {
-        const long long k = KIND == CSR ? (long long)a.rows.col[e] : a.rows.labels[r];
-        if (k < 0 || k >= a.K) continue;  // the row's 16 lanes together
-        const u32q* w = (const u32q*)(a.w.at + k * a.w.ld);
-        float s = 0.f;
-        for (int q = sub; q < chunks; q += 16) s = dot_step(h[q], w[q], s, T());
-        s = sum16(s);
-        if (sub == 0) a.entry_z[e] = s + (a.bias ? a.bias[k] : 0.f);
+    for (long long e0 = p0 + first * 16; e0 < p1; e0 += step * 16) {
+        int col = -1;
+        if (e0 + sub < p1) {
+            const long long k = KIND == CSR ? (long long)a.rows.col[e0 + sub] : a.rows.labels[r];
+            col = k >= 0 && k < a.K ? (int)k : -1;
+        }
+        constexpr int DEEP = KIND == CSR ? 4 : 1;
+        int k[DEEP];
+        const u32q* w[DEEP];
+        float s[DEEP];
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) {
+            k[u] = __shfl(col, u * 4 + group);
+            w[u] = (const u32q*)(a.w.at + (k[u] < 0 ? 0 : k[u]) * a.w.ld);  // row 0 in place of none: read, not used
+            s[u] = 0.f;
+        }
+        for (int q = sub; q < chunks; q += 16) {
+            const u32q x = h[q];
+            u32q y[DEEP];
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u) y[u] = w[u][q];
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u) s[u] = dot_step(x, y[u], s[u], T());
+        }
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) {
+            s[u] = sum16(s[u]);
+            if (sub == 0 && k[u] >= 0) a.entry_z[e0 + u * 4 + group] = s[u] + (a.bias ? a.bias[k[u]] : 0.f);
+        }
     }
 }
 
 template <class T, int KIND>
 __global__ __launch_bounds__(256) void entry_kernel(TileArgs a) {
     const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r < a.nb) entries_of<T, KIND>(a, r, (threadIdx.x & 63) >> 4, 4);
+    if (r < a.nb) entries_of<T, KIND>(a, r, 0, 1);
+}
+
+__device__ __forceinline__ f32x2 merge(f32x2 v, f32x2 o) {
+    const float m = fmaxf(v[0], o[0]), base = m == -INFINITY ? 0.f : m;
+    return f32x2{m, v[1] * __builtin_amdgcn_exp2f(v[0] - base) + o[1] * __builtin_amdgcn_exp2f(o[0] - base)};
+}
+
+// The forward pass for up to 16 rows: a read of the weights and little else.  A wave makes 16 columns for all rows; its weights
+// go from memory straight into the matrix instructions' registers, WIDE loads of 16 bytes a lane ahead, and the rows wait in LDS.
+// Nothing is shared between waves but the rows, so many small workgroups keep ~200 KB a CU in flight.  Workgroups beyond the
+// columns make the rows' z at their counts, so that a call has two launches.
+template <class T, int KIND>
+__global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ f32x2 seen[4][16];
+    if (blockIdx.x >= a.tiles_c) {
+        if constexpr (KIND != DENSE) entries_of<T, KIND>(a, blockIdx.x - a.tiles_c, threadIdx.x >> 6, 4);
+        return;
+    }
+    constexpr int WIDE = 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int chunks = (int)((a.D * (long long)sizeof(T) + 15) / 16), rounds = (chunks + 3) / 4;  // a round: 64 bytes of each row
+    const long long k0 = (long long)blockIdx.x * 64 + wave * 16;
+    const long long k = k0 + c < a.K ? k0 + c : a.K - 1;
+    const u32q* w = (const u32q*)(a.w.at + k * a.w.ld);
+    const u32q none = u32q{0, 0, 0, 0};
+    u32q y[2][WIDE];
+    auto load = [&](u32q* to, int round) {
+#pragma unroll
+        for (int u = 0; u < WIDE; ++u) {
+            const int at = (round + u) * 4 + g;
+            to[u] = at < chunks ? __builtin_nontemporal_load(w + at) : none;
+        }
+    };
+    load(y[0], 0);
+    const int pitch = (rounds * 4 + 4) * 16;  // bytes; the four chunks more spread the rows over the banks
+    for (int i = tid; i < 16 * rounds * 4; i += 256) {
+        const int r = i / (rounds * 4), at = i - r * (rounds * 4);
+        u32q v = none;
+        if (r < a.nb && at < chunks) v = *(const u32q*)(a.h.at + r * a.h.ld + at * 16);
+        *(u32q*)(lds + r * pitch + at * 16) = v;
+    }
+    __syncthreads();
+    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    const char* h = lds + c * pitch + g * 16;
+    auto multiply = [&](const u32q* with, int round) {
+#pragma unroll
+        for (int u = 0; u < WIDE; ++u)
+            if (round + u < rounds) acc[u & 1] = dme_mma(with[u], *(const u32q*)(h + (round + u) * 64), acc[u & 1], T());
+    };
+    for (int round = 0; round < rounds; round += 2 * WIDE) {
+        load(y[1], round + WIDE);
+        multiply(y[0], round);
+        load(y[0], round + 2 * WIDE);
+        multiply(y[1], round + WIDE);
+    }
+    const f32x4 z = acc[0] + acc[1] + bias_of(a, k0 + g * 4);
+    float m = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = LOG2E * fmaxf(m, __shfl_xor(m, 32));
+    const float base = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[q], LOG2E, -base));
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (g == 0) seen[wave][c] = f32x2{m, s};
+    __syncthreads();
+    if (tid < 16 && tid < a.nb) a.part[blockIdx.x * a.nb + tid] = merge(merge(seen[0][tid], seen[1][tid]), merge(seen[2][tid], seen[3][tid]));
 }
 
 // Tiles of z, reduced where the matrix instructions left them: a lane has NJ rows and 4 NI columns of each.
@@ -206,21 +323,15 @@ __global__ __launch_bounds__(256) void entry_kernel(TileArgs a) {
 //             the same M that the sum is kept with, so that its rounding costs nothing
 //   backward  2^(z log2 e - l log2 e) coef, rounded to T (the gradient's one rounding before its products), and the columns' sums
 //             of the unrounded values.  The counts are not looked at: patch_kernel puts them in.
-// With TR = 16 (few rows) the weights are read once from memory and each workgroup beyond the tiles makes one row's z at
-// its counts, so that a call has two launches.
-template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD>
+template <class T, int TR, int TC, int WR, int WC, bool BACKWARD>
 __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DmeTile<T, TR, TC, WR, WC> Tile;
-    if (TR == 16 && !BACKWARD && blockIdx.x >= a.tiles_r * a.tiles_c) {
-        if constexpr (KIND != DENSE) entries_of<T, KIND>(a, blockIdx.x - a.tiles_r * a.tiles_c, threadIdx.x >> 4, WR * WC * 4);
-        return;
-    }
     long long tr, tc;
     dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * TC, k0 = a.column + c0;
     Tile t;
-    t.run(a.h, a.w, a.D, a.zeros, lds, r0, c0, 0, a.slices);
+    t.run(a.h, a.w, a.D, lds, r0, c0, 0, a.slices);
     const int tid = threadIdx.x, g = (tid & 63) >> 4, wc = (tid >> 6) % WC, wr = (tid >> 6) / WC;
 #pragma unroll
     for (int i = 0; i < Tile::NI; ++i) {
@@ -254,12 +365,7 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
         if (tid < TR && r0 + tid < a.nb) {
             f32x2 v = seen[tid];
 #pragma unroll
-            for (int w = 1; w < WC; ++w) {
-                const f32x2 o = seen[w * TR + tid];
-                const float m = fmaxf(v[0], o[0]), base = m == -INFINITY ? 0.f : m;
-                v[1] = v[1] * __builtin_amdgcn_exp2f(v[0] - base) + o[1] * __builtin_amdgcn_exp2f(o[0] - base);
-                v[0] = m;
-            }
+            for (int w = 1; w < WC; ++w) v = merge(v, seen[w * TR + tid]);
             a.part[tc * a.nb + r0 + tid] = v;
         }
         return;
@@ -306,8 +412,42 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
 constexpr int DT = 128;      // columns of a tile with dense counts
 constexpr int ZP = DT + 4;   // its pitch in LDS (a multiple of 16 bytes that spreads the rows over the banks)
 
+// Eight neighbouring counts of a row, as they lie (16 or 32 bytes); 0 beyond K.
+struct Counts {
+    u32q lo, hi;
+    __device__ __forceinline__ void load(const Rows& rows, long long r, long long k, long long K) {
+        const char* at = rows.X + (r * rows.ldx + k) * rows.elem;
+        lo = hi = u32q{0, 0, 0, 0};
+        if (k + 8 <= K && ((uintptr_t)at & 15) == 0) {
+            lo = __builtin_nontemporal_load((const u32q*)at);
+            if (rows.elem == 4) hi = __builtin_nontemporal_load((const u32q*)at + 1);
+        } else if (rows.elem == 2) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (k + q < K) lo[q / 2] |= (u32)((const unsigned short*)at)[q] << (q % 2 * 16);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (k + q < K) lo[q] = ((const u32*)at)[q];
+                if (k + 4 + q < K) hi[q] = ((const u32*)at)[4 + q];
+            }
+        }
+    }
+    template <int Q>
+    __device__ __forceinline__ int get(int elem) const {
+        if (elem == 2) return (int)(lo[Q / 2] >> (Q % 2 * 16) & 0xffff);
+        return (int)(Q < 4 ? lo[Q & 3] : hi[Q & 3]);
+    }
+};
+
+template <int Q = 0, class F>
+__device__ __forceinline__ void each_count(const Counts& c, int elem, F f) {
+    f(Q, c.get<Q>(elem));
+    if constexpr (Q < 7) each_count<Q + 1>(c, elem, f);
+}
+
 // Tiles of z with a dense matrix of counts: every value of z may meet a count, so the tile lies in LDS in 32 bits, where a row's
-// 16 lanes read it beside the counts (both in order of the columns) in a loop short enough for F and G.
+// 16 lanes read it beside the counts, eight neighbouring columns a lane, the next rows' counts on their way.
 template <class T, int TR, bool BACKWARD>
 __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -316,9 +456,12 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * DT, k0 = a.column + c0;
     float* z = (float*)lds;
+    const int tid = threadIdx.x, sub = tid & 15;
+    Counts next;
+    if (r0 + (tid >> 4) < a.nb) next.load(a.rows, r0 + (tid >> 4), k0 + sub * 8, a.K);
     {
         Tile t;
-        t.run(a.h, a.w, a.D, a.zeros, lds, r0, c0, 0, a.slices);
+        t.run(a.h, a.w, a.D, lds, r0, c0, 0, a.slices);
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) {
             const int c = Tile::col_of(i);
@@ -328,69 +471,64 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
         }
     }
     __syncthreads();
-    const int tid = threadIdx.x, sub = tid & 15;
-    if (!BACKWARD) {
+    const bool dirichlet = a.likelihood == DME_LIKELIHOOD_DIRICHLET;
+    T* dz = (T*)a.dz;
 #pragma unroll 1
-        for (int row = tid >> 4; row < TR; row += 16) {
-            const long long r = r0 + row;
-            if (r >= a.nb) break;  // all of a row's lanes, and rows only ascend
-            const float* zr = z + row * ZP;
-            const f32x4 u = *(const f32x4*)(zr + sub * 4), w = *(const f32x4*)(zr + 64 + sub * 4);
+    for (int row = tid >> 4; row < TR; row += 16) {
+        const long long r = r0 + row;
+        float* zr = z + row * ZP + sub * 8;
+        if (r >= a.nb) {  // all of a row's lanes
+            if (!BACKWARD) break;
+            *(f32x4*)zr = *(f32x4*)(zr + 4) = f32x4{0.f, 0.f, 0.f, 0.f};
+            continue;
+        }
+        const Counts x = next;
+        if (row + 16 < TR && r + 16 < a.nb) next.load(a.rows, r + 16, k0 + sub * 8, a.K);
+        const f32x4 u = *(const f32x4*)zr, w = *(const f32x4*)(zr + 4);
+        if (!BACKWARD) {
             const float m = LOG2E * max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))));
             const float base = m == -INFINITY ? 0.f : m;
-            float s = 0.f;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                s += __builtin_amdgcn_exp2f(__builtin_fmaf(u[q], LOG2E, -base)) + __builtin_amdgcn_exp2f(__builtin_fmaf(w[q], LOG2E, -base));
-            s = sum16(s);
+            float s = 0.f, near = 0.f;
             double f = 0.0, t = 0.0;
             bool bad = false;
-#pragma unroll 1
-            for (int q = 0; q < 8; ++q) {
-                const int c = q * 16 + sub;
-                if (k0 + c >= a.K) break;
-                const int x = count_at(a.rows, r, k0 + c);
-                if (x < 0) bad = true;
-                if (x > 0) {
-                    t += (double)x;
-                    f += f_of(a.likelihood, (double)zr[c], (double)x);
+            each_count(x, a.rows.elem, [&](int q, int v) {
+                const float zq = q < 4 ? u[q & 3] : w[q & 3];
+                s += __builtin_amdgcn_exp2f(__builtin_fmaf(zq, LOG2E, -base));
+                bad |= v < 0;
+                t += (double)v;
+                if (v > 0) {
+                    if (!dirichlet)
+                        f += (double)v * (double)zq;
+                    else if (is_small(zq, v))
+                        near += small_f(zq, v);
+                    else
+                        f += dirichlet_f((double)zq, (double)v);
                 }
-            }
-            f = sum16(f);
+            });
+            s = sum16(s);
+            f = sum16(f + (double)near);
             t = sum16(bad ? __builtin_nan("") : t);
             if (sub == 0) {
                 a.part[tc * a.nb + r] = f32x2{m, s};
                 a.part_f[tc * a.nb + r] = f;
                 a.part_t[tc * a.nb + r] = t;
             }
-        }
-        return;
-    }
-    T* dz = (T*)a.dz;
-#pragma unroll 1
-    for (int row = tid >> 4; row < TR; row += 16) {
-        const long long r = r0 + row;
-        const bool real = r < a.nb;
-        const float l2 = real ? a.lse2[r] : INFINITY, cf = real ? a.coef[r] : 0.f, weight = real ? a.weight[r] : 0.f;
-        float* zr = z + row * ZP;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int c = h * 64 + sub * 4;
-            const f32x4 v = *(const f32x4*)(zr + c);
-            f32x4 d;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                d[q] = real ? __builtin_amdgcn_exp2f(__builtin_fmaf(v[q], LOG2E, -l2)) * cf : 0.f;
-                if (real && k0 + c + q < a.K) {
-                    const int x = count_at(a.rows, r, k0 + c + q);
-                    if (x != 0) d[q] -= weight * (float)g_of(a.likelihood, (double)v[q], (double)x);
-                }
-            }
-            *(f32x4*)(zr + c) = d;
-            if (real) dme_store4(dz + r * a.lddz + c0 + c, d);
+        } else {
+            const float l2 = a.lse2[r], cf = a.coef[r], weight = a.weight[r];
+            f32x4 d[2];
+            each_count(x, a.rows.elem, [&](int q, int v) {
+                const float zq = q < 4 ? u[q & 3] : w[q & 3];
+                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(zq, LOG2E, -l2)) * cf;
+                if (v > 0) e -= weight * (!dirichlet ? (float)v : is_small(zq, v) ? small_g(zq, v) : (float)dirichlet_g((double)zq, (double)v));
+                d[q >> 2][q & 3] = e;
+            });
+            *(f32x4*)zr = d[0];
+            *(f32x4*)(zr + 4) = d[1];
+            dme_store4(dz + r * a.lddz + c0 + sub * 8, d[0]);
+            dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, d[1]);
         }
     }
-    if (!a.dbias) return;
+    if (!BACKWARD || !a.dbias) return;
     __syncthreads();
     const int c = tid & 127, half = tid >> 7;
     float sum = 0.f;
@@ -401,30 +539,6 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     __syncthreads();
     if (!half && k0 + c < a.K) a.dbias[tr * a.K + k0 + c] = sum + z[c];
 }
-
-// Reductions over the lanes that share a row: 16, or a workgroup's 256.
-template <int LANES>
-struct Together {
-    double* shared;  // [4] (LANES == 256)
-    template <class F>
-    __device__ __forceinline__ double over_waves(double v, F f) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-        __syncthreads();
-        return f(f(shared[0], shared[1]), f(shared[2], shared[3]));
-    }
-    __device__ __forceinline__ double sum(double v) {
-        if constexpr (LANES == 16) return sum16(v);
-        return over_waves(dme_wave_sum_f64(v), [](double x, double y) { return x + y; });
-    }
-    __device__ __forceinline__ float max(float v) {
-        v = max16(v);
-        if constexpr (LANES == 16) return v;
-        v = fmaxf(v, __shfl_xor(v, 16));
-        v = fmaxf(v, __shfl_xor(v, 32));
-        return (float)over_waves((double)v, [](double x, double y) { return x > y ? x : y; });
-    }
-};
 
 struct RowArgs {
     long long nb, K;
@@ -445,35 +559,74 @@ struct RowArgs {
 
 // The row's pieces become l, the loss, and what the gradient needs of them, in 64 bits.  CSR rows are checked here: columns
 // strictly ascending and below K, no negative count, rowptr in order; a row that breaks this has total NaN.
+// A workgroup takes 256 / LANES rows.  The pieces lie row beside row, so neighbouring lanes take neighbouring rows there; the counts lie
+// entry beside entry, so neighbouring lanes take a row's neighbouring entries.
 template <int LANES>
 __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
-    __shared__ double shared[4];
-    Together<LANES> row{shared};
-    const int sub = threadIdx.x % LANES;
-    const long long r = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    constexpr int ROWS = 256 / LANES;
+    __shared__ float m_seen[LANES][ROWS];
+    __shared__ double s_seen[LANES][ROWS], f_seen[LANES][ROWS], t_seen[LANES][ROWS];
+    const long long first = (long long)blockIdx.x * ROWS;
+    {
+        const int row = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
+        const long long r = first + row < a.nb ? first + row : a.nb - 1;
+        float m = -INFINITY;
+        double s = 0.0, f = 0.0, t = 0.0;
+        for (int tile = lane; tile < a.tiles; tile += 4 * LANES) {
+            f32x2 p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = tile + u * LANES < a.tiles ? a.part[(tile + u * LANES) * a.nb + r] : f32x2{-INFINITY, 0.f};
+            const float top = fmaxf(fmaxf(m, fmaxf(p[0][0], p[1][0])), fmaxf(p[2][0], p[3][0])), base = top == -INFINITY ? 0.f : top;
+            s *= (double)__builtin_amdgcn_exp2f(m - base);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s += (double)p[u][1] * (double)__builtin_amdgcn_exp2f(p[u][0] - base);
+            m = top;
+        }
+        if (a.kind == DENSE)
+            for (int tile = lane; tile < a.tiles; tile += LANES) {
+                f += a.part_f[tile * a.nb + r];
+                t += a.part_t[tile * a.nb + r];
+            }
+        m_seen[lane][row] = m;
+        s_seen[lane][row] = s;
+        f_seen[lane][row] = f;
+        t_seen[lane][row] = t;
+    }
+    __syncthreads();
+    const int row = threadIdx.x / LANES, sub = threadIdx.x % LANES;
+    const long long r = first + row;
     const bool real = r < a.nb;
     const long long rr = real ? r : a.nb - 1;
-    float m = -INFINITY;
-    for (int t = sub; t < a.tiles; t += LANES) m = fmaxf(m, a.part[t * a.nb + rr][0]);
-    m = row.max(m);
-    const float base = m == -INFINITY ? 0.f : m;
-    double s = 0.0, f = 0.0, total = 0.0;
-    for (int t = sub; t < a.tiles; t += LANES) {
-        const f32x2 p = a.part[t * a.nb + rr];
-        s += (double)p[1] * (double)__builtin_amdgcn_exp2f(p[0] - base);
+    float m;
+    double s, f, total;
+    if constexpr (LANES == 16) {
+        m = max16(m_seen[sub][row]);
+        const float base = m == -INFINITY ? 0.f : m;
+        s = sum16(s_seen[sub][row] * (double)__builtin_amdgcn_exp2f(m_seen[sub][row] - base));
+        f = sum16(f_seen[sub][row]);
+        total = sum16(t_seen[sub][row]);
+    } else {  // one row: each wave makes the same sums of all
+        const int l = threadIdx.x & 63;
+        m = fmaxf(fmaxf(m_seen[l][0], m_seen[l + 64][0]), fmaxf(m_seen[l + 128][0], m_seen[l + 192][0]));
+        m = max16(m);
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const float base = m == -INFINITY ? 0.f : m;
+        s = f = total = 0.0;
+#pragma unroll
+        for (int u = 0; u < 256; u += 64) {
+            s += s_seen[l + u][0] * (double)__builtin_amdgcn_exp2f(m_seen[l + u][0] - base);
+            f += f_seen[l + u][0];
+            total += t_seen[l + u][0];
+        }
+        s = dme_wave_sum_f64(s);
+        f = dme_wave_sum_f64(f);
+        total = dme_wave_sum_f64(total);
     }
-    s = row.sum(s);
-    const double exact2 = s == 0.0 ? -INFINITY : (double)base + log2(s), lse = exact2 * (1.0 / (double)LOG2E);
+    const double exact2 = s == 0.0 ? -INFINITY : (double)m + log2(s), lse = exact2 * (1.0 / (double)LOG2E);
     const float weight = a.weights ? a.weights[rr] : 1.f;
     float most = 0.f;
-    if (a.kind == DENSE) {
-        for (int t = sub; t < a.tiles; t += LANES) {
-            f += a.part_f[t * a.nb + rr];
-            total += a.part_t[t * a.nb + rr];
-        }
-        f = row.sum(f);
-        total = row.sum(total);
-    } else if (a.kind == CSR) {
+    if (a.kind == CSR) {
         const long long q0 = a.rows.rowptr[rr], q1 = a.rows.rowptr[rr + 1];
         const long long e0 = row_begin(a.rows, rr), e1 = row_begin(a.rows, rr + 1);
         bool bad = q0 < 0 || q1 < q0 || q1 > a.rows.nnz;
@@ -483,18 +636,33 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
                 bad = true;
                 continue;
             }
-            const double z = (double)a.entry_z[e];
+            const float z = a.entry_z[e];
             total += (double)x;
-            f += f_of(a.likelihood, z, (double)x);
+            const bool near = a.likelihood == DME_LIKELIHOOD_DIRICHLET && x > 0 && is_small(z, x);
+            f += near ? (double)small_f(z, x) : f_of(a.likelihood, (double)z, (double)x);
             if (a.lse2 && real) {
-                const float v = weight * (float)g_of(a.likelihood, z, (double)x);
+                const float v = weight * (near ? small_g(z, x) : (float)g_of(a.likelihood, (double)z, (double)x));
                 a.entry_g[e] = v;
                 most = fmaxf(most, fabsf(v));
             }
         }
-        f = row.sum(f);
-        total = row.sum(bad ? __builtin_nan("") : total);
-    } else {
+        if (bad) total = __builtin_nan("");
+        if constexpr (LANES == 16) {
+            f = sum16(f);
+            total = sum16(total);
+        } else {  // through LDS, in the waves' order
+            f = dme_wave_sum_f64(f);
+            total = dme_wave_sum_f64(total);
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) {
+                f_seen[threadIdx.x >> 6][0] = f;
+                t_seen[threadIdx.x >> 6][0] = total;
+            }
+            __syncthreads();
+            f = (f_seen[0][0] + f_seen[1][0]) + (f_seen[2][0] + f_seen[3][0]);
+            total = (t_seen[0][0] + t_seen[1][0]) + (t_seen[2][0] + t_seen[3][0]);
+        }
+    } else if (a.kind == LABELS) {
         const long long k = a.rows.labels[rr];
         total = k < 0 ? 0.0 : k < a.K ? 1.0 : __builtin_nan("");
         f = k >= 0 && k < a.K ? (double)a.entry_z[rr] : 0.0;  // F(z, 1) = z, G(z, 1) = 1 in both likelihoods
@@ -503,13 +671,11 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
             most = k >= 0 ? fabsf(weight) : 0.f;
         }
     }
-    if (a.lse2 && a.kind != DENSE) {
-        most = row.max(most);
-        if (LANES == 16) {  // one atomic a wave
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-        }
-        if ((threadIdx.x & 63) == 0 && most > 0.f && (LANES == 16 || threadIdx.x == 0)) atomicMax(a.largest, __builtin_bit_cast(u32, most));
+    if (a.lse2 && a.kind != DENSE) {  // one atomic a wave
+        most = max16(most);
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(a.largest, __builtin_bit_cast(u32, most));
     }
     if (!real || sub != 0) return;
     a.loss[r] = total == 0.0 ? 0.f : (float)(f_of(a.likelihood, lse, total) - f);
@@ -542,29 +708,57 @@ __device__ __forceinline__ int fixed_shift(const u32* largest, int headroom) {
 }
 
 // d loss / d z at the counts: the tiles' value made again, minus G, in its place.  What dbias needs of G is added up in fixed
-// point, 64 bits wide: sums of whole numbers do not depend on their order.  16 lanes a row.
-template <class T, int KIND>
-__global__ __launch_bounds__(256) void patch_kernel(PatchArgs a) {
-    const int sub = threadIdx.x & 15;
-    const long long r = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (r >= a.nb) return;
-    const float l2 = a.lse2[r], cf = a.coef[r];
-    const int shift = a.fixed ? fixed_shift(a.largest, a.headroom) : 0;
-    const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
-    for (long long e = p0 + sub; e < p1; e += 16) {
-        const long long k = KIND == CSR ? (long long)a.rows.col[e] : a.rows.labels[r];
-        const long long c = k - a.column;
-        if (c < 0 || c >= a.width || k >= a.K) continue;
-        const float g = a.entry_g[e];
-        ((T*)a.dz)[r * a.lddz + c] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(a.entry_z[e], LOG2E, -l2)) * cf - g);
-        if (a.fixed && __builtin_isfinite(g)) atomicAdd((u64*)(a.fixed + k), (u64)llrint(ldexp((double)g, shift)));
+// point, 64 bits wide: sums of whole numbers do not depend on their order.  A workgroup adds its entries up by column in LDS first:
+// word frequencies send thousands of entries to one address, where memory takes one at a time (4099 rows, 144 000 entries: 88 us with
+// an atomic each).  LANES lanes a row.
+template <class T, int KIND, int LANES>
+__global__ __launch_bounds__(1024) void patch_kernel(PatchArgs a) {
+    constexpr int SLOTS = 2048;
+    __shared__ int keys[SLOTS];
+    __shared__ u64 sums[SLOTS];
+    const bool add = a.fixed != nullptr;
+    if (add) {
+        for (int i = threadIdx.x; i < SLOTS; i += 1024) {
+            keys[i] = -1;
+            sums[i] = 0;
+        }
+        __syncthreads();
     }
+    const int sub = threadIdx.x % LANES;
+    const long long r = (long long)blockIdx.x * (1024 / LANES) + threadIdx.x / LANES;
+    if (r < a.nb) {
+        const float l2 = a.lse2[r], cf = a.coef[r];
+        const int shift = add ? fixed_shift(a.largest, a.headroom) : 0;
+        const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
+        for (long long e = p0 + sub; e < p1; e += LANES) {
+            const long long k = KIND == CSR ? (long long)a.rows.col[e] : a.rows.labels[r];
+            const long long c = k - a.column;
+            if (c < 0 || c >= a.width || k >= a.K) continue;
+            const float g = a.entry_g[e];
+            ((T*)a.dz)[r * a.lddz + c] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(a.entry_z[e], LOG2E, -l2)) * cf - g);
+            if (!add || !__builtin_isfinite(g)) continue;
+            const u64 v = (u64)llrint(ldexp((double)g, shift));
+            u32 slot = ((u32)k * 2654435761u) >> 21;
+            bool done = false;
+            for (int probe = 0; probe < 8 && !done; ++probe, slot = (slot + 1) % SLOTS) {
+                const int was = atomicCAS(&keys[slot], -1, (int)k);
+                if (was == -1 || was == (int)k) {
+                    atomicAdd(&sums[slot], v);
+                    done = true;
+                }
+            }
+            if (!done) atomicAdd((u64*)(a.fixed + k), v);
+        }
+    }
+    if (!add) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < SLOTS; i += 1024)
+        if (keys[i] >= 0 && sums[i] != 0) atomicAdd((u64*)(a.fixed + keys[i]), sums[i]);
 }
 
 struct ProductArgs {
     DmeOperand p, q;
     long long k;
-    const char* zeros;
     long long tiles_r, tiles_c;
     int slices, per_split;
     float* part;        // [split][R][ldpart], or null: the result goes to out in T
@@ -586,7 +780,7 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void product_kernel(Produc
     int s1 = s0 + a.per_split;
     s1 = s1 < a.slices ? s1 : a.slices;
     Tile t;
-    t.run(a.p, a.q, a.k, a.zeros, lds, tr * SIDE, tc * SIDE, s0, s1);
+    t.run(a.p, a.q, a.k, lds, tr * SIDE, tc * SIDE, s0, s1);
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
         const long long r = tr * SIDE + Tile::row_of(j);
@@ -649,16 +843,20 @@ struct Plan {
     long long dpad;           // k of the first product in a packed operand
     long long nb;             // rows of a block
     int side;                 // of the tiles of z: 256, 128, or 16 rows x 128 columns
-    long long tile_rows, tile_cols, tiles;
+    bool few;                 // the forward pass goes by few_kernel
+    long long tile_rows, tile_cols;
+    long long tiles;          // pieces that the forward pass leaves of a row
     long long chunk;          // columns of a piece of d loss / d z
     DmeCut cut_w, cut_h;
     bool part_w, part_h;      // the products leave 32-bit pieces
     long long ldpart;
     int headroom;
     // places in the workspace
-    long long zeros, h, w, part, part_f, part_t, entry_z, entry_g, lse2, coef, weight, dbias, fixed, dz, pw, ph, bytes;
-    long long zero_words;     // from the beginning: the zeros, the largest entry, the fixed-point sums
+    long long largest, fixed, h, w, part, part_f, part_t, entry_z, entry_g, lse2, coef, weight, dbias, dz, pw, ph, bytes;
+    long long zero_words;     // from the beginning: the largest entry and the fixed-point sums
 };
+
+inline long long few_lds(long long bytes) { return 16 * (up(bytes, 64) + 64); }
 
 Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int type, long long N, long long K, long long D,
                const dme_count_rows_t* rows, bool gradient) {
@@ -675,16 +873,21 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     p.side = p.nb <= 16 ? 16 : rows->kind == DENSE ? 128 : dme_cut(p.nb, K, slices, p.size, false, 4.0).side < 256 ? 128 : 256;
     p.tile_rows = p.side;
     p.tile_cols = p.side == 16 ? 128 : p.side;
-    p.tiles = (K + p.tile_cols - 1) / p.tile_cols;
+    const long long tiles = (K + p.tile_cols - 1) / p.tile_cols;
+    // up to 16 rows, while they fit into the LDS that needs no attribute
+    p.few = p.side == 16 && rows->kind != DENSE && few_lds(D * p.size) <= 61440;
+    p.tiles = p.few ? (K + 63) / 64 : tiles;
     long long at = 0;
     const auto take = [&](long long bytes) {
         const long long here = at;
         at += up(bytes, 256);
         return here;
     };
-    p.zeros = take(256);
-    if (gradient && rows->kind != DENSE) p.fixed = take(K * 8);
-    p.zero_words = at / 4;
+    if (gradient && rows->kind != DENSE) {
+        p.largest = take(256);
+        p.fixed = take(K * 8);
+        p.zero_words = at / 4;
+    }
     if (p.pack_h) p.h = take(p.nb * p.dpad * p.size);
     if (p.pack_w) p.w = take(K * p.dpad * p.size);
     p.part = take(p.tiles * p.nb * 8);
@@ -705,15 +908,15 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         p.dbias = take((p.nb + p.tile_rows - 1) / p.tile_rows * K * 4);
         long long c = PIECE_BYTES / (p.nb * p.size) / p.tile_cols;
         if (c < 1) c = 1;
-        if (c > p.tiles) c = p.tiles;
-        const long long pieces = (p.tiles + c - 1) / c;
-        p.chunk = (p.tiles + pieces - 1) / pieces * p.tile_cols;  // pieces of like width
+        if (c > tiles) c = tiles;
+        const long long pieces = (tiles + c - 1) / c;
+        p.chunk = (tiles + pieces - 1) / pieces * p.tile_cols;  // pieces of like width
         p.dz = take(p.nb * p.chunk * p.size);
         p.ldpart = up(D, 4);
         p.cut_w = dme_cut(p.chunk < K ? p.chunk : K, D, (p.nb * p.size + DME_SLICE - 1) / DME_SLICE, p.size, true);
         p.cut_h = dme_cut(p.nb, D, (p.chunk * p.size + DME_SLICE - 1) / DME_SLICE, p.size, true);
         p.part_w = p.cut_w.splits > 1 || N > p.nb;
-        p.part_h = p.cut_h.splits > 1 || p.chunk < p.tiles * p.tile_cols;
+        p.part_h = p.cut_h.splits > 1 || pieces > 1;
         if (p.part_w) p.pw = take((long long)p.cut_w.splits * K * p.ldpart * 4);
         if (p.part_h) p.ph = take((long long)p.cut_h.splits * p.nb * p.ldpart * 4);
     }
@@ -732,15 +935,14 @@ int set_lds(std::atomic<bool>* done, F kernel, int bytes) {
     return DME_OK;
 }
 
-template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD>
+template <class T, int TR, int TC, int WR, int WC, bool BACKWARD>
 int launch_tile(const TileArgs& a, hipStream_t s) {
     typedef DmeTile<T, TR, TC, WR, WC> Tile;
     static_assert(2 * Tile::STAGE >= WC * TR * 8 && 2 * Tile::STAGE >= WR * TC * 4, "the reductions use the tiles' LDS");
     static std::atomic<bool> done[64];
-    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD>, 2 * Tile::STAGE);
+    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, BACKWARD>, 2 * Tile::STAGE);
     if (rc) return rc;
-    const long long blocks = a.tiles_r * a.tiles_c + (TR == 16 && !BACKWARD ? a.nb : 0);
-    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD>), dim3((unsigned)blocks), dim3(Tile::NT), 2 * Tile::STAGE, s, a);
+    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c)), dim3(Tile::NT), 2 * Tile::STAGE, s, a);
     return DME_OK;
 }
 
@@ -755,19 +957,13 @@ int launch_dense(const TileArgs& a, hipStream_t s) {
     return DME_OK;
 }
 
-template <class T, int KIND, bool BACKWARD>
-int launch_side(const TileArgs& a, int side, hipStream_t s) {
-    if (side == 256) return launch_tile<T, 256, 256, 4, 2, KIND, BACKWARD>(a, s);
-    if (side == 128) return launch_tile<T, 128, 128, 2, 2, KIND, BACKWARD>(a, s);
-    return launch_tile<T, 16, 128, 1, 4, KIND, BACKWARD>(a, s);
-}
-
-// The tiles of z (the workgroups that make z at the counts are part of the forward launch where rows are few).
+// The tiles of z.
 template <class T, bool BACKWARD>
 int tiles_of_z(const TileArgs& a, int kind, int side, hipStream_t s) {
     if (kind == DENSE) return side == 16 ? launch_dense<T, 16, BACKWARD>(a, s) : launch_dense<T, 128, BACKWARD>(a, s);
-    if (BACKWARD || side != 16) return launch_side<T, LABELS, BACKWARD>(a, side, s);  // the kind does not matter
-    return kind == CSR ? launch_side<T, CSR, false>(a, 16, s) : launch_side<T, LABELS, false>(a, 16, s);
+    if (side == 256) return launch_tile<T, 256, 256, 4, 2, BACKWARD>(a, s);
+    if (side == 128) return launch_tile<T, 128, 128, 2, 2, BACKWARD>(a, s);
+    return launch_tile<T, 16, 128, 1, 4, BACKWARD>(a, s);
 }
 
 template <class T, int SIDE, bool PK>
@@ -818,12 +1014,13 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
                            (T*)(ws + p.w), p.dpad);
         w = DmeOperand{ws + p.w, p.dpad * size, c.K};
     }
-    u32* largest = (u32*)(ws + p.zeros) + 32;  // the zeros are its first bytes
+    u32* largest = (u32*)(ws + p.largest);
     long long* fixed = gradient && kind != DENSE && c.dbias ? (long long*)(ws + p.fixed) : nullptr;
     for (long long n0 = 0; n0 < c.N; n0 += p.nb) {
         const long long nb = c.N - n0 < p.nb ? c.N - n0 : p.nb;
         // each block of rows has fixed-point sums of its own: their scale is the block's
-        hipLaunchKernelGGL(zero_kernel, dim3(dme_blocks(p.zero_words, 1024, 1024)), dim3(256), 0, s, (u32*)ws, p.zero_words);
+        if (p.zero_words)
+            hipLaunchKernelGGL(zero_kernel, dim3(dme_blocks(p.zero_words, 1024, 1024)), dim3(256), 0, s, (u32*)ws, p.zero_words);
         DmeOperand h{(const char*)c.H + n0 * c.ldh * size, c.ldh * size, nb};
         if (p.pack_h) {
             hipLaunchKernelGGL(dme_pack_kernel<T>, dim3(dme_blocks(nb * p.dpad, 1024, 8192)), dim3(256), 0, s, (const T*)h.at, c.ldh, nb, c.D,
@@ -834,7 +1031,6 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         a.h = h;
         a.w = w;
         a.D = c.D;
-        a.zeros = ws + p.zeros;
         a.tiles_r = (nb + p.tile_rows - 1) / p.tile_rows;
         a.tiles_c = p.tiles;
         a.slices = (int)((c.D * size + DME_SLICE - 1) / DME_SLICE);
@@ -859,11 +1055,20 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         a.part_f = (double*)(ws + p.part_f);
         a.part_t = (double*)(ws + p.part_t);
         a.entry_z = (float*)(ws + p.entry_z);
-        if (kind == CSR && p.side != 16)
-            hipLaunchKernelGGL((entry_kernel<T, CSR>), dim3((unsigned)((nb + 3) / 4)), dim3(256), 0, s, a);
-        else if (kind == LABELS && p.side != 16)
-            hipLaunchKernelGGL((entry_kernel<T, LABELS>), dim3((unsigned)((nb + 3) / 4)), dim3(256), 0, s, a);
-        int rc = tiles_of_z<T, false>(a, kind, p.side, s);
+        int rc = DME_OK;
+        if (p.few) {
+            const unsigned blocks = (unsigned)(p.tiles + nb), bytes = (unsigned)few_lds(c.D * size);
+            if (kind == CSR)
+                hipLaunchKernelGGL((few_kernel<T, CSR>), dim3(blocks), dim3(256), bytes, s, a);
+            else
+                hipLaunchKernelGGL((few_kernel<T, LABELS>), dim3(blocks), dim3(256), bytes, s, a);
+        } else {
+            if (kind == CSR)
+                hipLaunchKernelGGL((entry_kernel<T, CSR>), dim3((unsigned)((nb + 3) / 4)), dim3(256), 0, s, a);
+            else if (kind == LABELS)
+                hipLaunchKernelGGL((entry_kernel<T, LABELS>), dim3((unsigned)((nb + 3) / 4)), dim3(256), 0, s, a);
+            rc = tiles_of_z<T, false>(a, kind, p.side, s);
+        }
         if (rc) return rc;
         RowArgs ra{};
         ra.nb = nb;
@@ -885,7 +1090,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             ra.entry_g = (float*)(ws + p.entry_g);
             ra.largest = largest;
         }
-        if (nb <= 1024)  // too few rows to fill the card with 16 lanes each
+        if (nb <= 128)  // too few rows to fill the card with 16 lanes each
             hipLaunchKernelGGL(row_kernel<256>, dim3((unsigned)nb), dim3(256), 0, s, ra);
         else
             hipLaunchKernelGGL(row_kernel<16>, dim3((unsigned)((nb + 15) / 16)), dim3(256), 0, s, ra);
@@ -906,16 +1111,15 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             if (kind != DENSE) {
                 PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.lse2, ra.coef, a.dz, a.lddz, fixed, largest, p.headroom};
                 if (kind == CSR)
-                    hipLaunchKernelGGL((patch_kernel<T, CSR>), dim3((unsigned)((nb + 15) / 16)), dim3(256), 0, s, pa);
+                    hipLaunchKernelGGL((patch_kernel<T, CSR, 16>), dim3((unsigned)((nb + 63) / 64)), dim3(1024), 0, s, pa);
                 else
-                    hipLaunchKernelGGL((patch_kernel<T, LABELS>), dim3((unsigned)((nb + 15) / 16)), dim3(256), 0, s, pa);
+                    hipLaunchKernelGGL((patch_kernel<T, LABELS, 1>), dim3((unsigned)((nb + 1023) / 1024)), dim3(1024), 0, s, pa);
             }
             const char* dz = (const char*)a.dz;
             ProductArgs m{};  // dW of the piece = dz' H
             m.p = DmeOperand{dz, a.lddz * size, width};
             m.q = DmeOperand{h.at, h.ld, c.D};
             m.k = nb;
-            m.zeros = a.zeros;
             if (p.part_w) {
                 m.part = (float*)(ws + p.pw) + k0 * p.ldpart;
                 m.ldpart = p.ldpart;
@@ -932,7 +1136,6 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             m.p = DmeOperand{dz, a.lddz * size, nb};
             m.q = DmeOperand{a.w.at, a.w.ld, c.D};
             m.k = width;
-            m.zeros = a.zeros;
             if (p.part_h) {
                 m.part = (float*)(ws + p.ph);
                 m.ldpart = p.ldpart;

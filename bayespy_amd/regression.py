@@ -100,15 +100,12 @@ class CountRows:
         return self
 
     def _arg(self):
-        t, a = self._tensors, _lib.CountRowsArg()
-        a.kind = self._kind
+        t = self._tensors
         if self._kind == _LABELS:
-            a.labels = t[0].data_ptr()
-        elif self._kind == _CSR:
-            a.rowptr, a.colidx, a.vals, a.nnz = t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), t[1].numel()
-        else:
-            a.X, a.elem, a.ld = t[0].data_ptr(), self._elem, self._ld
-        return a
+            return _lib.CountRowsArg(_LABELS, 0, t[0].data_ptr())
+        if self._kind == _CSR:
+            return _lib.CountRowsArg(_CSR, 0, None, t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), t[1].numel())
+        return _lib.CountRowsArg(_DENSE, self._elem, None, None, None, None, 0, t[0].data_ptr(), self._ld)
 
 
 def _pitch(t, name):
@@ -147,11 +144,20 @@ def _call(features, weights, rows, bias, likelihood):
     return (features.data_ptr(), _pitch(features, "features"), weights.data_ptr(), _pitch(weights, "weights")), (N, rows.K, D)
 
 
-def _workspace(operands, kind, shape, arg, gradient, device):
-    need = _lib.lib().dme_log_loss_workspace_bytes(*operands, kind, *shape, ctypes.addressof(arg), gradient)
-    if need < 0:
-        _lib.check(_lib.ERR_INVALID_ARG)
-    return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+_NEEDS = {}  # scratch bytes by what they depend on: sizes, pitches, alignment
+
+
+def _workspace(operands, kind, shape, rows, arg, gradient):
+    key = (operands[0] % 16, operands[1], operands[2] % 16, operands[3], kind, shape, rows._kind, arg.nnz, gradient)
+    need = _NEEDS.get(key)
+    if need is None:
+        need = _lib.lib().dme_log_loss_workspace_bytes(*operands, kind, *shape, ctypes.addressof(arg), gradient)
+        if need < 0:
+            _lib.check(_lib.ERR_INVALID_ARG)
+        if len(_NEEDS) >= 1024:
+            _NEEDS.clear()
+        _NEEDS[key] = need
+    return torch.empty(max(need, 256), dtype=torch.uint8, device=rows.device)
 
 
 def log_loss(features, weights, rows, bias=None, likelihood="multinomial"):
@@ -164,7 +170,7 @@ def log_loss(features, weights, rows, bias=None, likelihood="multinomial"):
         if rows.N == 0:
             return loss
         arg, kind = rows._arg(), _TYPES[features.dtype]
-        ws = _workspace(operands, kind, shape, arg, 0, rows.device)
+        ws = _workspace(operands, kind, shape, rows, arg, 0)
         _lib.check(_lib.lib().dme_log_loss(*operands, _ptr(bias), kind, *shape, ctypes.addressof(arg),
                                            _LIKELIHOODS[likelihood], loss.data_ptr(), ws.data_ptr(), ws.numel(), _stream()))
     return loss
@@ -186,7 +192,7 @@ def log_loss_gradient(features, weights, rows, bias=None, likelihood="multinomia
         dweights = torch.empty(weights.shape, dtype=weights.dtype, device=dev)
         dbias = None if bias is None else torch.empty(rows.K, dtype=torch.float32, device=dev)
         arg, kind = rows._arg(), _TYPES[features.dtype]
-        ws = _workspace(operands, kind, shape, arg, 1, dev)
+        ws = _workspace(operands, kind, shape, rows, arg, 1)
         _lib.check(_lib.lib().dme_log_loss_gradient(
             *operands, _ptr(bias), kind, *shape, ctypes.addressof(arg), _LIKELIHOODS[likelihood], _ptr(row_weights),
             loss.data_ptr(), dfeatures.data_ptr(), dweights.data_ptr(), _ptr(dbias), ws.data_ptr(), ws.numel(), _stream()))
