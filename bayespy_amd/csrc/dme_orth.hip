@@ -148,9 +148,9 @@ __device__ __forceinline__ void put_s(const Matrices<W>& x, long long so, long l
 // S = X X' (X' X for a tall X), the tiles on and below the diagonal; what lies above is their mirror image.  Where the tiles are
 // too few for the card, k is split and join_kernel adds the pieces.
 template <class T, class W, int SIDE, bool TALL>
-__global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void square_kernel(StepArgs<T, W> a) {
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArgs<T, W> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2, TALL, TALL> Tile;
+    typedef DmeSquare<W, SIDE, TALL, TALL> Tile;
     const Matrices<W>& x = a.mat;
     const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
     const DmeOperand op{(const char*)(x.Xw[a.from] + blockIdx.y * x.stride_x), x.ldx * (long long)sizeof(W), x.m};
@@ -200,9 +200,9 @@ __global__ __launch_bounds__(256) void join_kernel(Matrices<W> x, int splits) {
 
 // B = b S + c S S.  With S = d + O (diagonal, rest): (S S)[r][c] = (O O)[r][c] + (d_r + d_c) O[r][c], + d_r^2 where r = c.
 template <class T, class W, int SIDE>
-__global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void poly_kernel(StepArgs<T, W> a) {
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<T, W> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2> Tile;
+    typedef DmeSquare<W, SIDE> Tile;
     const Matrices<W>& x = a.mat;
     const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
     const DmeOperand op{(const char*)(x.Sw + so), x.lds * (long long)sizeof(W), x.m};
@@ -241,9 +241,9 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void poly_kernel(StepArgs<
 
 // X <- a X + B X (a X + X B for a tall X)
 template <class T, class W, int SIDE, bool TALL>
-__global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void update_kernel(StepArgs<T, W> a) {
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArgs<T, W> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2, false, !TALL> Tile;
+    typedef DmeSquare<W, SIDE, false, !TALL> Tile;
     const Matrices<W>& x = a.mat;
     const long long xo = blockIdx.y * x.stride_x, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
     constexpr long long size = sizeof(W);
@@ -331,14 +331,14 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
 
 template <class W, int SIDE, class F, class A>
 int launch(F kernel, std::atomic<bool>* done, const A& a, long long tiles, int splits, hipStream_t s) {
-    constexpr int bytes = 2 * DmeTile<W, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2>::STAGE;
+    constexpr int bytes = 2 * DmeSquare<W, SIDE>::STAGE;
     int dev = 0;
     DME_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
         DME_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)splits), dim3(SIDE == 256 ? 512 : 256), bytes, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)splits), dim3(SIDE >= 192 ? 512 : 256), bytes, s, a);
     return DME_OK;
 }
 
@@ -371,14 +371,19 @@ int update(StepArgs<T, W> a, hipStream_t s) {
 template <class T, class W, bool TALL>
 int one_step(const StepArgs<T, W>& k, const StepPlan& p, hipStream_t s) {
     int rc = p.square.side == 256   ? square<T, W, 256, TALL>(k, p.square, s)
+             : p.square.side == 192 ? square<T, W, 192, TALL>(k, p.square, s)
              : p.square.side == 128 ? square<T, W, 128, TALL>(k, p.square, s)
                                     : square<T, W, 64, TALL>(k, p.square, s);
     if (rc) return rc;
     if (p.square.splits > 1)
         hipLaunchKernelGGL(join_kernel<W>, dim3((unsigned)dme_blocks(p.m * p.lds, 256, 2048), (unsigned)k.batch), dim3(256), 0, s, k.mat, p.square.splits);
-    rc = p.poly.side == 256 ? poly<T, W, 256>(k, s) : p.poly.side == 128 ? poly<T, W, 128>(k, s) : poly<T, W, 64>(k, s);
+    rc = p.poly.side == 256   ? poly<T, W, 256>(k, s)
+         : p.poly.side == 192 ? poly<T, W, 192>(k, s)
+         : p.poly.side == 128 ? poly<T, W, 128>(k, s)
+                              : poly<T, W, 64>(k, s);
     if (rc) return rc;
     return p.update.side == 256   ? update<T, W, 256, TALL>(k, s)
+           : p.update.side == 192 ? update<T, W, 192, TALL>(k, s)
            : p.update.side == 128 ? update<T, W, 128, TALL>(k, s)
                                   : update<T, W, 64, TALL>(k, s);
 }

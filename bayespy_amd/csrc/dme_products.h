@@ -53,6 +53,16 @@ struct DmeOperand {
 
 constexpr int DME_SLICE = 128;  // bytes of k in a slice
 
+// 16 bytes a lane from memory to LDS at `to` + lane * 16 (`to` uniform).  In assembly because the compiler waits for every copy it knows
+// of before a transposing LDS read, whatever buffer that reads; who calls this waits with s_waitcnt vmcnt(0) itself.  No register
+// is written.  One wait state belongs between a write of m0 and its use here.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: that is why its change is said
+__device__ __forceinline__ void dme_copy_to_lds(const char* from, u32 to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // What products read in place of what lies outside an operand.  Never written.
 static __device__ __attribute__((aligned(256))) u32 dme_zeros[64];
 
@@ -80,7 +90,7 @@ struct DmeTile {
     template <int TM>
     __device__ __forceinline__ static int spread(int k) {
         if (SIZE == 4) return (k >> 2) & 3;
-        return TM == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;
+        return TM % 128 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;
     }
 
     // source of one lane's 16 bytes of piece `piece` (1 KB) of an operand, and in how many slices from the first on it lies
@@ -146,14 +156,14 @@ struct DmeTile {
                 src[t] += s0 * qstep;
             }
         }
+        const u32 to = (u32)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
         auto copy = [&](int s, int buf) {
 #pragma unroll
             for (int t = 0; t < PER_WAVE; ++t) {
                 const int piece = t * NW + wave;
                 if (COPIES % NW == 0 || piece < COPIES) {
                     const char* from = s < limit[t] ? src[t] : (const char*)dme_zeros;
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                                     (__attribute__((address_space(3))) void*)(lds + buf * STAGE + piece * 1024), 16, 0, 0);
+                    dme_copy_to_lds(from, to + buf * STAGE + piece * 1024);
                     src[t] += piece < TR / 8 ? pstep : qstep;
                 }
             }
@@ -227,19 +237,27 @@ inline int dme_blocks(long long work, long long per, long long most) {
     return (int)(b < 1 ? 1 : b > most ? most : b);
 }
 
-// How a product of R x C outputs over `slices` slices of k is cut: tiles of 256, 128 or 64 a side, and into how many pieces of
-// k.  A workgroup of 256 x 256 has a CU to itself and makes 1230 TFLOP/s in bf16 at 8192^3, 128 x 128 two to a CU 970,
-// 64 x 64 four to a CU about 700 (fp32: 141, 138, 128); small products are bound by how many CUs have a tile at all, and pieces of k
-// cost a pass over their 32-bit sums.
+// The waves of a SIDE x SIDE tile.
+template <class T, int SIDE, bool PK = false, bool QK = false>
+using DmeSquare = DmeTile<T, SIDE, SIDE, (SIDE == 256 ? 4 : 2), (SIDE == 192 ? 4 : 2), PK, QK>;
+
+// How a product of R x C outputs over `slices` slices of k is cut: tiles of 256, 192, 128 or 64 a side, and into how many pieces
+// of k.  Measured in bf16 (fp32) at 4096^3 and 8192^3: 256 a side, one workgroup to a CU, 1150-1290 (141) TFLOP/s; 192, one to a CU, 960-1010;
+// 128, two to a CU, 910-1110 (138); 64, four to a CU, 700 (128).  Small products are bound by how many CUs have a tile at all, and
+// pieces of k cost a pass over their 32-bit sums.
 struct DmeCut {
     int side, splits;
     double us;
 };
 inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool split, double extra_per_tile_us = 0.0, bool symmetric = false) {
+    static const struct {
+        int side, per_cu;
+        double bf16, f32;
+    } kinds[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6}, {128, 2, 980e6, 138e6}, {64, 4, 700e6, 128e6}};
     DmeCut best{0, 1, 0.0};
-    for (int side = 256; side >= 64; side /= 2) {
-        const int per_cu = side == 256 ? 1 : side == 128 ? 2 : 4;
-        const double rate = size == 4 ? (side == 256 ? 141e6 : side == 128 ? 138e6 : 128e6) : (side == 256 ? 1230e6 : side == 128 ? 970e6 : 700e6);
+    for (const auto& kind : kinds) {
+        const int side = kind.side, per_cu = kind.per_cu;
+        const double rate = size == 4 ? kind.f32 : kind.bf16;
         const long long along = (R + side - 1) / side, slots = 256ll * per_cu;
         const long long tiles = symmetric ? along * (along + 1) / 2 : along * ((C + side - 1) / side);
         // one slice of one tile while the CU's other places are taken too

@@ -771,9 +771,9 @@ struct ProductArgs {
 
 // out = P Q' (R x C), Q k-major, in T, or as 32-bit pieces where k is split over workgroups or over launches.
 template <class T, int SIDE, bool PK>
-__global__ __launch_bounds__(SIDE == 256 ? 512 : 256) void product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void product_kernel(ProductArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeTile<T, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2, PK, true> Tile;
+    typedef DmeSquare<T, SIDE, PK, true> Tile;
     long long tr, tc;
     dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
     const int s0 = (int)blockIdx.y * a.per_split;
@@ -870,7 +870,7 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     p.dpad = up(D, 16 / p.size);
     p.nb = N < 1 ? 1 : N < ROW_BLOCK ? N : ROW_BLOCK;
     const long long slices = (D * p.size + DME_SLICE - 1) / DME_SLICE;
-    p.side = p.nb <= 16 ? 16 : rows->kind == DENSE ? 128 : dme_cut(p.nb, K, slices, p.size, false, 4.0).side < 256 ? 128 : 256;
+    p.side = p.nb <= 16 ? 16 : rows->kind == DENSE || dme_cut(p.nb, K, slices, p.size, false, 4.0).side < 192 ? 128 : 256;
     p.tile_rows = p.side;
     p.tile_cols = p.side == 16 ? 128 : p.side;
     const long long tiles = (K + p.tile_cols - 1) / p.tile_cols;
@@ -968,7 +968,7 @@ int tiles_of_z(const TileArgs& a, int kind, int side, hipStream_t s) {
 
 template <class T, int SIDE, bool PK>
 int launch_product(const ProductArgs& a, int splits, hipStream_t s) {
-    typedef DmeTile<T, SIDE, SIDE, (SIDE == 256 ? 4 : 2), 2, PK, true> Tile;
+    typedef DmeSquare<T, SIDE, PK, true> Tile;
     static std::atomic<bool> done[64];
     const int rc = set_lds(done, product_kernel<T, SIDE, PK>, 2 * Tile::STAGE);
     if (rc) return rc;
@@ -983,6 +983,7 @@ int product(ProductArgs a, const DmeCut& cut, hipStream_t s) {
     a.slices = (int)((a.k * (long long)sizeof(T) + DME_SLICE - 1) / DME_SLICE);
     a.per_split = (a.slices + cut.splits - 1) / cut.splits;
     if (cut.side == 256) return launch_product<T, 256, PK>(a, cut.splits, s);
+    if (cut.side == 192) return launch_product<T, 192, PK>(a, cut.splits, s);
     if (cut.side == 128) return launch_product<T, 128, PK>(a, cut.splits, s);
     return launch_product<T, 64, PK>(a, cut.splits, s);
 }
