@@ -222,14 +222,11 @@ __device__ __forceinline__ void dme_tile_of(long long block, long long tiles_r, 
     tc = t / high;
 }
 
-// dst [rows][ldd bytes] = src [rows][cols] (any pitch and alignment), zero beyond cols: a row pitch of whole slices.
+// dst [rows][ldd] = src [rows][cols] (any pitch and alignment), zero beyond cols.  A wave takes a row.
 template <class T>
-__global__ void dme_pack_kernel(const T* src, long long lds_, long long rows, long long cols, T* dst, long long ldd) {
-    const long long n = rows * ldd;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / ldd, c = i - r * ldd;
-        dst[i] = c < cols ? src[r * lds_ + c] : (T)0.f;
-    }
+__global__ __launch_bounds__(256) void dme_pack_kernel(const T* src, long long lds_, long long rows, long long cols, T* dst, long long ldd) {
+    for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (long long)gridDim.x * 4)
+        for (long long c = threadIdx.x & 63; c < ldd; c += 64) dst[r * ldd + c] = c < cols ? src[r * lds_ + c] : (T)0.f;
 }
 
 inline int dme_blocks(long long work, long long per, long long most) {

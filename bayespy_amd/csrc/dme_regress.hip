@@ -18,7 +18,10 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr long long ROW_BLOCK = 16384;             // rows worked on at a time
-constexpr long long PIECE_BYTES = 512ll << 20;     // of d loss / d z held at a time
+// of d loss / d z held at a time: about the memory-side cache, so that the two products read it from there, and pieces still
+// large enough to fill the card (N = 8192, K = 50000, D = 1024: 3508 us with 512 MB, 3400 with 256, 3419 with 128, 3582 with 64;
+// N = 4099, D = 128: 707, 653, 724, 790)
+constexpr long long PIECE_BYTES = 256ll << 20;
 
 enum { LABELS = DME_ROWS_LABELS, CSR = DME_ROWS_CSR, DENSE = DME_ROWS_DENSE };
 
@@ -86,21 +89,63 @@ __device__ __forceinline__ float exp_f32(float z) {
 // (64 + 15)^15 < 2^96.  F = z + log prod_{1 <= n < x} (e^z + n) with one logarithm, G = 1 + e^z sum 1 / (e^z + n) with one
 // reciprocal of the same product: 15 roundings of 2^-24 at most.  Others take the 64-bit functions above.
 __device__ __forceinline__ bool is_small(float z, int x) { return x <= 16 && z <= 4.1f; }
+// N cells of a lane at once, x = 0 where a cell is none of these: the chains of products are independent of each other, and the loop runs
+// as far as the wave's largest count, so that no lane has a branch of its own.
+template <int N>
+__device__ __forceinline__ int most_of(const int (&x)[N]) {
+    int most = x[0];
+#pragma unroll
+    for (int q = 1; q < N; ++q) most = most > x[q] ? most : x[q];
+    return most;
+}
+template <int N>
+__device__ __forceinline__ float small_f(const float (&z)[N], const int (&x)[N]) {  // the sum over the cells
+    float a[N], prod[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        a[q] = exp_f32(z[q]);
+        prod[q] = 1.f;
+    }
+    const int most = most_of(x);
+    for (int n = 1; __any(n < most); ++n)
+#pragma unroll
+        for (int q = 0; q < N; ++q) prod[q] *= n < x[q] ? a[q] + (float)n : 1.f;
+    float f = 0.f;
+#pragma unroll
+    for (int q = 0; q < N; ++q) f += x[q] > 0 ? __builtin_fmaf(__builtin_amdgcn_logf(prod[q]), 0.69314718f, z[q]) : 0.f;
+    return f;
+}
+template <int N>
+__device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], float (&g)[N]) {
+    float a[N], den[N], num[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        a[q] = exp_f32(z[q]);
+        den[q] = 1.f;
+        num[q] = 0.f;
+    }
+    const int most = most_of(x);
+    for (int n = 1; __any(n < most); ++n)
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            const float term = n < x[q] ? a[q] + (float)n : 1.f;
+            num[q] = n < x[q] ? __builtin_fmaf(num[q], term, den[q]) : num[q];
+            den[q] *= term;
+        }
+#pragma unroll
+    for (int q = 0; q < N; ++q) g[q] = x[q] > 0 ? __builtin_fmaf(a[q] * num[q], __builtin_amdgcn_rcpf(den[q]), 1.f) : 0.f;
+}
 __device__ __forceinline__ float small_f(float z, int x) {
-    const float a = exp_f32(z);
-    float prod = 1.f;
-    for (int n = 1; n < x; ++n) prod *= a + (float)n;
-    return __builtin_fmaf(__builtin_amdgcn_logf(prod), 0.69314718f, z);
+    const float zs[1] = {z};
+    const int xs[1] = {x};
+    return small_f(zs, xs);
 }
 __device__ __forceinline__ float small_g(float z, int x) {
-    const float a = exp_f32(z);
-    float den = 1.f, num = 0.f;
-    for (int n = 1; n < x; ++n) {
-        const float term = a + (float)n;
-        num = __builtin_fmaf(num, term, den);
-        den *= term;
-    }
-    return __builtin_fmaf(a * num, __builtin_amdgcn_rcpf(den), 1.f);
+    const float zs[1] = {z};
+    const int xs[1] = {x};
+    float g[1];
+    small_g(zs, xs, g);
+    return g[0];
 }
 
 // Reductions over the 16 lanes that share a row.
@@ -377,28 +422,48 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
         l2[j] = r < a.nb ? a.lse2[r] : INFINITY;
         cf[j] = r < a.nb ? a.coef[r] : 0.f;
     }
-    float* sums = (float*)lds;  // [WR][TC]
+    // In 16 bits a wave's part goes through LDS (its own piece of it), so that whole lines of rows are stored: the lanes of a matrix
+    // instruction hold 8 bytes each of 16 rows, and such stores took 27 us for a round of tiles where the memory needs 7.
+    constexpr bool TURN = sizeof(T) == 2 && TR >= 128;
+    constexpr int PITCH = Tile::WTC * (int)sizeof(T) + 16;
+    char* mine = lds + (tid >> 6) * Tile::WTR * PITCH;
+    f32x4 sum[Tile::NI];
 #pragma unroll
     for (int i = 0; i < Tile::NI; ++i) {
-        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+        sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < Tile::NJ; ++j) {
             f32x4 d;
 #pragma unroll
             for (int q = 0; q < 4; ++q) d[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][q], LOG2E, -l2[j])) * cf[j];
             const long long r = r0 + Tile::row_of(j);
-            if (r < a.nb) {
-                sum += d;
+            if (r < a.nb) sum[i] += d;
+            if constexpr (TURN)
+                dme_store4((T*)(mine + (j * 16 + (tid & 15)) * PITCH) + i * 16 + g * 4, d);
+            else if (r < a.nb)
                 dme_store4((T*)a.dz + r * a.lddz + c0 + Tile::col_of(i), d);
-            }
         }
-        if (a.dbias) {
+    }
+    if constexpr (TURN) {
+        constexpr int PER = Tile::WTC * (int)sizeof(T) / 16;  // lanes that store a row
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-            for (int q = 0; q < 4; ++q) sum[q] = sum16(sum[q]);
-            if ((tid & 15) == 0) *(f32x4*)(sums + wr * TC + Tile::col_of(i)) = sum;
+        for (int q = 0; q < Tile::WTR * PER / 64; ++q) {
+            const int row = q * (64 / PER) + (tid & 63) / PER, at = (tid & 63) % PER;
+            const long long r = r0 + wr * Tile::WTR + row;
+            const u32q v = *(const u32q*)(mine + row * PITCH + at * 16);
+            if (r < a.nb) *(u32q*)((T*)a.dz + r * a.lddz + c0 + wc * Tile::WTC + at * 8) = v;
         }
     }
     if (a.dbias) {
+        float* sums = (float*)lds;  // [WR][TC]
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < Tile::NI; ++i) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum[i][q] = sum16(sum[i][q]);
+            if ((tid & 15) == 0) *(f32x4*)(sums + wr * TC + Tile::col_of(i)) = sum[i];
+        }
         __syncthreads();
         for (int c = tid; c < TC; c += Tile::NT) {
             float v = 0.f;
@@ -488,26 +553,30 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
         if (!BACKWARD) {
             const float m = LOG2E * max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))));
             const float base = m == -INFINITY ? 0.f : m;
-            float s = 0.f, near = 0.f;
-            double f = 0.0, t = 0.0;
+            float s = 0.f;
+            double f = 0.0;
+            long long total = 0;
             bool bad = false;
+            float zs[8];
+            int xs[8];
             each_count(x, a.rows.elem, [&](int q, int v) {
                 const float zq = q < 4 ? u[q & 3] : w[q & 3];
                 s += __builtin_amdgcn_exp2f(__builtin_fmaf(zq, LOG2E, -base));
                 bad |= v < 0;
-                t += (double)v;
-                if (v > 0) {
-                    if (!dirichlet)
-                        f += (double)v * (double)zq;
-                    else if (is_small(zq, v))
-                        near += small_f(zq, v);
-                    else
-                        f += dirichlet_f((double)zq, (double)v);
+                total += v;
+                const bool small = v > 0 && is_small(zq, v);
+                zs[q] = small ? zq : 0.f;
+                xs[q] = small ? v : 0;
+                if (!dirichlet) {
+                    if (v > 0) f += (double)v * (double)zq;
+                } else if (v > 0 && !small) {
+                    f += dirichlet_f((double)zq, (double)v);
                 }
             });
+            if (dirichlet) f += (double)small_f(zs, xs);
             s = sum16(s);
-            f = sum16(f + (double)near);
-            t = sum16(bad ? __builtin_nan("") : t);
+            f = sum16(f);
+            const double t = sum16(bad ? __builtin_nan("") : (double)total);
             if (sub == 0) {
                 a.part[tc * a.nb + r] = f32x2{m, s};
                 a.part_f[tc * a.nb + r] = f;
@@ -516,10 +585,19 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
         } else {
             const float l2 = a.lse2[r], cf = a.coef[r], weight = a.weight[r];
             f32x4 d[2];
+            float zs[8], gs[8];
+            int xs[8];
+            each_count(x, a.rows.elem, [&](int q, int v) {
+                const float zq = q < 4 ? u[q & 3] : w[q & 3];
+                const bool small = v > 0 && is_small(zq, v);
+                zs[q] = small ? zq : 0.f;
+                xs[q] = small ? v : 0;
+            });
+            if (dirichlet) small_g(zs, xs, gs);
             each_count(x, a.rows.elem, [&](int q, int v) {
                 const float zq = q < 4 ? u[q & 3] : w[q & 3];
                 float e = __builtin_amdgcn_exp2f(__builtin_fmaf(zq, LOG2E, -l2)) * cf;
-                if (v > 0) e -= weight * (!dirichlet ? (float)v : is_small(zq, v) ? small_g(zq, v) : (float)dirichlet_g((double)zq, (double)v));
+                if (v > 0) e -= weight * (!dirichlet ? (float)v : xs[q] > 0 ? gs[q] : (float)dirichlet_g((double)zq, (double)v));
                 d[q >> 2][q & 3] = e;
             });
             *(f32x4*)zr = d[0];
@@ -638,10 +716,10 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
             }
             const float z = a.entry_z[e];
             total += (double)x;
-            const bool near = a.likelihood == DME_LIKELIHOOD_DIRICHLET && x > 0 && is_small(z, x);
-            f += near ? (double)small_f(z, x) : f_of(a.likelihood, (double)z, (double)x);
+            const bool small = a.likelihood == DME_LIKELIHOOD_DIRICHLET && x > 0 && is_small(z, x);
+            f += small ? (double)small_f(z, x) : f_of(a.likelihood, (double)z, (double)x);
             if (a.lse2 && real) {
-                const float v = weight * (near ? small_g(z, x) : (float)g_of(a.likelihood, (double)z, (double)x));
+                const float v = weight * (small ? small_g(z, x) : (float)g_of(a.likelihood, (double)z, (double)x));
                 a.entry_g[e] = v;
                 most = fmaxf(most, fabsf(v));
             }
@@ -712,20 +790,20 @@ __device__ __forceinline__ int fixed_shift(const u32* largest, int headroom) {
 // word frequencies send thousands of entries to one address, where memory takes one at a time (4099 rows, 144 000 entries: 88 us with
 // an atomic each).  LANES lanes a row.
 template <class T, int KIND, int LANES>
-__global__ __launch_bounds__(1024) void patch_kernel(PatchArgs a) {
+__global__ __launch_bounds__(512) void patch_kernel(PatchArgs a) {
     constexpr int SLOTS = 2048;
     __shared__ int keys[SLOTS];
     __shared__ u64 sums[SLOTS];
     const bool add = a.fixed != nullptr;
     if (add) {
-        for (int i = threadIdx.x; i < SLOTS; i += 1024) {
+        for (int i = threadIdx.x; i < SLOTS; i += 512) {
             keys[i] = -1;
             sums[i] = 0;
         }
         __syncthreads();
     }
     const int sub = threadIdx.x % LANES;
-    const long long r = (long long)blockIdx.x * (1024 / LANES) + threadIdx.x / LANES;
+    const long long r = (long long)blockIdx.x * (512 / LANES) + threadIdx.x / LANES;
     if (r < a.nb) {
         const float l2 = a.lse2[r], cf = a.coef[r];
         const int shift = add ? fixed_shift(a.largest, a.headroom) : 0;
@@ -752,7 +830,7 @@ __global__ __launch_bounds__(1024) void patch_kernel(PatchArgs a) {
     }
     if (!add) return;
     __syncthreads();
-    for (int i = threadIdx.x; i < SLOTS; i += 1024)
+    for (int i = threadIdx.x; i < SLOTS; i += 512)
         if (keys[i] >= 0 && sums[i] != 0) atomicAdd((u64*)(a.fixed + keys[i]), sums[i]);
 }
 
@@ -805,27 +883,59 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void product_kernel(Produc
     }
 }
 
-// out [R][C] = the sum of `splits` pieces, in their order.
+// out [R][C] = the sum of `splits` pieces, in their order.  `lines` lines of `length` values, the pieces' `ldpart` apart (a
+// multiple of four); one line where there are no gaps.  A wave takes 256 values of a line.
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const float* part, long long ldpart, long long split_stride, int splits, long long R, long long C,
-                                                   T* out) {
-    const long long n = R * C;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long r = i / C, c = i - r * C;
-        const float* at = part + r * ldpart + c;
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += at[s * split_stride];
-        out[i] = (T)v;
+__global__ __launch_bounds__(256) void join_kernel(const float* part, long long ldpart, long long split_stride, int splits, long long lines,
+                                                   long long length, T* out, int vector) {
+    const int lane = threadIdx.x & 63;
+    const long long across = (length + 255) / 256, all = lines * across, waves = (long long)gridDim.x * 4;
+    for (long long t = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); t < all; t += waves) {
+        const long long line = across == 1 ? t : t / across, c = (across == 1 ? 0 : t - line * across) * 256 + lane * 4;
+        if (c >= length) continue;
+        const float* at = part + line * ldpart + c;
+        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+        int s = 0;
+        for (; s + 4 <= splits; s += 4) {
+            f32x4 p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = *(const f32x4*)(at + (s + u) * split_stride);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v += p[u];
+        }
+        for (; s < splits; ++s) v += *(const f32x4*)(at + s * split_stride);
+        T* o = out + line * length + c;
+        if (vector) {
+            dme_store4(o, v);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < length) o[q] = (T)v[q];
+        }
     }
 }
 
-// dbias [K] (+)= the row tiles' sums, in their order, minus the counts' (fixed, null for dense rows).
+// dbias [K] (+)= the row tiles' sums, minus the counts' (fixed, null for dense rows).  64 columns a workgroup, a quarter of the
+// tiles a wave, the quarters added in their order.
 __global__ __launch_bounds__(256) void bias_kernel(const float* part, long long tiles, long long K, const long long* fixed, const u32* largest,
                                                    int headroom, int add, float* dbias) {
-    const long long k = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (k >= K) return;
-    double v = add ? (double)dbias[k] : 0.0;
-    for (long long t = 0; t < tiles; ++t) v += (double)part[t * K + k];
+    __shared__ double sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long k = (long long)blockIdx.x * 64 + lane;
+    double v = 0.0;
+    if (k < K)
+        for (long long t = wave; t < tiles; t += 16) {
+            float p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = t + u * 4 < tiles ? part[(t + u * 4) * K + k] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v += (double)p[u];
+        }
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave != 0 || k >= K) return;
+    v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    if (add) v += (double)dbias[k];
     if (fixed) v -= ldexp((double)fixed[k], -fixed_shift(largest, headroom));
     dbias[k] = (float)v;
 }
@@ -940,9 +1050,11 @@ int launch_tile(const TileArgs& a, hipStream_t s) {
     typedef DmeTile<T, TR, TC, WR, WC> Tile;
     static_assert(2 * Tile::STAGE >= WC * TR * 8 && 2 * Tile::STAGE >= WR * TC * 4, "the reductions use the tiles' LDS");
     static std::atomic<bool> done[64];
-    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, BACKWARD>, 2 * Tile::STAGE);
+    constexpr int turned = BACKWARD && sizeof(T) == 2 && TR >= 128 ? TR * WC * (Tile::WTC * (int)sizeof(T) + 16) : 0;
+    constexpr int bytes = turned > 2 * Tile::STAGE ? turned : 2 * Tile::STAGE;
+    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, BACKWARD>, bytes);
     if (rc) return rc;
-    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c)), dim3(Tile::NT), 2 * Tile::STAGE, s, a);
+    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c)), dim3(Tile::NT), bytes, s, a);
     return DME_OK;
 }
 
@@ -988,6 +1100,14 @@ int product(ProductArgs a, const DmeCut& cut, hipStream_t s) {
     return launch_product<T, 64, PK>(a, cut.splits, s);
 }
 
+template <class T>
+void join(const float* part, long long ldpart, long long split_stride, int splits, long long R, long long C, T* out, hipStream_t s) {
+    const bool whole = ldpart == C;
+    const long long lines = whole ? 1 : R, length = whole ? R * C : C;
+    hipLaunchKernelGGL(join_kernel<T>, dim3(dme_blocks(lines * ((length + 255) / 256), 4, 8192)), dim3(256), 0, s, part, ldpart, split_stride, splits, lines,
+                       length, out, (int)(C % 4 == 0));
+}
+
 struct Call {
     const void* H;
     long long ldh;
@@ -1011,7 +1131,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
     char* ws = c.ws;
     DmeOperand w{(const char*)c.W, c.ldw * size, c.K};
     if (p.pack_w) {
-        hipLaunchKernelGGL(dme_pack_kernel<T>, dim3(dme_blocks(c.K * p.dpad, 1024, 8192)), dim3(256), 0, s, (const T*)c.W, c.ldw, c.K, c.D,
+        hipLaunchKernelGGL(dme_pack_kernel<T>, dim3(dme_blocks(c.K, 4, 16384)), dim3(256), 0, s, (const T*)c.W, c.ldw, c.K, c.D,
                            (T*)(ws + p.w), p.dpad);
         w = DmeOperand{ws + p.w, p.dpad * size, c.K};
     }
@@ -1024,7 +1144,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             hipLaunchKernelGGL(zero_kernel, dim3(dme_blocks(p.zero_words, 1024, 1024)), dim3(256), 0, s, (u32*)ws, p.zero_words);
         DmeOperand h{(const char*)c.H + n0 * c.ldh * size, c.ldh * size, nb};
         if (p.pack_h) {
-            hipLaunchKernelGGL(dme_pack_kernel<T>, dim3(dme_blocks(nb * p.dpad, 1024, 8192)), dim3(256), 0, s, (const T*)h.at, c.ldh, nb, c.D,
+            hipLaunchKernelGGL(dme_pack_kernel<T>, dim3(dme_blocks(nb, 4, 16384)), dim3(256), 0, s, (const T*)h.at, c.ldh, nb, c.D,
                                (T*)(ws + p.h), p.dpad);
             h = DmeOperand{ws + p.h, p.dpad * size, nb};
         }
@@ -1112,9 +1232,9 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             if (kind != DENSE) {
                 PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.lse2, ra.coef, a.dz, a.lddz, fixed, largest, p.headroom};
                 if (kind == CSR)
-                    hipLaunchKernelGGL((patch_kernel<T, CSR, 16>), dim3((unsigned)((nb + 63) / 64)), dim3(1024), 0, s, pa);
+                    hipLaunchKernelGGL((patch_kernel<T, CSR, 16>), dim3((unsigned)((nb + 31) / 32)), dim3(512), 0, s, pa);
                 else
-                    hipLaunchKernelGGL((patch_kernel<T, LABELS, 1>), dim3((unsigned)((nb + 1023) / 1024)), dim3(1024), 0, s, pa);
+                    hipLaunchKernelGGL((patch_kernel<T, LABELS, 1>), dim3((unsigned)((nb + 511) / 512)), dim3(512), 0, s, pa);
             }
             const char* dz = (const char*)a.dz;
             ProductArgs m{};  // dW of the piece = dz' H
@@ -1151,15 +1271,13 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             if (rc) return rc;
         }
         if (p.part_h)
-            hipLaunchKernelGGL(join_kernel<T>, dim3(dme_blocks(nb * c.D, 1024, 8192)), dim3(256), 0, s, (const float*)(ws + p.ph), p.ldpart,
-                               p.nb * p.ldpart, p.cut_h.splits, nb, c.D, (T*)c.dH + n0 * c.D);
+            join<T>((const float*)(ws + p.ph), p.ldpart, p.nb * p.ldpart, p.cut_h.splits, nb, c.D, (T*)c.dH + n0 * c.D, s);
         if (c.dbias)
-            hipLaunchKernelGGL(bias_kernel, dim3((unsigned)((c.K + 255) / 256)), dim3(256), 0, s, (const float*)a.dbias, a.tiles_r, c.K,
+            hipLaunchKernelGGL(bias_kernel, dim3((unsigned)((c.K + 63) / 64)), dim3(256), 0, s, (const float*)a.dbias, a.tiles_r, c.K,
                                fixed, largest, p.headroom, (int)(n0 > 0), c.dbias);
     }
     if (gradient && p.part_w)
-        hipLaunchKernelGGL(join_kernel<T>, dim3(dme_blocks(c.K * c.D, 1024, 8192)), dim3(256), 0, s, (const float*)(ws + p.pw), p.ldpart,
-                           c.K * p.ldpart, p.cut_w.splits, c.K, c.D, (T*)c.dW);
+        join<T>((const float*)(ws + p.pw), p.ldpart, c.K * p.ldpart, p.cut_w.splits, c.K, c.D, (T*)c.dW, s);
     DME_HIP_CHECK(hipGetLastError());
     return DME_OK;
 }
@@ -1219,8 +1337,8 @@ extern "C" int dme_log_loss_gradient(const void* H, int64_t ldh, const void* W, 
     const long long size = type == DME_TYPE_BF16 ? 2 : 4;
     DME_REQUIRE((uintptr_t)dW % 16 == 0 && (uintptr_t)dH % 16 == 0, "gradients must be aligned to 16 bytes");
     if (N == 0) {  // a sum over no rows
-        hipLaunchKernelGGL(dme_pack_kernel<char>, dim3(dme_blocks(K * D * size, 4096, 8192)), dim3(256), 0, (hipStream_t)stream, (const char*)nullptr, 0,
-                           K * D * size, 0, (char*)dW, 1);
+        hipLaunchKernelGGL(dme_pack_kernel<unsigned short>, dim3(dme_blocks(K, 4, 16384)), dim3(256), 0, (hipStream_t)stream, (const unsigned short*)nullptr, 0,
+                           K, 0, (unsigned short*)dW, D * size / 2);
         if (dbias) hipLaunchKernelGGL(zero_kernel, dim3(dme_blocks(K, 1024, 4096)), dim3(256), 0, (hipStream_t)stream, (u32*)dbias, K);
         DME_HIP_CHECK(hipGetLastError());
         return DME_OK;
