@@ -4,12 +4,17 @@
 // losses; the quintic iteration is Bjorck and Bowie's, 1971).
 //
 // S is the square of the smaller side: X X' for a wide X, X' X for a tall one (then X <- a X + X (b S + c S S)); X keeps G's
-// orientation.  Operands of the products are fp16 for bf16 matrices, scaled by powers of two, and X itself stays in 32 bits
-// beside them: what fp16 drops of X then only passes through b S + c S S, which is small where X's singular values are, instead
-// of being amplified by a at every step.  The diagonals of S and of b S + c S S are kept out of the operands and applied in 32 bits:
-// where singular values are alike the diagonal is nearly one number, and its rounding would not average out (50000 x 256 of
-// near-flat spectrum, five steps: 3.7e-3 of the result with the diagonal in fp16, below 1e-3 without).  For fp32 matrices everything
-// is fp32.
+// orientation.
+//
+// The products run on the fp16 matrix instructions, sums in 32 bits.  A value v, scaled by a power of two, is kept as fp16 pairs
+// hi + lo of 22 bits together; |X| = 1 at the start and singular values stay below 3 (checked), so nothing leaves fp16's range.
+//   fp32 matrices  P Q = Ph Qh + Ph Ql + Pl Qh: what is dropped is 2^-22 of a product, less than 32-bit sums of as many terms round
+//                  off (4.4e-7 of the result with fp32 instructions; see the table of errors), at 2.5 times their rate
+//   bf16 matrices  P Q = Ph Qh; X itself keeps its lo part, so that what fp16 drops of X only passes through b S + c S S, which is
+//                  small where X's singular values are, instead of being amplified by a at every step.
+// The diagonals of S and of b S + c S S are kept out of the operands and applied in 32 bits: where singular values are alike the diagonal is
+// nearly one number, and its rounding would not average out (50000 x 256 of near-flat spectrum, five steps: 3.7e-3 of the result with
+// the diagonal in fp16, below 1e-3 without).
 #include <math.h>
 
 #include <atomic>
@@ -20,14 +25,9 @@ namespace {
 
 // Powers of two that keep the operands inside fp16: X and S hold values up to 3 and 9, b S + c S S up to 60 (checked on
 // the host), and what falls below 2^-14 / scale is small beside their norms.
-template <class W>
-struct Scale {
-    static constexpr float X = 1.f, S = 1.f, B = 1.f;
-};
-template <>
-struct Scale<_Float16> {
-    static constexpr float X = 4096.f, S = 4096.f, B = 1024.f;
-};
+constexpr float SCALE_X = 4096.f, SCALE_S = 4096.f, SCALE_B = 1024.f;
+
+typedef _Float16 half;
 
 constexpr int NORM_BLOCKS = 256;
 
@@ -64,67 +64,96 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, lon
     if (threadIdx.x == 0) part[blockIdx.y * NORM_BLOCKS + blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
-template <class W>
+// hi + lo of four values
+__device__ __forceinline__ void split4(half* hi, half* lo, f32x4 v) {
+    f16x4 h, l;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        h[q] = (half)v[q];
+        l[q] = (half)(v[q] - (float)h[q]);
+    }
+    *(f16x4*)hi = h;
+    *(f16x4*)lo = l;
+}
+__device__ __forceinline__ void split1(half* hi, half* lo, float v) {
+    const half h = (half)v;
+    *hi = h;
+    if (lo) *lo = (half)(v - (float)h);
+}
+
 struct Matrices {
-    float* X;      // [rows][ldx]; not used for fp32 matrices
-    W* Xw[2];      // [rows][ldx]: the operand, read and written in turn
-    float* S;      // [m][lds]
-    W* Sw;         // [m][lds]: S without its diagonal
-    W* Bw;         // [m][lds]: b S + c S S without its diagonal
-    float* Sd;     // [m]: the diagonals
+    half* X[2][2];  // [which of two][hi, lo]: [rows][ldx], read and written in turn
+    float* S;       // [m][lds]
+    half* Sw[2];    // [hi, lo]: S without its diagonal; lo for fp32 matrices
+    half* Bw[2];    // b S + c S S without its diagonal
+    float* Sd;      // [m]: the diagonals
     float* Bd;
-    float* part;   // [split][m][lds]: pieces of S
+    float* part;    // [split][m][lds]: pieces of S
     long long stride_x, stride_s, stride_part;  // from matrix to matrix
     long long rows, cols, ldx, m, lds;
 };
 
 // X = G / |G|, zero in the padding of its pitch.
-template <class T, class W>
-__global__ __launch_bounds__(256) void begin_kernel(const T* G, long long sb, long long rs, long long cs, const double* part, Matrices<W> a) {
+template <class T>
+__global__ __launch_bounds__(256) void begin_kernel(const T* G, long long sb, long long rs, long long cs, const double* part, Matrices a) {
     __shared__ float tile[64][65];
     __shared__ double sums[4];
     double s = dme_wave_sum_f64(part[blockIdx.y * NORM_BLOCKS + threadIdx.x]);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
     __syncthreads();
     s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    const double scale = s > 0.0 || s != s ? 1.0 / sqrt(s) : 0.0;
+    const double scale = s > 0.0 || s != s ? (double)SCALE_X / sqrt(s) : 0.0;
     const T* g = G + blockIdx.y * sb;
     const long long xo = blockIdx.y * a.stride_x;
-    const int lo = threadIdx.x & 63, hi = threadIdx.x >> 6;
     const bool along = cs == 1 || a.cols == 1;  // neighbouring values are neighbours in G too; otherwise tiles are turned in LDS
     const long long tiles_c = (a.ldx + 63) / 64, tiles_r = (a.rows + 63) / 64;
+    const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * 4;  // four neighbouring values a thread
     for (long long t = blockIdx.x; t < tiles_c * tiles_r; t += gridDim.x) {
         const long long r0 = t / tiles_c * 64, c0 = t % tiles_c * 64;
         if (!along) {
             __syncthreads();
-            for (int q = hi; q < 64; q += 4) {
-                const long long r = r0 + lo, c = c0 + q;
-                if (r < a.rows && c < a.cols) tile[lo][q] = (float)g[r * rs + c * cs];
+            for (int q = threadIdx.x >> 6; q < 64; q += 4) {
+                const long long r = r0 + (threadIdx.x & 63), c = c0 + q;
+                if (r < a.rows && c < a.cols) tile[threadIdx.x & 63][q] = (float)g[r * rs + c * cs];
             }
             __syncthreads();
         }
-        for (int q = hi; q < 64; q += 4) {
-            const long long r = r0 + q, c = c0 + lo;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const long long r = r0 + row + q * 16, c = c0 + col;
             if (r >= a.rows || c >= a.ldx) continue;
-            float v = 0.f;
-            if (c < a.cols) v = (float)((double)(along ? (float)g[r * rs + c * cs] : tile[q][lo]) * scale);
-            if (sizeof(W) == 2) a.X[xo + r * a.ldx + c] = v;
-            a.Xw[0][xo + r * a.ldx + c] = (W)(v * Scale<W>::X);
+            f32x4 v;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                v[u] = c + u < a.cols ? (float)((double)(along ? (float)g[r * rs + (c + u) * cs] : tile[row + q * 16][col + u]) * scale) : 0.f;
+            split4(a.X[0][0] + xo + r * a.ldx + c, a.X[0][1] + xo + r * a.ldx + c, v);
         }
     }
 }
 
-template <class T, class W>
+template <class T>
 struct StepArgs {
-    Matrices<W> mat;
+    Matrices mat;
     float a, b, c;
-    int from;  // which of Xw is read
+    int from;  // which of X is read
     T* out;    // the last step's result, or null
     long long out_batch;
     int vector;  // its rows are aligned to four values
     long long tiles_r, tiles_c, batch;
     int slices, per_split;
 };
+
+// acc = P Q' of operands in one part or two
+template <int PARTS, class Tile>
+__device__ __forceinline__ void multiply(Tile& t, half* const* P, const DmeOperand& p, half* const* Q, const DmeOperand& q, long long po, long long qo,
+                                         long long K, char* lds, long long r0, long long c0, int s0, int s1) {
+    t.clear();
+#pragma unroll
+    for (int i = 0; i < (PARTS == 2 ? 3 : 1); ++i) {
+        const DmeOperand x{(const char*)(P[i == 2] + po), p.ld, p.rows}, y{(const char*)(Q[i == 1] + qo), q.ld, q.rows};
+        t.run(x, y, K, lds, r0, c0, s0, s1);
+    }
+}
 
 // Tile `t` of the lower triangle of a square of tiles, numbered along its rows; XCDs take eighths of them (dme_tile_of).
 __device__ __forceinline__ void triangle_tile(long long block, long long n, long long& tr, long long& tc) {
@@ -138,30 +167,31 @@ __device__ __forceinline__ void triangle_tile(long long block, long long n, long
 }
 
 // what becomes of S[r][c] = v
-template <class W>
-__device__ __forceinline__ void put_s(const Matrices<W>& x, long long so, long long mo, long long r, long long c, float v) {
-    x.S[so + r * x.lds + c] = v;
-    x.Sw[so + r * x.lds + c] = r == c ? (W)0.f : (W)(v * Scale<W>::S);
+template <int PARTS>
+__device__ __forceinline__ void put_s(const Matrices& x, long long so, long long mo, long long r, long long c, float v) {
+    const long long at = so + r * x.lds + c;
+    x.S[at] = v;
+    split1(x.Sw[0] + at, PARTS == 2 ? x.Sw[1] + at : nullptr, r == c ? 0.f : v * SCALE_S);
     if (r == c) x.Sd[mo + r] = v;
 }
 
 // S = X X' (X' X for a tall X), the tiles on and below the diagonal; what lies above is their mirror image.  Where the tiles are
 // too few for the card, k is split and join_kernel adds the pieces.
-template <class T, class W, int SIDE, bool TALL>
-__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArgs<T, W> a) {
+template <class T, int PARTS, int SIDE, bool TALL>
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeSquare<W, SIDE, TALL, TALL> Tile;
-    const Matrices<W>& x = a.mat;
-    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
-    const DmeOperand op{(const char*)(x.Xw[a.from] + blockIdx.y * x.stride_x), x.ldx * (long long)sizeof(W), x.m};
+    typedef DmeSquare<half, SIDE, TALL, TALL> Tile;
+    const Matrices& x = a.mat;
+    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m, xo = blockIdx.y * x.stride_x;
+    const DmeOperand op{nullptr, x.ldx * 2, x.m};
     long long tr, tc;
     triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
     const int s0 = (int)blockIdx.z * a.per_split;
     int s1 = s0 + a.per_split;
     s1 = s1 < a.slices ? s1 : a.slices;
     Tile t;
-    t.run(op, op, TALL ? x.rows : x.cols, lds, tr * SIDE, tc * SIDE, s0, s1);
-    constexpr float UNIT = 1.f / (Scale<W>::X * Scale<W>::X);
+    multiply<PARTS>(t, x.X[a.from], op, x.X[a.from], op, xo, xo, TALL ? x.rows : x.cols, lds, tr * SIDE, tc * SIDE, s0, s1);
+    constexpr float UNIT = 1.f / (SCALE_X * SCALE_X);
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
         const long long r = tr * SIDE + Tile::row_of(j);
@@ -177,40 +207,56 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArg
 #pragma unroll
             for (int q = 0; q < 4; ++q) {  // the pitch's padding is zero, below the diagonal and above it
                 const bool in = r < x.m && c + q < x.m;
-                if (tr != tc && c + q < x.m) put_s(x, so, mo, c + q, r, in ? v[q] : 0.f);
-                if (r < x.m) put_s(x, so, mo, r, c + q, in ? v[q] : 0.f);
+                if (tr != tc && c + q < x.m) put_s<PARTS>(x, so, mo, c + q, r, in ? v[q] : 0.f);
+                if (r < x.m) put_s<PARTS>(x, so, mo, r, c + q, in ? v[q] : 0.f);
             }
         }
     }
 }
 
-template <class W>
-__global__ __launch_bounds__(256) void join_kernel(Matrices<W> x, int splits) {
-    const long long n = x.m * x.lds, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long r = i / x.lds, c = i - r * x.lds;
-        float v = 0.f;
-        if (c < x.m) {
-            const float* at = x.part + blockIdx.y * x.stride_part + (r > c ? r * x.lds + c : c * x.lds + r);
-            for (int s = 0; s < splits; ++s) v += at[s * x.stride_s];
+// 16 x 16 values of S on and below the diagonal, and their mirror image.
+template <int PARTS>
+__global__ __launch_bounds__(256) void join_kernel(Matrices x, int splits) {
+    __shared__ float turn[16][17];
+    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    long long tr, tc;
+    triangle_tile(blockIdx.x, (x.lds + 15) / 16, tr, tc);
+    const int lo = threadIdx.x & 15, hi = threadIdx.x >> 4;
+    const long long r = tr * 16 + hi, c = tc * 16 + lo;
+    float v = 0.f;
+    if (r < x.m && c < x.m) {
+        const float* at = x.part + blockIdx.y * x.stride_part + (r > c ? r * x.lds + c : c * x.lds + r);  // above the diagonal: the same sum
+        int s = 0;
+        for (; s + 8 <= splits; s += 8) {
+            float p[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) p[u] = at[(s + u) * x.stride_s];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v += p[u];
         }
-        put_s(x, so, mo, r, c, v);
+        for (; s < splits; ++s) v += at[s * x.stride_s];
     }
+    turn[hi][lo] = v;
+    if (r < x.m && c < x.lds) put_s<PARTS>(x, so, mo, r, c, v);
+    if (tr == tc) return;  // uniform
+    __syncthreads();
+    const long long rr = tc * 16 + hi, cc = tr * 16 + lo;
+    if (rr < x.m && cc < x.lds) put_s<PARTS>(x, so, mo, rr, cc, turn[lo][hi]);
 }
 
 // B = b S + c S S.  With S = d + O (diagonal, rest): (S S)[r][c] = (O O)[r][c] + (d_r + d_c) O[r][c], + d_r^2 where r = c.
-template <class T, class W, int SIDE>
-__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<T, W> a) {
+template <class T, int PARTS, int SIDE>
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeSquare<W, SIDE> Tile;
-    const Matrices<W>& x = a.mat;
+    typedef DmeSquare<half, SIDE> Tile;
+    const Matrices& x = a.mat;
     const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
-    const DmeOperand op{(const char*)(x.Sw + so), x.lds * (long long)sizeof(W), x.m};
+    const DmeOperand op{nullptr, x.lds * 2, x.m};
     long long tr, tc;
     triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
     Tile t;
-    t.run(op, op, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
-    constexpr float UNIT = 1.f / (Scale<W>::S * Scale<W>::S);
+    multiply<PARTS>(t, x.Sw, op, x.Sw, op, so, so, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+    constexpr float UNIT = 1.f / (SCALE_S * SCALE_S);
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
         const long long r = tr * SIDE + Tile::row_of(j);
@@ -231,30 +277,39 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
                 const float ss = t.acc[i][j][q] * UNIT + (on ? dr * dr : (dr + dc) * s[q]);
                 const float poly = __builtin_fmaf(a.c, ss, a.b * s[q]);
                 if (on) x.Bd[mo + r] = poly;
-                v[q] = in && !on ? poly * Scale<W>::B : 0.f;
-                if (tr != tc && c + q < x.m) x.Bw[so + (c + q) * x.lds + r] = (W)v[q];
+                v[q] = in && !on ? poly * SCALE_B : 0.f;
+                if (tr != tc && c + q < x.m) {
+                    const long long at = so + (c + q) * x.lds + r;
+                    split1(x.Bw[0] + at, PARTS == 2 ? x.Bw[1] + at : nullptr, v[q]);
+                }
             }
-            if (real) dme_store4(x.Bw + so + r * x.lds + c, v);
+            if (!real) continue;
+            if (PARTS == 2)
+                split4(x.Bw[0] + so + r * x.lds + c, x.Bw[1] + so + r * x.lds + c, v);
+            else
+                dme_store4(x.Bw[0] + so + r * x.lds + c, v);
         }
     }
 }
 
 // X <- a X + B X (a X + X B for a tall X)
-template <class T, class W, int SIDE, bool TALL>
-__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArgs<T, W> a) {
+template <class T, int PARTS, int SIDE, bool TALL>
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeSquare<W, SIDE, false, !TALL> Tile;
-    const Matrices<W>& x = a.mat;
+    typedef DmeSquare<half, SIDE, false, !TALL> Tile;
+    const Matrices& x = a.mat;
     const long long xo = blockIdx.y * x.stride_x, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
-    constexpr long long size = sizeof(W);
-    const DmeOperand b{(const char*)(x.Bw + so), x.lds * size, x.m};
-    const DmeOperand y{(const char*)(x.Xw[a.from] + xo), x.ldx * size, TALL ? x.rows : x.cols};
+    const DmeOperand b{nullptr, x.lds * 2, x.m}, y{nullptr, x.ldx * 2, TALL ? x.rows : x.cols};
+    half* const* X = x.X[a.from];
     long long tr, tc;
     dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
     Tile t;
-    t.run(TALL ? y : b, TALL ? b : y, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
-    constexpr float UNIT = 1.f / (Scale<W>::B * Scale<W>::X);
-    W* to = x.Xw[a.from ^ 1] + xo;
+    if (TALL)
+        multiply<PARTS>(t, X, y, x.Bw, b, xo, so, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+    else
+        multiply<PARTS>(t, x.Bw, b, X, y, so, xo, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+    constexpr float UNIT = 1.f / SCALE_B;  // X's scale stays
+    half *hi = x.X[a.from ^ 1][0] + xo, *lo = x.X[a.from ^ 1][1] + xo;
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
         const long long r = tr * SIDE + Tile::row_of(j);
@@ -265,18 +320,18 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArg
             const long long c = tc * SIDE + Tile::col_of(i);
             if (c >= x.ldx) continue;
             const long long at = r * x.ldx + c;
-            const f32x4 old = size == 2 ? *(const f32x4*)(x.X + xo + at) : *(const f32x4*)((const float*)(x.Xw[a.from] + xo) + at);
+            const f16x4 h = *(const f16x4*)(X[0] + xo + at), l = *(const f16x4*)(X[1] + xo + at);
             f32x4 v;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const bool in = c + q < x.cols;
                 const float d = TALL ? (in ? a.a + x.Bd[mo + c + q] : 0.f) : dr;
-                v[q] = in ? __builtin_fmaf(d, old[q], t.acc[i][j][q] * UNIT) : 0.f;
+                v[q] = in ? __builtin_fmaf(d, (float)h[q], __builtin_fmaf(d, (float)l[q], t.acc[i][j][q] * UNIT)) : 0.f;
             }
             if (!a.out) {
-                if (size == 2) *(f32x4*)(x.X + xo + at) = v;
-                dme_store4(to + at, v * Scale<W>::X);
+                split4(hi + at, lo + at, v);
             } else if (c < x.cols) {  // the result has no padding
+                v *= 1.f / SCALE_X;
                 T* o = a.out + blockIdx.y * a.out_batch + r * x.cols + c;
                 if (a.vector) {
                     dme_store4(o, v);
@@ -295,21 +350,21 @@ inline long long up(long long v, long long to) { return (v + to - 1) / to * to; 
 struct StepPlan {
     long long m, n, ldx, lds;
     DmeCut square, poly, update;
-    long long norm, X, Xw[2], S, Sw, Bw, Sd, Bd, part, bytes;
+    long long norm, X[2][2], S, Sw[2], Bw[2], Sd, Bd, part, bytes;
 };
 
 StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     StepPlan p{};
-    const bool half = type == DME_TYPE_BF16;
-    const long long size = half ? 2 : 4, per = 16 / size;
+    const int parts = type == DME_TYPE_BF16 ? 1 : 2;
     p.m = rows < cols ? rows : cols;
     p.n = rows < cols ? cols : rows;
-    p.ldx = up(cols, per);
-    p.lds = up(p.m, per);
-    const auto slices = [&](long long k) { return (k * size + DME_SLICE - 1) / DME_SLICE; };
-    p.square = dme_cut(p.m, p.m, slices(p.n), (int)size, true, 0.0, true);
-    p.poly = dme_cut(p.m, p.m, slices(p.m), (int)size, false, 0.0, true);
-    p.update = dme_cut(rows, cols, slices(p.m), (int)size, false);
+    p.ldx = up(cols, 8);
+    p.lds = up(p.m, 8);
+    // three products of halves cost three times the slices
+    const auto slices = [&](long long k) { return (k * 2 + DME_SLICE - 1) / DME_SLICE * (parts == 2 ? 3 : 1); };
+    p.square = dme_cut(p.m, p.m, slices(p.n), 2, true, 0.0, true);
+    p.poly = dme_cut(p.m, p.m, slices(p.m), 2, false, 0.0, true);
+    p.update = dme_cut(rows, cols, slices(p.m), 2, false);
     long long at = 0;
     const auto take = [&](long long bytes) {
         const long long here = at;
@@ -317,11 +372,12 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
         return here;
     };
     p.norm = take(batch * NORM_BLOCKS * 8);
-    if (half) p.X = take(batch * rows * p.ldx * 4);
-    for (int i = 0; i < 2; ++i) p.Xw[i] = take(batch * rows * p.ldx * size);
+    for (int i = 0; i < 4; ++i) p.X[i / 2][i % 2] = take(batch * rows * p.ldx * 2);
     p.S = take(batch * p.m * p.lds * 4);
-    p.Sw = take(batch * p.m * p.lds * size);
-    p.Bw = take(batch * p.m * p.lds * size);
+    for (int i = 0; i < parts; ++i) {
+        p.Sw[i] = take(batch * p.m * p.lds * 2);
+        p.Bw[i] = take(batch * p.m * p.lds * 2);
+    }
     p.Sd = take(batch * p.m * 4);
     p.Bd = take(batch * p.m * 4);
     if (p.square.splits > 1) p.part = take(batch * p.square.splits * p.m * p.lds * 4);
@@ -329,9 +385,9 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     return p;
 }
 
-template <class W, int SIDE, class F, class A>
+template <int SIDE, class F, class A>
 int launch(F kernel, std::atomic<bool>* done, const A& a, long long tiles, int splits, hipStream_t s) {
-    constexpr int bytes = 2 * DmeSquare<W, SIDE>::STAGE;
+    constexpr int bytes = 2 * DmeSquare<half, SIDE>::STAGE;
     int dev = 0;
     DME_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
@@ -342,63 +398,66 @@ int launch(F kernel, std::atomic<bool>* done, const A& a, long long tiles, int s
     return DME_OK;
 }
 
-template <class T, class W, int SIDE, bool TALL>
-int square(StepArgs<T, W> a, const DmeCut& cut, hipStream_t s) {
+template <class T, int PARTS, int SIDE, bool TALL>
+int square(StepArgs<T> a, const DmeCut& cut, hipStream_t s) {
     static std::atomic<bool> done[64];
     a.tiles_r = (a.mat.m + SIDE - 1) / SIDE;
-    a.slices = (int)(((TALL ? a.mat.rows : a.mat.cols) * (long long)sizeof(W) + DME_SLICE - 1) / DME_SLICE);
+    a.slices = (int)(((TALL ? a.mat.rows : a.mat.cols) * 2 + DME_SLICE - 1) / DME_SLICE);
     a.per_split = (a.slices + cut.splits - 1) / cut.splits;
-    return launch<W, SIDE>(square_kernel<T, W, SIDE, TALL>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, cut.splits, s);
+    return launch<SIDE>(square_kernel<T, PARTS, SIDE, TALL>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, cut.splits, s);
 }
 
-template <class T, class W, int SIDE>
-int poly(StepArgs<T, W> a, hipStream_t s) {
+template <class T, int PARTS, int SIDE>
+int poly(StepArgs<T> a, hipStream_t s) {
     static std::atomic<bool> done[64];
     a.tiles_r = (a.mat.m + SIDE - 1) / SIDE;
-    a.slices = (int)((a.mat.m * (long long)sizeof(W) + DME_SLICE - 1) / DME_SLICE);
-    return launch<W, SIDE>(poly_kernel<T, W, SIDE>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, 1, s);
+    a.slices = (int)((a.mat.m * 2 + DME_SLICE - 1) / DME_SLICE);
+    return launch<SIDE>(poly_kernel<T, PARTS, SIDE>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, 1, s);
 }
 
-template <class T, class W, int SIDE, bool TALL>
-int update(StepArgs<T, W> a, hipStream_t s) {
+template <class T, int PARTS, int SIDE, bool TALL>
+int update(StepArgs<T> a, hipStream_t s) {
     static std::atomic<bool> done[64];
     a.tiles_r = (a.mat.rows + SIDE - 1) / SIDE;
     a.tiles_c = (a.mat.cols + SIDE - 1) / SIDE;
-    a.slices = (int)((a.mat.m * (long long)sizeof(W) + DME_SLICE - 1) / DME_SLICE);
-    return launch<W, SIDE>(update_kernel<T, W, SIDE, TALL>, done, a, a.tiles_r * a.tiles_c, 1, s);
+    a.slices = (int)((a.mat.m * 2 + DME_SLICE - 1) / DME_SLICE);
+    return launch<SIDE>(update_kernel<T, PARTS, SIDE, TALL>, done, a, a.tiles_r * a.tiles_c, 1, s);
 }
 
-template <class T, class W, bool TALL>
-int one_step(const StepArgs<T, W>& k, const StepPlan& p, hipStream_t s) {
-    int rc = p.square.side == 256   ? square<T, W, 256, TALL>(k, p.square, s)
-             : p.square.side == 192 ? square<T, W, 192, TALL>(k, p.square, s)
-             : p.square.side == 128 ? square<T, W, 128, TALL>(k, p.square, s)
-                                    : square<T, W, 64, TALL>(k, p.square, s);
+template <class T, int PARTS, bool TALL>
+int one_step(const StepArgs<T>& k, const StepPlan& p, hipStream_t s) {
+    int rc = p.square.side == 256   ? square<T, PARTS, 256, TALL>(k, p.square, s)
+             : p.square.side == 192 ? square<T, PARTS, 192, TALL>(k, p.square, s)
+             : p.square.side == 128 ? square<T, PARTS, 128, TALL>(k, p.square, s)
+                                    : square<T, PARTS, 64, TALL>(k, p.square, s);
     if (rc) return rc;
-    if (p.square.splits > 1)
-        hipLaunchKernelGGL(join_kernel<W>, dim3((unsigned)dme_blocks(p.m * p.lds, 256, 2048), (unsigned)k.batch), dim3(256), 0, s, k.mat, p.square.splits);
-    rc = p.poly.side == 256   ? poly<T, W, 256>(k, s)
-         : p.poly.side == 192 ? poly<T, W, 192>(k, s)
-         : p.poly.side == 128 ? poly<T, W, 128>(k, s)
-                              : poly<T, W, 64>(k, s);
+    if (p.square.splits > 1) {
+        const long long along = (p.lds + 15) / 16;
+        hipLaunchKernelGGL(join_kernel<PARTS>, dim3((unsigned)(along * (along + 1) / 2), (unsigned)k.batch), dim3(256), 0, s, k.mat, p.square.splits);
+    }
+    rc = p.poly.side == 256   ? poly<T, PARTS, 256>(k, s)
+         : p.poly.side == 192 ? poly<T, PARTS, 192>(k, s)
+         : p.poly.side == 128 ? poly<T, PARTS, 128>(k, s)
+                              : poly<T, PARTS, 64>(k, s);
     if (rc) return rc;
-    return p.update.side == 256   ? update<T, W, 256, TALL>(k, s)
-           : p.update.side == 192 ? update<T, W, 192, TALL>(k, s)
-           : p.update.side == 128 ? update<T, W, 128, TALL>(k, s)
-                                  : update<T, W, 64, TALL>(k, s);
+    return p.update.side == 256   ? update<T, PARTS, 256, TALL>(k, s)
+           : p.update.side == 192 ? update<T, PARTS, 192, TALL>(k, s)
+           : p.update.side == 128 ? update<T, PARTS, 128, TALL>(k, s)
+                                  : update<T, PARTS, 64, TALL>(k, s);
 }
 
-template <class T, class W>
+template <class T, int PARTS>
 int run(const T* G, long long sb, long long rs, long long cs, long long batch, long long rows, long long cols, int steps, double a, double b, double c,
         T* out, char* ws, const StepPlan& p, hipStream_t s) {
     const bool tall = rows > cols;
-    StepArgs<T, W> k{};
-    Matrices<W>& x = k.mat;
-    x.X = (float*)(ws + p.X);
-    for (int i = 0; i < 2; ++i) x.Xw[i] = (W*)(ws + p.Xw[i]);
+    StepArgs<T> k{};
+    Matrices& x = k.mat;
+    for (int i = 0; i < 4; ++i) x.X[i / 2][i % 2] = (half*)(ws + p.X[i / 2][i % 2]);
+    for (int i = 0; i < PARTS; ++i) {
+        x.Sw[i] = (half*)(ws + p.Sw[i]);
+        x.Bw[i] = (half*)(ws + p.Bw[i]);
+    }
     x.S = (float*)(ws + p.S);
-    x.Sw = (W*)(ws + p.Sw);
-    x.Bw = (W*)(ws + p.Bw);
     x.Sd = (float*)(ws + p.Sd);
     x.Bd = (float*)(ws + p.Bd);
     x.part = (float*)(ws + p.part);
@@ -424,11 +483,11 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
     hipLaunchKernelGGL(norm_kernel<T>, dim3(NORM_BLOCKS, (unsigned)batch), dim3(256), 0, s, G, sb, line, step, whole ? 1 : lines,
                        whole ? lines * length : length, part);
     const long long tiles = (p.ldx + 63) / 64 * ((rows + 63) / 64);
-    hipLaunchKernelGGL((begin_kernel<T, W>), dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, part, x);
+    hipLaunchKernelGGL(begin_kernel<T>, dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, part, x);
     for (int i = 0; i < steps; ++i) {
         k.from = i & 1;
         k.out = i + 1 < steps ? nullptr : out;
-        const int rc = tall ? one_step<T, W, true>(k, p, s) : one_step<T, W, false>(k, p, s);
+        const int rc = tall ? one_step<T, PARTS, true>(k, p, s) : one_step<T, PARTS, false>(k, p, s);
         if (rc) return rc;
     }
     DME_HIP_CHECK(hipGetLastError());
@@ -478,8 +537,8 @@ extern "C" int dme_orthogonal_step(const void* G, int64_t batch_stride, int64_t 
     if (ws == nullptr || (uintptr_t)ws % 256 != 0 || ws_bytes < p.bytes)
         return dme_set_error(DME_ERR_WORKSPACE, "workspace of %lld bytes, aligned to 256, needed", p.bytes);
     if (type == DME_TYPE_BF16)
-        return run<__bf16, _Float16>((const __bf16*)G, batch_stride, row_stride, col_stride, batch, rows, cols, steps, a, b, c, (__bf16*)out, (char*)ws, p,
-                                     (hipStream_t)stream);
-    return run<float, float>((const float*)G, batch_stride, row_stride, col_stride, batch, rows, cols, steps, a, b, c, (float*)out, (char*)ws, p,
-                             (hipStream_t)stream);
+        return run<__bf16, 1>((const __bf16*)G, batch_stride, row_stride, col_stride, batch, rows, cols, steps, a, b, c, (__bf16*)out, (char*)ws, p,
+                              (hipStream_t)stream);
+    return run<float, 2>((const float*)G, batch_stride, row_stride, col_stride, batch, rows, cols, steps, a, b, c, (float*)out, (char*)ws, p,
+                         (hipStream_t)stream);
 }

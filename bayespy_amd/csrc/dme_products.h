@@ -138,7 +138,14 @@ struct DmeTile {
         }
     }
 
-    // acc = the tile at (r0, c0) over the slices [s0, s1) of k < K.  lds: 2 * STAGE bytes, free for the caller afterwards (a
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // acc += the tile at (r0, c0) over the slices [s0, s1) of k < K.  lds: 2 * STAGE bytes, free for the caller afterwards (a
     // barrier has been passed).  Every thread of the workgroup calls this.
     __device__ __forceinline__ void run(const DmeOperand& P, const DmeOperand& Q, long long K, char* lds, long long r0, long long c0, int s0, int s1) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -169,10 +176,6 @@ struct DmeTile {
             }
         };
         const int wr = wave / WC * NJ, wc = wave % WC * NI;
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         copy(s0, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();

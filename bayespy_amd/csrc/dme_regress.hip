@@ -41,7 +41,7 @@ __device__ __attribute__((noinline)) double dirichlet_f(double z, double x) {
     const int head = x < 16.0 ? (int)x : 16;
     for (int n = 1; n < head; ++n) {
         prod *= a + n;
-        if ((n & 3) == 0) {
+        if (prod > 1e200) {
             r += log(prod);
             prod = 1.0;
         }
@@ -376,6 +376,7 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
     dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * TC, k0 = a.column + c0;
     Tile t;
+    t.clear();
     t.run(a.h, a.w, a.D, lds, r0, c0, 0, a.slices);
     const int tid = threadIdx.x, g = (tid & 63) >> 4, wc = (tid >> 6) % WC, wr = (tid >> 6) / WC;
 #pragma unroll
@@ -526,6 +527,7 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     if (r0 + (tid >> 4) < a.nb) next.load(a.rows, r0 + (tid >> 4), k0 + sub * 8, a.K);
     {
         Tile t;
+        t.clear();
         t.run(a.h, a.w, a.D, lds, r0, c0, 0, a.slices);
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) {
@@ -858,6 +860,7 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void product_kernel(Produc
     int s1 = s0 + a.per_split;
     s1 = s1 < a.slices ? s1 : a.slices;
     Tile t;
+    t.clear();
     t.run(a.p, a.q, a.k, lds, tr * SIDE, tc * SIDE, s0, s1);
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
