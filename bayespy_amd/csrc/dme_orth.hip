@@ -148,10 +148,12 @@ template <int PARTS, class Tile>
 __device__ __forceinline__ void multiply(Tile& t, half* const* P, const DmeOperand& p, half* const* Q, const DmeOperand& q, long long po, long long qo,
                                          long long K, char* lds, long long r0, long long c0, int s0, int s1) {
     t.clear();
-#pragma unroll
-    for (int i = 0; i < (PARTS == 2 ? 3 : 1); ++i) {
-        const DmeOperand x{(const char*)(P[i == 2] + po), p.ld, p.rows}, y{(const char*)(Q[i == 1] + qo), q.ld, q.rows};
-        t.run(x, y, K, lds, r0, c0, s0, s1);
+    if constexpr (PARTS == 2) {
+        const char* const x[3] = {(const char*)(P[0] + po), (const char*)(P[0] + po), (const char*)(P[1] + po)};
+        const char* const y[3] = {(const char*)(Q[0] + qo), (const char*)(Q[1] + qo), (const char*)(Q[0] + qo)};
+        t.run(p, q, x, y, K, lds, r0, c0, s0, s1);
+    } else {
+        t.run(DmeOperand{(const char*)(P[0] + po), p.ld, p.rows}, DmeOperand{(const char*)(Q[0] + qo), q.ld, q.rows}, K, lds, r0, c0, s0, s1);
     }
 }
 
@@ -255,6 +257,18 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
     long long tr, tc;
     triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
     Tile t;
+    // a small tile's own values are on their way while it is made
+    constexpr bool EARLY = SIDE == 64;
+    f32x4 early[EARLY ? Tile::NI : 1][EARLY ? Tile::NJ : 1];
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int j = 0; j < Tile::NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < Tile::NI; ++i) {
+                const long long r = tr * SIDE + Tile::row_of(j), c = tc * SIDE + Tile::col_of(i);
+                early[i][j] = r < x.m && c < x.lds ? *(const f32x4*)(x.S + so + r * x.lds + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+    }
     multiply<PARTS>(t, x.Sw, op, x.Sw, op, so, so, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
     constexpr float UNIT = 1.f / (SCALE_S * SCALE_S);
 #pragma unroll
@@ -268,7 +282,10 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
             const long long c = tc * SIDE + Tile::col_of(i);
             if (c >= x.lds) continue;
             f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (real) s = *(const f32x4*)(x.S + so + r * x.lds + c);
+            if constexpr (EARLY)
+                s = early[i][j];
+            else if (real)
+                s = *(const f32x4*)(x.S + so + r * x.lds + c);
             f32x4 v;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -304,6 +321,20 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArg
     long long tr, tc;
     dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
     Tile t;
+    // a small tile's own values are on their way while it is made
+    constexpr bool EARLY = SIDE == 64;
+    f16x4 early[2][EARLY ? Tile::NI : 1][EARLY ? Tile::NJ : 1];
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int j = 0; j < Tile::NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < Tile::NI; ++i) {
+                const long long r = tr * SIDE + Tile::row_of(j), c = tc * SIDE + Tile::col_of(i);
+                const bool in = r < x.rows && c < x.ldx;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) early[u][i][j] = in ? *(const f16x4*)(X[u] + xo + r * x.ldx + c) : f16x4{0, 0, 0, 0};
+            }
+    }
     if (TALL)
         multiply<PARTS>(t, X, y, x.Bw, b, xo, so, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
     else
@@ -320,7 +351,14 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArg
             const long long c = tc * SIDE + Tile::col_of(i);
             if (c >= x.ldx) continue;
             const long long at = r * x.ldx + c;
-            const f16x4 h = *(const f16x4*)(X[0] + xo + at), l = *(const f16x4*)(X[1] + xo + at);
+            f16x4 h, l;
+            if constexpr (EARLY) {
+                h = early[0][i][j];
+                l = early[1][i][j];
+            } else {
+                h = *(const f16x4*)(X[0] + xo + at);
+                l = *(const f16x4*)(X[1] + xo + at);
+            }
             f32x4 v;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -345,9 +383,160 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArg
     }
 }
 
+// ---- up to 64 singular values, up to 4096 the other way ---------------------------------------------------------------
+//
+// Such a matrix is all latency: the four launches of a step above take 25 us, most of it waiting for memory once or twice each.  Here
+// a step is one launch.  X lies n x 64 in 32 bits, a workgroup owns tiles of 64 lines of it; it adds up the workgroups' pieces of S, makes
+// the polynomial of S for itself (64 x 64 x 64 products in LDS, fp32 instructions), updates its tiles and leaves its piece of the next S.
+
+constexpr int SMALL = 64, SMALL_GROUPS = 16, SP = SMALL + 4;  // SP: pitch in LDS, a multiple of 16 bytes that spreads the lines over the banks
+
+struct SmallArgs {
+    float* X;             // [batch][n][64]
+    const float* part;    // [batch][groups][64][64]
+    float* next;
+    long long n, m, tiles;
+    int groups;
+    float a, b, c;
+    void* out;            // the last step's result, or null
+    long long out_batch, out_n, out_m;
+};
+
+// acc[i] += P[r][k] Q[c][k] over 64 k; this wave's 16 r, all c in four blocks.  P, Q: lines of SP values in LDS.
+__device__ __forceinline__ void small_product(f32x4 (&acc)[4], const float* P, const float* Q) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < SMALL; k += 16) {
+        const u32q p = *(const u32q*)(P + (wave * 16 + c) * SP + k + g * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = dme_mma(*(const u32q*)(Q + (i * 16 + c) * SP + k + g * 4), p, acc[i], float());
+    }
+}
+
+// acc[i] += X[k][r] X[k][c] over 64 lines k
+__device__ __forceinline__ void small_square(f32x4 (&acc)[4], const float* X) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < SMALL; k += 4) {
+        const float* line = X + (k + g) * SP + c;
+        const float p = line[wave * 16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(line[i * 16], p, acc[i], 0, 0, 0);
+    }
+}
+
+// this workgroup's piece of S
+__device__ __forceinline__ void small_leave(const f32x4 (&acc)[4], float* part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(f32x4*)(part + (wave * 16 + c) * SMALL + i * 16 + g * 4) = acc[i];
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void small_begin_kernel(const T* G, long long sb, long long sn, long long sm, const double* norm, SmallArgs a) {
+    __shared__ __attribute__((aligned(16))) float tile[SMALL * SP];
+    __shared__ double sums[4];
+    double s = dme_wave_sum_f64(norm[blockIdx.y * NORM_BLOCKS + threadIdx.x]);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const double scale = s > 0.0 || s != s ? 1.0 / sqrt(s) : 0.0;
+    const T* g = G + blockIdx.y * sb;
+    f32x4 acc[4] = {};
+    const int lo = threadIdx.x & 63, hi = threadIdx.x >> 6;
+    for (long long t = blockIdx.x; t < a.tiles; t += a.groups) {
+        __syncthreads();
+        for (int q = hi; q < SMALL; q += 4) {  // neighbouring lanes along G's contiguous direction
+            const int y = sm == 1 ? q : lo, x = sm == 1 ? lo : q;
+            const long long r = t * SMALL + y;
+            tile[y * SP + x] = r < a.n && x < a.m ? (float)((double)(float)g[r * sn + x * sm] * scale) : 0.f;
+        }
+        __syncthreads();
+        float* X = a.X + (blockIdx.y * a.tiles + t) * SMALL * SMALL;
+        for (int f = threadIdx.x; f < SMALL * SMALL / 4; f += 256) *(f32x4*)(X + f * 4) = *(const f32x4*)(tile + (f >> 4) * SP + (f & 15) * 4);
+        small_square(acc, tile);
+    }
+    small_leave(acc, a.next + (blockIdx.y * a.groups + blockIdx.x) * SMALL * SMALL);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void small_step_kernel(SmallArgs a) {
+    __shared__ __attribute__((aligned(16))) float S[SMALL * SP], B[SMALL * SP], X[SMALL * SP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    float* mine = a.X + blockIdx.y * a.tiles * SMALL * SMALL;
+    f32x4 x[4];  // the first tile is on its way while S is added up
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = *(const f32x4*)(mine + blockIdx.x * SMALL * SMALL + (q * 256 + tid) * 4);
+    {
+        f32x4 s[4] = {};
+        const float* part = a.part + blockIdx.y * a.groups * SMALL * SMALL;
+#pragma unroll 8
+        for (int u = 0; u < a.groups; ++u)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] += *(const f32x4*)(part + u * SMALL * SMALL + (q * 256 + tid) * 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int f = q * 256 + tid;
+            *(f32x4*)(S + (f >> 4) * SP + (f & 15) * 4) = s[q];
+        }
+    }
+    __syncthreads();
+    f32x4 acc[4] = {};
+    small_product(acc, S, S);
+    const int r = wave * 16 + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = i * 16 + g * 4;
+        const f32x4 s = *(const f32x4*)(S + r * SP + k);
+        f32x4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = __builtin_fmaf(a.c, acc[i][q], a.b * s[q]) + (k + q == r ? a.a : 0.f);
+        *(f32x4*)(B + r * SP + k) = v;
+    }
+    f32x4 next[4] = {};
+    for (long long t = blockIdx.x; t < a.tiles; t += a.groups) {
+        float* at = mine + t * SMALL * SMALL;
+        __syncthreads();  // B is written, and X of the tile before read
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int f = q * 256 + tid;
+            if (t != blockIdx.x) x[q] = *(const f32x4*)(at + f * 4);
+            *(f32x4*)(X + (f >> 4) * SP + (f & 15) * 4) = x[q];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        small_product(acc, X, B);  // B is symmetric
+        if (a.out) {
+            const long long line = t * SMALL + r;
+            T* o = (T*)a.out + blockIdx.y * a.out_batch + line * a.out_n;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int k = i * 16 + g * 4 + q;
+                    if (line < a.n && k < a.m) o[k * a.out_m] = (T)acc[i][q];
+                }
+            continue;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            *(f32x4*)(X + r * SP + i * 16 + g * 4) = acc[i];
+            *(f32x4*)(at + r * SMALL + i * 16 + g * 4) = acc[i];
+        }
+        __syncthreads();
+        small_square(next, X);
+    }
+    if (!a.out) small_leave(next, a.next + (blockIdx.y * a.groups + blockIdx.x) * SMALL * SMALL);
+}
+
 inline long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 struct StepPlan {
+    bool small;
+    long long tiles;  // small: of 64 lines
+    int groups;
     long long m, n, ldx, lds;
     DmeCut square, poly, update;
     long long norm, X[2][2], S, Sw[2], Bw[2], Sd, Bd, part, bytes;
@@ -362,9 +551,11 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     p.lds = up(p.m, 8);
     // three products of halves cost three times the slices
     const auto slices = [&](long long k) { return (k * 2 + DME_SLICE - 1) / DME_SLICE * (parts == 2 ? 3 : 1); };
-    p.square = dme_cut(p.m, p.m, slices(p.n), 2, true, 0.0, true);
-    p.poly = dme_cut(p.m, p.m, slices(p.m), 2, false, 0.0, true);
-    p.update = dme_cut(rows, cols, slices(p.m), 2, false);
+    p.square = dme_cut(p.m, p.m, slices(p.n), 2, true, 0.0, true, batch);
+    p.poly = dme_cut(p.m, p.m, slices(p.m), 2, false, 0.0, true, batch);
+    p.update = dme_cut(rows, cols, slices(p.m), 2, false, 0.0, false, batch);
+    // few slices: the update is bound by its passes over X, which small tiles overlap (50000 x 256: 50 us with 256, 41 with 64)
+    if (slices(p.m) <= 8) p.update.side = 64;
     long long at = 0;
     const auto take = [&](long long bytes) {
         const long long here = at;
@@ -372,6 +563,15 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
         return here;
     };
     p.norm = take(batch * NORM_BLOCKS * 8);
+    p.small = p.m <= SMALL && p.n <= 4096;
+    if (p.small) {
+        p.tiles = (p.n + SMALL - 1) / SMALL;
+        p.groups = (int)(p.tiles < SMALL_GROUPS ? p.tiles : SMALL_GROUPS);
+        p.S = take(batch * p.tiles * SMALL * SMALL * 4);                        // X
+        p.part = take(2 * batch * p.groups * SMALL * SMALL * 4);  // the pieces of S, read and written in turn
+        p.bytes = at;
+        return p;
+    }
     for (int i = 0; i < 4; ++i) p.X[i / 2][i % 2] = take(batch * rows * p.ldx * 2);
     p.S = take(batch * p.m * p.lds * 4);
     for (int i = 0; i < parts; ++i) {
@@ -387,7 +587,7 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
 
 template <int SIDE, class F, class A>
 int launch(F kernel, std::atomic<bool>* done, const A& a, long long tiles, int splits, hipStream_t s) {
-    constexpr int bytes = 2 * DmeSquare<half, SIDE>::STAGE;
+    constexpr int bytes = DmeSquare<half, SIDE>::LDS;
     int dev = 0;
     DME_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
@@ -482,6 +682,32 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
     const bool whole = step == 1 && line == length;
     hipLaunchKernelGGL(norm_kernel<T>, dim3(NORM_BLOCKS, (unsigned)batch), dim3(256), 0, s, G, sb, line, step, whole ? 1 : lines,
                        whole ? lines * length : length, part);
+    if (p.small) {
+        SmallArgs y{};
+        float* pieces[2] = {(float*)(ws + p.part), (float*)(ws + p.part) + batch * p.groups * SMALL * SMALL};
+        y.X = (float*)(ws + p.S);
+        y.next = pieces[0];
+        y.n = p.n;
+        y.m = p.m;
+        y.tiles = p.tiles;
+        y.groups = p.groups;
+        y.a = (float)a;
+        y.b = (float)b;
+        y.c = (float)c;
+        y.out_batch = rows * cols;
+        y.out_n = tall ? cols : 1;
+        y.out_m = tall ? 1 : cols;
+        const dim3 grid((unsigned)p.groups, (unsigned)batch);
+        hipLaunchKernelGGL(small_begin_kernel<T>, grid, dim3(256), 0, s, G, sb, tall ? rs : cs, tall ? cs : rs, part, y);
+        for (int i = 0; i < steps; ++i) {
+            y.part = pieces[i & 1];
+            y.next = pieces[(i & 1) ^ 1];
+            y.out = i + 1 < steps ? nullptr : out;
+            hipLaunchKernelGGL(small_step_kernel<T>, grid, dim3(256), 0, s, y);
+        }
+        DME_HIP_CHECK(hipGetLastError());
+        return DME_OK;
+    }
     const long long tiles = (p.ldx + 63) / 64 * ((rows + 63) / 64);
     hipLaunchKernelGGL(begin_kernel<T>, dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, part, x);
     for (int i = 0; i < steps; ++i) {

@@ -3,7 +3,8 @@
 //
 // A workgroup of NW = WR x WC waves makes a tile of TR x TC outputs.  k goes by slices of 128 bytes (64 bf16 / fp16,
 // 32 fp32 values): a slice of the tile's TR + TC rows is copied from memory straight into LDS (16 bytes a lane, no
-// registers in between), two buffers, so that the copies of slice s + 1 fly while slice s is multiplied.  A row's eight
+// registers in between), two buffers (four for small tiles, whose products are short beside the memory's answer), so that the
+// copies of later slices fly while slice s is multiplied.  A row's eight
 // 16-byte chunks are stored at chunk ^ (row & 7): lanes of a wave that read the same chunk of 8 neighbouring rows then
 // touch all banks once.  Q is the matrix instruction's first operand, so a lane ends up with ONE r (lane & 15) and four
 // neighbouring c: rows are reduced and stored in vectors.
@@ -78,6 +79,8 @@ struct DmeTile {
     static constexpr int WTR = TR / WR, WTC = TC / WC;  // a wave's part
     static constexpr int NJ = WTR / 16, NI = WTC / 16;  // its 16 x 16 blocks
     static constexpr int STAGE = (TR + TC) * DME_SLICE;  // bytes of one buffer
+    static constexpr int STAGES = TR + TC <= 144 ? 4 : 2;
+    static constexpr int LDS = STAGES * STAGE;
     static constexpr int COPIES = (TR + TC) / 8;         // wave copies (1 KB) of one slice
     static constexpr int PER_WAVE = (COPIES + NW - 1) / NW;
     static constexpr int SIZE = sizeof(T);
@@ -145,9 +148,18 @@ struct DmeTile {
             for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // acc += the tile at (r0, c0) over the slices [s0, s1) of k < K.  lds: 2 * STAGE bytes, free for the caller afterwards (a
+    // acc += the tile at (r0, c0) over the slices [s0, s1) of k < K.  lds: LDS bytes, free for the caller afterwards (a
     // barrier has been passed).  Every thread of the workgroup calls this.
     __device__ __forceinline__ void run(const DmeOperand& P, const DmeOperand& Q, long long K, char* lds, long long r0, long long c0, int s0, int s1) {
+        const char *p[1] = {P.at}, *q[1] = {Q.at};
+        run(P, Q, p, q, K, lds, r0, c0, s0, s1);
+    }
+
+    // acc += the sum of PARTS products whose operands lie alike, part i at p[i] and q[i] (P.at, Q.at are not used), as one run of slices.
+    template <int PARTS>
+    __device__ __forceinline__ void run(const DmeOperand& P, const DmeOperand& Q, const char* const (&p)[PARTS], const char* const (&q)[PARTS],
+                                        long long K, char* lds, long long r0, long long c0, int s0, int s1) {
+        if (s0 >= s1) return;
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const char* src[PER_WAVE];
         int limit[PER_WAVE];
@@ -156,47 +168,86 @@ struct DmeTile {
         for (int t = 0; t < PER_WAVE; ++t) {
             const int piece = t * NW + wave;
             if (piece < TR / 8) {
-                source<TR, PK>(P, r0, K, piece, lane, src[t], limit[t]);
+                source<TR, PK>(DmeOperand{p[0], P.ld, P.rows}, r0, K, piece, lane, src[t], limit[t]);
                 src[t] += s0 * pstep;
             } else {
-                source<TC, QK>(Q, c0, K, piece - TR / 8, lane, src[t], limit[t]);
+                source<TC, QK>(DmeOperand{q[0], Q.ld, Q.rows}, c0, K, piece - TR / 8, lane, src[t], limit[t]);
                 src[t] += s0 * qstep;
             }
         }
         const u32 to = (u32)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-        auto copy = [&](int s, int buf) {
+        int slice = s0, part = 0;  // the next one to be copied
+        auto copy = [&](int buf) {
 #pragma unroll
             for (int t = 0; t < PER_WAVE; ++t) {
                 const int piece = t * NW + wave;
                 if (COPIES % NW == 0 || piece < COPIES) {
-                    const char* from = s < limit[t] ? src[t] : (const char*)dme_zeros;
+                    const char* from = slice < limit[t] ? src[t] : (const char*)dme_zeros;
                     dme_copy_to_lds(from, to + buf * STAGE + piece * 1024);
                     src[t] += piece < TR / 8 ? pstep : qstep;
                 }
             }
+            ++slice;
+            if (PARTS > 1 && slice == s1 && part + 1 < PARTS) {
+                slice = s0;
+                long long dp = 0, dq = 0;  // from this part's end to the next one's beginning
+#pragma unroll
+                for (int i = 0; i + 1 < PARTS; ++i)
+                    if (part == i) {
+                        dp = p[i + 1] - p[i];
+                        dq = q[i + 1] - q[i];
+                    }
+                dp -= (s1 - s0) * pstep;
+                dq -= (s1 - s0) * qstep;
+                ++part;
+#pragma unroll
+                for (int t = 0; t < PER_WAVE; ++t) src[t] += t * NW + wave < TR / 8 ? dp : dq;
+            }
         };
         const int wr = wave / WC * NJ, wc = wave % WC * NI;
-        copy(s0, 0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        for (int s = s0; s < s1; ++s) {
-            const int buf = (s - s0) & 1;
-            if (s + 1 < s1) copy(s + 1, buf ^ 1);
-            const char* at = lds + buf * STAGE;
+        auto multiply = [&](const char* at) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                u32q p[NJ], q[NI];
+                u32q x[NJ], y[NI];
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) p[j] = fragment<TR, PK>(at, wr + j, h);
+                for (int j = 0; j < NJ; ++j) x[j] = fragment<TR, PK>(at, wr + j, h);
 #pragma unroll
-                for (int i = 0; i < NI; ++i) q[i] = fragment<TC, QK>(at + TR * DME_SLICE, wc + i, h);
+                for (int i = 0; i < NI; ++i) y[i] = fragment<TC, QK>(at + TR * DME_SLICE, wc + i, h);
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc[i][j] = dme_mma(q[i], p[j], acc[i][j], T());
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = dme_mma(y[i], x[j], acc[i][j], T());
             }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // slice s + 1 is in LDS ...
-            __syncthreads();                                  // ... and everybody has read slice s
+        };
+        const int n = (s1 - s0) * PARTS;
+        if constexpr (STAGES == 2) {
+            copy(0);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            for (int u = 0; u < n; ++u) {
+                if (u + 1 < n) copy((u + 1) & 1);
+                multiply(lds + (u & 1) * STAGE);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // slice u + 1 is in LDS ...
+                __syncthreads();                                  // ... and everybody has read slice u
+            }
+        } else {
+            // every wave issues COPIES / NW copies of a slice at least, so that many times the slices that may still be on their
+            // way are what it may have outstanding (copies come back in their order)
+            constexpr int AHEAD = STAGES - 2, OUT = AHEAD * (COPIES / NW);
+            static_assert(OUT < 64, "vmcnt has six bits");
+#pragma unroll
+            for (int u = 0; u < STAGES - 1; ++u)
+                if (u < n) copy(u);
+            for (int u = 0; u < n; ++u) {
+                if (u + AHEAD < n)
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OUT) : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();  // slice u is in LDS, and everybody has read slice u - 1
+                if (u + STAGES - 1 < n) copy((u + STAGES - 1) % STAGES);
+                multiply(lds + u % STAGES * STAGE);
+            }
+            __syncthreads();
         }
     }
 
@@ -243,30 +294,31 @@ using DmeSquare = DmeTile<T, SIDE, SIDE, (SIDE == 256 ? 4 : 2), (SIDE == 192 ? 4
 
 // How a product of R x C outputs over `slices` slices of k is cut: tiles of 256, 192, 128 or 64 a side, and into how many pieces
 // of k.  Measured in bf16 (fp32) at 4096^3 and 8192^3: 256 a side, one workgroup to a CU, 1150-1290 (141) TFLOP/s; 192, one to a CU, 960-1010;
-// 128, two to a CU, 910-1110 (138); 64, four to a CU, 700 (128).  Small products are bound by how many CUs have a tile at all, and
+// 128, two to a CU, 910-1110 (138); 64, two to a CU, 600 (128).  Small products are bound by how many CUs have a tile at all, and
 // pieces of k cost a pass over their 32-bit sums.
 struct DmeCut {
     int side, splits;
     double us;
 };
-inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool split, double extra_per_tile_us = 0.0, bool symmetric = false) {
+inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool split, double extra_per_tile_us = 0.0, bool symmetric = false,
+                      long long batch = 1) {
     static const struct {
         int side, per_cu;
         double bf16, f32;
-    } kinds[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6}, {128, 2, 980e6, 138e6}, {64, 4, 700e6, 128e6}};
+    } kinds[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6}, {128, 2, 980e6, 138e6}, {64, 2, 600e6, 128e6}};
     DmeCut best{0, 1, 0.0};
     for (const auto& kind : kinds) {
         const int side = kind.side, per_cu = kind.per_cu;
         const double rate = size == 4 ? kind.f32 : kind.bf16;
         const long long along = (R + side - 1) / side, slots = 256ll * per_cu;
-        const long long tiles = symmetric ? along * (along + 1) / 2 : along * ((C + side - 1) / side);
+        const long long tiles = batch * (symmetric ? along * (along + 1) / 2 : along * ((C + side - 1) / side));
         // one slice of one tile while the CU's other places are taken too
         const double slice = (double)side * side * (DME_SLICE / size) * 2.0 * slots / rate;
         for (int s = 1; s <= (split ? 64 : 1); s *= 2) {
             if (s > 1 && slices / s < 2) break;
             const double rounds = (double)((tiles * s + slots - 1) / slots);
             double us = rounds * ((double)((slices + s - 1) / s + 2) * slice + extra_per_tile_us * side * side / 65536.0 * per_cu);
-            if (s > 1) us += 4.0 + (double)s * R * C * 8.0 / 4e6;
+            if (s > 1) us += 4.0 + (double)s * batch * R * C * 8.0 / 4e6;
             if (best.side == 0 || us < best.us) best = DmeCut{side, s, us};
         }
     }

@@ -1051,10 +1051,10 @@ int set_lds(std::atomic<bool>* done, F kernel, int bytes) {
 template <class T, int TR, int TC, int WR, int WC, bool BACKWARD>
 int launch_tile(const TileArgs& a, hipStream_t s) {
     typedef DmeTile<T, TR, TC, WR, WC> Tile;
-    static_assert(2 * Tile::STAGE >= WC * TR * 8 && 2 * Tile::STAGE >= WR * TC * 4, "the reductions use the tiles' LDS");
+    static_assert(Tile::LDS >= WC * TR * 8 && Tile::LDS >= WR * TC * 4, "the reductions use the tiles' LDS");
     static std::atomic<bool> done[64];
     constexpr int turned = BACKWARD && sizeof(T) == 2 && TR >= 128 ? TR * WC * (Tile::WTC * (int)sizeof(T) + 16) : 0;
-    constexpr int bytes = turned > 2 * Tile::STAGE ? turned : 2 * Tile::STAGE;
+    constexpr int bytes = turned > Tile::LDS ? turned : Tile::LDS;
     const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, BACKWARD>, bytes);
     if (rc) return rc;
     hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c)), dim3(Tile::NT), bytes, s, a);
@@ -1064,7 +1064,7 @@ int launch_tile(const TileArgs& a, hipStream_t s) {
 template <class T, int TR, bool BACKWARD>
 int launch_dense(const TileArgs& a, hipStream_t s) {
     typedef DmeTile<T, TR, DT, (TR == 16 ? 1 : 2), (TR == 16 ? 4 : 2)> Tile;
-    constexpr int bytes = 2 * Tile::STAGE > TR * ZP * 4 ? 2 * Tile::STAGE : TR * ZP * 4;
+    constexpr int bytes = Tile::LDS > TR * ZP * 4 ? Tile::LDS : TR * ZP * 4;
     static std::atomic<bool> done[64];
     const int rc = set_lds(done, dense_kernel<T, TR, BACKWARD>, bytes);
     if (rc) return rc;
@@ -1085,9 +1085,9 @@ template <class T, int SIDE, bool PK>
 int launch_product(const ProductArgs& a, int splits, hipStream_t s) {
     typedef DmeSquare<T, SIDE, PK, true> Tile;
     static std::atomic<bool> done[64];
-    const int rc = set_lds(done, product_kernel<T, SIDE, PK>, 2 * Tile::STAGE);
+    const int rc = set_lds(done, product_kernel<T, SIDE, PK>, Tile::LDS);
     if (rc) return rc;
-    hipLaunchKernelGGL((product_kernel<T, SIDE, PK>), dim3((unsigned)(a.tiles_r * a.tiles_c), (unsigned)splits), dim3(Tile::NT), 2 * Tile::STAGE, s, a);
+    hipLaunchKernelGGL((product_kernel<T, SIDE, PK>), dim3((unsigned)(a.tiles_r * a.tiles_c), (unsigned)splits), dim3(Tile::NT), Tile::LDS, s, a);
     return DME_OK;
 }
 
