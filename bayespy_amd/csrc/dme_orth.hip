@@ -157,11 +157,10 @@ __device__ __forceinline__ void multiply(Tile& t, half* const* P, const DmeOpera
     }
 }
 
-// Tile `t` of the lower triangle of a square of tiles, numbered along its rows; XCDs take eighths of them (dme_tile_of).
-__device__ __forceinline__ void triangle_tile(long long block, long long n, long long& tr, long long& tc) {
-    const long long all = n * (n + 1) / 2, per = all / 8, more = all % 8, x = block & 7, at = block >> 3;
-    const long long t = x * per + (x < more ? x : more) + at;
-    long long r = (long long)((sqrt(8.0 * (double)t + 1.0) - 1.0) * 0.5);
+// The tiles of the lower triangle of a square of n x n tiles, numbered along its rows; XCDs take eighths of them (dme_xcd_order).
+__device__ __forceinline__ void triangle_tile(u32 block, u32 n, long long& tr, long long& tc) {
+    const u32 t = dme_xcd_order(block, n * (n + 1) / 2);
+    u32 r = (u32)((__builtin_sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);  // near enough: set right below
     while (r * (r + 1) / 2 > t) --r;
     while ((r + 1) * (r + 2) / 2 <= t) ++r;
     tr = r;
@@ -187,7 +186,7 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArg
     const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m, xo = blockIdx.y * x.stride_x;
     const DmeOperand op{nullptr, x.ldx * 2, x.m};
     long long tr, tc;
-    triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
+    triangle_tile(blockIdx.x, (u32)a.tiles_r, tr, tc);
     const int s0 = (int)blockIdx.z * a.per_split;
     int s1 = s0 + a.per_split;
     s1 = s1 < a.slices ? s1 : a.slices;
@@ -222,7 +221,7 @@ __global__ __launch_bounds__(256) void join_kernel(Matrices x, int splits) {
     __shared__ float turn[16][17];
     const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
     long long tr, tc;
-    triangle_tile(blockIdx.x, (x.lds + 15) / 16, tr, tc);
+    triangle_tile(blockIdx.x, (u32)((x.lds + 15) / 16), tr, tc);
     const int lo = threadIdx.x & 15, hi = threadIdx.x >> 4;
     const long long r = tr * 16 + hi, c = tc * 16 + lo;
     float v = 0.f;
@@ -255,7 +254,7 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
     const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
     const DmeOperand op{nullptr, x.lds * 2, x.m};
     long long tr, tc;
-    triangle_tile(blockIdx.x, a.tiles_r, tr, tc);
+    triangle_tile(blockIdx.x, (u32)a.tiles_r, tr, tc);
     Tile t;
     // a small tile's own values are on their way while it is made
     constexpr bool EARLY = SIDE == 64;
@@ -310,16 +309,16 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
 }
 
 // X <- a X + B X (a X + X B for a tall X)
-template <class T, int PARTS, int SIDE, bool TALL>
+template <class T, int PARTS, int SIDE, bool TALL, int STAGES = 0>
 __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeSquare<half, SIDE, false, !TALL> Tile;
+    typedef DmeSquare<half, SIDE, false, !TALL, STAGES> Tile;
     const Matrices& x = a.mat;
     const long long xo = blockIdx.y * x.stride_x, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
     const DmeOperand b{nullptr, x.lds * 2, x.m}, y{nullptr, x.ldx * 2, TALL ? x.rows : x.cols};
     half* const* X = x.X[a.from];
     long long tr, tc;
-    dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
+    dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
     Tile t;
     // a small tile's own values are on their way while it is made
     constexpr bool EARLY = SIDE == 64;
@@ -470,7 +469,6 @@ __global__ __launch_bounds__(256) void small_step_kernel(SmallArgs a) {
     {
         f32x4 s[4] = {};
         const float* part = a.part + blockIdx.y * a.groups * SMALL * SMALL;
-#pragma unroll 8
         for (int u = 0; u < a.groups; ++u)
 #pragma unroll
             for (int q = 0; q < 4; ++q) s[q] += *(const f32x4*)(part + u * SMALL * SMALL + (q * 256 + tid) * 4);
@@ -585,9 +583,9 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     return p;
 }
 
-template <int SIDE, class F, class A>
+template <int SIDE, int STAGES = 0, class F, class A>
 int launch(F kernel, std::atomic<bool>* done, const A& a, long long tiles, int splits, hipStream_t s) {
-    constexpr int bytes = DmeSquare<half, SIDE>::LDS;
+    constexpr int bytes = DmeSquare<half, SIDE, false, false, STAGES>::LDS;
     int dev = 0;
     DME_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
@@ -617,10 +615,14 @@ int poly(StepArgs<T> a, hipStream_t s) {
 
 template <class T, int PARTS, int SIDE, bool TALL>
 int update(StepArgs<T> a, hipStream_t s) {
-    static std::atomic<bool> done[64];
+    static std::atomic<bool> done[64], done2[64];
     a.tiles_r = (a.mat.rows + SIDE - 1) / SIDE;
     a.tiles_c = (a.mat.cols + SIDE - 1) / SIDE;
     a.slices = (int)((a.mat.m * 2 + DME_SLICE - 1) / DME_SLICE);
+    // small tiles: a deep pipeline where a CU has one or two of them, two buffers where it can hold five
+    if constexpr (SIDE == 64)
+        if (a.tiles_r * a.tiles_c * a.batch > 512)
+            return launch<SIDE, 2>(update_kernel<T, PARTS, SIDE, TALL, 2>, done2, a, a.tiles_r * a.tiles_c, 1, s);
     return launch<SIDE>(update_kernel<T, PARTS, SIDE, TALL>, done, a, a.tiles_r * a.tiles_c, 1, s);
 }
 

@@ -73,13 +73,13 @@ static __device__ __attribute__((aligned(256))) u32 dme_zeros[64];
 // transposing LDS read (16 lanes read 4 lines of 16 values, each lane gets one row's 4 k), 32-bit ones by four reads of a
 // word.  The 16 lines that a wave reads at once begin in the same bank, so the 16-value groups of line k are stored at
 // group ^ f(k), f spreading them over the banks.
-template <class T, int TR, int TC, int WR, int WC, bool PK = false, bool QK = false>
+template <class T, int TR, int TC, int WR, int WC, bool PK = false, bool QK = false, int STAGES_ = 0>
 struct DmeTile {
     static constexpr int NW = WR * WC, NT = NW * 64;
     static constexpr int WTR = TR / WR, WTC = TC / WC;  // a wave's part
     static constexpr int NJ = WTR / 16, NI = WTC / 16;  // its 16 x 16 blocks
     static constexpr int STAGE = (TR + TC) * DME_SLICE;  // bytes of one buffer
-    static constexpr int STAGES = TR + TC <= 144 ? 4 : 2;
+    static constexpr int STAGES = STAGES_ ? STAGES_ : TR + TC <= 144 ? 4 : 2;
     static constexpr int LDS = STAGES * STAGE;
     static constexpr int COPIES = (TR + TC) / 8;         // wave copies (1 KB) of one slice
     static constexpr int PER_WAVE = (COPIES + NW - 1) / NW;
@@ -265,13 +265,15 @@ struct DmeTile {
 // Which tile a workgroup makes.  Workgroups go round the 8 XCDs one by one, and each XCD has an L2 of its own: XCD x
 // takes the x-th eighth of the tiles, in columns of 8 row tiles, so that the operand rows that its 32 CUs read at the
 // same time overlap.
-__device__ __forceinline__ void dme_tile_of(long long block, long long tiles_r, long long tiles_c, long long& tr, long long& tc) {
-    const long long n = tiles_r * tiles_c;
-    const long long per = n / 8, more = n % 8, x = block & 7, at = block >> 3;
-    long long t = x * per + (x < more ? x : more) + at;
-    const long long band = t / (8 * tiles_c), first = band * 8;
-    const long long high = tiles_r - first < 8 ? tiles_r - first : 8;
-    t -= band * 8 * tiles_c;
+__device__ __forceinline__ u32 dme_xcd_order(u32 block, u32 n) {
+    const u32 per = n / 8, more = n % 8, x = block & 7;
+    return x * per + (x < more ? x : more) + (block >> 3);
+}
+__device__ __forceinline__ void dme_tile_of(u32 block, u32 tiles_r, u32 tiles_c, long long& tr, long long& tc) {
+    u32 t = dme_xcd_order(block, tiles_r * tiles_c);  // fits: the launch has as many workgroups
+    const u32 band = t / (8 * tiles_c), first = band * 8;
+    const u32 high = tiles_r - first < 8 ? tiles_r - first : 8;
+    t -= first * tiles_c;
     tr = first + t % high;
     tc = t / high;
 }
@@ -289,8 +291,8 @@ inline int dme_blocks(long long work, long long per, long long most) {
 }
 
 // The waves of a SIDE x SIDE tile.
-template <class T, int SIDE, bool PK = false, bool QK = false>
-using DmeSquare = DmeTile<T, SIDE, SIDE, (SIDE == 256 ? 4 : 2), (SIDE == 192 ? 4 : 2), PK, QK>;
+template <class T, int SIDE, bool PK = false, bool QK = false, int STAGES = 0>
+using DmeSquare = DmeTile<T, SIDE, SIDE, (SIDE == 256 ? 4 : 2), (SIDE == 192 ? 4 : 2), PK, QK, STAGES>;
 
 // How a product of R x C outputs over `slices` slices of k is cut: tiles of 256, 192, 128 or 64 a side, and into how many pieces
 // of k.  Measured in bf16 (fp32) at 4096^3 and 8192^3: 256 a side, one workgroup to a CU, 1150-1290 (141) TFLOP/s; 192, one to a CU, 960-1010;

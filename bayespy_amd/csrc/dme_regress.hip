@@ -373,7 +373,7 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DmeTile<T, TR, TC, WR, WC> Tile;
     long long tr, tc;
-    dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
+    dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * TC, k0 = a.column + c0;
     Tile t;
     t.clear();
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DmeTile<T, TR, DT, (TR == 16 ? 1 : 2), (TR == 16 ? 4 : 2)> Tile;
     long long tr, tc;
-    dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
+    dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * DT, k0 = a.column + c0;
     float* z = (float*)lds;
     const int tid = threadIdx.x, sub = tid & 15;
@@ -855,7 +855,7 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void product_kernel(Produc
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DmeSquare<T, SIDE, PK, true> Tile;
     long long tr, tc;
-    dme_tile_of(blockIdx.x, a.tiles_r, a.tiles_c, tr, tc);
+    dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
     const int s0 = (int)blockIdx.y * a.per_split;
     int s1 = s0 + a.per_split;
     s1 = s1 < a.slices ? s1 : a.slices;
