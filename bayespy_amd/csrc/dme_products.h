@@ -278,11 +278,12 @@ __device__ __forceinline__ void dme_tile_of(u32 block, u32 tiles_r, u32 tiles_c,
     tc = t / high;
 }
 
-// dst [rows][ldd] = src [rows][cols] (any pitch and alignment), zero beyond cols.  A wave takes a row.
-template <class T>
-__global__ __launch_bounds__(256) void dme_pack_kernel(const T* src, long long lds_, long long rows, long long cols, T* dst, long long ldd) {
+// dst [rows][ldd] = src [rows][cols], zero beyond cols, all counted in values of V (as many bytes as every row's beginning and length
+// allow).  A wave takes a row.
+template <class V>
+__global__ __launch_bounds__(256) void dme_pack_kernel(const V* src, long long lds_, long long rows, long long cols, V* dst, long long ldd) {
     for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (long long)gridDim.x * 4)
-        for (long long c = threadIdx.x & 63; c < ldd; c += 64) dst[r * ldd + c] = c < cols ? src[r * lds_ + c] : (T)0.f;
+        for (long long c = threadIdx.x & 63; c < ldd; c += 64) dst[r * ldd + c] = c < cols ? src[r * lds_ + c] : V(0);
 }
 
 inline int dme_blocks(long long work, long long per, long long most) {
@@ -296,7 +297,7 @@ using DmeSquare = DmeTile<T, SIDE, SIDE, (SIDE == 256 ? 4 : 2), (SIDE == 192 ? 4
 
 // How a product of R x C outputs over `slices` slices of k is cut: tiles of 256, 192, 128 or 64 a side, and into how many pieces
 // of k.  Measured in bf16 (fp32) at 4096^3 and 8192^3: 256 a side, one workgroup to a CU, 1150-1290 (141) TFLOP/s; 192, one to a CU, 960-1010;
-// 128, two to a CU, 910-1110 (138); 64, two to a CU, 600 (128).  Small products are bound by how many CUs have a tile at all, and
+// 128, two to a CU, 910-1110 (138); 64, two to a CU, 600 (105).  Small products are bound by how many CUs have a tile at all, and
 // pieces of k cost a pass over their 32-bit sums.
 struct DmeCut {
     int side, splits;
@@ -307,7 +308,7 @@ inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool
     static const struct {
         int side, per_cu;
         double bf16, f32;
-    } kinds[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6}, {128, 2, 980e6, 138e6}, {64, 2, 600e6, 128e6}};
+    } kinds[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6}, {128, 2, 980e6, 138e6}, {64, 2, 600e6, 105e6}};
     DmeCut best{0, 1, 0.0};
     for (const auto& kind : kinds) {
         const int side = kind.side, per_cu = kind.per_cu;

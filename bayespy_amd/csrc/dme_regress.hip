@@ -955,7 +955,7 @@ struct Plan {
     bool pack_h, pack_w;      // the operand is copied with a pitch of whole 16-byte chunks first
     long long dpad;           // k of the first product in a packed operand
     long long nb;             // rows of a block
-    int side;                 // of the tiles of z: 256, 128, or 16 rows x 128 columns
+    int side;                 // of the tiles of z: 256, 128, 64, or 16 rows x 128 columns
     bool few;                 // the forward pass goes by few_kernel
     long long tile_rows, tile_cols;
     long long tiles;          // pieces that the forward pass leaves of a row
@@ -983,7 +983,8 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     p.dpad = up(D, 16 / p.size);
     p.nb = N < 1 ? 1 : N < ROW_BLOCK ? N : ROW_BLOCK;
     const long long slices = (D * p.size + DME_SLICE - 1) / DME_SLICE;
-    p.side = p.nb <= 16 ? 16 : rows->kind == DENSE || dme_cut(p.nb, K, slices, p.size, false, 4.0).side < 192 ? 128 : 256;
+    const int cut = dme_cut(p.nb, K, slices, p.size, false, 4.0).side;
+    p.side = p.nb <= 16 ? 16 : rows->kind == DENSE ? 128 : cut >= 192 ? 256 : cut;
     p.tile_rows = p.side;
     p.tile_cols = p.side == 16 ? 128 : p.side;
     const long long tiles = (K + p.tile_cols - 1) / p.tile_cols;
@@ -1078,6 +1079,7 @@ int tiles_of_z(const TileArgs& a, int kind, int side, hipStream_t s) {
     if (kind == DENSE) return side == 16 ? launch_dense<T, 16, BACKWARD>(a, s) : launch_dense<T, 128, BACKWARD>(a, s);
     if (side == 256) return launch_tile<T, 256, 256, 4, 2, BACKWARD>(a, s);
     if (side == 128) return launch_tile<T, 128, 128, 2, 2, BACKWARD>(a, s);
+    if (side == 64) return launch_tile<T, 64, 64, 2, 2, BACKWARD>(a, s);
     return launch_tile<T, 16, 128, 1, 4, BACKWARD>(a, s);
 }
 
@@ -1111,6 +1113,19 @@ void join(const float* part, long long ldpart, long long split_stride, int split
                        length, out, (int)(C % 4 == 0));
 }
 
+// dst (rows of `width` bytes) = src (rows of `bytes` bytes, `pitch` apart), zero in what is more
+void pack(const char* src, long long pitch, long long rows, long long bytes, char* dst, long long width, hipStream_t s) {
+    const dim3 grid(dme_blocks(rows, 4, 16384)), block(256);
+    const uintptr_t all = (uintptr_t)src | (uintptr_t)(rows > 1 ? pitch : 0) | (uintptr_t)bytes;  // width: a multiple of 16
+    if (all % 8 == 0)
+        hipLaunchKernelGGL(dme_pack_kernel<u64>, grid, block, 0, s, (const u64*)src, pitch / 8, rows, bytes / 8, (u64*)dst, width / 8);
+    else if (all % 4 == 0)
+        hipLaunchKernelGGL(dme_pack_kernel<u32>, grid, block, 0, s, (const u32*)src, pitch / 4, rows, bytes / 4, (u32*)dst, width / 4);
+    else
+        hipLaunchKernelGGL(dme_pack_kernel<unsigned short>, grid, block, 0, s, (const unsigned short*)src, pitch / 2, rows, bytes / 2,
+                           (unsigned short*)dst, width / 2);
+}
+
 struct Call {
     const void* H;
     long long ldh;
@@ -1134,8 +1149,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
     char* ws = c.ws;
     DmeOperand w{(const char*)c.W, c.ldw * size, c.K};
     if (p.pack_w) {
-        hipLaunchKernelGGL(dme_pack_kernel<T>, dim3(dme_blocks(c.K, 4, 16384)), dim3(256), 0, s, (const T*)c.W, c.ldw, c.K, c.D,
-                           (T*)(ws + p.w), p.dpad);
+        pack((const char*)c.W, c.ldw * size, c.K, c.D * size, ws + p.w, p.dpad * size, s);
         w = DmeOperand{ws + p.w, p.dpad * size, c.K};
     }
     u32* largest = (u32*)(ws + p.largest);
@@ -1147,8 +1161,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             hipLaunchKernelGGL(zero_kernel, dim3(dme_blocks(p.zero_words, 1024, 1024)), dim3(256), 0, s, (u32*)ws, p.zero_words);
         DmeOperand h{(const char*)c.H + n0 * c.ldh * size, c.ldh * size, nb};
         if (p.pack_h) {
-            hipLaunchKernelGGL(dme_pack_kernel<T>, dim3(dme_blocks(nb, 4, 16384)), dim3(256), 0, s, (const T*)h.at, c.ldh, nb, c.D,
-                               (T*)(ws + p.h), p.dpad);
+            pack(h.at, c.ldh * size, nb, c.D * size, ws + p.h, p.dpad * size, s);
             h = DmeOperand{ws + p.h, p.dpad * size, nb};
         }
         TileArgs a{};
