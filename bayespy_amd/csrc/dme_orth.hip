@@ -9,9 +9,10 @@
 // The products run on the fp16 matrix instructions, sums in 32 bits.  A value v, scaled by a power of two, is kept as fp16 pairs
 // hi + lo of 22 bits together; |X| = 1 at the start and singular values stay below 3 (checked), so nothing leaves fp16's range.
 //   fp32 matrices  P Q = Ph Qh + Ph Ql + Pl Qh: what is dropped is 2^-22 of a product, less than 32-bit sums of as many terms round
-//                  off (4.4e-7 of the result with fp32 instructions; see the table of errors), at 2.5 times their rate
-//   bf16 matrices  P Q = Ph Qh; X itself keeps its lo part, so that what fp16 drops of X only passes through b S + c S S, which is
-//                  small where X's singular values are, instead of being amplified by a at every step.
+//                  off, at 2.5 times the rate of the fp32 instructions.  X itself stays in 32 bits beside its pair.
+//   bf16 matrices  P Q = Ph Qh; X itself keeps its lo part.
+// What the operands drop of X then only passes through b S + c S S, which is small where X's singular values are, instead of being
+// amplified by a at every step (fp32, 16 strong directions over weak noise: 1.7e-6 of the result when X was its pair alone).
 // The diagonals of S and of b S + c S S are kept out of the operands and applied in 32 bits: where singular values are alike the diagonal is
 // nearly one number, and its rounding would not average out (50000 x 256 of near-flat spectrum, five steps: 3.7e-3 of the result with
 // the diagonal in fp16, below 1e-3 without).
@@ -83,6 +84,7 @@ __device__ __forceinline__ void split1(half* hi, half* lo, float v) {
 
 struct Matrices {
     half* X[2][2];  // [which of two][hi, lo]: [rows][ldx], read and written in turn
+    float* Xf;      // fp32 matrices: X itself, scaled like its pair
     float* S;       // [m][lds]
     half* Sw[2];    // [hi, lo]: S without its diagonal; lo for fp32 matrices
     half* Bw[2];    // b S + c S S without its diagonal
@@ -94,7 +96,7 @@ struct Matrices {
 };
 
 // X = G / |G|, zero in the padding of its pitch.
-template <class T>
+template <class T, int PARTS>
 __global__ __launch_bounds__(256) void begin_kernel(const T* G, long long sb, long long rs, long long cs, const double* part, Matrices a) {
     __shared__ float tile[64][65];
     __shared__ double sums[4];
@@ -127,6 +129,7 @@ __global__ __launch_bounds__(256) void begin_kernel(const T* G, long long sb, lo
             for (int u = 0; u < 4; ++u)
                 v[u] = c + u < a.cols ? (float)((double)(along ? (float)g[r * rs + (c + u) * cs] : tile[row + q * 16][col + u]) * scale) : 0.f;
             split4(a.X[0][0] + xo + r * a.ldx + c, a.X[0][1] + xo + r * a.ldx + c, v);
+            if (PARTS == 2) *(f32x4*)(a.Xf + xo + r * a.ldx + c) = v;
         }
     }
 }
@@ -322,16 +325,19 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArg
     Tile t;
     // a small tile's own values are on their way while it is made
     constexpr bool EARLY = SIDE == 64;
-    f16x4 early[2][EARLY ? Tile::NI : 1][EARLY ? Tile::NJ : 1];
+    const auto own = [&](long long at) {
+        if (PARTS == 2) return *(const f32x4*)(x.Xf + xo + at);
+        const f16x4 h = *(const f16x4*)(X[0] + xo + at), l = *(const f16x4*)(X[1] + xo + at);
+        return f32x4{(float)h[0] + (float)l[0], (float)h[1] + (float)l[1], (float)h[2] + (float)l[2], (float)h[3] + (float)l[3]};
+    };
+    f32x4 early[EARLY ? Tile::NI : 1][EARLY ? Tile::NJ : 1];
     if constexpr (EARLY) {
 #pragma unroll
         for (int j = 0; j < Tile::NJ; ++j)
 #pragma unroll
             for (int i = 0; i < Tile::NI; ++i) {
                 const long long r = tr * SIDE + Tile::row_of(j), c = tc * SIDE + Tile::col_of(i);
-                const bool in = r < x.rows && c < x.ldx;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) early[u][i][j] = in ? *(const f16x4*)(X[u] + xo + r * x.ldx + c) : f16x4{0, 0, 0, 0};
+                early[i][j] = r < x.rows && c < x.ldx ? own(r * x.ldx + c) : f32x4{0.f, 0.f, 0.f, 0.f};
             }
     }
     if (TALL)
@@ -350,23 +356,21 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArg
             const long long c = tc * SIDE + Tile::col_of(i);
             if (c >= x.ldx) continue;
             const long long at = r * x.ldx + c;
-            f16x4 h, l;
-            if constexpr (EARLY) {
-                h = early[0][i][j];
-                l = early[1][i][j];
-            } else {
-                h = *(const f16x4*)(X[0] + xo + at);
-                l = *(const f16x4*)(X[1] + xo + at);
-            }
+            f32x4 old;
+            if constexpr (EARLY)
+                old = early[i][j];
+            else
+                old = own(at);
             f32x4 v;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const bool in = c + q < x.cols;
                 const float d = TALL ? (in ? a.a + x.Bd[mo + c + q] : 0.f) : dr;
-                v[q] = in ? __builtin_fmaf(d, (float)h[q], __builtin_fmaf(d, (float)l[q], t.acc[i][j][q] * UNIT)) : 0.f;
+                v[q] = in ? __builtin_fmaf(d, old[q], t.acc[i][j][q] * UNIT) : 0.f;
             }
             if (!a.out) {
                 split4(hi + at, lo + at, v);
+                if (PARTS == 2) *(f32x4*)(x.Xf + xo + at) = v;
             } else if (c < x.cols) {  // the result has no padding
                 v *= 1.f / SCALE_X;
                 T* o = a.out + blockIdx.y * a.out_batch + r * x.cols + c;
@@ -537,7 +541,7 @@ struct StepPlan {
     int groups;
     long long m, n, ldx, lds;
     DmeCut square, poly, update;
-    long long norm, X[2][2], S, Sw[2], Bw[2], Sd, Bd, part, bytes;
+    long long norm, X[2][2], Xf, S, Sw[2], Bw[2], Sd, Bd, part, bytes;
 };
 
 StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
@@ -571,6 +575,7 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
         return p;
     }
     for (int i = 0; i < 4; ++i) p.X[i / 2][i % 2] = take(batch * rows * p.ldx * 2);
+    if (parts == 2) p.Xf = take(batch * rows * p.ldx * 4);
     p.S = take(batch * p.m * p.lds * 4);
     for (int i = 0; i < parts; ++i) {
         p.Sw[i] = take(batch * p.m * p.lds * 2);
@@ -659,6 +664,7 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
         x.Sw[i] = (half*)(ws + p.Sw[i]);
         x.Bw[i] = (half*)(ws + p.Bw[i]);
     }
+    x.Xf = (float*)(ws + p.Xf);
     x.S = (float*)(ws + p.S);
     x.Sd = (float*)(ws + p.Sd);
     x.Bd = (float*)(ws + p.Bd);
@@ -711,7 +717,7 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
         return DME_OK;
     }
     const long long tiles = (p.ldx + 63) / 64 * ((rows + 63) / 64);
-    hipLaunchKernelGGL(begin_kernel<T>, dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, part, x);
+    hipLaunchKernelGGL((begin_kernel<T, PARTS>), dim3((unsigned)(tiles < 4096 ? tiles : 4096), (unsigned)batch), dim3(256), 0, s, G, sb, rs, cs, part, x);
     for (int i = 0; i < steps; ++i) {
         k.from = i & 1;
         k.out = i + 1 < steps ? nullptr : out;

@@ -7,7 +7,12 @@
 // Dirichlet likelihood with one z for all rows):
 //     loss = F(l, T) - sum_k F(z_k, x_k)         d loss / d z_k = exp(z_k - l) G(l, T) - G(z_k, x_k)
 //     multinomial  F = x z, G = x;               Dirichlet  F = lgamma(e^z + x) - lgamma(e^z), G = dF/dz
-// so both likelihoods share the pass over the columns; F and G are needed at the counts alone, in 64 bits.
+// so both likelihoods share the pass over the columns; F and G are needed at the counts alone.  With m the row's largest z and
+// s = sum_k e^(z_k - m) the terms are taken relative to m, so that a row whose z are all far out (masks of the type's lowest value)
+// loses nothing:
+//     multinomial  loss = T log s - sum_k x_k (z_k - m)
+//     Dirichlet    F(z, x) = z + R(z, x):  loss = log s + R(l, T) - sum_{x_k > 0} [(z_k - m) + R(z_k, x_k)] + (1 - J) m, J = #{x_k > 0}
+// and e^(z - l) = e^(z - m) / s.
 #include <math.h>
 
 #include <atomic>
@@ -31,13 +36,13 @@ __device__ double stirling_rest(double v) {
     return i * (1.0 / 12.0 - q * (1.0 / 360.0 - q * (1.0 / 1260.0)));
 }
 
-// F of the Dirichlet likelihood: sum_{n < x} log(e^z + n).  The first 16 terms are multiplied out (n = 0 gives z itself,
-// however small e^z), the rest is a difference of two Stirling formulas written without their cancelling parts.
-__device__ __attribute__((noinline)) double dirichlet_f(double z, double x) {
-    if (!(x > 0.0)) return 0.0 * x;
-    if (z > 60.0) return x * z;  // e^z + n is e^z in 64 bits
+// R(z, x) = sum_{1 <= n < x} log(e^z + n) (F without its first term, z itself).  Up to 15 terms are multiplied out, the rest is a difference
+// of two Stirling formulas written without their cancelling parts.
+__device__ __attribute__((noinline)) double dirichlet_rest(double z, double x) {
+    if (!(x > 1.0)) return 0.0 * x;
+    if (z > 60.0) return (x - 1.0) * z;  // e^z + n is e^z in 64 bits
     const double a = exp(z);
-    double r = z, prod = 1.0;
+    double r = 0.0, prod = 1.0;
     const int head = x < 16.0 ? (int)x : 16;
     for (int n = 1; n < head; ++n) {
         prod *= a + n;
@@ -70,10 +75,6 @@ __device__ __attribute__((noinline)) double dirichlet_g(double z, double x) {
     return g;
 }
 
-__device__ __forceinline__ double f_of(int likelihood, double z, double x) {
-    if (likelihood == DME_LIKELIHOOD_DIRICHLET) return dirichlet_f(z, x);
-    return x == 0.0 ? 0.0 : x * z;
-}
 __device__ __forceinline__ double g_of(int likelihood, double z, double x) {
     return likelihood == DME_LIKELIHOOD_DIRICHLET ? dirichlet_g(z, x) : x;
 }
@@ -86,7 +87,7 @@ __device__ __forceinline__ float exp_f32(float z) {
 }
 
 // The counts that most cells of a dense matrix hold: 1 <= x <= 16, and e^z small enough for 32-bit products of the 15 terms
-// (64 + 15)^15 < 2^96.  F = z + log prod_{1 <= n < x} (e^z + n) with one logarithm, G = 1 + e^z sum 1 / (e^z + n) with one
+// (64 + 15)^15 < 2^96.  R = log prod_{1 <= n < x} (e^z + n) with one logarithm, G = 1 + e^z sum 1 / (e^z + n) with one
 // reciprocal of the same product: 15 roundings of 2^-24 at most.  Others take the 64-bit functions above.
 __device__ __forceinline__ bool is_small(float z, int x) { return x <= 16 && z <= 4.1f; }
 // N cells of a lane at once, x = 0 where a cell is none of these: the chains of products are independent of each other, and the loop runs
@@ -99,7 +100,7 @@ __device__ __forceinline__ int most_of(const int (&x)[N]) {
     return most;
 }
 template <int N>
-__device__ __forceinline__ float small_f(const float (&z)[N], const int (&x)[N]) {  // the sum over the cells
+__device__ __forceinline__ float small_rest(const float (&z)[N], const int (&x)[N]) {  // the sum over the cells
     float a[N], prod[N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
@@ -112,8 +113,8 @@ __device__ __forceinline__ float small_f(const float (&z)[N], const int (&x)[N])
         for (int q = 0; q < N; ++q) prod[q] *= n < x[q] ? a[q] + (float)n : 1.f;
     float f = 0.f;
 #pragma unroll
-    for (int q = 0; q < N; ++q) f += x[q] > 0 ? __builtin_fmaf(__builtin_amdgcn_logf(prod[q]), 0.69314718f, z[q]) : 0.f;
-    return f;
+    for (int q = 0; q < N; ++q) f += __builtin_amdgcn_logf(prod[q]);  // of 1 where there is no cell
+    return f * 0.69314718f;
 }
 template <int N>
 __device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], float (&g)[N]) {
@@ -135,10 +136,10 @@ __device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], 
 #pragma unroll
     for (int q = 0; q < N; ++q) g[q] = x[q] > 0 ? __builtin_fmaf(a[q] * num[q], __builtin_amdgcn_rcpf(den[q]), 1.f) : 0.f;
 }
-__device__ __forceinline__ float small_f(float z, int x) {
+__device__ __forceinline__ float small_rest(float z, int x) {
     const float zs[1] = {z};
     const int xs[1] = {x};
-    return small_f(zs, xs);
+    return small_rest(zs, xs);
 }
 __device__ __forceinline__ float small_g(float z, int x) {
     const float zs[1] = {z};
@@ -204,14 +205,15 @@ struct TileArgs {
     long long column;  // first column of the piece
     Rows rows;
     // forward
-    f32x2* part;       // [tile][nb]: largest z log2 e, sum of 2^(z log2 e - that)
-    double* part_f;    // DENSE: [tile][nb]: sum F(z, x)
+    f32x2* part;       // [tile][nb]: largest z, sum of e^(z - that)
+    double* part_f;    // DENSE: [tile][nb]: the counts' sum of the loss, relative to the tile's largest z (0 if that is -inf)
+    double* part_w;    // DENSE: [tile][nb]: how often that z goes into it: sum x (multinomial), number of counts (Dirichlet)
     double* part_t;    // DENSE: [tile][nb]: sum x, NaN where a count is negative
     float* entry_z;    // CSR: [nnz], LABELS: [nb]: z at the counts
     int likelihood;
     // backward
-    const float* lse2;     // [nb]: l * log2 e
-    const float* coef;     // [nb]: weight * G(l, T) * 2^(lse2 - l log2 e)
+    const float* largest_z;  // [nb]: m
+    const float* coef;     // [nb]: weight * G(l, T) / s
     const float* weight;   // [nb]
     void* dz;              // [nb][lddz]
     long long lddz;
@@ -230,6 +232,23 @@ __device__ __forceinline__ f32x4 bias_of(const TileArgs& a, long long k) {
     }
     return b;
 }
+
+// whether one of the wave's columns is out: only then is there anything to choose
+__device__ __forceinline__ bool any_out(f32x4 b) {
+    return __any(b[0] == -INFINITY || b[1] == -INFINITY || b[2] == -INFINITY || b[3] == -INFINITY);
+}
+
+// z = products + bias; a column that is out has z = -inf whatever its weights hold
+__device__ __forceinline__ f32x4 with_bias(f32x4 v, f32x4 b, bool out) {
+    v += b;
+    if (out)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = b[q] == -INFINITY ? -INFINITY : v[q];
+    return v;
+}
+
+// e^(z - m).  The difference is taken first: z log2 e may leave 32 bits where a mask is the type's lowest value.
+__device__ __forceinline__ float exp_of(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * LOG2E); }
 
 __device__ __forceinline__ float dot_step(const u32q& h, const u32q& w, float s, __bf16) {
 #pragma unroll
@@ -283,7 +302,10 @@ __device__ __forceinline__ void entries_of(const TileArgs& a, long long r, int f
 #pragma unroll
         for (int u = 0; u < DEEP; ++u) {
             s[u] = sum16(s[u]);
-            if (sub == 0 && k[u] >= 0) a.entry_z[e0 + u * 4 + group] = s[u] + (a.bias ? a.bias[k[u]] : 0.f);
+            if (sub == 0 && k[u] >= 0) {
+                const float b = a.bias ? a.bias[k[u]] : 0.f;
+                a.entry_z[e0 + u * 4 + group] = b == -INFINITY ? b : s[u] + b;
+            }
         }
     }
 }
@@ -296,7 +318,7 @@ __global__ __launch_bounds__(256) void entry_kernel(TileArgs a) {
 
 __device__ __forceinline__ f32x2 merge(f32x2 v, f32x2 o) {
     const float m = fmaxf(v[0], o[0]), base = m == -INFINITY ? 0.f : m;
-    return f32x2{m, v[1] * __builtin_amdgcn_exp2f(v[0] - base) + o[1] * __builtin_amdgcn_exp2f(o[0] - base)};
+    return f32x2{m, v[1] * exp_of(v[0], base) + o[1] * exp_of(o[0], base)};
 }
 
 // The forward pass for up to 16 rows: a read of the weights and little else.  A wave makes 16 columns for all rows; its weights
@@ -348,14 +370,14 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
         load(y[0], round + 2 * WIDE);
         multiply(y[1], round + WIDE);
     }
-    const f32x4 z = acc[0] + acc[1] + bias_of(a, k0 + g * 4);
+    const f32x4 b = bias_of(a, k0 + g * 4), z = with_bias(acc[0] + acc[1], b, any_out(b));
     float m = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
     m = fmaxf(m, __shfl_xor(m, 16));
-    m = LOG2E * fmaxf(m, __shfl_xor(m, 32));
+    m = fmaxf(m, __shfl_xor(m, 32));
     const float base = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[q], LOG2E, -base));
+    for (int q = 0; q < 4; ++q) s += exp_of(z[q], base);
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
     if (g == 0) seen[wave][c] = f32x2{m, s};
@@ -364,9 +386,8 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
 }
 
 // Tiles of z, reduced where the matrix instructions left them: a lane has NJ rows and 4 NI columns of each.
-//   forward   largest exponent and sum of exponentials of each row: 2^(z log2 e - M) with M = max z log2 e rounded to 32 bits,
-//             the same M that the sum is kept with, so that its rounding costs nothing
-//   backward  2^(z log2 e - l log2 e) coef, rounded to T (the gradient's one rounding before its products), and the columns' sums
+//   forward   the largest z of each row and the sum of e^(z - that)
+//   backward  e^(z - m) coef, rounded to T (the gradient's one rounding before its products), and the columns' sums
 //             of the unrounded values.  The counts are not looked at: patch_kernel puts them in.
 template <class T, int TR, int TC, int WR, int WC, bool BACKWARD>
 __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
@@ -382,8 +403,9 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
 #pragma unroll
     for (int i = 0; i < Tile::NI; ++i) {
         const f32x4 b = bias_of(a, k0 + Tile::col_of(i));
+        const bool out = any_out(b);
 #pragma unroll
-        for (int j = 0; j < Tile::NJ; ++j) t.acc[i][j] += b;
+        for (int j = 0; j < Tile::NJ; ++j) t.acc[i][j] = with_bias(t.acc[i][j], b, out);
     }
     if (!BACKWARD) {
         f32x2* seen = (f32x2*)lds;  // [WC][TR]
@@ -396,13 +418,12 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
                 for (int q = 0; q < 4; ++q) m = fmaxf(m, t.acc[i][j][q]);
             m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
-            m *= LOG2E;
             const float base = m == -INFINITY ? 0.f : m;
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < Tile::NI; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) s += __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][q], LOG2E, -base));
+                for (int q = 0; q < 4; ++q) s += exp_of(t.acc[i][j][q], base);
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
             if (g == 0) seen[wc * TR + wr * Tile::WTR + j * 16 + (tid & 15)] = f32x2{m, s};
@@ -416,11 +437,11 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
         }
         return;
     }
-    float l2[Tile::NJ], cf[Tile::NJ];
+    float m[Tile::NJ], cf[Tile::NJ];
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
         const long long r = r0 + Tile::row_of(j);
-        l2[j] = r < a.nb ? a.lse2[r] : INFINITY;
+        m[j] = r < a.nb ? a.largest_z[r] : INFINITY;
         cf[j] = r < a.nb ? a.coef[r] : 0.f;
     }
     // In 16 bits a wave's part goes through LDS (its own piece of it), so that whole lines of rows are stored: the lanes of a matrix
@@ -436,7 +457,7 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
         for (int j = 0; j < Tile::NJ; ++j) {
             f32x4 d;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) d[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][q], LOG2E, -l2[j])) * cf[j];
+            for (int q = 0; q < 4; ++q) d[q] = exp_of(t.acc[i][j][q], m[j]) * cf[j];
             const long long r = r0 + Tile::row_of(j);
             if (r < a.nb) sum[i] += d;
             if constexpr (TURN)
@@ -533,8 +554,9 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
         for (int i = 0; i < Tile::NI; ++i) {
             const int c = Tile::col_of(i);
             const f32x4 b = bias_of(a, k0 + c);
+            const bool out = any_out(b);
 #pragma unroll
-            for (int j = 0; j < Tile::NJ; ++j) *(f32x4*)(z + Tile::row_of(j) * ZP + c) = t.acc[i][j] + b;
+            for (int j = 0; j < Tile::NJ; ++j) *(f32x4*)(z + Tile::row_of(j) * ZP + c) = with_bias(t.acc[i][j], b, out);
         }
     }
     __syncthreads();
@@ -551,54 +573,55 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
         }
         const Counts x = next;
         if (row + 16 < TR && r + 16 < a.nb) next.load(a.rows, r + 16, k0 + sub * 8, a.K);
-        const f32x4 u = *(const f32x4*)zr, w = *(const f32x4*)(zr + 4);
+        const f32x4 u = *(const f32x4*)zr, u2 = *(const f32x4*)(zr + 4);
         if (!BACKWARD) {
-            const float m = LOG2E * max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))));
+            const float m = max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(u2[0], u2[1]), fmaxf(u2[2], u2[3]))));
             const float base = m == -INFINITY ? 0.f : m;
             float s = 0.f;
             double f = 0.0;
             long long total = 0;
+            int counts = 0;
             bool bad = false;
             float zs[8];
             int xs[8];
             each_count(x, a.rows.elem, [&](int q, int v) {
-                const float zq = q < 4 ? u[q & 3] : w[q & 3];
-                s += __builtin_amdgcn_exp2f(__builtin_fmaf(zq, LOG2E, -base));
+                const float zq = q < 4 ? u[q & 3] : u2[q & 3];
+                s += exp_of(zq, base);
                 bad |= v < 0;
                 total += v;
                 const bool small = v > 0 && is_small(zq, v);
                 zs[q] = small ? zq : 0.f;
                 xs[q] = small ? v : 0;
-                if (!dirichlet) {
-                    if (v > 0) f += (double)v * (double)zq;
-                } else if (v > 0 && !small) {
-                    f += dirichlet_f((double)zq, (double)v);
-                }
+                counts += v > 0;
+                if (v > 0) f += ((double)zq - (double)base) * (dirichlet ? 1.0 : (double)v);
+                if (dirichlet && v > 0 && !small) f += dirichlet_rest((double)zq, (double)v);
             });
-            if (dirichlet) f += (double)small_f(zs, xs);
+            if (dirichlet) f += (double)small_rest(zs, xs);
             s = sum16(s);
             f = sum16(f);
+            const double w = sum16(dirichlet ? (double)counts : (double)total);
             const double t = sum16(bad ? __builtin_nan("") : (double)total);
             if (sub == 0) {
                 a.part[tc * a.nb + r] = f32x2{m, s};
                 a.part_f[tc * a.nb + r] = f;
+                a.part_w[tc * a.nb + r] = w;
                 a.part_t[tc * a.nb + r] = t;
             }
         } else {
-            const float l2 = a.lse2[r], cf = a.coef[r], weight = a.weight[r];
+            const float m = a.largest_z[r], cf = a.coef[r], weight = a.weight[r];
             f32x4 d[2];
             float zs[8], gs[8];
             int xs[8];
             each_count(x, a.rows.elem, [&](int q, int v) {
-                const float zq = q < 4 ? u[q & 3] : w[q & 3];
+                const float zq = q < 4 ? u[q & 3] : u2[q & 3];
                 const bool small = v > 0 && is_small(zq, v);
                 zs[q] = small ? zq : 0.f;
                 xs[q] = small ? v : 0;
             });
             if (dirichlet) small_g(zs, xs, gs);
             each_count(x, a.rows.elem, [&](int q, int v) {
-                const float zq = q < 4 ? u[q & 3] : w[q & 3];
-                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(zq, LOG2E, -l2)) * cf;
+                const float zq = q < 4 ? u[q & 3] : u2[q & 3];
+                float e = exp_of(zq, m) * cf;
                 if (v > 0) e -= weight * (!dirichlet ? (float)v : xs[q] > 0 ? gs[q] : (float)dirichlet_g((double)zq, (double)v));
                 d[q >> 2][q & 3] = e;
             });
@@ -625,12 +648,13 @@ struct RowArgs {
     int tiles, kind, likelihood;
     const f32x2* part;
     const double* part_f;
+    const double* part_w;
     const double* part_t;
     const float* entry_z;
     Rows rows;
     const float* weights;  // [nb] or null
     float* loss;           // [nb]
-    float* lse2;           // [nb] or null: no gradient is wanted
+    float* largest_z;      // [nb] or null: no gradient is wanted
     float* coef;
     float* weight;
     float* entry_g;        // CSR: [nnz], LABELS: [nb]: weight * G(z, x)
@@ -645,32 +669,25 @@ template <int LANES>
 __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     constexpr int ROWS = 256 / LANES;
     __shared__ float m_seen[LANES][ROWS];
-    __shared__ double s_seen[LANES][ROWS], f_seen[LANES][ROWS], t_seen[LANES][ROWS];
+    __shared__ double s_seen[LANES][ROWS], sums[3][4];
     const long long first = (long long)blockIdx.x * ROWS;
     {
         const int row = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
         const long long r = first + row < a.nb ? first + row : a.nb - 1;
         float m = -INFINITY;
-        double s = 0.0, f = 0.0, t = 0.0;
+        double s = 0.0;
         for (int tile = lane; tile < a.tiles; tile += 4 * LANES) {
             f32x2 p[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) p[u] = tile + u * LANES < a.tiles ? a.part[(tile + u * LANES) * a.nb + r] : f32x2{-INFINITY, 0.f};
             const float top = fmaxf(fmaxf(m, fmaxf(p[0][0], p[1][0])), fmaxf(p[2][0], p[3][0])), base = top == -INFINITY ? 0.f : top;
-            s *= (double)__builtin_amdgcn_exp2f(m - base);
+            s *= (double)exp_of(m, base);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s += (double)p[u][1] * (double)__builtin_amdgcn_exp2f(p[u][0] - base);
+            for (int u = 0; u < 4; ++u) s += (double)p[u][1] * (double)exp_of(p[u][0], base);
             m = top;
         }
-        if (a.kind == DENSE)
-            for (int tile = lane; tile < a.tiles; tile += LANES) {
-                f += a.part_f[tile * a.nb + r];
-                t += a.part_t[tile * a.nb + r];
-            }
         m_seen[lane][row] = m;
         s_seen[lane][row] = s;
-        f_seen[lane][row] = f;
-        t_seen[lane][row] = t;
     }
     __syncthreads();
     const int row = threadIdx.x / LANES, sub = threadIdx.x % LANES;
@@ -678,13 +695,11 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     const bool real = r < a.nb;
     const long long rr = real ? r : a.nb - 1;
     float m;
-    double s, f, total;
+    double s;
     if constexpr (LANES == 16) {
         m = max16(m_seen[sub][row]);
         const float base = m == -INFINITY ? 0.f : m;
-        s = sum16(s_seen[sub][row] * (double)__builtin_amdgcn_exp2f(m_seen[sub][row] - base));
-        f = sum16(f_seen[sub][row]);
-        total = sum16(t_seen[sub][row]);
+        s = sum16(s_seen[sub][row] * (double)exp_of(m_seen[sub][row], base));
     } else {  // one row: each wave makes the same sums of all
         const int l = threadIdx.x & 63;
         m = fmaxf(fmaxf(m_seen[l][0], m_seen[l + 64][0]), fmaxf(m_seen[l + 128][0], m_seen[l + 192][0]));
@@ -692,21 +707,27 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
         const float base = m == -INFINITY ? 0.f : m;
-        s = f = total = 0.0;
+        s = 0.0;
 #pragma unroll
-        for (int u = 0; u < 256; u += 64) {
-            s += s_seen[l + u][0] * (double)__builtin_amdgcn_exp2f(m_seen[l + u][0] - base);
-            f += f_seen[l + u][0];
-            total += t_seen[l + u][0];
-        }
+        for (int u = 0; u < 256; u += 64) s += s_seen[l + u][0] * (double)exp_of(m_seen[l + u][0], base);
         s = dme_wave_sum_f64(s);
-        f = dme_wave_sum_f64(f);
-        total = dme_wave_sum_f64(total);
     }
-    const double exact2 = s == 0.0 ? -INFINITY : (double)m + log2(s), lse = exact2 * (1.0 / (double)LOG2E);
+    // the counts: their part of the loss relative to m, their total, and how often m goes into their part
+    const bool dirichlet = a.likelihood == DME_LIKELIHOOD_DIRICHLET;
+    const double top = (double)m, over = log(s);
     const float weight = a.weights ? a.weights[rr] : 1.f;
     float most = 0.f;
-    if (a.kind == CSR) {
+    double f = 0.0, total = 0.0, times = 0.0;
+    if (a.kind == DENSE) {
+        for (int tile = sub; tile < a.tiles; tile += LANES) {
+            const long long at = tile * a.nb + rr;
+            const double w = a.part_w[at];
+            const float mt = a.part[at][0];
+            if (w != 0.0) f += a.part_f[at] + w * ((mt == -INFINITY ? 0.0 : (double)mt) - top);
+            total += a.part_t[at];
+            times += w;
+        }
+    } else if (a.kind == CSR) {
         const long long q0 = a.rows.rowptr[rr], q1 = a.rows.rowptr[rr + 1];
         const long long e0 = row_begin(a.rows, rr), e1 = row_begin(a.rows, rr + 1);
         bool bad = q0 < 0 || q1 < q0 || q1 > a.rows.nnz;
@@ -718,52 +739,67 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
             }
             const float z = a.entry_z[e];
             total += (double)x;
-            const bool small = a.likelihood == DME_LIKELIHOOD_DIRICHLET && x > 0 && is_small(z, x);
-            f += small ? (double)small_f(z, x) : f_of(a.likelihood, (double)z, (double)x);
-            if (a.lse2 && real) {
+            const bool small = dirichlet && x > 0 && is_small(z, x);
+            if (x > 0) {
+                times += dirichlet ? 1.0 : (double)x;
+                f += ((double)z - top) * (dirichlet ? 1.0 : (double)x);
+                if (dirichlet) f += small ? (double)small_rest(z, x) : dirichlet_rest((double)z, (double)x);
+            }
+            if (a.largest_z && real) {
                 const float v = weight * (small ? small_g(z, x) : (float)g_of(a.likelihood, (double)z, (double)x));
                 a.entry_g[e] = v;
                 most = fmaxf(most, fabsf(v));
             }
         }
         if (bad) total = __builtin_nan("");
-        if constexpr (LANES == 16) {
-            f = sum16(f);
-            total = sum16(total);
-        } else {  // through LDS, in the waves' order
-            f = dme_wave_sum_f64(f);
-            total = dme_wave_sum_f64(total);
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) {
-                f_seen[threadIdx.x >> 6][0] = f;
-                t_seen[threadIdx.x >> 6][0] = total;
-            }
-            __syncthreads();
-            f = (f_seen[0][0] + f_seen[1][0]) + (f_seen[2][0] + f_seen[3][0]);
-            total = (t_seen[0][0] + t_seen[1][0]) + (t_seen[2][0] + t_seen[3][0]);
-        }
-    } else if (a.kind == LABELS) {
+    } else if (sub == 0) {  // F(z, 1) = z, G(z, 1) = 1 in both likelihoods
         const long long k = a.rows.labels[rr];
-        total = k < 0 ? 0.0 : k < a.K ? 1.0 : __builtin_nan("");
-        f = k >= 0 && k < a.K ? (double)a.entry_z[rr] : 0.0;  // F(z, 1) = z, G(z, 1) = 1 in both likelihoods
-        if (a.lse2 && real && sub == 0) {
+        const bool in = k >= 0 && k < a.K;
+        total = k < 0 ? 0.0 : in ? 1.0 : __builtin_nan("");
+        f = in ? (double)a.entry_z[rr] - top : 0.0;
+        times = in ? 1.0 : 0.0;
+        if (a.largest_z && real) {
             a.entry_g[r] = weight;
             most = k >= 0 ? fabsf(weight) : 0.f;
         }
     }
-    if (a.lse2 && a.kind != DENSE) {  // one atomic a wave
+    if constexpr (LANES == 16) {
+        f = sum16(f);
+        total = sum16(total);
+        times = sum16(times);
+    } else {  // through LDS, in the waves' order
+        f = dme_wave_sum_f64(f);
+        total = dme_wave_sum_f64(total);
+        times = dme_wave_sum_f64(times);
+        if ((threadIdx.x & 63) == 0) {
+            sums[0][threadIdx.x >> 6] = f;
+            sums[1][threadIdx.x >> 6] = total;
+            sums[2][threadIdx.x >> 6] = times;
+        }
+        __syncthreads();
+        f = (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]);
+        total = (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]);
+        times = (sums[2][0] + sums[2][1]) + (sums[2][2] + sums[2][3]);
+    }
+    if (a.largest_z && a.kind != DENSE) {  // one atomic a wave
         most = max16(most);
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
         if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(a.largest, __builtin_bit_cast(u32, most));
     }
     if (!real || sub != 0) return;
-    a.loss[r] = total == 0.0 ? 0.f : (float)(f_of(a.likelihood, lse, total) - f);
-    if (!a.lse2) return;
-    // what lse2's rounding to 32 bits drops goes into the coefficient
-    const float l2 = total == 0.0 ? INFINITY : (float)exact2;
-    a.lse2[r] = l2;
-    a.coef[r] = total == 0.0 ? 0.f : (float)((double)weight * g_of(a.likelihood, lse, total) * exp2((double)l2 - exact2));
+    const double l = top + over;
+    double loss = total == total ? -f : total;
+    if (dirichlet) {
+        loss += over + dirichlet_rest(l, total);
+        if (times != 1.0) loss += (1.0 - times) * top;
+    } else {
+        loss += total * over;
+    }
+    a.loss[r] = total == 0.0 ? 0.f : (float)loss;
+    if (!a.largest_z) return;
+    a.largest_z[r] = total == 0.0 ? INFINITY : m;
+    a.coef[r] = total == 0.0 ? 0.f : (float)((double)weight * g_of(a.likelihood, l, total) / s);
     a.weight[r] = weight;
 }
 
@@ -772,7 +808,7 @@ struct PatchArgs {
     Rows rows;
     const float* entry_z;
     const float* entry_g;
-    const float* lse2;
+    const float* largest_z;
     const float* coef;
     void* dz;
     long long lddz;
@@ -807,7 +843,7 @@ __global__ __launch_bounds__(512) void patch_kernel(PatchArgs a) {
     const int sub = threadIdx.x % LANES;
     const long long r = (long long)blockIdx.x * (512 / LANES) + threadIdx.x / LANES;
     if (r < a.nb) {
-        const float l2 = a.lse2[r], cf = a.coef[r];
+        const float m = a.largest_z[r], cf = a.coef[r];
         const int shift = add ? fixed_shift(a.largest, a.headroom) : 0;
         const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
         for (long long e = p0 + sub; e < p1; e += LANES) {
@@ -815,7 +851,7 @@ __global__ __launch_bounds__(512) void patch_kernel(PatchArgs a) {
             const long long c = k - a.column;
             if (c < 0 || c >= a.width || k >= a.K) continue;
             const float g = a.entry_g[e];
-            ((T*)a.dz)[r * a.lddz + c] = (T)(__builtin_amdgcn_exp2f(__builtin_fmaf(a.entry_z[e], LOG2E, -l2)) * cf - g);
+            ((T*)a.dz)[r * a.lddz + c] = (T)(exp_of(a.entry_z[e], m) * cf - g);
             if (!add || !__builtin_isfinite(g)) continue;
             const u64 v = (u64)llrint(ldexp((double)g, shift));
             u32 slot = ((u32)k * 2654435761u) >> 21;
@@ -961,11 +997,11 @@ struct Plan {
     long long tiles;          // pieces that the forward pass leaves of a row
     long long chunk;          // columns of a piece of d loss / d z
     DmeCut cut_w, cut_h;
-    bool part_w, part_h;      // the products leave 32-bit pieces
+    bool pieces_w, pieces_h;  // the products leave 32-bit pieces
     long long ldpart;
     int headroom;
     // places in the workspace
-    long long largest, fixed, h, w, part, part_f, part_t, entry_z, entry_g, lse2, coef, weight, dbias, dz, pw, ph, bytes;
+    long long largest, fixed, h, w, part, part_f, part_w, part_t, entry_z, entry_g, largest_z, coef, weight, dbias, dz, pw, ph, bytes;
     long long zero_words;     // from the beginning: the largest entry and the fixed-point sums
 };
 
@@ -1009,6 +1045,7 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         p.entry_z = take(rows->nnz * 4);
     } else if (rows->kind == DENSE) {
         p.part_f = take(p.tiles * p.nb * 8);
+        p.part_w = take(p.tiles * p.nb * 8);
         p.part_t = take(p.tiles * p.nb * 8);
     } else {
         p.entry_z = take(p.nb * 4);
@@ -1016,7 +1053,7 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     if (gradient) {
         if (rows->kind != DENSE) p.entry_g = take((rows->kind == CSR ? rows->nnz : p.nb) * 4);
         for (p.headroom = 1; (rows->kind == CSR ? rows->nnz : N) >> p.headroom; ++p.headroom) {}
-        p.lse2 = take(p.nb * 4);
+        p.largest_z = take(p.nb * 4);
         p.coef = take(p.nb * 4);
         p.weight = take(p.nb * 4);
         p.dbias = take((p.nb + p.tile_rows - 1) / p.tile_rows * K * 4);
@@ -1029,10 +1066,10 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         p.ldpart = up(D, 4);
         p.cut_w = dme_cut(p.chunk < K ? p.chunk : K, D, (p.nb * p.size + DME_SLICE - 1) / DME_SLICE, p.size, true);
         p.cut_h = dme_cut(p.nb, D, (p.chunk * p.size + DME_SLICE - 1) / DME_SLICE, p.size, true);
-        p.part_w = p.cut_w.splits > 1 || N > p.nb;
-        p.part_h = p.cut_h.splits > 1 || pieces > 1;
-        if (p.part_w) p.pw = take((long long)p.cut_w.splits * K * p.ldpart * 4);
-        if (p.part_h) p.ph = take((long long)p.cut_h.splits * p.nb * p.ldpart * 4);
+        p.pieces_w = p.cut_w.splits > 1 || N > p.nb;
+        p.pieces_h = p.cut_h.splits > 1 || pieces > 1;
+        if (p.pieces_w) p.pw = take((long long)p.cut_w.splits * K * p.ldpart * 4);
+        if (p.pieces_h) p.ph = take((long long)p.cut_h.splits * p.nb * p.ldpart * 4);
     }
     p.bytes = at;
     return p;
@@ -1190,6 +1227,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         }
         a.part = (f32x2*)(ws + p.part);
         a.part_f = (double*)(ws + p.part_f);
+        a.part_w = (double*)(ws + p.part_w);
         a.part_t = (double*)(ws + p.part_t);
         a.entry_z = (float*)(ws + p.entry_z);
         int rc = DME_OK;
@@ -1215,13 +1253,14 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         ra.likelihood = c.likelihood;
         ra.part = a.part;
         ra.part_f = a.part_f;
+        ra.part_w = a.part_w;
         ra.part_t = a.part_t;
         ra.entry_z = a.entry_z;
         ra.rows = rows;
         ra.loss = c.loss + n0;
         if (gradient) {
             ra.weights = c.weights ? c.weights + n0 : nullptr;
-            ra.lse2 = (float*)(ws + p.lse2);
+            ra.largest_z = (float*)(ws + p.largest_z);
             ra.coef = (float*)(ws + p.coef);
             ra.weight = (float*)(ws + p.weight);
             ra.entry_g = (float*)(ws + p.entry_g);
@@ -1232,7 +1271,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         else
             hipLaunchKernelGGL(row_kernel<16>, dim3((unsigned)((nb + 15) / 16)), dim3(256), 0, s, ra);
         if (!gradient) continue;
-        a.lse2 = ra.lse2;
+        a.largest_z = ra.largest_z;
         a.coef = ra.coef;
         a.weight = ra.weight;
         a.dz = ws + p.dz;
@@ -1246,7 +1285,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             rc = tiles_of_z<T, true>(a, kind, p.side, s);
             if (rc) return rc;
             if (kind != DENSE) {
-                PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.lse2, ra.coef, a.dz, a.lddz, fixed, largest, p.headroom};
+                PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.largest_z, ra.coef, a.dz, a.lddz, fixed, largest, p.headroom};
                 if (kind == CSR)
                     hipLaunchKernelGGL((patch_kernel<T, CSR, 16>), dim3((unsigned)((nb + 31) / 32)), dim3(512), 0, s, pa);
                 else
@@ -1257,7 +1296,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             m.p = DmeOperand{dz, a.lddz * size, width};
             m.q = DmeOperand{h.at, h.ld, c.D};
             m.k = nb;
-            if (p.part_w) {
+            if (p.pieces_w) {
                 m.part = (float*)(ws + p.pw) + k0 * p.ldpart;
                 m.ldpart = p.ldpart;
                 m.split_stride = c.K * p.ldpart;
@@ -1273,7 +1312,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             m.p = DmeOperand{dz, a.lddz * size, nb};
             m.q = DmeOperand{a.w.at, a.w.ld, c.D};
             m.k = width;
-            if (p.part_h) {
+            if (p.pieces_h) {
                 m.part = (float*)(ws + p.ph);
                 m.ldpart = p.ldpart;
                 m.split_stride = p.nb * p.ldpart;
@@ -1286,13 +1325,13 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             rc = product<T, false>(m, p.cut_h, s);
             if (rc) return rc;
         }
-        if (p.part_h)
+        if (p.pieces_h)
             join<T>((const float*)(ws + p.ph), p.ldpart, p.nb * p.ldpart, p.cut_h.splits, nb, c.D, (T*)c.dH + n0 * c.D, s);
         if (c.dbias)
             hipLaunchKernelGGL(bias_kernel, dim3((unsigned)((c.K + 63) / 64)), dim3(256), 0, s, (const float*)a.dbias, a.tiles_r, c.K,
                                fixed, largest, p.headroom, (int)(n0 > 0), c.dbias);
     }
-    if (gradient && p.part_w)
+    if (gradient && p.pieces_w)
         join<T>((const float*)(ws + p.pw), p.ldpart, c.K * p.ldpart, p.cut_w.splits, c.K, c.D, (T*)c.dW, s);
     DME_HIP_CHECK(hipGetLastError());
     return DME_OK;

@@ -14,22 +14,29 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
+special = pytest.importorskip("scipy.special")
 
 TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
 
 
 def f_of(z, x, likelihood):
+    """lgamma(a + x) - lgamma(a) = lgamma(x) - log B(a, x): scipy takes the beta function where the difference cancels."""
     if likelihood == "multinomial":
         return torch.where(x > 0, x * z, torch.zeros_like(z))
-    a = z.exp()
-    return torch.where(x > 0, torch.lgamma(a + x) - torch.lgamma(a), torch.zeros_like(z))
+    a, n = z.exp().numpy(), np.where(x.numpy() > 0, x.numpy(), 1.0)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        f = torch.from_numpy(special.gammaln(n) - special.betaln(a, n))
+    return torch.where(x > 0, f, torch.zeros_like(z))
 
 
 def g_of(z, x, likelihood):
+    """a (psi(a + x) - psi(a)); from a = e^20 on by psi's series, whose next term is below 1 / (12 a^2)."""
     if likelihood == "multinomial":
         return x
     a = z.exp()
-    return torch.where(x > 0, a * (torch.digamma(a + x) - torch.digamma(a)), torch.zeros_like(z))
+    near = a * (torch.digamma(a + x) - torch.digamma(a))
+    far = a * (torch.log1p(x / a) + x / (2 * a * (a + x)))
+    return torch.where(x > 0, torch.where(z > 20, far, near), torch.zeros_like(z))
 
 
 def oracle(h, w, b, x, g, likelihood, dtype):
@@ -193,3 +200,430 @@ def test_orthogonal_step(shape, dtype, steps):
     want = step_oracle(g, steps)
     off = float(torch.linalg.vector_norm(got.double().cpu() - want))
     assert off <= step_tolerance(want, TYPES[dtype], steps, shape[-2], shape[-1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(256, 640), (640, 256), (193, 1000), (300, 129)])
+def test_orthogonal_step_larger(shape, dtype):
+    """Several tiles a side, split k, the padding of odd pitches; wide and tall."""
+    from bayespy_amd import regression
+    r = np.random.default_rng(5)
+    g = torch.from_numpy(r.standard_normal(shape)).to(TYPES[dtype]).cuda()
+    got, want = regression.orthogonal_step(g), step_oracle(g, 5)
+    off = float(torch.linalg.vector_norm(got.double().cpu() - want))
+    assert off <= step_tolerance(want, TYPES[dtype], 5, *shape)
+
+
+def test_orthogonal_step_precision():
+    """Rounded once from 64 bits bf16 is off by 2^-8 / sqrt(3) / 1.4 of the norm (a uniform rounding error, values spread over a
+    power of two); the products in fp16 may add as much again.  fp32: no further off than the same steps in 32-bit arithmetic are, which is
+    what weak directions beside strong ones make of roundings of 2^-24 (1.7e-6 of the norm here)."""
+    from bayespy_amd import regression
+    r = np.random.default_rng(8)
+    left, right = r.standard_normal((2000, 16)) * np.arange(1, 17) ** -1.0, r.standard_normal((16, 130))
+    g = torch.from_numpy(left @ right + 0.1 * r.standard_normal((2000, 130))).float().cuda()
+    want = step_oracle(g, 5)
+    off = torch.linalg.vector_norm(regression.orthogonal_step(g).double().cpu() - want) / torch.linalg.vector_norm(want)
+    a, b, c = COEFFICIENTS
+    y = g.cpu() / torch.linalg.vector_norm(g.cpu().double()).float()
+    for _ in range(5):
+        t = y.t() @ y
+        y = a * y + y @ (b * t + c * (t @ t))
+    assert float(off) <= float(torch.linalg.vector_norm(y.double() - want) / torch.linalg.vector_norm(want))
+    h = g.bfloat16()
+    want = step_oracle(h, 5)
+    off = torch.linalg.vector_norm(regression.orthogonal_step(h).double().cpu() - want) / torch.linalg.vector_norm(want)
+    assert float(off) < 2 * 2.0**-8 / 3**0.5 / 1.4
+
+
+def test_orthogonal_step_strides_zero_and_scale():
+    from bayespy_amd import regression
+    r = np.random.default_rng(2)
+    whole = torch.from_numpy(r.standard_normal((6, 90, 200))).float().cuda()
+    for view in (whole[:, 3:70, 5:140], whole[:, 3:70, 5:140].transpose(1, 2), whole[::2, ::3, ::2], whole[1:2].expand(3, 90, 200),
+                 whole[0].t(), whole[0, :33, ::3], whole[0, ::3, :33].t()):
+        want = step_oracle(view, 5)
+        off = float(torch.linalg.vector_norm(regression.orthogonal_step(view).double().cpu() - want))
+        assert off <= step_tolerance(want, torch.float32, 5, view.shape[-2], view.shape[-1])
+    for dtype in (torch.float32, torch.bfloat16):
+        zero = torch.zeros(70, 130, dtype=dtype, device="cuda")
+        assert not bool(regression.orthogonal_step(zero).any())
+        # |G| beyond the range of its squares, powers of two: the same result to the bit
+        g = whole[0].to(dtype)
+        one = regression.orthogonal_step(g)
+        for scale in (2.0**100, 2.0**-100):
+            assert torch.equal(regression.orthogonal_step(g * scale), one)
+        pair = torch.stack([g, zero[:1, :1].expand_as(g)])
+        got = regression.orthogonal_step(pair)
+        assert torch.equal(got[0], one) and not bool(got[1].any())
+        g = g.clone()
+        g[3, 4] = float("nan")
+        assert bool(torch.isnan(regression.orthogonal_step(g)).all())
+    assert regression.orthogonal_step(torch.zeros(0, 5, 7, device="cuda")).shape == (0, 5, 7)
+    narrow = regression.orthogonal_step(whole[0], steps=3, coefficients=(1.5, -0.5, 0.0))  # the cubic iteration
+    want = step_oracle(whole[0], 3, (1.5, -0.5, 0.0))
+    assert float(torch.linalg.vector_norm(narrow.double().cpu() - want)) <= step_tolerance(want, torch.float32, 3, 90, 200)
+
+
+# ---- masks, empty rows, formats ----------------------------------------------------------------------------------
+
+def test_columns_taken_out():
+    """bias = -inf: probability 0, no gradient, whatever the weights hold; a count there costs +inf."""
+    from bayespy_amd import regression
+    for n, k, d in ((5, 300, 24), (40, 300, 24)):
+        h, w, b, x, g = make(n, k, d, torch.float32, 11)
+        out = torch.zeros(k, dtype=torch.bool)
+        out[[0, 7, 129, 255, 299]] = True
+        x[:, out] = 0
+        keep = ~out
+        b = b.clone()
+        b[out.cuda()] = -float("inf")
+        for likelihood in ("multinomial", "dirichlet"):
+            want = oracle(h, w[keep.cuda()], b[keep.cuda()], x[:, keep], g, likelihood, torch.float32)
+            for kind in ("csr", "dense32"):
+                loss, dh, dw, db = regression.log_loss_gradient(h, w, as_rows(x, kind), bias=b, likelihood=likelihood, row_weights=g)
+                near(loss, want["loss"], "loss")
+                near(dh, want["dh"], "dfeatures")
+                near(dw[keep.cuda()], want["dw"], "dweights")
+                near(db[keep.cuda()], want["db"], "dbias")
+                assert not bool(dw[out.cuda()].any()) and not bool(db[out.cuda()].any())
+                broken = w.clone()
+                broken[7], broken[299] = float("nan"), float("inf")
+                near(regression.log_loss(h, broken, as_rows(x, kind), bias=b, likelihood=likelihood), want["loss"], "NaN in weights that are out")
+        y = x.clone()
+        y[1, 7] = 2
+        for kind in ("csr", "dense32"):
+            loss = regression.log_loss(h, w, as_rows(y, kind), bias=b)
+            assert loss[1] == float("inf") and bool(torch.isfinite(loss[[0, 2, 3, 4]]).all())
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_masks_of_the_lowest_value(n):
+    """All columns at the type's lowest value are all alike: the loss is T log K; one spared column takes everything."""
+    from bayespy_amd import regression
+    k, d = 500, 16
+    h, w, _, x, _ = make(n, k, d, torch.bfloat16, 3)
+    low = torch.full((k,), torch.finfo(torch.float32).min, device="cuda")
+    y = torch.arange(n, device="cuda") % k
+    loss = regression.log_loss(h, w, regression.CountRows.from_labels(y, k), bias=low)
+    assert bool(((loss - np.log(k)).abs() <= 2.0**-20).all())  # log, exp and one rounding of a value near 6
+    for kind in ("csr", "dense32"):  # every likelihood and form of rows; the gradient's p is 1 / K
+        one = torch.zeros(n, k, dtype=torch.int32)
+        one[torch.arange(n), y.cpu()] = 1
+        for likelihood in ("multinomial", "dirichlet"):
+            loss, _, _, db = regression.log_loss_gradient(h, w, as_rows(one, kind), bias=low, likelihood=likelihood)
+            assert bool(((loss - np.log(k)).abs() <= 2.0**-20).all())
+            assert bool(((db.cpu() - (n / k - one.sum(0))).abs() <= n * 2.0**-22).all())
+    low[9] = 0.0
+    y[:] = 9
+    loss = regression.log_loss(h, w, regression.CountRows.from_labels(y, k), bias=low)
+    # l = z_9, which is summed twice in two orders: once among the row's columns, once for the label; each is off by d 2^-24 sum |h w| at most
+    assert bool((loss.abs() <= 2 * d * 2.0**-24 * float((h.double().abs() @ w[9].double().abs()).max())).all())
+
+
+def test_rows_without_counts_and_no_rows():
+    from bayespy_amd import regression
+    k, d = 200, 40
+    for n in (4, 50):
+        h, w, b, x, g = make(n, k, d, torch.float32, 1)
+        x[:] = 0
+        labels = torch.full((n,), -1, device="cuda")
+        for rows in (as_rows(x, "csr"), as_rows(x, "dense16"), regression.CountRows.from_labels(labels, k)):
+            h2 = h.clone()
+            loss, dh, dw, db = regression.log_loss_gradient(h2, w, rows, bias=b, row_weights=g, likelihood="dirichlet")
+            for t in (loss, dh, dw, db):
+                assert not bool(t.any())
+    for dtype in (torch.float32, torch.bfloat16):
+        for rows in (regression.CountRows.from_labels(torch.zeros(0, dtype=torch.int64, device="cuda"), 7),
+                     regression.CountRows.from_dense(torch.zeros(0, 7, dtype=torch.int32, device="cuda")),
+                     regression.CountRows.from_csr(torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda"),
+                                                   torch.zeros(0, dtype=torch.int32, device="cuda"), 7)):
+            h, w = torch.zeros(0, 3, dtype=dtype, device="cuda"), torch.ones(7, 3, dtype=dtype, device="cuda")
+            loss, dh, dw, db = regression.log_loss_gradient(h, w, rows.check(), bias=torch.zeros(7, device="cuda"))
+            assert loss.shape == (0,) and dh.shape == (0, 3) and not bool(dw.any()) and not bool(db.any())
+            assert regression.log_loss(h, w, rows).shape == (0,)
+
+
+def test_rows_that_break_their_format():
+    """check() names it; the loss of such a row is NaN, other rows keep theirs, and nothing out of range is followed."""
+    from bayespy_amd import regression
+    k, d = 300, 8
+    for n in (6, 40):
+        h, w, b, x, _ = make(n, k, d, torch.float32, 4)
+        x[n // 2, 5] = 1
+        good = as_rows(x, "csr")
+        want = regression.log_loss(h, w, good, bias=b, likelihood="dirichlet")
+        rowptr, col, val = good._tensors
+        first = int(rowptr[1])
+        breaks = {"ascend strictly": lambda p, c, v: c.__setitem__(first + 1, int(c[first])), "out of range": lambda p, c, v: c.__setitem__(first, k),
+                  "column is out": lambda p, c, v: c.__setitem__(first, -3), "negative": lambda p, c, v: v.__setitem__(first, -1)}
+        for text, change in breaks.items():
+            p, c, v = rowptr.clone(), col.clone(), val.clone()
+            change(p, c, v)
+            rows = regression.CountRows.from_csr(p, c, v, k)
+            with pytest.raises(ValueError):
+                rows.check()
+            loss = regression.log_loss(h, w, rows, bias=b, likelihood="dirichlet")
+            other = [i for i in range(n) if i != 1]
+            assert bool(torch.isnan(loss[1])) and torch.equal(loss[other], want[other])
+            loss, dh, dw, db = regression.log_loss_gradient(h, w, rows, bias=b, likelihood="dirichlet")
+            assert bool(torch.isnan(dh[1]).all()) and bool(torch.isnan(dw).all()) and bool(torch.isnan(db).all()) and bool(torch.isfinite(dh[other]).all())
+        for i, value in ((1, 1 << 40), (1, -5), (2, 0)):
+            p = rowptr.clone()
+            p[i] = value
+            rows = regression.CountRows.from_csr(p, col, val, k)
+            with pytest.raises(ValueError, match="rowptr"):
+                rows.check()
+            assert bool(torch.isnan(regression.log_loss(h, w, rows, bias=b)[i - 1 if value != 0 else 1]))
+        y = torch.zeros(n, dtype=torch.int64, device="cuda")
+        y[1], y[2] = k, 1 << 50
+        rows = regression.CountRows.from_labels(y, k)
+        with pytest.raises(ValueError, match="below K"):
+            rows.check()
+        loss = regression.log_loss_gradient(h, w, rows, bias=b)[0]
+        assert torch.isnan(loss).tolist() == [i in (1, 2) for i in range(n)]
+        z = x.clone()
+        z[1, 3] = -1
+        rows = as_rows(z, "dense32")
+        with pytest.raises(ValueError, match="negative"):
+            rows.check()
+        assert torch.isnan(regression.log_loss(h, w, rows, bias=b)).tolist() == [i == 1 for i in range(n)]
+
+
+@pytest.mark.parametrize("likelihood", ["multinomial", "dirichlet"])
+@pytest.mark.parametrize("kind", ["csr", "dense32"])
+def test_large_counts_and_far_values(kind, likelihood):
+    """Counts to 2^30, z from -80 to 80: where 32-bit lgamma and exp would leave their range."""
+    from bayespy_amd import regression
+    n, k, d = 20, 150, 16
+    h, w, b, x, g = make(n, k, d, torch.float32, 21)
+    r = np.random.default_rng(0)
+    b = torch.from_numpy(r.uniform(-80, 80, size=k)).float().cuda()
+    b[:20] = torch.linspace(-8, 8, 20)
+    big = torch.from_numpy(np.floor(2.0 ** r.uniform(0, 30, size=(n, k))).astype(np.int32))
+    x = torch.where(torch.from_numpy(r.random((n, k)) < 0.1), big, x)
+    x[:3] = 0
+    x[0, 4], x[1, 120], x[2, 10] = 17, 16, 1 << 30
+    want = oracle(h, w, b, x, g, likelihood, torch.float32)
+    loss, dh, dw, db = regression.log_loss_gradient(h, w, as_rows(x, kind), bias=b, likelihood=likelihood, row_weights=g)
+    near(loss, want["loss"], "loss")
+    near(dh, want["dh"], "dfeatures")
+    near(dw, want["dw"], "dweights")
+    near(db, want["db"], "dbias")
+
+
+# ---- layout --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [7, 90])
+def test_pitches_and_alignment(n, dtype):
+    from bayespy_amd import regression
+    k, d = 333, 56
+    h, w, b, x, g = make(n, k, d, TYPES[dtype], 9)
+    plain = regression.log_loss_gradient(h, w, as_rows(x, "dense16"), bias=b, row_weights=g)
+    for shift in (1, 2, 8):
+        big_h = torch.full((n, d + 19), float("nan"), dtype=h.dtype, device="cuda")
+        big_w = torch.full((k, d + 24), float("nan"), dtype=h.dtype, device="cuda")
+        big_x = torch.full((n, k + 13), 9, dtype=torch.int32, device="cuda").to(torch.uint16)
+        hh, ww, xx = big_h[:, shift:shift + d], big_w[:, shift:shift + d], big_x[:, shift:shift + k]
+        hh.copy_(h), ww.copy_(w), xx.copy_(x.to(torch.uint16))
+        bb = torch.empty(k + 1, device="cuda")[1:]
+        bb.copy_(b)
+        got = regression.log_loss_gradient(hh, ww, regression.CountRows.from_dense(xx), bias=bb, row_weights=g)
+        for a, c in zip(plain, got):  # the same sums in the same order, whatever the layout
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("d", [2500, 5000])
+def test_few_rows_of_many_features(d):
+    """Rows too long for LDS take tiles."""
+    from bayespy_amd import regression
+    for dtype in ("bf16", "f32"):
+        h, w, b, x, g = make(3, 200, d, TYPES[dtype], 2)
+        want = oracle(h, w, b, x, g, "multinomial", TYPES[dtype])
+        near(regression.log_loss(h, w, as_rows(x, "csr"), bias=b), want["loss"], "loss")
+
+
+def test_more_rows_than_a_block():
+    from bayespy_amd import regression
+    n, k, d = 16384 + 37, 140, 8
+    h, w, b, x, g = make(n, k, d, torch.float32, 6, density=0.05)
+    want = oracle(h, w, b, x, g, "dirichlet", torch.float32)
+    for kind in ("csr", "dense16"):
+        loss, dh, dw, db = regression.log_loss_gradient(h, w, as_rows(x, kind), bias=b, likelihood="dirichlet", row_weights=g)
+        near(loss, want["loss"], "loss")
+        near(dh, want["dh"], "dfeatures")
+        near(dw, want["dw"], "dweights")
+        near(db, want["db"], "dbias")
+
+
+def test_more_columns_than_a_piece():
+    """d loss / d z of 1500 x 60000 in fp32 is 360 MB: two pieces."""
+    from bayespy_amd import regression
+    n, k, d = 1500, 60000, 8
+    h, w, b, _, g = make(n, 16, d, torch.float32, 6)
+    r = np.random.default_rng(1)
+    w = torch.from_numpy(r.standard_normal((k, d)) * 0.2).float().cuda()
+    b = torch.from_numpy(r.standard_normal(k)).float().cuda()
+    y = torch.from_numpy(r.integers(0, k, size=n))
+    x = torch.zeros(n, k, dtype=torch.int32)
+    x[torch.arange(n), y] = 1
+    want = oracle(h, w, b, x, g, "multinomial", torch.float32)
+    loss, dh, dw, db = regression.log_loss_gradient(h, w, regression.CountRows.from_labels(y.cuda(), k), bias=b, row_weights=g)
+    near(loss, want["loss"], "loss")
+    near(dh, want["dh"], "dfeatures")
+    near(dw, want["dw"], "dweights")
+    near(db, want["db"], "dbias")
+
+
+@pytest.mark.parametrize("n", [2, 130])
+def test_weights_beyond_32_bit_offsets(n):
+    """2^31 + values: zero but for the last columns."""
+    from bayespy_amd import regression
+    d = 1024
+    k = (1 << 31) // d + 1000
+    w = torch.zeros(k, d, dtype=torch.bfloat16, device="cuda")
+    w[-3:] = 0.125
+    h = torch.ones(n, d, dtype=torch.bfloat16, device="cuda") * 0.0625
+    y = torch.full((n,), k - 2, device="cuda")
+    loss, dh, dw, _ = regression.log_loss_gradient(h, w, regression.CountRows.from_labels(y, k))
+    z = 0.125 * 0.0625 * d
+    mass = (k - 3) + 3 * np.exp(z)
+    # l and z in 32 bits: a few roundings of 2^-24 of values up to 15
+    assert bool(((loss - (np.log(mass) - z)).abs() <= 2.0**-19).all())
+    u = 2.0**-8
+    p = np.exp(z) / mass
+    assert float((dw[-2].double() - n * (p - 1) * 0.0625).abs().max()) <= 3 * u * n * 0.0625
+    assert float((dw[-1].double() - n * p * 0.0625).abs().max()) <= 3 * u * n * p * 0.0625
+    assert float((dw[0].double() - n / mass * 0.0625).abs().max()) <= 3 * u * n / mass * 0.0625
+    assert float((dh.double() - 0.125 * (3 * p - 1)).abs().max()) <= 3 * u * 0.125 * (1 + 3 * p)
+
+
+# ---- how they are run ------------------------------------------------------------------------------------------------
+
+def _call_all(h, w, b, x, g, kind, likelihood):
+    from bayespy_amd import regression
+    loss, dh, dw, db = regression.log_loss_gradient(h, w, as_rows(x, kind), bias=b, likelihood=likelihood, row_weights=g)
+    return [regression.log_loss(h, w, as_rows(x, kind), bias=b, likelihood=likelihood), loss, dh, dw, db, regression.orthogonal_step(dw)]
+
+
+@pytest.mark.parametrize("kind", ["csr", "dense32"])
+def test_same_bits_every_time_and_on_any_stream(kind):
+    h, w, b, x, g = make(300, 700, 72, torch.bfloat16, 13)
+    want = _call_all(h, w, b, x, g, kind, "dirichlet")
+    side = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for s in side * 3:  # calls that overlap
+        with torch.cuda.stream(s):
+            got.append(_call_all(h, w, b, x, g, kind, "dirichlet"))
+    torch.cuda.synchronize()
+    for one in got:
+        for a, c in zip(want, one):
+            assert torch.equal(a, c)
+
+
+def test_captured_and_replayed():
+    """Two graphs, replayed in turn with eager calls between: each replay gives the eager bits for the inputs of the time."""
+    from bayespy_amd import regression
+    cases = []
+    for n, k, d in ((200, 500, 64), (6, 900, 32)):
+        h, w, b, x, g = make(n, k, d, torch.float32, n)
+        rows = as_rows(x, "csr")
+        run = lambda h=h, w=w, b=b, rows=rows, g=g: (lambda r: list(r) + [regression.orthogonal_step(r[2])])(  # noqa: E731
+            regression.log_loss_gradient(h, w, rows, bias=b, likelihood="dirichlet", row_weights=g))
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        cases.append((graph, out, run, h))
+    for turn in range(4):
+        for graph, out, run, h in cases:
+            h.mul_(1.125)
+            graph.replay()
+            kept = [t.clone() for t in out]
+            want = run()
+            torch.cuda.synchronize()
+            for a, c in zip(want, kept):
+                assert torch.equal(a, c)
+
+
+def test_gradient_against_differences():
+    """Central differences of the loss in 64 bits (its definition, which the tests above hold the kernels to) against the kernels' fp32
+    gradient: step e = 1e-4, truncation e^2 / 6 of the third derivative (below 1e-6 here) and fp32's 2^-24 of sums near 100."""
+    from bayespy_amd import regression
+    n, k, d = 12, 60, 5
+    h, w, b, x, g = make(n, k, d, torch.float32, 17)
+    for likelihood in ("multinomial", "dirichlet"):
+        _, dh, dw, db = regression.log_loss_gradient(h, w, as_rows(x, "csr"), bias=b, likelihood=likelihood, row_weights=g)
+
+        def total(h, w, b):
+            return float((oracle(h, w, b, x, torch.ones(n), likelihood, torch.float32)["loss"][0] * g.double().cpu()).sum())
+        at = [h.double().cpu(), w.double().cpu(), b.double().cpu()]
+        for i, (grad, where) in enumerate(((dh, (2, 3)), (dw, (10, 1)), (dw, (59, 4)), (db, (0,)), (db, (33,)))):
+            which = 0 if grad is dh else 1 if grad is dw else 2
+            ends = []
+            for sign in (1, -1):
+                moved = [t.clone() for t in at]
+                moved[which][where] += sign * 1e-4
+                ends.append(total(*moved))
+            assert abs((ends[0] - ends[1]) / 2e-4 - float(grad[where])) < 1e-4
+
+
+def test_bias_alone_is_the_prior_s_likelihood():
+    """weights = 0, bias = log(alphas): the loss summed over rows is the total loss that the estimator minimises."""
+    from bayespy_amd import dirichletMultinomialEstimation as DME
+    from bayespy_amd import regression
+    r = np.random.default_rng(4)
+    k = 30
+    x = r.poisson(1.5, size=(400, k)).astype(np.int32)
+    data = DME.CompressedRowData(k)
+    data.appendMatrix(x)
+    priors = DME.findDirichletPriors(data, [1.0] * k, 50)
+    want = DME.getTotalLoss(priors, data)
+    h, w = torch.ones(400, 8, device="cuda"), torch.zeros(k, 8, device="cuda")
+    b = torch.log(torch.tensor(priors, dtype=torch.float64)).float().cuda()
+    rows = regression.CountRows.from_dense(torch.from_numpy(x).cuda())
+    loss, _, _, db = regression.log_loss_gradient(h, w, rows, bias=b, likelihood="dirichlet")
+    # each alpha is off by the 2^-24 |log alpha| of its bias's rounding, a loss by 2^-20 of its terms
+    assert abs(float(loss.double().sum()) - want) <= 2.0**-20 * abs(want)
+    # at the maximum the gradient vanishes: what is left is the solver's stop (|g|^2 < 2^-10, here times alpha) and the sums' rounding
+    assert float(db.abs().max()) <= 2.0**-5 * max(priors) + 2.0**-20 * float(x.sum())
+
+
+def test_a_run_of_them():
+    """A few steps of a decoder as a user takes them: loss, gradient, orthogonalised step, weights; every step against the same in 64 bits."""
+    from bayespy_amd import regression
+    n, k, d = 200, 400, 32
+    h, w, b, x, g = make(n, k, d, torch.float32, 30)
+    rows = as_rows(x, "csr").check()
+    for _ in range(3):
+        want = oracle(h, w, b, x, g, "dirichlet", torch.float32)
+        loss, dh, dw, db = regression.log_loss_gradient(h, w, rows, bias=b, likelihood="dirichlet", row_weights=g)
+        near(loss, want["loss"], "loss")
+        near(dw, want["dw"], "dweights")
+        step = regression.orthogonal_step(dw)
+        exact = step_oracle(dw, 5)
+        assert float(torch.linalg.vector_norm(step.double().cpu() - exact)) <= step_tolerance(exact, torch.float32, 5, k, d)
+        w = w - 0.02 * step
+        b = b - 1e-4 * db
+
+
+def test_refusals():
+    from bayespy_amd import regression as R
+    h, w = torch.zeros(4, 8, device="cuda"), torch.zeros(9, 8, device="cuda")
+    rows = R.CountRows.from_labels(torch.zeros(4, dtype=torch.int64, device="cuda"), 9)
+    for bad in (lambda: R.log_loss(h.half(), w.half(), rows), lambda: R.log_loss(h, w.bfloat16(), rows), lambda: R.log_loss(h[:3], w, rows),
+                lambda: R.log_loss(h, w[:8], rows), lambda: R.log_loss(h[:, :7], w, rows), lambda: R.log_loss(h, w, rows, likelihood="poisson"),
+                lambda: R.log_loss(h, w, "rows"), lambda: R.log_loss(h, w, rows, bias=torch.zeros(8, device="cuda")),
+                lambda: R.log_loss(h, w, rows, bias=torch.zeros(9)), lambda: R.log_loss(h.cpu(), w, rows), lambda: R.log_loss(h[:1].expand(4, 8), w, rows),
+                lambda: R.log_loss(torch.zeros(8, 4, device="cuda").t(), w, rows), lambda: R.log_loss_gradient(h, w, rows, row_weights=torch.zeros(3, device="cuda")),
+                lambda: R.log_loss_gradient(h, w, rows, row_weights=torch.zeros(4, dtype=torch.float64, device="cuda")),
+                lambda: R.CountRows.from_dense(torch.zeros(4, 9, device="cuda")), lambda: R.CountRows.from_dense(torch.zeros(9, 4, dtype=torch.int32, device="cuda").t()),
+                lambda: R.orthogonal_step(h.half()), lambda: R.orthogonal_step(h[0]), lambda: R.orthogonal_step(h, steps=0), lambda: R.orthogonal_step(h[:0]),
+                lambda: R.orthogonal_step(h, coefficients=(9.0, 0.0, 0.0)), lambda: R.orthogonal_step(h, coefficients=(float("nan"), 0.0, 0.0))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        R.orthogonal_step(h.cpu())
