@@ -221,8 +221,8 @@ struct TileArgs {
 };
 
 // bias of four columns; columns from K on get -inf, which leaves them out of every sum
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
 __device__ __forceinline__ f32x4 bias_of(const TileArgs& a, long long k) {
-    typedef f32x4 f32x4_u __attribute__((aligned(4)));
     f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
     if (k + 4 <= a.K) {
         if (a.bias) b = *(const f32x4_u*)(a.bias + k);
@@ -249,6 +249,18 @@ __device__ __forceinline__ f32x4 with_bias(f32x4 v, f32x4 b, bool out) {
 
 // e^(z - m).  The difference is taken first: z log2 e may leave 32 bits where a mask is the type's lowest value.
 __device__ __forceinline__ float exp_of(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * LOG2E); }
+
+// The same for many z of one m, one operation less: 2^(z log2 e - r) e^rest with r = m log2 e rounded to 32 bits and what that drops.
+// Not for |m| > FAR, where r's rounding is no small number.
+constexpr float FAR = 1e30f;
+struct Reference {
+    float r, rest;
+    __device__ __forceinline__ explicit Reference(float m) {
+        r = m * LOG2E;
+        rest = fabsf(m) <= FAR ? __builtin_amdgcn_exp2f(-__builtin_fmaf(m, LOG2E, -r)) : 1.f;
+    }
+    __device__ __forceinline__ float operator()(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, LOG2E, -r)); }
+};
 
 __device__ __forceinline__ float dot_step(const u32q& h, const u32q& w, float s, __bf16) {
 #pragma unroll
@@ -400,12 +412,26 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
     t.clear();
     t.run(a.h, a.w, a.D, lds, r0, c0, 0, a.slices);
     const int tid = threadIdx.x, g = (tid & 63) >> 4, wc = (tid >> 6) % WC, wr = (tid >> 6) / WC;
+    bool out = false;
+    if (a.bias || k0 + TC > a.K) {
+        const bool inside = k0 + TC <= a.K;  // then no lane looks at its columns
 #pragma unroll
-    for (int i = 0; i < Tile::NI; ++i) {
-        const f32x4 b = bias_of(a, k0 + Tile::col_of(i));
-        const bool out = any_out(b);
+        for (int i = 0; i < Tile::NI; ++i) {
+            const f32x4 b = inside ? *(const f32x4_u*)(a.bias + k0 + Tile::col_of(i)) : bias_of(a, k0 + Tile::col_of(i));
+            out |= b[0] == -INFINITY || b[1] == -INFINITY || b[2] == -INFINITY || b[3] == -INFINITY;
 #pragma unroll
-        for (int j = 0; j < Tile::NJ; ++j) t.acc[i][j] = with_bias(t.acc[i][j], b, out);
+            for (int j = 0; j < Tile::NJ; ++j) t.acc[i][j] += b;
+        }
+    }
+    if (__any(out)) {  // rare: the bias is read again
+#pragma unroll
+        for (int i = 0; i < Tile::NI; ++i) {
+            const f32x4 b = bias_of(a, k0 + Tile::col_of(i));
+#pragma unroll
+            for (int j = 0; j < Tile::NJ; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) t.acc[i][j][q] = b[q] == -INFINITY ? -INFINITY : t.acc[i][j][q];
+        }
     }
     if (!BACKWARD) {
         f32x2* seen = (f32x2*)lds;  // [WC][TR]
@@ -420,10 +446,19 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
             m = fmaxf(m, __shfl_xor(m, 32));
             const float base = m == -INFINITY ? 0.f : m;
             float s = 0.f;
+            if (!__any(fabsf(base) > FAR)) {
+                const Reference e(base);
 #pragma unroll
-            for (int i = 0; i < Tile::NI; ++i)
+                for (int i = 0; i < Tile::NI; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) s += exp_of(t.acc[i][j][q], base);
+                    for (int q = 0; q < 4; ++q) s += e(t.acc[i][j][q]);
+                s *= e.rest;
+            } else {
+#pragma unroll
+                for (int i = 0; i < Tile::NI; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) s += exp_of(t.acc[i][j][q], base);
+            }
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
             if (g == 0) seen[wc * TR + wr * Tile::WTR + j * 16 + (tid & 15)] = f32x2{m, s};
@@ -438,11 +473,13 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
         return;
     }
     float m[Tile::NJ], cf[Tile::NJ];
+    bool far = false;
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
         const long long r = r0 + Tile::row_of(j);
         m[j] = r < a.nb ? a.largest_z[r] : INFINITY;
         cf[j] = r < a.nb ? a.coef[r] : 0.f;
+        far |= fabsf(m[j]) > FAR && fabsf(m[j]) < INFINITY;
     }
     // In 16 bits a wave's part goes through LDS (its own piece of it), so that whole lines of rows are stored: the lanes of a matrix
     // instruction hold 8 bytes each of 16 rows, and such stores took 27 us for a round of tiles where the memory needs 7.
@@ -450,21 +487,35 @@ __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
     constexpr int PITCH = Tile::WTC * (int)sizeof(T) + 16;
     char* mine = lds + (tid >> 6) * Tile::WTR * PITCH;
     f32x4 sum[Tile::NI];
+    const auto each = [&](auto exp_j) {  // exp_j(j, z): e^(z - m[j])
 #pragma unroll
-    for (int i = 0; i < Tile::NI; ++i) {
-        sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < Tile::NI; ++i) {
+            sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < Tile::NJ; ++j) {
+                f32x4 d;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) d[q] = exp_j(j, t.acc[i][j][q]) * cf[j];
+                const long long r = r0 + Tile::row_of(j);
+                sum[i] += d;  // rows beyond the block have coefficient 0 (and the last row's z)
+                if constexpr (TURN)
+                    dme_store4((T*)(mine + (j * 16 + (tid & 15)) * PITCH) + i * 16 + g * 4, d);
+                else if (r < a.nb)
+                    dme_store4((T*)a.dz + r * a.lddz + c0 + Tile::col_of(i), d);
+            }
+        }
+    };
+    if (!__any(far)) {
+        float r[Tile::NJ];
 #pragma unroll
         for (int j = 0; j < Tile::NJ; ++j) {
-            f32x4 d;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) d[q] = exp_of(t.acc[i][j][q], m[j]) * cf[j];
-            const long long r = r0 + Tile::row_of(j);
-            if (r < a.nb) sum[i] += d;
-            if constexpr (TURN)
-                dme_store4((T*)(mine + (j * 16 + (tid & 15)) * PITCH) + i * 16 + g * 4, d);
-            else if (r < a.nb)
-                dme_store4((T*)a.dz + r * a.lddz + c0 + Tile::col_of(i), d);
+            const Reference e(m[j]);
+            r[j] = e.r;
+            cf[j] *= e.rest;
         }
+        each([&](int j, float z) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, LOG2E, -r[j])); });
+    } else {
+        each([&](int j, float z) { return exp_of(z, m[j]); });
     }
     if constexpr (TURN) {
         constexpr int PER = Tile::WTC * (int)sizeof(T) / 16;  // lanes that store a row
