@@ -473,9 +473,19 @@ __global__ __launch_bounds__(256) void small_step_kernel(SmallArgs a) {
     {
         f32x4 s[4] = {};
         const float* part = a.part + blockIdx.y * a.groups * SMALL * SMALL;
-        for (int u = 0; u < a.groups; ++u)
+        for (int u = 0; u < a.groups; u += 4) {  // four pieces on their way at a time
+            f32x4 p[4][4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) s[q] += *(const f32x4*)(part + u * SMALL * SMALL + (q * 256 + tid) * 4);
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    p[v][q] = *(const f32x4*)(part + (u + v < a.groups ? u + v : u) * SMALL * SMALL + (q * 256 + tid) * 4);
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (u + v < a.groups) s[q] += p[v][q];
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int f = q * 256 + tid;

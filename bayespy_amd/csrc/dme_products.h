@@ -303,27 +303,59 @@ struct DmeCut {
     int side, splits;
     double us;
 };
+struct DmeKind {
+    int side, per_cu;
+    double bf16, f32;  // in FLOP / us
+};
+constexpr DmeKind DME_KINDS[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6}, {128, 2, 980e6, 138e6}, {64, 2, 600e6, 105e6}};
+
+// us of one slice of one tile while the CU's other places are taken too
+inline double dme_slice_us(const DmeKind& kind, int size) {
+    return (double)kind.side * kind.side * (DME_SLICE / size) * 2.0 * 256.0 * kind.per_cu / (size == 4 ? kind.f32 : kind.bf16);
+}
+// us of writing and adding up pieces of 32-bit sums
+inline double dme_join_us(int splits, double values) { return splits > 1 ? 4.0 + splits * values * 8.0 / 4e6 : 0.0; }
+
 inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool split, double extra_per_tile_us = 0.0, bool symmetric = false,
                       long long batch = 1) {
-    static const struct {
-        int side, per_cu;
-        double bf16, f32;
-    } kinds[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6}, {128, 2, 980e6, 138e6}, {64, 2, 600e6, 105e6}};
     DmeCut best{0, 1, 0.0};
-    for (const auto& kind : kinds) {
+    for (const DmeKind& kind : DME_KINDS) {
         const int side = kind.side, per_cu = kind.per_cu;
-        const double rate = size == 4 ? kind.f32 : kind.bf16;
         const long long along = (R + side - 1) / side, slots = 256ll * per_cu;
         const long long tiles = batch * (symmetric ? along * (along + 1) / 2 : along * ((C + side - 1) / side));
-        // one slice of one tile while the CU's other places are taken too
-        const double slice = (double)side * side * (DME_SLICE / size) * 2.0 * slots / rate;
+        const double slice = dme_slice_us(kind, size);
         for (int s = 1; s <= (split ? 64 : 1); s *= 2) {
             if (s > 1 && slices / s < 2) break;
             const double rounds = (double)((tiles * s + slots - 1) / slots);
-            double us = rounds * ((double)((slices + s - 1) / s + 2) * slice + extra_per_tile_us * side * side / 65536.0 * per_cu);
-            if (s > 1) us += 4.0 + (double)s * batch * R * C * 8.0 / 4e6;
+            const double us = rounds * ((double)((slices + s - 1) / s + 2) * slice + extra_per_tile_us * side * side / 65536.0 * per_cu) +
+                              dme_join_us(s, (double)batch * R * C);
             if (best.side == 0 || us < best.us) best = DmeCut{side, s, us};
         }
+    }
+    return best;
+}
+
+// The same for two products launched together, Rw x C over sw slices and Rh x C over sh: one side for both, each with its own pieces
+// of k.  The workgroups go out as CUs fall free, so what counts is the whole work over the card and, at its end, about half of the
+// shorter kind.  `joined_w`, `joined_h`: the product leaves 32-bit sums in any case.
+struct DmePair {
+    int side, splits_w, splits_h;
+    double us;
+};
+inline DmePair dme_pair(long long Rw, long long sw, long long Rh, long long sh, long long C, int size, bool joined_w, bool joined_h) {
+    DmePair best{0, 1, 1, 0.0};
+    for (const DmeKind& kind : DME_KINDS) {
+        const long long side = kind.side, across = (C + side - 1) / side, tw = (Rw + side - 1) / side * across, th = (Rh + side - 1) / side * across;
+        const double slots = 256.0 * kind.per_cu, slice = dme_slice_us(kind, size);
+        for (int a = 1; a <= 64 && (a == 1 || sw / a >= 2); a *= 2)
+            for (int b = 1; b <= 64 && (b == 1 || sh / b >= 2); b *= 2) {
+                const double lw = (double)((sw + a - 1) / a + 2), lh = (double)((sh + b - 1) / b + 2);
+                const double whole = ((double)tw * a * lw + (double)th * b * lh) / slots, last = lw < lh ? lw : lh, longest = lw < lh ? lh : lw;
+                double us = whole + 0.5 * last;
+                if (us < longest) us = longest;
+                us = us * slice + dme_join_us(joined_w && a == 1 ? 2 : a, (double)Rw * C) + dme_join_us(joined_h && b == 1 ? 2 : b, (double)Rh * C);
+                if (best.side == 0 || us < best.us) best = DmePair{(int)side, a, b, us};
+            }
     }
     return best;
 }

@@ -91,50 +91,65 @@ __device__ __forceinline__ float exp_f32(float z) {
 // reciprocal of the same product: 15 roundings of 2^-24 at most.  Others take the 64-bit functions above.
 __device__ __forceinline__ bool is_small(float z, int x) { return x <= 16 && z <= 4.1f; }
 // N cells of a lane at once, x = 0 where a cell is none of these: the chains of products are independent of each other, and the loop runs
-// as far as the wave's largest count, so that no lane has a branch of its own.
+// as far as the wave's largest count, so that no lane has a branch of its own.  Terms n and x - n are taken together,
+// (a + n) (a + x - n) = a (a + x) + n (x - n), which halves the loop; an even x leaves the term in the middle.
 template <int N>
-__device__ __forceinline__ int most_of(const int (&x)[N]) {
-    int most = x[0];
+__device__ __forceinline__ float most_of(const float (&x)[N]) {
+    float most = x[0];
 #pragma unroll
-    for (int q = 1; q < N; ++q) most = most > x[q] ? most : x[q];
+    for (int q = 1; q < N; ++q) most = fmaxf(most, x[q]);
     return most;
 }
 template <int N>
 __device__ __forceinline__ float small_rest(const float (&z)[N], const int (&x)[N]) {  // the sum over the cells
-    float a[N], prod[N];
+    float xf[N], ends[N], prod[N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-        a[q] = exp_f32(z[q]);
-        prod[q] = 1.f;
+        const float a = exp_f32(z[q]);
+        xf[q] = (float)x[q];
+        ends[q] = a * (a + xf[q]);
+        prod[q] = x[q] > 0 && !(x[q] & 1) ? __builtin_fmaf(0.5f, xf[q], a) : 1.f;
     }
-    const int most = most_of(x);
-    for (int n = 1; __any(n < most); ++n)
+    const float half = 0.5f * most_of(xf);
+    for (float n = 1.f; __any(n < half); n += 1.f)
 #pragma unroll
-        for (int q = 0; q < N; ++q) prod[q] *= n < x[q] ? a[q] + (float)n : 1.f;
+        for (int q = 0; q < N; ++q) {
+            const float other = xf[q] - n;
+            prod[q] *= n < other ? __builtin_fmaf(n, other, ends[q]) : 1.f;
+        }
     float f = 0.f;
 #pragma unroll
     for (int q = 0; q < N; ++q) f += __builtin_amdgcn_logf(prod[q]);  // of 1 where there is no cell
     return f * 0.69314718f;
 }
+// Two terms of sum 1 / (a + n) make (2 a + x) / ((a + n) (a + x - n)).
 template <int N>
 __device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], float (&g)[N]) {
-    float a[N], den[N], num[N];
+    float a[N], xf[N], ends[N], den[N], num[N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
         a[q] = exp_f32(z[q]);
+        xf[q] = (float)x[q];
+        ends[q] = a[q] * (a[q] + xf[q]);
         den[q] = 1.f;
         num[q] = 0.f;
     }
-    const int most = most_of(x);
-    for (int n = 1; __any(n < most); ++n)
+    const float half = 0.5f * most_of(xf);
+    for (float n = 1.f; __any(n < half); n += 1.f)
 #pragma unroll
         for (int q = 0; q < N; ++q) {
-            const float term = n < x[q] ? a[q] + (float)n : 1.f;
-            num[q] = n < x[q] ? __builtin_fmaf(num[q], term, den[q]) : num[q];
-            den[q] *= term;
+            const float other = xf[q] - n, pair = __builtin_fmaf(n, other, ends[q]);
+            const bool in = n < other;
+            num[q] = in ? __builtin_fmaf(num[q], pair, den[q]) : num[q];
+            den[q] = in ? den[q] * pair : den[q];
         }
 #pragma unroll
-    for (int q = 0; q < N; ++q) g[q] = x[q] > 0 ? __builtin_fmaf(a[q] * num[q], __builtin_amdgcn_rcpf(den[q]), 1.f) : 0.f;
+    for (int q = 0; q < N; ++q) {
+        const float middle = __builtin_fmaf(0.5f, xf[q], a[q]);  // 2 a + x is twice that
+        float sum = 2.f * middle * num[q] * __builtin_amdgcn_rcpf(den[q]);
+        sum += !(x[q] & 1) ? __builtin_amdgcn_rcpf(middle) : 0.f;
+        g[q] = x[q] > 0 ? __builtin_fmaf(a[q], sum, 1.f) : 0.f;
+    }
 }
 __device__ __forceinline__ float small_rest(float z, int x) {
     const float zs[1] = {z};
@@ -629,7 +644,8 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
             const float m = max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(u2[0], u2[1]), fmaxf(u2[2], u2[3]))));
             const float base = m == -INFINITY ? 0.f : m;
             float s = 0.f;
-            double f = 0.0;
+            double far = 0.0;
+            float f = 0.f;
             long long total = 0;
             int counts = 0;
             bool bad = false;
@@ -644,17 +660,17 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
                 zs[q] = small ? zq : 0.f;
                 xs[q] = small ? v : 0;
                 counts += v > 0;
-                if (v > 0) f += ((double)zq - (double)base) * (dirichlet ? 1.0 : (double)v);
-                if (dirichlet && v > 0 && !small) f += dirichlet_rest((double)zq, (double)v);
+                f += v > 0 ? (zq - base) * (dirichlet ? 1.f : (float)v) : 0.f;
+                if (dirichlet && v > 0 && !small) far += dirichlet_rest((double)zq, (double)v);
             });
-            if (dirichlet) f += (double)small_rest(zs, xs);
+            if (dirichlet) f += small_rest(zs, xs);
             s = sum16(s);
-            f = sum16(f);
+            far = sum16(far + (double)f);
             const double w = sum16(dirichlet ? (double)counts : (double)total);
             const double t = sum16(bad ? __builtin_nan("") : (double)total);
             if (sub == 0) {
                 a.part[tc * a.nb + r] = f32x2{m, s};
-                a.part_f[tc * a.nb + r] = f;
+                a.part_f[tc * a.nb + r] = far;
                 a.part_w[tc * a.nb + r] = w;
                 a.part_t[tc * a.nb + r] = t;
             }
@@ -938,12 +954,12 @@ struct ProductArgs {
 
 // out = P Q' (R x C), Q k-major, in T, or as 32-bit pieces where k is split over workgroups or over launches.
 template <class T, int SIDE, bool PK>
-__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void product_kernel(ProductArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+__device__ __forceinline__ void product(const ProductArgs& a, u32 block, char* lds) {
     typedef DmeSquare<T, SIDE, PK, true> Tile;
+    const u32 tiles = (u32)(a.tiles_r * a.tiles_c), split = block / tiles;
     long long tr, tc;
-    dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
-    const int s0 = (int)blockIdx.y * a.per_split;
+    dme_tile_of(block - split * tiles, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
+    const int s0 = (int)split * a.per_split;
     int s1 = s0 + a.per_split;
     s1 = s1 < a.slices ? s1 : a.slices;
     Tile t;
@@ -959,7 +975,7 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void product_kernel(Produc
             if (c >= a.q.rows) continue;
             f32x4 v = t.acc[i][j];
             if (a.part) {  // the pitch is a multiple of four: a row's last vector stays inside it
-                f32x4* to = (f32x4*)(a.part + blockIdx.y * a.split_stride + r * a.ldpart + c);
+                f32x4* to = (f32x4*)(a.part + split * a.split_stride + r * a.ldpart + c);
                 if (a.add) v += *to;
                 *to = v;
             } else if (a.vector) {
@@ -971,6 +987,19 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void product_kernel(Produc
             }
         }
     }
+}
+
+// Both products of a piece of d loss / d z: dW = dz' H and dH = dz W, in one launch or (no workgroups for the other) one alone.  Their
+// tiles are many and few, short and long; together they leave fewer CUs idle than one after the other.  The longer ones begin.
+template <class T, int SIDE>
+__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void products_kernel(ProductArgs w, ProductArgs h, u32 blocks_w, u32 blocks_h, int h_first) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const u32 block = blockIdx.x;
+    const bool is_h = h_first ? block < blocks_h : block >= blocks_w;
+    if (is_h)
+        product<T, SIDE, false>(h, h_first ? block : block - blocks_w, lds);
+    else
+        product<T, SIDE, true>(w, h_first ? block - blocks_h : block, lds);
 }
 
 // out [R][C] = the sum of `splits` pieces, in their order.  `lines` lines of `length` values, the pieces' `ldpart` apart (a
@@ -1047,7 +1076,8 @@ struct Plan {
     long long tile_rows, tile_cols;
     long long tiles;          // pieces that the forward pass leaves of a row
     long long chunk;          // columns of a piece of d loss / d z
-    DmeCut cut_w, cut_h;
+    bool together;            // the two products of a piece go out in one launch
+    DmePair cut_w, cut_h;     // how they are cut: one cut for both, or each its own
     bool pieces_w, pieces_h;  // the products leave 32-bit pieces
     long long ldpart;
     int headroom;
@@ -1115,12 +1145,22 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         p.chunk = (tiles + pieces - 1) / pieces * p.tile_cols;  // pieces of like width
         p.dz = take(p.nb * p.chunk * p.size);
         p.ldpart = up(D, 4);
-        p.cut_w = dme_cut(p.chunk < K ? p.chunk : K, D, (p.nb * p.size + DME_SLICE - 1) / DME_SLICE, p.size, true);
-        p.cut_h = dme_cut(p.nb, D, (p.chunk * p.size + DME_SLICE - 1) / DME_SLICE, p.size, true);
-        p.pieces_w = p.cut_w.splits > 1 || N > p.nb;
-        p.pieces_h = p.cut_h.splits > 1 || pieces > 1;
-        if (p.pieces_w) p.pw = take((long long)p.cut_w.splits * K * p.ldpart * 4);
-        if (p.pieces_h) p.ph = take((long long)p.cut_h.splits * p.nb * p.ldpart * 4);
+        const auto slices_of = [&](long long k) { return (k * p.size + DME_SLICE - 1) / DME_SLICE; };
+        const long long width = p.chunk < K ? p.chunk : K;
+        // Together they fill the card better; where a piece's rows are long each fills it alone, and side by side they only take the caches
+        // from each other (N = 4099, D = 128: 229 us apart, 162 together; N = 8192, D = 1024: 1567 apart, 1690 together; D = 256: alike).
+        p.together = D <= 512;
+        if (p.together) {
+            p.cut_w = p.cut_h = dme_pair(width, slices_of(p.nb), p.nb, slices_of(width), D, p.size, N > p.nb, pieces > 1);
+        } else {
+            const DmeCut w = dme_cut(width, D, slices_of(p.nb), p.size, true), h = dme_cut(p.nb, D, slices_of(width), p.size, true);
+            p.cut_w = DmePair{w.side, w.splits, 1, w.us};
+            p.cut_h = DmePair{h.side, 1, h.splits, h.us};
+        }
+        p.pieces_w = p.cut_w.splits_w > 1 || N > p.nb;
+        p.pieces_h = p.cut_h.splits_h > 1 || pieces > 1;
+        if (p.pieces_w) p.pw = take((long long)p.cut_w.splits_w * K * p.ldpart * 4);
+        if (p.pieces_h) p.ph = take((long long)p.cut_h.splits_h * p.nb * p.ldpart * 4);
     }
     p.bytes = at;
     return p;
@@ -1171,26 +1211,31 @@ int tiles_of_z(const TileArgs& a, int kind, int side, hipStream_t s) {
     return launch_tile<T, 16, 128, 1, 4, BACKWARD>(a, s);
 }
 
-template <class T, int SIDE, bool PK>
-int launch_product(const ProductArgs& a, int splits, hipStream_t s) {
-    typedef DmeSquare<T, SIDE, PK, true> Tile;
+template <class T, int SIDE>
+int launch_products(ProductArgs w, ProductArgs h, const DmePair& cut, bool do_w, bool do_h, hipStream_t s) {
+    typedef DmeSquare<T, SIDE, true, true> Tile;
     static std::atomic<bool> done[64];
-    const int rc = set_lds(done, product_kernel<T, SIDE, PK>, Tile::LDS);
+    const int rc = set_lds(done, products_kernel<T, SIDE>, Tile::LDS);
     if (rc) return rc;
-    hipLaunchKernelGGL((product_kernel<T, SIDE, PK>), dim3((unsigned)(a.tiles_r * a.tiles_c), (unsigned)splits), dim3(Tile::NT), Tile::LDS, s, a);
+    const auto lay = [](ProductArgs& a, int splits) {
+        a.tiles_r = (a.p.rows + SIDE - 1) / SIDE;
+        a.tiles_c = (a.q.rows + SIDE - 1) / SIDE;
+        a.slices = (int)((a.k * (long long)sizeof(T) + DME_SLICE - 1) / DME_SLICE);
+        a.per_split = (a.slices + splits - 1) / splits;
+        return (u32)(a.tiles_r * a.tiles_c * splits);
+    };
+    const u32 blocks_w = do_w ? lay(w, cut.splits_w) : 0, blocks_h = do_h ? lay(h, cut.splits_h) : 0;
+    hipLaunchKernelGGL((products_kernel<T, SIDE>), dim3(blocks_w + blocks_h), dim3(Tile::NT), Tile::LDS, s, w, h, blocks_w, blocks_h,
+                       (int)(h.per_split > w.per_split));
     return DME_OK;
 }
 
-template <class T, bool PK>
-int product(ProductArgs a, const DmeCut& cut, hipStream_t s) {
-    a.tiles_r = (a.p.rows + cut.side - 1) / cut.side;
-    a.tiles_c = (a.q.rows + cut.side - 1) / cut.side;
-    a.slices = (int)((a.k * (long long)sizeof(T) + DME_SLICE - 1) / DME_SLICE);
-    a.per_split = (a.slices + cut.splits - 1) / cut.splits;
-    if (cut.side == 256) return launch_product<T, 256, PK>(a, cut.splits, s);
-    if (cut.side == 192) return launch_product<T, 192, PK>(a, cut.splits, s);
-    if (cut.side == 128) return launch_product<T, 128, PK>(a, cut.splits, s);
-    return launch_product<T, 64, PK>(a, cut.splits, s);
+template <class T>
+int products(const ProductArgs& w, const ProductArgs& h, const DmePair& cut, bool do_w, bool do_h, hipStream_t s) {
+    if (cut.side == 256) return launch_products<T, 256>(w, h, cut, do_w, do_h, s);
+    if (cut.side == 192) return launch_products<T, 192>(w, h, cut, do_w, do_h, s);
+    if (cut.side == 128) return launch_products<T, 128>(w, h, cut, do_w, do_h, s);
+    return launch_products<T, 64>(w, h, cut, do_w, do_h, s);
 }
 
 template <class T>
@@ -1343,47 +1388,49 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
                     hipLaunchKernelGGL((patch_kernel<T, LABELS, 1>), dim3((unsigned)((nb + 511) / 512)), dim3(512), 0, s, pa);
             }
             const char* dz = (const char*)a.dz;
-            ProductArgs m{};  // dW of the piece = dz' H
-            m.p = DmeOperand{dz, a.lddz * size, width};
-            m.q = DmeOperand{h.at, h.ld, c.D};
-            m.k = nb;
+            ProductArgs mw{}, mh{};
+            mw.p = DmeOperand{dz, a.lddz * size, width};  // dW of the piece = dz' H
+            mw.q = DmeOperand{h.at, h.ld, c.D};
+            mw.k = nb;
             if (p.pieces_w) {
-                m.part = (float*)(ws + p.pw) + k0 * p.ldpart;
-                m.ldpart = p.ldpart;
-                m.split_stride = c.K * p.ldpart;
-                m.add = n0 > 0;
+                mw.part = (float*)(ws + p.pw) + k0 * p.ldpart;
+                mw.ldpart = p.ldpart;
+                mw.split_stride = c.K * p.ldpart;
+                mw.add = n0 > 0;
             } else {
-                m.out = (T*)c.dW + k0 * c.D;
-                m.ldout = c.D;
-                m.vector = c.D % 4 == 0;
+                mw.out = (T*)c.dW + k0 * c.D;
+                mw.ldout = c.D;
+                mw.vector = c.D % 4 == 0;
             }
-            rc = product<T, true>(m, p.cut_w, s);
-            if (rc) return rc;
-            m = ProductArgs{};  // dH (+)= dz W
-            m.p = DmeOperand{dz, a.lddz * size, nb};
-            m.q = DmeOperand{a.w.at, a.w.ld, c.D};
-            m.k = width;
+            mh.p = DmeOperand{dz, a.lddz * size, nb};  // dH (+)= dz W
+            mh.q = DmeOperand{a.w.at, a.w.ld, c.D};
+            mh.k = width;
             if (p.pieces_h) {
-                m.part = (float*)(ws + p.ph);
-                m.ldpart = p.ldpart;
-                m.split_stride = p.nb * p.ldpart;
-                m.add = k0 > 0;
+                mh.part = (float*)(ws + p.ph);
+                mh.ldpart = p.ldpart;
+                mh.split_stride = p.nb * p.ldpart;
+                mh.add = k0 > 0;
             } else {
-                m.out = (T*)c.dH + n0 * c.D;
-                m.ldout = c.D;
-                m.vector = c.D % 4 == 0;
+                mh.out = (T*)c.dH + n0 * c.D;
+                mh.ldout = c.D;
+                mh.vector = c.D % 4 == 0;
             }
-            rc = product<T, false>(m, p.cut_h, s);
+            if (p.together) {
+                rc = products<T>(mw, mh, p.cut_w, true, true, s);
+            } else {
+                rc = products<T>(mw, mh, p.cut_w, true, false, s);
+                if (!rc) rc = products<T>(mw, mh, p.cut_h, false, true, s);
+            }
             if (rc) return rc;
         }
         if (p.pieces_h)
-            join<T>((const float*)(ws + p.ph), p.ldpart, p.nb * p.ldpart, p.cut_h.splits, nb, c.D, (T*)c.dH + n0 * c.D, s);
+            join<T>((const float*)(ws + p.ph), p.ldpart, p.nb * p.ldpart, p.cut_h.splits_h, nb, c.D, (T*)c.dH + n0 * c.D, s);
         if (c.dbias)
             hipLaunchKernelGGL(bias_kernel, dim3((unsigned)((c.K + 63) / 64)), dim3(256), 0, s, (const float*)a.dbias, a.tiles_r, c.K,
                                fixed, largest, p.headroom, (int)(n0 > 0), c.dbias);
     }
     if (gradient && p.pieces_w)
-        join<T>((const float*)(ws + p.pw), p.ldpart, c.K * p.ldpart, p.cut_w.splits, c.K, c.D, (T*)c.dW, s);
+        join<T>((const float*)(ws + p.pw), p.ldpart, c.K * p.ldpart, p.cut_w.splits_w, c.K, c.D, (T*)c.dW, s);
     DME_HIP_CHECK(hipGetLastError());
     return DME_OK;
 }
