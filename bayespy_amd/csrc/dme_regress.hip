@@ -225,6 +225,8 @@ struct TileArgs {
     double* part_w;    // DENSE: [tile][nb]: how often that z goes into it: sum x (multinomial), number of counts (Dirichlet)
     double* part_t;    // DENSE: [tile][nb]: sum x, NaN where a count is negative
     float* entry_z;    // CSR: [nnz], LABELS: [nb]: z at the counts
+    u32* clear;        // cleared on the way
+    long long clear_words;
     int likelihood;
     // backward
     const float* largest_z;  // [nb]: m
@@ -337,9 +339,13 @@ __device__ __forceinline__ void entries_of(const TileArgs& a, long long r, int f
     }
 }
 
-template <class T, int KIND>
-__global__ __launch_bounds__(256) void entry_kernel(TileArgs a) {
-    const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+// What workgroups beyond the tiles do in the forward launch: a wave makes a row's z at its counts, and together they clear the words
+// that the gradient adds into later.
+template <class T, int KIND, int WAVES>
+__device__ __forceinline__ void beyond_tiles(const TileArgs& a, u32 block) {
+    const u32 blocks = (u32)((a.nb + WAVES - 1) / WAVES);
+    for (long long i = (long long)block * WAVES * 64 + threadIdx.x; i < a.clear_words; i += (long long)blocks * WAVES * 64) a.clear[i] = 0;
+    const long long r = (long long)block * WAVES + (threadIdx.x >> 6);
     if (r < a.nb) entries_of<T, KIND>(a, r, 0, 1);
 }
 
@@ -357,7 +363,9 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ f32x2 seen[4][16];
     if (blockIdx.x >= a.tiles_c) {
-        if constexpr (KIND != DENSE) entries_of<T, KIND>(a, blockIdx.x - a.tiles_c, threadIdx.x >> 6, 4);
+        const u32 r = blockIdx.x - (u32)a.tiles_c;
+        for (long long i = (long long)r * 256 + threadIdx.x; i < a.clear_words; i += a.nb * 256) a.clear[i] = 0;
+        entries_of<T, KIND>(a, r, threadIdx.x >> 6, 4);
         return;
     }
     constexpr int WIDE = 8;
@@ -416,10 +424,14 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
 //   forward   the largest z of each row and the sum of e^(z - that)
 //   backward  e^(z - m) coef, rounded to T (the gradient's one rounding before its products), and the columns' sums
 //             of the unrounded values.  The counts are not looked at: patch_kernel puts them in.
-template <class T, int TR, int TC, int WR, int WC, bool BACKWARD>
+template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD>
 __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DmeTile<T, TR, TC, WR, WC> Tile;
+    if (!BACKWARD && blockIdx.x >= (u32)(a.tiles_r * a.tiles_c)) {
+        beyond_tiles<T, KIND, WR * WC>(a, blockIdx.x - (u32)(a.tiles_r * a.tiles_c));
+        return;
+    }
     long long tr, tc;
     dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * TC, k0 = a.column + c0;
@@ -1004,59 +1016,87 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void products_kernel(Produ
 
 // out [R][C] = the sum of `splits` pieces, in their order.  `lines` lines of `length` values, the pieces' `ldpart` apart (a
 // multiple of four); one line where there are no gaps.  A wave takes 256 values of a line.
+struct JoinArgs {
+    const float* part;
+    long long ldpart, split_stride;
+    int splits;
+    long long lines, length;
+    void* out;
+    int vector;
+    u32 blocks;
+};
+
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const float* part, long long ldpart, long long split_stride, int splits, long long lines,
-                                                   long long length, T* out, int vector) {
+__device__ __forceinline__ void join(const JoinArgs& a, u32 block) {
     const int lane = threadIdx.x & 63;
-    const long long across = (length + 255) / 256, all = lines * across, waves = (long long)gridDim.x * 4;
-    for (long long t = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); t < all; t += waves) {
+    const long long across = (a.length + 255) / 256, all = a.lines * across, waves = (long long)a.blocks * 4;
+    for (long long t = (long long)block * 4 + (threadIdx.x >> 6); t < all; t += waves) {
         const long long line = across == 1 ? t : t / across, c = (across == 1 ? 0 : t - line * across) * 256 + lane * 4;
-        if (c >= length) continue;
-        const float* at = part + line * ldpart + c;
+        if (c >= a.length) continue;
+        const float* at = a.part + line * a.ldpart + c;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
         int s = 0;
-        for (; s + 4 <= splits; s += 4) {
+        for (; s + 4 <= a.splits; s += 4) {
             f32x4 p[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) p[u] = *(const f32x4*)(at + (s + u) * split_stride);
+            for (int u = 0; u < 4; ++u) p[u] = *(const f32x4*)(at + (s + u) * a.split_stride);
 #pragma unroll
             for (int u = 0; u < 4; ++u) v += p[u];
         }
-        for (; s < splits; ++s) v += *(const f32x4*)(at + s * split_stride);
-        T* o = out + line * length + c;
-        if (vector) {
+        for (; s < a.splits; ++s) v += *(const f32x4*)(at + s * a.split_stride);
+        T* o = (T*)a.out + line * a.length + c;
+        if (a.vector) {
             dme_store4(o, v);
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (c + q < length) o[q] = (T)v[q];
+                if (c + q < a.length) o[q] = (T)v[q];
         }
     }
 }
 
 // dbias [K] (+)= the row tiles' sums, minus the counts' (fixed, null for dense rows).  64 columns a workgroup, a quarter of the
 // tiles a wave, the quarters added in their order.
-__global__ __launch_bounds__(256) void bias_kernel(const float* part, long long tiles, long long K, const long long* fixed, const u32* largest,
-                                                   int headroom, int add, float* dbias) {
-    __shared__ double sums[4][64];
+struct BiasArgs {
+    const float* part;
+    long long tiles, K;
+    const long long* fixed;
+    const u32* largest;
+    int headroom, add;
+    float* dbias;
+    u32 blocks;
+};
+
+__device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*sums)[64]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long k = (long long)blockIdx.x * 64 + lane;
+    const long long k = (long long)block * 64 + lane;
     double v = 0.0;
-    if (k < K)
-        for (long long t = wave; t < tiles; t += 16) {
+    if (k < a.K)
+        for (long long t = wave; t < a.tiles; t += 16) {
             float p[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) p[u] = t + u * 4 < tiles ? part[(t + u * 4) * K + k] : 0.f;
+            for (int u = 0; u < 4; ++u) p[u] = t + u * 4 < a.tiles ? a.part[(t + u * 4) * a.K + k] : 0.f;
 #pragma unroll
             for (int u = 0; u < 4; ++u) v += (double)p[u];
         }
     sums[wave][lane] = v;
     __syncthreads();
-    if (wave != 0 || k >= K) return;
+    if (wave != 0 || k >= a.K) return;
     v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
-    if (add) v += (double)dbias[k];
-    if (fixed) v -= ldexp((double)fixed[k], -fixed_shift(largest, headroom));
-    dbias[k] = (float)v;
+    if (a.add) v += (double)a.dbias[k];
+    if (a.fixed) v -= ldexp((double)a.fixed[k], -fixed_shift(a.largest, a.headroom));
+    a.dbias[k] = (float)v;
+}
+
+// What is left when the products are through, in one launch: the pieces of dH and dW, and dbias (0 workgroups: not this time).
+template <class T>
+__global__ __launch_bounds__(256) void finish_kernel(JoinArgs w, JoinArgs h, BiasArgs b) {
+    __shared__ double sums[4][64];
+    u32 block = blockIdx.x;
+    if (block < w.blocks) return join<T>(w, block);
+    block -= w.blocks;
+    if (block < h.blocks) return join<T>(h, block);
+    add_bias(b, block - h.blocks, sums);
 }
 
 __global__ void zero_kernel(u32* p, long long words) {
@@ -1177,17 +1217,26 @@ int set_lds(std::atomic<bool>* done, F kernel, int bytes) {
     return DME_OK;
 }
 
-template <class T, int TR, int TC, int WR, int WC, bool BACKWARD>
+template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD>
 int launch_tile(const TileArgs& a, hipStream_t s) {
     typedef DmeTile<T, TR, TC, WR, WC> Tile;
     static_assert(Tile::LDS >= WC * TR * 8 && Tile::LDS >= WR * TC * 4, "the reductions use the tiles' LDS");
     static std::atomic<bool> done[64];
     constexpr int turned = BACKWARD && sizeof(T) == 2 && TR >= 128 ? TR * WC * (Tile::WTC * (int)sizeof(T) + 16) : 0;
     constexpr int bytes = turned > Tile::LDS ? turned : Tile::LDS;
-    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, BACKWARD>, bytes);
+    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD>, bytes);
     if (rc) return rc;
-    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c)), dim3(Tile::NT), bytes, s, a);
+    const long long more = BACKWARD ? 0 : (a.nb + Tile::NW - 1) / Tile::NW;
+    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c + more)), dim3(Tile::NT), bytes, s, a);
     return DME_OK;
+}
+
+template <class T, int KIND, bool BACKWARD>
+int launch_side(const TileArgs& a, int side, hipStream_t s) {
+    if (side == 256) return launch_tile<T, 256, 256, 4, 2, KIND, BACKWARD>(a, s);
+    if (side == 128) return launch_tile<T, 128, 128, 2, 2, KIND, BACKWARD>(a, s);
+    if (side == 64) return launch_tile<T, 64, 64, 2, 2, KIND, BACKWARD>(a, s);
+    return launch_tile<T, 16, 128, 1, 4, KIND, BACKWARD>(a, s);
 }
 
 template <class T, int TR, bool BACKWARD>
@@ -1201,14 +1250,12 @@ int launch_dense(const TileArgs& a, hipStream_t s) {
     return DME_OK;
 }
 
-// The tiles of z.
+// The tiles of z, forward with z at the counts.
 template <class T, bool BACKWARD>
 int tiles_of_z(const TileArgs& a, int kind, int side, hipStream_t s) {
     if (kind == DENSE) return side == 16 ? launch_dense<T, 16, BACKWARD>(a, s) : launch_dense<T, 128, BACKWARD>(a, s);
-    if (side == 256) return launch_tile<T, 256, 256, 4, 2, BACKWARD>(a, s);
-    if (side == 128) return launch_tile<T, 128, 128, 2, 2, BACKWARD>(a, s);
-    if (side == 64) return launch_tile<T, 64, 64, 2, 2, BACKWARD>(a, s);
-    return launch_tile<T, 16, 128, 1, 4, BACKWARD>(a, s);
+    if (!BACKWARD && kind == CSR) return launch_side<T, CSR, false>(a, side, s);
+    return launch_side<T, LABELS, BACKWARD>(a, side, s);  // backward the kind does not matter
 }
 
 template <class T, int SIDE>
@@ -1238,12 +1285,11 @@ int products(const ProductArgs& w, const ProductArgs& h, const DmePair& cut, boo
     return launch_products<T, 64>(w, h, cut, do_w, do_h, s);
 }
 
-template <class T>
-void join(const float* part, long long ldpart, long long split_stride, int splits, long long R, long long C, T* out, hipStream_t s) {
+JoinArgs join_args(const void* part, long long ldpart, long long split_stride, int splits, long long R, long long C, void* out) {
     const bool whole = ldpart == C;
-    const long long lines = whole ? 1 : R, length = whole ? R * C : C;
-    hipLaunchKernelGGL(join_kernel<T>, dim3(dme_blocks(lines * ((length + 255) / 256), 4, 8192)), dim3(256), 0, s, part, ldpart, split_stride, splits, lines,
-                       length, out, (int)(C % 4 == 0));
+    JoinArgs a{(const float*)part, ldpart, split_stride, splits, whole ? 1 : R, whole ? R * C : C, out, (int)(C % 4 == 0), 0};
+    a.blocks = (u32)dme_blocks(a.lines * ((a.length + 255) / 256), 4, 8192);
+    return a;
 }
 
 // dst (rows of `width` bytes) = src (rows of `bytes` bytes, `pitch` apart), zero in what is more
@@ -1289,9 +1335,6 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
     long long* fixed = gradient && kind != DENSE && c.dbias ? (long long*)(ws + p.fixed) : nullptr;
     for (long long n0 = 0; n0 < c.N; n0 += p.nb) {
         const long long nb = c.N - n0 < p.nb ? c.N - n0 : p.nb;
-        // each block of rows has fixed-point sums of its own: their scale is the block's
-        if (p.zero_words)
-            hipLaunchKernelGGL(zero_kernel, dim3(dme_blocks(p.zero_words, 1024, 1024)), dim3(256), 0, s, (u32*)ws, p.zero_words);
         DmeOperand h{(const char*)c.H + n0 * c.ldh * size, c.ldh * size, nb};
         if (p.pack_h) {
             pack(h.at, c.ldh * size, nb, c.D * size, ws + p.h, p.dpad * size, s);
@@ -1326,6 +1369,8 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         a.part_w = (double*)(ws + p.part_w);
         a.part_t = (double*)(ws + p.part_t);
         a.entry_z = (float*)(ws + p.entry_z);
+        a.clear = (u32*)ws;  // each block of rows has fixed-point sums of its own: their scale is the block's
+        a.clear_words = p.zero_words;
         int rc = DME_OK;
         if (p.few) {
             const unsigned blocks = (unsigned)(p.tiles + nb), bytes = (unsigned)few_lds(c.D * size);
@@ -1334,10 +1379,6 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             else
                 hipLaunchKernelGGL((few_kernel<T, LABELS>), dim3(blocks), dim3(256), bytes, s, a);
         } else {
-            if (kind == CSR)
-                hipLaunchKernelGGL((entry_kernel<T, CSR>), dim3((unsigned)((nb + 3) / 4)), dim3(256), 0, s, a);
-            else if (kind == LABELS)
-                hipLaunchKernelGGL((entry_kernel<T, LABELS>), dim3((unsigned)((nb + 3) / 4)), dim3(256), 0, s, a);
             rc = tiles_of_z<T, false>(a, kind, p.side, s);
         }
         if (rc) return rc;
@@ -1423,14 +1464,15 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             }
             if (rc) return rc;
         }
-        if (p.pieces_h)
-            join<T>((const float*)(ws + p.ph), p.ldpart, p.nb * p.ldpart, p.cut_h.splits_h, nb, c.D, (T*)c.dH + n0 * c.D, s);
+        JoinArgs jw{}, jh{};
+        BiasArgs bias{};
+        if (p.pieces_w && n0 + nb == c.N) jw = join_args(ws + p.pw, p.ldpart, c.K * p.ldpart, p.cut_w.splits_w, c.K, c.D, c.dW);
+        if (p.pieces_h) jh = join_args(ws + p.ph, p.ldpart, p.nb * p.ldpart, p.cut_h.splits_h, nb, c.D, (T*)c.dH + n0 * c.D);
         if (c.dbias)
-            hipLaunchKernelGGL(bias_kernel, dim3((unsigned)((c.K + 63) / 64)), dim3(256), 0, s, (const float*)a.dbias, a.tiles_r, c.K,
-                               fixed, largest, p.headroom, (int)(n0 > 0), c.dbias);
+            bias = BiasArgs{a.dbias, a.tiles_r, c.K, fixed, largest, p.headroom, (int)(n0 > 0), c.dbias, (u32)((c.K + 63) / 64)};
+        const u32 blocks = jw.blocks + jh.blocks + bias.blocks;
+        if (blocks) hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks), dim3(256), 0, s, jw, jh, bias);
     }
-    if (gradient && p.pieces_w)
-        join<T>((const float*)(ws + p.pw), p.ldpart, c.K * p.ldpart, p.cut_w.splits_w, c.K, c.D, (T*)c.dW, s);
     DME_HIP_CHECK(hipGetLastError());
     return DME_OK;
 }
