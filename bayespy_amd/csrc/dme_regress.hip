@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
 #pragma unroll
         for (int u = 0; u < WIDE; ++u) {
             const int at = (round + u) * 4 + g;
-            to[u] = at < chunks ? __builtin_nontemporal_load(w + at) : none;
+            to[u] = at < chunks ? w[at] : none;
         }
     };
     load(y[0], 0);
@@ -424,10 +424,10 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
 //   forward   the largest z of each row and the sum of e^(z - that)
 //   backward  e^(z - m) coef, rounded to T (the gradient's one rounding before its products), and the columns' sums
 //             of the unrounded values.  The counts are not looked at: patch_kernel puts them in.
-template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD>
+template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD, int STAGES = 0>
 __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeTile<T, TR, TC, WR, WC> Tile;
+    typedef DmeTile<T, TR, TC, WR, WC, false, false, STAGES> Tile;
     if (!BACKWARD && blockIdx.x >= (u32)(a.tiles_r * a.tiles_c)) {
         beyond_tiles<T, KIND, WR * WC>(a, blockIdx.x - (u32)(a.tiles_r * a.tiles_c));
         return;
@@ -965,9 +965,9 @@ struct ProductArgs {
 };
 
 // out = P Q' (R x C), Q k-major, in T, or as 32-bit pieces where k is split over workgroups or over launches.
-template <class T, int SIDE, bool PK>
+template <class T, int SIDE, bool PK, int STAGES>
 __device__ __forceinline__ void product(const ProductArgs& a, u32 block, char* lds) {
-    typedef DmeSquare<T, SIDE, PK, true> Tile;
+    typedef DmeSquare<T, SIDE, PK, true, STAGES> Tile;
     const u32 tiles = (u32)(a.tiles_r * a.tiles_c), split = block / tiles;
     long long tr, tc;
     dme_tile_of(block - split * tiles, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
@@ -1003,15 +1003,15 @@ __device__ __forceinline__ void product(const ProductArgs& a, u32 block, char* l
 
 // Both products of a piece of d loss / d z: dW = dz' H and dH = dz W, in one launch or (no workgroups for the other) one alone.  Their
 // tiles are many and few, short and long; together they leave fewer CUs idle than one after the other.  The longer ones begin.
-template <class T, int SIDE>
+template <class T, int SIDE, int STAGES>
 __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void products_kernel(ProductArgs w, ProductArgs h, u32 blocks_w, u32 blocks_h, int h_first) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const u32 block = blockIdx.x;
     const bool is_h = h_first ? block < blocks_h : block >= blocks_w;
     if (is_h)
-        product<T, SIDE, false>(h, h_first ? block : block - blocks_w, lds);
+        product<T, SIDE, false, STAGES>(h, h_first ? block : block - blocks_w, lds);
     else
-        product<T, SIDE, true>(w, h_first ? block - blocks_h : block, lds);
+        product<T, SIDE, true, STAGES>(w, h_first ? block - blocks_h : block, lds);
 }
 
 // out [R][C] = the sum of `splits` pieces, in their order.  `lines` lines of `length` values, the pieces' `ldpart` apart (a
@@ -1217,17 +1217,17 @@ int set_lds(std::atomic<bool>* done, F kernel, int bytes) {
     return DME_OK;
 }
 
-template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD>
+template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD, int STAGES = 0>
 int launch_tile(const TileArgs& a, hipStream_t s) {
-    typedef DmeTile<T, TR, TC, WR, WC> Tile;
+    typedef DmeTile<T, TR, TC, WR, WC, false, false, STAGES> Tile;
     static_assert(Tile::LDS >= WC * TR * 8 && Tile::LDS >= WR * TC * 4, "the reductions use the tiles' LDS");
     static std::atomic<bool> done[64];
     constexpr int turned = BACKWARD && sizeof(T) == 2 && TR >= 128 ? TR * WC * (Tile::WTC * (int)sizeof(T) + 16) : 0;
     constexpr int bytes = turned > Tile::LDS ? turned : Tile::LDS;
-    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD>, bytes);
+    const int rc = set_lds(done, tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD, STAGES>, bytes);
     if (rc) return rc;
     const long long more = BACKWARD ? 0 : (a.nb + Tile::NW - 1) / Tile::NW;
-    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c + more)), dim3(Tile::NT), bytes, s, a);
+    hipLaunchKernelGGL((tile_kernel<T, TR, TC, WR, WC, KIND, BACKWARD, STAGES>), dim3((unsigned)(a.tiles_r * a.tiles_c + more)), dim3(Tile::NT), bytes, s, a);
     return DME_OK;
 }
 
@@ -1235,7 +1235,10 @@ template <class T, int KIND, bool BACKWARD>
 int launch_side(const TileArgs& a, int side, hipStream_t s) {
     if (side == 256) return launch_tile<T, 256, 256, 4, 2, KIND, BACKWARD>(a, s);
     if (side == 128) return launch_tile<T, 128, 128, 2, 2, KIND, BACKWARD>(a, s);
-    if (side == 64) return launch_tile<T, 64, 64, 2, 2, KIND, BACKWARD>(a, s);
+    if (side == 64) {  // a deep pipeline where a CU has one or two of them, two buffers where it can hold five
+        if (a.tiles_r * a.tiles_c > 512) return launch_tile<T, 64, 64, 2, 2, KIND, BACKWARD, 2>(a, s);
+        return launch_tile<T, 64, 64, 2, 2, KIND, BACKWARD>(a, s);
+    }
     return launch_tile<T, 16, 128, 1, 4, KIND, BACKWARD>(a, s);
 }
 
@@ -1258,11 +1261,11 @@ int tiles_of_z(const TileArgs& a, int kind, int side, hipStream_t s) {
     return launch_side<T, LABELS, BACKWARD>(a, side, s);  // backward the kind does not matter
 }
 
-template <class T, int SIDE>
+template <class T, int SIDE, int STAGES = 0>
 int launch_products(ProductArgs w, ProductArgs h, const DmePair& cut, bool do_w, bool do_h, hipStream_t s) {
-    typedef DmeSquare<T, SIDE, true, true> Tile;
+    typedef DmeSquare<T, SIDE, true, true, STAGES> Tile;
     static std::atomic<bool> done[64];
-    const int rc = set_lds(done, products_kernel<T, SIDE>, Tile::LDS);
+    const int rc = set_lds(done, products_kernel<T, SIDE, STAGES>, Tile::LDS);
     if (rc) return rc;
     const auto lay = [](ProductArgs& a, int splits) {
         a.tiles_r = (a.p.rows + SIDE - 1) / SIDE;
@@ -1272,7 +1275,7 @@ int launch_products(ProductArgs w, ProductArgs h, const DmePair& cut, bool do_w,
         return (u32)(a.tiles_r * a.tiles_c * splits);
     };
     const u32 blocks_w = do_w ? lay(w, cut.splits_w) : 0, blocks_h = do_h ? lay(h, cut.splits_h) : 0;
-    hipLaunchKernelGGL((products_kernel<T, SIDE>), dim3(blocks_w + blocks_h), dim3(Tile::NT), Tile::LDS, s, w, h, blocks_w, blocks_h,
+    hipLaunchKernelGGL((products_kernel<T, SIDE, STAGES>), dim3(blocks_w + blocks_h), dim3(Tile::NT), Tile::LDS, s, w, h, blocks_w, blocks_h,
                        (int)(h.per_split > w.per_split));
     return DME_OK;
 }
@@ -1282,6 +1285,9 @@ int products(const ProductArgs& w, const ProductArgs& h, const DmePair& cut, boo
     if (cut.side == 256) return launch_products<T, 256>(w, h, cut, do_w, do_h, s);
     if (cut.side == 192) return launch_products<T, 192>(w, h, cut, do_w, do_h, s);
     if (cut.side == 128) return launch_products<T, 128>(w, h, cut, do_w, do_h, s);
+    const long long along = (w.q.rows + 63) / 64;
+    const long long all = ((w.p.rows + 63) / 64 * cut.splits_w * do_w + (h.p.rows + 63) / 64 * cut.splits_h * do_h) * along;
+    if (all > 512) return launch_products<T, 64, 2>(w, h, cut, do_w, do_h, s);
     return launch_products<T, 64>(w, h, cut, do_w, do_h, s);
 }
 
