@@ -23,6 +23,8 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr long long ROW_BLOCK = 16384;             // rows worked on at a time
+// ... and less of them where K is vast: a launch has fewer than 2^32 threads, and tiles of 64 take a thread for 16 values of z
+constexpr long long MOST_CELLS = 1ll << 35;
 // of d loss / d z held at a time: about the memory-side cache, so that the two products read it from there, and pieces still
 // large enough to fill the card (N = 8192, K = 50000, D = 1024: 3508 us with 512 MB, 3400 with 256, 3419 with 128, 3582 with 64;
 // N = 4099, D = 128: 707, 653, 724, 790)
@@ -827,7 +829,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
             if (a.largest_z && real) {
                 const float v = weight * (small ? small_g(z, x) : (float)g_of(a.likelihood, (double)z, (double)x));
                 a.entry_g[e] = v;
-                most = fmaxf(most, fabsf(v));
+                if (__builtin_isfinite(v)) most = fmaxf(most, fabsf(v));
             }
         }
         if (bad) total = __builtin_nan("");
@@ -839,7 +841,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         times = in ? 1.0 : 0.0;
         if (a.largest_z && real) {
             a.entry_g[r] = weight;
-            most = k >= 0 ? fabsf(weight) : 0.f;
+            most = k >= 0 && __builtin_isfinite(weight) ? fabsf(weight) : 0.f;
         }
     }
     if constexpr (LANES == 16) {
@@ -899,7 +901,7 @@ struct PatchArgs {
 // The exponent of the fixed-point sums of entry_g: the largest one takes 62 - headroom bits, whatever its size.
 __device__ __forceinline__ int fixed_shift(const u32* largest, int headroom) {
     const float v = __builtin_bit_cast(float, *largest);
-    return 62 - headroom - (v > 0.f && v < INFINITY ? ilogbf(v) + 1 : 0);
+    return 62 - headroom - (v > 0.f ? ilogbf(v) + 1 : 0);
 }
 
 // d loss / d z at the counts: the tiles' value made again, minus G, in its place.  What dbias needs of G is added up in fixed
@@ -1139,6 +1141,7 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     p.pack_w = loose(W, ldw);
     p.dpad = up(D, 16 / p.size);
     p.nb = N < 1 ? 1 : N < ROW_BLOCK ? N : ROW_BLOCK;
+    while (p.nb * K > MOST_CELLS) p.nb = (p.nb + 1) / 2;
     const long long slices = (D * p.size + DME_SLICE - 1) / DME_SLICE;
     const int cut = dme_cut(p.nb, K, slices, p.size, false, 4.0).side;
     p.side = p.nb <= 16 ? 16 : rows->kind == DENSE ? 128 : cut >= 192 ? 256 : cut;
@@ -1487,7 +1490,7 @@ int check_call(const void* H, int64_t ldh, const void* W, int64_t ldw, int type,
                int likelihood) {
     DME_REQUIRE(type == DME_TYPE_BF16 || type == DME_TYPE_F32, "features and weights are bf16 or fp32");
     DME_REQUIRE(N >= 0 && K >= 1 && D >= 1, "bad shape: N = %lld, K = %lld, D = %lld", (long long)N, (long long)K, (long long)D);
-    DME_REQUIRE(K <= 0x7fffffffll && D <= (1ll << 20) && N <= (1ll << 40), "shape out of range");
+    DME_REQUIRE(K <= (1ll << 29) && D <= (1ll << 20) && N <= (1ll << 40), "shape out of range");
     DME_REQUIRE(ldh >= D && ldw >= D, "pitch smaller than a row");
     DME_REQUIRE(likelihood == DME_LIKELIHOOD_MULTINOMIAL || likelihood == DME_LIKELIHOOD_DIRICHLET, "unknown likelihood %d", likelihood);
     DME_REQUIRE(rows != nullptr, "no count rows");

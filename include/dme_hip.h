@@ -577,14 +577,17 @@ int dme_synth_dirmult(void* X /*[dev]*/, int elem_bytes, int64_t N, int64_t K, i
  *   multinomial   loss = T l - sum_k x_k z_k                          (softmax; the multinomial coefficient left out)
  *   Dirichlet     loss = lgamma(e^l + T) - lgamma(e^l) - sum_k [lgamma(e^z_k + x_k) - lgamma(e^z_k)]
  * z is never stored whole: the loss takes one pass over the columns, the gradient makes z again in pieces of the
- * columns (1 GB of scratch at most beside the rows' own).
+ * columns (256 MB of d loss / d z at a time, at most 16384 rows at a time; beside it dW and dH in 32 bits where a sum is split, and
+ * what each entry of the rows needs).
  *
  *   H [dev][N][ldh], W [dev][K][ldw]: bf16 or fp32 (type), values contiguous within a row, any pitch
  *     and alignment (rows that are not whole 16-byte groups cost a copy of the operand).
- *   bias [dev][K] fp32 or NULL.  -inf takes a column out: its probability is 0, a count in it costs +inf.
+ *   K up to 2^29, D up to 2^20.
+ *   bias [dev][K] fp32 or NULL.  -inf takes a column out: its probability is 0, a count in it costs +inf.  Its weights do not
+ *     enter the loss, whatever they hold; dH has 0 times them.
  *   rows: what the counts are (a host struct of device pointers), see below.
  *   row_weights [dev][N] fp32 or NULL (ones): the gradient is that of sum_i row_weights[i] loss[i].
- *   loss [dev][N] fp32, unweighted.  A row without counts has loss 0 and gradient 0.
+ *   loss [dev][N] fp32, unweighted.  A row without counts has loss 0 and gradient 0; its features must be finite like all others.
  *   dH [dev][N][D], dW [dev][K][D] in H's type, dbias [dev][K] fp32 or NULL: overwritten, aligned to 16 bytes.
  * Sums, l and the row terms are held in 32 bits or more; d loss / d z is rounded once to H's type
  * before its products with W and H (dbias is summed before that rounding).  Results do not depend on timing:
@@ -594,6 +597,7 @@ int dme_synth_dirmult(void* X /*[dev]*/, int elem_bytes, int64_t N, int64_t K, i
  *       DME_ROWS_DENSE   X [N][ld], uint16 (elem 2) or int32 >= 0 (elem 4).
  * A row that breaks its format (a column out of range or out of order, a negative count, a label >= K,
  * a rowptr that runs backwards or beyond nnz) has loss NaN and makes the gradient NaN; nothing out of range is read.
+ * Where rowptr runs backwards, rows that take the same entries have no defined loss.
  * ------------------------------------------------------------------------------------------- */
 #define DME_TYPE_F32 0
 #define DME_TYPE_BF16 1
@@ -629,9 +633,10 @@ int dme_log_loss_gradient(const void* H /*[dev]*/, int64_t ldh, const void* W /*
 /* ---------------------------------------------------------------------------------------------
  * The orthogonalised step: `batch` matrices G (rows x cols, any strides, in elements) become
  * X = G / |G|_F, then `steps` times X <- a X + b X X'X + c X X'X X'X (products over the smaller side);
- * out [dev][batch][rows][cols], contiguous, in G's type.  A zero matrix stays zero.  bf16 matrices go through
- * fp16 products with 32-bit sums and a 32-bit X, fp32 matrices through fp32 products.  The coefficients
- * must keep singular values that begin in [0, 1] below 3.  The step that dme_predicted_step takes from a Hessian is taken
+ * out [dev][batch][rows][cols], contiguous, in G's type.  A zero matrix stays zero.  Products run on fp16
+ * operands with 32-bit sums: one for bf16 matrices, whose X is kept as a pair of fp16 values (22 bits); three, of pairs, for fp32
+ * matrices, whose X is kept in 32 bits (min(rows, cols) <= 64: fp32 products throughout).  The coefficients
+ * must keep singular values that begin in [0, 1] below 3.  The smaller side is at most 2^16, the larger one 2^28.  The step that dme_predicted_step takes from a Hessian is taken
  * here from the gradient alone: log-sum-exp losses are smooth in the spectral norm.
  * ------------------------------------------------------------------------------------------- */
 int64_t dme_orthogonal_step_workspace_bytes(int type, int64_t batch, int64_t rows, int64_t cols);

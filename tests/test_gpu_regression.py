@@ -499,6 +499,41 @@ def test_weights_beyond_32_bit_offsets(n):
     assert float((dh.double() - 0.125 * (3 * p - 1)).abs().max()) <= 3 * u * 0.125 * (1 + 3 * p)
 
 
+def test_more_tiles_than_a_launch_takes():
+    """16384 rows of 2^25 columns: tiles of 256 with a thread for 128 values each would be 2^32 threads."""
+    from bayespy_amd import regression
+    n, k, d = 16384, 1 << 25, 8
+    w = torch.zeros(k, d, dtype=torch.bfloat16, device="cuda")
+    w[-3:] = 0.5
+    h = torch.zeros(n, d, dtype=torch.bfloat16, device="cuda")
+    z = torch.tensor([0.0, 4.0, 8.0, 16.0], dtype=torch.float64)
+    h[:] = (z[torch.arange(n) % 4, None] / (0.5 * d)).to(torch.bfloat16).cuda()  # exact
+    y = torch.full((n,), k - 1, device="cuda")
+    loss = regression.log_loss(h, w, regression.CountRows.from_labels(y, k))
+    want = (torch.log((k - 3) + 3 * z.exp()) - z)[torch.arange(n) % 4]
+    # l - m in 64 bits from pieces that hold at most 2^14 ones each, and one rounding of a value up to 18
+    assert bool(((loss.cpu().double() - want).abs() <= 2.0**-19).all())
+
+
+def test_a_weight_at_the_end_of_its_range():
+    """weight * count leaves 32 bits in one row: its column is lost, columns without it are not."""
+    from bayespy_amd import regression
+    n, k, d = 40, 600, 16
+    h, w, b, x, _ = make(n, k, d, torch.float32, 4)
+    g = torch.ones(n, device="cuda")
+    b[:] = 0.0
+    b[300:] = -200.0  # p = 0 in 32 bits there
+    x[:, 300:] = 0
+    x[1:, 400] = 3000000
+    x[0, :] = 0
+    x[0, 5] = 2
+    g[0] = 3e38
+    for likelihood in ("multinomial", "dirichlet"):
+        _, _, _, db = regression.log_loss_gradient(h, w, as_rows(x, "csr"), bias=b, likelihood=likelihood, row_weights=g)
+        want = oracle(h[1:], w, b, x[1:], g[1:], likelihood, torch.float32)["db"]
+        near(db[300:], (want[0][300:], want[1][300:]), "dbias of columns that the row has not")
+
+
 # ---- how they are run ------------------------------------------------------------------------------------------------
 
 def _call_all(h, w, b, x, g, kind, likelihood):

@@ -26,7 +26,7 @@ def test_workspace_of_what_is_taken_and_refused():
     assert _bytes(_rows(), N=0) > 0
     assert _bytes(_rows(), gradient=0) < _bytes(_rows())
     assert _bytes(_rows(), D=15, ldh=16, ldw=16) > _bytes(_rows(), D=16)  # copies of the operands
-    for bad in (dict(type_=2), dict(N=-1), dict(K=0), dict(D=0), dict(ldh=8), dict(ldw=8), dict(H=0), dict(W=0), dict(W=8193), dict(K=1 << 31),
+    for bad in (dict(type_=2), dict(N=-1), dict(K=0), dict(D=0), dict(ldh=8), dict(ldw=8), dict(H=0), dict(W=0), dict(W=8193), dict(K=1 << 31), dict(K=(1 << 29) + 1),
                 dict(D=(1 << 20) + 1)):
         assert _bytes(_rows(), **bad) == -1, bad
     for rows in (_rows(kind=3), _rows(labels=0), _rows(kind=1, rowptr=0), _rows(kind=1, rowptr=8, nnz=-1), _rows(kind=1, rowptr=8, nnz=5),
