@@ -92,9 +92,9 @@ __device__ __forceinline__ float exp_f32(float z) {
 // (64 + 15)^15 < 2^96.  R = log prod_{1 <= n < x} (e^z + n) with one logarithm, G = 1 + e^z sum 1 / (e^z + n) with one
 // reciprocal of the same product: 15 roundings of 2^-24 at most.  Others take the 64-bit functions above.
 __device__ __forceinline__ bool is_small(float z, int x) { return x <= 16 && z <= 4.1f; }
-// N cells of a lane at once, x = 0 where a cell is none of these: the chains of products are independent of each other, and the loop runs
-// as far as the wave's largest count, so that no lane has a branch of its own.  Terms n and x - n are taken together,
-// (a + n) (a + x - n) = a (a + x) + n (x - n), which halves the loop; an even x leaves the term in the middle.
+// N cells of a lane at once, x = 0 where a cell is none of these: the chains of products are independent of each other.  The loop takes
+// PAIRS pairs of terms (x <= 2 PAIRS + 2), or runs as far as the wave's largest count (PAIRS = 0), so that no lane has a branch of its own.
+// A pair is terms n and x - n, (a + n) (a + x - n) = a (a + x) + n (x - n); an even x leaves the term in the middle.
 template <int N>
 __device__ __forceinline__ float most_of(const float (&x)[N]) {
     float most = x[0];
@@ -102,7 +102,7 @@ __device__ __forceinline__ float most_of(const float (&x)[N]) {
     for (int q = 1; q < N; ++q) most = fmaxf(most, x[q]);
     return most;
 }
-template <int N>
+template <int PAIRS, int N>
 __device__ __forceinline__ float small_rest(const float (&z)[N], const int (&x)[N]) {  // the sum over the cells
     float xf[N], ends[N], prod[N];
 #pragma unroll
@@ -112,20 +112,27 @@ __device__ __forceinline__ float small_rest(const float (&z)[N], const int (&x)[
         ends[q] = a * (a + xf[q]);
         prod[q] = x[q] > 0 && !(x[q] & 1) ? __builtin_fmaf(0.5f, xf[q], a) : 1.f;
     }
-    const float half = 0.5f * most_of(xf);
-    for (float n = 1.f; __any(n < half); n += 1.f)
+    const auto pair = [&](float n) {
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             const float other = xf[q] - n;
             prod[q] *= n < other ? __builtin_fmaf(n, other, ends[q]) : 1.f;
         }
+    };
+    if constexpr (PAIRS > 0) {
+#pragma unroll
+        for (int n = 1; n <= PAIRS; ++n) pair((float)n);
+    } else {
+        const float half = 0.5f * most_of(xf);
+        for (float n = 1.f; __any(n < half); n += 1.f) pair(n);
+    }
     float f = 0.f;
 #pragma unroll
     for (int q = 0; q < N; ++q) f += __builtin_amdgcn_logf(prod[q]);  // of 1 where there is no cell
     return f * 0.69314718f;
 }
 // Two terms of sum 1 / (a + n) make (2 a + x) / ((a + n) (a + x - n)).
-template <int N>
+template <int PAIRS, int N>
 __device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], float (&g)[N]) {
     float a[N], xf[N], ends[N], den[N], num[N];
 #pragma unroll
@@ -136,15 +143,22 @@ __device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], 
         den[q] = 1.f;
         num[q] = 0.f;
     }
-    const float half = 0.5f * most_of(xf);
-    for (float n = 1.f; __any(n < half); n += 1.f)
+    const auto pair = [&](float n) {
 #pragma unroll
         for (int q = 0; q < N; ++q) {
-            const float other = xf[q] - n, pair = __builtin_fmaf(n, other, ends[q]);
+            const float other = xf[q] - n, both = __builtin_fmaf(n, other, ends[q]);
             const bool in = n < other;
-            num[q] = in ? __builtin_fmaf(num[q], pair, den[q]) : num[q];
-            den[q] = in ? den[q] * pair : den[q];
+            num[q] = in ? __builtin_fmaf(num[q], both, den[q]) : num[q];
+            den[q] = in ? den[q] * both : den[q];
         }
+    };
+    if constexpr (PAIRS > 0) {
+#pragma unroll
+        for (int n = 1; n <= PAIRS; ++n) pair((float)n);
+    } else {
+        const float half = 0.5f * most_of(xf);
+        for (float n = 1.f; __any(n < half); n += 1.f) pair(n);
+    }
 #pragma unroll
     for (int q = 0; q < N; ++q) {
         const float middle = __builtin_fmaf(0.5f, xf[q], a[q]);  // 2 a + x is twice that
@@ -156,13 +170,13 @@ __device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], 
 __device__ __forceinline__ float small_rest(float z, int x) {
     const float zs[1] = {z};
     const int xs[1] = {x};
-    return small_rest(zs, xs);
+    return small_rest<0>(zs, xs);
 }
 __device__ __forceinline__ float small_g(float z, int x) {
     const float zs[1] = {z};
     const int xs[1] = {x};
     float g[1];
-    small_g(zs, xs, g);
+    small_g<0>(zs, xs, g);
     return g[0];
 }
 
@@ -600,17 +614,35 @@ struct Counts {
             }
         }
     }
-    template <int Q>
-    __device__ __forceinline__ int get(int elem) const {
-        if (elem == 2) return (int)(lo[Q / 2] >> (Q % 2 * 16) & 0xffff);
-        return (int)(Q < 4 ? lo[Q & 3] : hi[Q & 3]);
+    __device__ __forceinline__ void get(int elem, int (&v)[8]) const {
+        if (elem == 2) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (int)(lo[q / 2] >> (q % 2 * 16) & 0xffff);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (int)(q < 4 ? lo[q & 3] : hi[q & 3]);
+        }
     }
 };
 
-template <int Q = 0, class F>
-__device__ __forceinline__ void each_count(const Counts& c, int elem, F f) {
-    f(Q, c.get<Q>(elem));
-    if constexpr (Q < 7) each_count<Q + 1>(c, elem, f);
+// Dirichlet terms of a dense matrix: most counts are small, and a wave that runs each cell's loop to its largest count works for few
+// lanes.  Counts up to 6 take two pairs of terms where they are; the cells with others are put on a list of the wave in LDS and
+// taken 64 at a time, those for the 64-bit functions on a second one (16384 x 1000, counts of mean 1.1 and 45% of them above 0: LISTS).
+constexpr int NEAR = 6;             // two pairs and a middle term
+constexpr float NEAR_Z = 17.f;      // (e^17 + 6)^5 < 2^126
+constexpr int LIST = 512;           // cells that a wave makes at a time
+struct Lists {
+    u32 cell[4][LIST];              // row 7 b | column 7 b | count 18 b (all ones: to be read again); forward, later: R as a float
+    unsigned short far[4][128];     // places in `cell`
+    double f[128];                  // forward: of each row: the other cells' sum
+    unsigned short begin[128], end[128];  // forward: of each row: its places in `cell`
+};
+
+__device__ __forceinline__ int scan16(int v) {  // over the 16 lanes of a row, this one's included
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr: 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
 }
 
 // Tiles of z with a dense matrix of counts: every value of z may meet a count, so the tile lies in LDS in 32 bits, where a row's
@@ -623,7 +655,8 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * DT, k0 = a.column + c0;
     float* z = (float*)lds;
-    const int tid = threadIdx.x, sub = tid & 15;
+    Lists& lists = *(Lists*)(lds + TR * ZP * 4);
+    const int tid = threadIdx.x, sub = tid & 15, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Counts next;
     if (r0 + (tid >> 4) < a.nb) next.load(a.rows, r0 + (tid >> 4), k0 + sub * 8, a.K);
     {
@@ -642,76 +675,172 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     __syncthreads();
     const bool dirichlet = a.likelihood == DME_LIKELIHOOD_DIRICHLET;
     T* dz = (T*)a.dz;
+    u32* cell = lists.cell[wave];
+    unsigned short* far = lists.far[wave];
+    const auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };
+
+    // What the cell at a place of the list adds, made by one lane: from 32 bits or, where that is too little and `wide`, from 64.
+    const auto make = [&](int place, bool real, bool wide) {  // whether it is one for the other functions
+        const u32 c = real ? cell[place] : 0;
+        const int row = c >> 7 & 127, col = c & 127;
+        int x = (int)(c >> 14);
+        if (x == 0x3ffff) x = count_at(a.rows, r0 + row, k0 + col);
+        float* at = z + row * ZP + col;
+        const float v = real ? *at : 0.f;
+        const bool small = is_small(v, x);
+        if (__builtin_amdgcn_ballot_w64(real && small != wide) == 0) return real && !small && !wide;
+        float value;
+        if (!BACKWARD)
+            value = wide ? (float)dirichlet_rest((double)v, (double)x) : small_rest(small ? v : 0.f, small ? x : 0);
+        else
+            value = wide ? (float)dirichlet_g((double)v, (double)x) : small_g(small ? v : 0.f, small ? x : 0);
+        if (real && small != wide) {
+            if (!BACKWARD) {
+                cell[place] = __builtin_bit_cast(u32, value);
+            } else {
+                const long long r = r0 + row;
+                *at = exp_of(v, a.largest_z[r]) * a.coef[r] - a.weight[r] * value;
+            }
+        }
+        return real && !small && !wide;
+    };
+    // The listed cells, and then what is left to do for the rows from `from` to `to` (of this wave's lanes' rows, 16 apart).
+    int filled = 0, from = tid >> 4;
+    const auto empty = [&](int to) {
+        fence();
+        int others = 0;
+        for (int e = 0; e < filled; e += 64) {
+            const bool other = make(e + lane, e + lane < filled, false);
+            const u64 b = __builtin_amdgcn_ballot_w64(other);
+            if (other) far[others + (int)__builtin_amdgcn_mbcnt_hi((u32)(b >> 32), __builtin_amdgcn_mbcnt_lo((u32)b, 0))] = (unsigned short)(e + lane);
+            others += __builtin_popcountll(b);
+            fence();
+            if (others >= 64) {
+                make(far[lane], true, true);
+                others -= 64;
+                const unsigned short rest = far[64 + lane];
+                fence();
+                far[lane] = rest;
+                fence();
+            }
+        }
+        if (others > 0) make(lane < others ? far[lane] : 0, lane < others, true);
+        fence();
+        for (int row = from; row < to; row += 16) {
+            const long long r = r0 + row;
+            if (r >= a.nb) break;
+            if (!BACKWARD) {
+                double f = 0.0;
+                for (int e = lists.begin[row] + sub; e < lists.end[row]; e += 16) f += (double)__builtin_bit_cast(float, cell[e]);
+                f = sum16(f);
+                if (sub == 0) a.part_f[tc * a.nb + r] = lists.f[row] + f;
+            } else {
+                const float* zr = z + row * ZP + sub * 8;
+                dme_store4(dz + r * a.lddz + c0 + sub * 8, *(const f32x4*)zr);
+                dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, *(const f32x4*)(zr + 4));
+            }
+        }
+        from = to;
+        filled = 0;
+        fence();
+    };
+
 #pragma unroll 1
     for (int row = tid >> 4; row < TR; row += 16) {
         const long long r = r0 + row;
+        const bool real = r < a.nb;  // the same for all of a row's lanes
         float* zr = z + row * ZP + sub * 8;
-        if (r >= a.nb) {  // all of a row's lanes
+        if (__builtin_amdgcn_ballot_w64(real) == 0) {
             if (!BACKWARD) break;
             *(f32x4*)zr = *(f32x4*)(zr + 4) = f32x4{0.f, 0.f, 0.f, 0.f};
             continue;
         }
-        const Counts x = next;
+        int v[8];
+        next.get(a.rows.elem, v);
         if (row + 16 < TR && r + 16 < a.nb) next.load(a.rows, r + 16, k0 + sub * 8, a.K);
-        const f32x4 u = *(const f32x4*)zr, u2 = *(const f32x4*)(zr + 4);
+        const f32x4 left = *(const f32x4*)zr, right = *(const f32x4*)(zr + 4);
+        const float u[8] = {left[0], left[1], left[2], left[3], right[0], right[1], right[2], right[3]};
+        bool listed[8];
+        if (dirichlet) {
+            int mine = 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                listed[q] = real && v[q] > 1 && (v[q] > NEAR || !(u[q] <= NEAR_Z));
+                mine += listed[q];
+            }
+            const int upto = scan16(mine), n0 = __builtin_amdgcn_readlane(upto, 15), n1 = __builtin_amdgcn_readlane(upto, 31),
+                      n2 = __builtin_amdgcn_readlane(upto, 47), n3 = __builtin_amdgcn_readlane(upto, 63), all = n0 + n1 + n2 + n3;
+            if (filled + all > LIST) empty(row);
+            const int g = lane >> 4;
+            int at = filled + upto - mine + (g > 0 ? n0 : 0) + (g > 1 ? n1 : 0) + (g > 2 ? n2 : 0);
+            if (!BACKWARD) {
+                if (sub == 0) lists.begin[row] = (unsigned short)at;
+                if (sub == 15) lists.end[row] = (unsigned short)(at + mine);
+            }
+            if (all)
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (listed[q]) cell[at++] = (u32)(row * DT + sub * 8 + q) | (u32)(v[q] < 0x3ffff ? v[q] : 0x3ffff) << 14;
+            filled += all;
+        }
+        float zs[8];
+        int xs[8];
+        if (dirichlet)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const bool here = real && v[q] > 0 && !listed[q];
+                zs[q] = here && v[q] > 1 ? u[q] : 0.f;  // R(z, 1) = 0 and G(z, 1) = 1 however large z is
+                xs[q] = here ? v[q] : 0;
+            }
         if (!BACKWARD) {
-            const float m = max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(u2[0], u2[1]), fmaxf(u2[2], u2[3]))));
+            const float m = max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(u[4], u[5]), fmaxf(u[6], u[7]))));
             const float base = m == -INFINITY ? 0.f : m;
-            float s = 0.f;
-            double far = 0.0;
-            float f = 0.f;
+            float s = 0.f, f = 0.f;
             long long total = 0;
             int counts = 0;
             bool bad = false;
-            float zs[8];
-            int xs[8];
-            each_count(x, a.rows.elem, [&](int q, int v) {
-                const float zq = q < 4 ? u[q & 3] : u2[q & 3];
-                s += exp_of(zq, base);
-                bad |= v < 0;
-                total += v;
-                const bool small = v > 0 && is_small(zq, v);
-                zs[q] = small ? zq : 0.f;
-                xs[q] = small ? v : 0;
-                counts += v > 0;
-                f += v > 0 ? (zq - base) * (dirichlet ? 1.f : (float)v) : 0.f;
-                if (dirichlet && v > 0 && !small) far += dirichlet_rest((double)zq, (double)v);
-            });
-            if (dirichlet) f += small_rest(zs, xs);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                s += exp_of(u[q], base);
+                bad |= v[q] < 0;
+                total += v[q];
+                counts += v[q] > 0;
+                f += v[q] > 0 ? (u[q] - base) * (dirichlet ? 1.f : (float)v[q]) : 0.f;
+            }
+            if (dirichlet) f += small_rest<NEAR / 2 - 1>(zs, xs);
             s = sum16(s);
-            far = sum16(far + (double)f);
+            const double all = sum16((double)f);
             const double w = sum16(dirichlet ? (double)counts : (double)total);
             const double t = sum16(bad ? __builtin_nan("") : (double)total);
-            if (sub == 0) {
+            if (sub == 0 && real) {
                 a.part[tc * a.nb + r] = f32x2{m, s};
-                a.part_f[tc * a.nb + r] = far;
                 a.part_w[tc * a.nb + r] = w;
                 a.part_t[tc * a.nb + r] = t;
+                if (dirichlet)
+                    lists.f[row] = all;
+                else
+                    a.part_f[tc * a.nb + r] = all;
             }
         } else {
-            const float m = a.largest_z[r], cf = a.coef[r], weight = a.weight[r];
-            f32x4 d[2];
-            float zs[8], gs[8];
-            int xs[8];
-            each_count(x, a.rows.elem, [&](int q, int v) {
-                const float zq = q < 4 ? u[q & 3] : u2[q & 3];
-                const bool small = v > 0 && is_small(zq, v);
-                zs[q] = small ? zq : 0.f;
-                xs[q] = small ? v : 0;
-            });
-            if (dirichlet) small_g(zs, xs, gs);
-            each_count(x, a.rows.elem, [&](int q, int v) {
-                const float zq = q < 4 ? u[q & 3] : u2[q & 3];
-                float e = exp_of(zq, m) * cf;
-                if (v > 0) e -= weight * (!dirichlet ? (float)v : xs[q] > 0 ? gs[q] : (float)dirichlet_g((double)zq, (double)v));
-                d[q >> 2][q & 3] = e;
-            });
-            *(f32x4*)zr = d[0];
-            *(f32x4*)(zr + 4) = d[1];
-            dme_store4(dz + r * a.lddz + c0 + sub * 8, d[0]);
-            dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, d[1]);
+            const float m = real ? a.largest_z[r] : 0.f, cf = real ? a.coef[r] : 0.f, weight = real ? a.weight[r] : 0.f;
+            float gs[8], d[8];
+            if (dirichlet) small_g<NEAR / 2 - 1>(zs, xs, gs);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                float e = exp_of(u[q], m) * cf;
+                if (v[q] > 0) e -= weight * (dirichlet ? gs[q] : (float)v[q]);
+                d[q] = !real ? 0.f : dirichlet && listed[q] ? u[q] : e;  // a listed cell waits as it is
+            }
+            const f32x4 d0 = f32x4{d[0], d[1], d[2], d[3]}, d1 = f32x4{d[4], d[5], d[6], d[7]};
+            *(f32x4*)zr = d0;
+            *(f32x4*)(zr + 4) = d1;
+            if (!dirichlet && real) {
+                dme_store4(dz + r * a.lddz + c0 + sub * 8, d0);
+                dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, d1);
+            }
         }
     }
+    if (dirichlet) empty(TR);
     if (!BACKWARD || !a.dbias) return;
     __syncthreads();
     const int c = tid & 127, half = tid >> 7;
@@ -795,7 +924,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     }
     // the counts: their part of the loss relative to m, their total, and how often m goes into their part
     const bool dirichlet = a.likelihood == DME_LIKELIHOOD_DIRICHLET;
-    const double top = (double)m, over = log(s);
+    const double top = (double)m;
     const float weight = a.weights ? a.weights[rr] : 1.f;
     float most = 0.f;
     double f = 0.0, total = 0.0, times = 0.0;
@@ -868,20 +997,43 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         most = fmaxf(most, __shfl_xor(most, 32));
         if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(a.largest, __builtin_bit_cast(u32, most));
     }
-    if (!real || sub != 0) return;
-    const double l = top + over;
-    double loss = total == total ? -f : total;
-    if (dirichlet) {
-        loss += over + dirichlet_rest(l, total);
-        if (times != 1.0) loss += (1.0 - times) * top;
-    } else {
-        loss += total * over;
+    // the row's own terms take a thousand instructions in 64 bits: one wave makes the loss of all rows here, one the gradient's coefficients
+    const int part = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if constexpr (LANES == 16) {
+        if (sub == 0) {
+            s_seen[0][row] = s;
+            s_seen[1][row] = f;
+            s_seen[2][row] = total;
+            s_seen[3][row] = times;
+            m_seen[0][row] = m;
+        }
+        __syncthreads();
     }
-    a.loss[r] = total == 0.0 ? 0.f : (float)loss;
-    if (!a.largest_z) return;
-    a.largest_z[r] = total == 0.0 ? INFINITY : m;
-    a.coef[r] = total == 0.0 ? 0.f : (float)((double)weight * g_of(a.likelihood, l, total) / s);
-    a.weight[r] = weight;
+    if (lane >= ROWS || first + lane >= a.nb) return;
+    if constexpr (LANES == 16) {
+        s = s_seen[0][lane];
+        f = s_seen[1][lane];
+        total = s_seen[2][lane];
+        times = s_seen[3][lane];
+        m = m_seen[0][lane];
+    }
+    const long long at = first + lane;
+    const double over = log(s), l = (double)m + over;
+    if (part == 0) {
+        double loss = total == total ? -f : total;
+        if (dirichlet) {
+            loss += over + dirichlet_rest(l, total);
+            if (times != 1.0) loss += (1.0 - times) * (double)m;
+        } else {
+            loss += total * over;
+        }
+        a.loss[at] = total == 0.0 ? 0.f : (float)loss;
+    } else if (part == 1 && a.largest_z) {
+        const float w = a.weights ? a.weights[at] : 1.f;
+        a.largest_z[at] = total == 0.0 ? INFINITY : m;
+        a.coef[at] = total == 0.0 ? 0.f : (float)((double)w * g_of(a.likelihood, l, total) / s);
+        a.weight[at] = w;
+    }
 }
 
 struct PatchArgs {
@@ -1248,7 +1400,8 @@ int launch_side(const TileArgs& a, int side, hipStream_t s) {
 template <class T, int TR, bool BACKWARD>
 int launch_dense(const TileArgs& a, hipStream_t s) {
     typedef DmeTile<T, TR, DT, (TR == 16 ? 1 : 2), (TR == 16 ? 4 : 2)> Tile;
-    constexpr int bytes = Tile::LDS > TR * ZP * 4 ? Tile::LDS : TR * ZP * 4;
+    constexpr int bytes = Tile::LDS > TR * ZP * 4 + (int)sizeof(Lists) ? Tile::LDS : TR * ZP * 4 + (int)sizeof(Lists);
+    static_assert(2 * bytes <= 160 * 1024, "two workgroups a CU");
     static std::atomic<bool> done[64];
     const int rc = set_lds(done, dense_kernel<T, TR, BACKWARD>, bytes);
     if (rc) return rc;
