@@ -81,102 +81,90 @@ __device__ __forceinline__ double g_of(int likelihood, double z, double x) {
     return likelihood == DME_LIKELIHOOD_DIRICHLET ? dirichlet_g(z, x) : x;
 }
 
-// e^z in 32 bits, good to a few last bits however large |z|: the exponent's rounding is made up for.
-__device__ __forceinline__ float exp_f32(float z) {
-    const float t = z * LOG2E, rest = __builtin_fmaf(z, LOG2E, -t) + z * 1.9259630e-8f;  // log2 e - LOG2E
-    const float e = __builtin_amdgcn_exp2f(t);
-    return z > -100.f ? __builtin_fmaf(e, rest * 0.69314718f, e) : 0.f;  // (-inf - -inf) kept out
-}
-
-// The counts that most cells of a dense matrix hold: 1 <= x <= 16, and e^z small enough for 32-bit products of the 15 terms
-// (64 + 15)^15 < 2^96.  R = log prod_{1 <= n < x} (e^z + n) with one logarithm, G = 1 + e^z sum 1 / (e^z + n) with one
-// reciprocal of the same product: 15 roundings of 2^-24 at most.  Others take the 64-bit functions above.
-__device__ __forceinline__ bool is_small(float z, int x) { return x <= 16 && z <= 4.1f; }
-// N cells of a lane at once, x = 0 where a cell is none of these: the chains of products are independent of each other.  The loop takes
-// PAIRS pairs of terms (x <= 2 PAIRS + 2), or runs as far as the wave's largest count (PAIRS = 0), so that no lane has a branch of its own.
-// A pair is terms n and x - n, (a + n) (a + x - n) = a (a + x) + n (x - n); an even x leaves the term in the middle.
+// The counts that most cells hold, 1 <= x <= 16, in 32 bits.  With a = e^z the terms a + n, 1 <= n < x, are multiplied out, so that R takes
+// one logarithm and G, as sum 1 / (a + n) over the same product, one reciprocal.  For z > 0 they are taken over a: with w = 1 / a
+//     R = (x - 1) z + log prod (1 + n w)      G = 1 + sum 1 / (1 + n w)
+// and no product leaves 16!, however large |z| is.  Terms n and x - n are taken together, (a + n) (a + x - n) = a (a + x) + n (x - n), which
+// halves the loop; an even x leaves the term in the middle.  e^-|z| as 2^(z log2 e) is off as a z rounded once more would be, and z comes out of 32-bit
+// sums; the products round 15 times 2^-24 at most.  The loop runs as far as the wave's largest count: no lane has a branch of its own.
+__device__ __forceinline__ bool is_small(int x) { return x <= 16; }
+struct SmallTerms {
+    float x, one, ww, ends, middle;  // one = a, ww = 1, ends = a (a + x), middle = a + x / 2, or those over a, a^2, a^2 and a
+    bool far;
+    SmallTerms() = default;
+    __device__ __forceinline__ SmallTerms(float z, int count) {
+        far = z > 0.f;
+        const float e = __builtin_amdgcn_exp2f(-fabsf(z) * LOG2E), w = far ? e : 1.f;
+        x = (float)count;
+        one = far ? 1.f : e;
+        ww = w * w;
+        ends = one * __builtin_fmaf(x, w, one);
+        middle = __builtin_fmaf(0.5f * x, w, one);
+    }
+    __device__ __forceinline__ float pair(float n, float other) const { return __builtin_fmaf(n * other, ww, ends); }
+};
+// N cells of a lane at once; 0 < count <= 16 where there is a cell, 0 elsewhere
 template <int N>
-__device__ __forceinline__ float most_of(const float (&x)[N]) {
-    float most = x[0];
-#pragma unroll
-    for (int q = 1; q < N; ++q) most = fmaxf(most, x[q]);
-    return most;
-}
-template <int PAIRS, int N>
-__device__ __forceinline__ float small_rest(const float (&z)[N], const int (&x)[N]) {  // the sum over the cells
-    float xf[N], ends[N], prod[N];
+__device__ __forceinline__ void small_rest(const float (&z)[N], const int (&count)[N], float (&r)[N]) {
+    SmallTerms t[N];
+    float most = 0.f;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-        const float a = exp_f32(z[q]);
-        xf[q] = (float)x[q];
-        ends[q] = a * (a + xf[q]);
-        prod[q] = x[q] > 0 && !(x[q] & 1) ? __builtin_fmaf(0.5f, xf[q], a) : 1.f;
+        t[q] = SmallTerms(z[q], count[q]);
+        most = fmaxf(most, t[q].x);
+        r[q] = count[q] > 0 && !(count[q] & 1) ? t[q].middle : 1.f;
     }
-    const auto pair = [&](float n) {
+    for (float n = 1.f; __any(n < most - n); n += 1.f)
 #pragma unroll
         for (int q = 0; q < N; ++q) {
-            const float other = xf[q] - n;
-            prod[q] *= n < other ? __builtin_fmaf(n, other, ends[q]) : 1.f;
+            const float other = t[q].x - n;
+            r[q] *= n < other ? t[q].pair(n, other) : 1.f;
         }
-    };
-    if constexpr (PAIRS > 0) {
 #pragma unroll
-        for (int n = 1; n <= PAIRS; ++n) pair((float)n);
-    } else {
-        const float half = 0.5f * most_of(xf);
-        for (float n = 1.f; __any(n < half); n += 1.f) pair(n);
+    for (int q = 0; q < N; ++q) {
+        r[q] = __builtin_amdgcn_logf(r[q]) * 0.69314718f;
+        if (t[q].far && count[q] > 1) r[q] = __builtin_fmaf(t[q].x - 1.f, z[q], r[q]);
     }
-    float f = 0.f;
-#pragma unroll
-    for (int q = 0; q < N; ++q) f += __builtin_amdgcn_logf(prod[q]);  // of 1 where there is no cell
-    return f * 0.69314718f;
 }
 // Two terms of sum 1 / (a + n) make (2 a + x) / ((a + n) (a + x - n)).
-template <int PAIRS, int N>
-__device__ __forceinline__ void small_g(const float (&z)[N], const int (&x)[N], float (&g)[N]) {
-    float a[N], xf[N], ends[N], den[N], num[N];
+template <int N>
+__device__ __forceinline__ void small_g(const float (&z)[N], const int (&count)[N], float (&g)[N]) {
+    SmallTerms t[N];
+    float most = 0.f, num[N], den[N];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-        a[q] = exp_f32(z[q]);
-        xf[q] = (float)x[q];
-        ends[q] = a[q] * (a[q] + xf[q]);
-        den[q] = 1.f;
+        t[q] = SmallTerms(z[q], count[q]);
+        most = fmaxf(most, t[q].x);
         num[q] = 0.f;
+        den[q] = 1.f;
     }
-    const auto pair = [&](float n) {
+    for (float n = 1.f; __any(n < most - n); n += 1.f)
 #pragma unroll
         for (int q = 0; q < N; ++q) {
-            const float other = xf[q] - n, both = __builtin_fmaf(n, other, ends[q]);
+            const float other = t[q].x - n, both = t[q].pair(n, other);
             const bool in = n < other;
             num[q] = in ? __builtin_fmaf(num[q], both, den[q]) : num[q];
             den[q] = in ? den[q] * both : den[q];
         }
-    };
-    if constexpr (PAIRS > 0) {
-#pragma unroll
-        for (int n = 1; n <= PAIRS; ++n) pair((float)n);
-    } else {
-        const float half = 0.5f * most_of(xf);
-        for (float n = 1.f; __any(n < half); n += 1.f) pair(n);
-    }
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-        const float middle = __builtin_fmaf(0.5f, xf[q], a[q]);  // 2 a + x is twice that
-        float sum = 2.f * middle * num[q] * __builtin_amdgcn_rcpf(den[q]);
-        sum += !(x[q] & 1) ? __builtin_amdgcn_rcpf(middle) : 0.f;
-        g[q] = x[q] > 0 ? __builtin_fmaf(a[q], sum, 1.f) : 0.f;
+        float sum = 2.f * t[q].middle * num[q] * __builtin_amdgcn_rcpf(den[q]);
+        sum += !(count[q] & 1) ? __builtin_amdgcn_rcpf(t[q].middle) : 0.f;
+        g[q] = count[q] > 0 ? __builtin_fmaf(t[q].one, sum, 1.f) : 0.f;
     }
 }
-__device__ __forceinline__ float small_rest(float z, int x) {
+__device__ __forceinline__ float small_rest(float z, int count) {
     const float zs[1] = {z};
-    const int xs[1] = {x};
-    return small_rest<0>(zs, xs);
+    const int xs[1] = {count};
+    float r[1];
+    small_rest(zs, xs, r);
+    return r[0];
 }
-__device__ __forceinline__ float small_g(float z, int x) {
+__device__ __forceinline__ float small_g(float z, int count) {
     const float zs[1] = {z};
-    const int xs[1] = {x};
+    const int xs[1] = {count};
     float g[1];
-    small_g<0>(zs, xs, g);
+    small_g(zs, xs, g);
     return g[0];
 }
 
@@ -625,17 +613,18 @@ struct Counts {
     }
 };
 
-// Dirichlet terms of a dense matrix: most counts are small, and a wave that runs each cell's loop to its largest count works for few
-// lanes.  Counts up to 6 take two pairs of terms where they are; the cells with others are put on a list of the wave in LDS and
-// taken 64 at a time, those for the 64-bit functions on a second one (16384 x 1000, counts of mean 1.1 and 45% of them above 0: LISTS).
-constexpr int NEAR = 6;             // two pairs and a middle term
-constexpr float NEAR_Z = 17.f;      // (e^17 + 6)^5 < 2^126
-constexpr int LIST = 512;           // cells that a wave makes at a time
+// Dirichlet terms of a dense matrix: R(z, 1) = 0 and G(z, 1) = 1, and a wave that ran every cell's loop to the largest of its counts would
+// work for few lanes.  A wave's cells with counts above 1 are put on a list in LDS instead, their z left where it is, and taken 128 at a time; those
+// for the 64-bit functions go on to a second list and are taken 64 at a time or at the end (LISTS).
+constexpr int LIST = 512;            // cells that a wave makes at a time
+template <int WAVES>
 struct Lists {
-    u32 cell[4][LIST];              // row 7 b | column 7 b | count 18 b (all ones: to be read again); forward, later: R as a float
-    unsigned short far[4][128];     // places in `cell`
-    double f[128];                  // forward: of each row: the other cells' sum
-    unsigned short begin[128], end[128];  // forward: of each row: its places in `cell`
+    unsigned short cell[WAVES][LIST + 64];  // row of the wave 4 b | column 7 b | count 5 b (31: or more); 64 places for what is not listed
+    unsigned short far[WAVES][128];
+    union {
+        double f[128];               // forward: of each row: what its sum has beside the listed cells
+        float row[128][3];           // backward: of each row: m, coefficient, weight
+    };
 };
 
 __device__ __forceinline__ int scan16(int v) {  // over the 16 lanes of a row, this one's included
@@ -645,17 +634,26 @@ __device__ __forceinline__ int scan16(int v) {  // over the 16 lanes of a row, t
     return v + __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
 }
 
+template <class T, int TR>
+struct Dense {
+    static constexpr int NT = TR == 16 ? 256 : 512, WAVES = NT / 64;
+    typedef DmeTile<T, TR, DT, (TR == 16 ? 1 : 4), (TR == 16 ? 4 : 2)> Tile;
+    static constexpr int USED = TR * ZP * 4 + (int)sizeof(Lists<WAVES>), LDS = Tile::LDS > USED ? Tile::LDS : USED;
+    static_assert(2 * LDS <= 160 * 1024, "two workgroups a CU");
+};
+
 // Tiles of z with a dense matrix of counts: every value of z may meet a count, so the tile lies in LDS in 32 bits, where a row's
 // 16 lanes read it beside the counts, eight neighbouring columns a lane, the next rows' counts on their way.
 template <class T, int TR, bool BACKWARD>
-__global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
+__global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeTile<T, TR, DT, (TR == 16 ? 1 : 2), (TR == 16 ? 4 : 2)> Tile;
+    typedef typename Dense<T, TR>::Tile Tile;
+    constexpr int NT = Dense<T, TR>::NT, WAVES = Dense<T, TR>::WAVES, STEP = NT / 16;  // rows at a time
     long long tr, tc;
     dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
     const long long r0 = tr * TR, c0 = tc * DT, k0 = a.column + c0;
     float* z = (float*)lds;
-    Lists& lists = *(Lists*)(lds + TR * ZP * 4);
+    Lists<WAVES>& lists = *(Lists<WAVES>*)(lds + TR * ZP * 4);
     const int tid = threadIdx.x, sub = tid & 15, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Counts next;
     if (r0 + (tid >> 4) < a.nb) next.load(a.rows, r0 + (tid >> 4), k0 + sub * 8, a.K);
@@ -675,78 +673,70 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
     __syncthreads();
     const bool dirichlet = a.likelihood == DME_LIKELIHOOD_DIRICHLET;
     T* dz = (T*)a.dz;
-    u32* cell = lists.cell[wave];
-    unsigned short* far = lists.far[wave];
+    unsigned short *cell = lists.cell[wave], *far = lists.far[wave];
     const auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };
-
-    // What the cell at a place of the list adds, made by one lane: from 32 bits or, where that is too little and `wide`, from 64.
-    const auto make = [&](int place, bool real, bool wide) {  // whether it is one for the other functions
-        const u32 c = real ? cell[place] : 0;
-        const int row = c >> 7 & 127, col = c & 127;
-        int x = (int)(c >> 14);
-        if (x == 0x3ffff) x = count_at(a.rows, r0 + row, k0 + col);
-        float* at = z + row * ZP + col;
-        const float v = real ? *at : 0.f;
-        const bool small = is_small(v, x);
-        if (__builtin_amdgcn_ballot_w64(real && small != wide) == 0) return real && !small && !wide;
-        float value;
-        if (!BACKWARD)
-            value = wide ? (float)dirichlet_rest((double)v, (double)x) : small_rest(small ? v : 0.f, small ? x : 0);
-        else
-            value = wide ? (float)dirichlet_g((double)v, (double)x) : small_g(small ? v : 0.f, small ? x : 0);
-        if (real && small != wide) {
-            if (!BACKWARD) {
-                cell[place] = __builtin_bit_cast(u32, value);
-            } else {
-                const long long r = r0 + row;
-                *at = exp_of(v, a.largest_z[r]) * a.coef[r] - a.weight[r] * value;
-            }
-        }
-        return real && !small && !wide;
+    const auto row_of = [&](int code) { return (code >> 9 & 3) * STEP + wave * 4 + (code >> 7 & 3); };
+    // the listed cell's value in place of its z
+    const auto put = [&](int code, float v, float value) {
+        const int row = row_of(code);
+        const float* of = lists.row[row];
+        z[row * ZP + (code & 127)] = BACKWARD ? exp_of(v, of[0]) * of[1] - of[2] * value : value;
     };
-    // The listed cells, and then what is left to do for the rows from `from` to `to` (of this wave's lanes' rows, 16 apart).
-    int filled = 0, from = tid >> 4;
-    const auto empty = [&](int to) {
+    int filled = 0, others = 0;
+    const auto make_others = [&](int n) {
+        const int code = lane < n ? far[lane] : 0, row = row_of(code);
+        int x = code >> 11;
+        if (x == 31) x = count_at(a.rows, r0 + row, k0 + (code & 127));
+        const float v = z[row * ZP + (code & 127)];
+        const float value = (float)(BACKWARD ? dirichlet_g((double)v, (double)x) : dirichlet_rest((double)v, (double)x));
+        if (lane < n) put(code, v, value);
+    };
+    const auto make = [&] {
+        constexpr int N = 2;
         fence();
-        int others = 0;
-        for (int e = 0; e < filled; e += 64) {
-            const bool other = make(e + lane, e + lane < filled, false);
-            const u64 b = __builtin_amdgcn_ballot_w64(other);
-            if (other) far[others + (int)__builtin_amdgcn_mbcnt_hi((u32)(b >> 32), __builtin_amdgcn_mbcnt_lo((u32)b, 0))] = (unsigned short)(e + lane);
-            others += __builtin_popcountll(b);
-            fence();
-            if (others >= 64) {
-                make(far[lane], true, true);
-                others -= 64;
-                const unsigned short rest = far[64 + lane];
-                fence();
-                far[lane] = rest;
-                fence();
+        for (int e = 0; e < filled; e += 64 * N) {
+            int code[N], x[N];
+            float v[N], value[N];
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int at = e + u * 64 + lane;
+                code[u] = at < filled ? cell[at] : 0;
+                x[u] = code[u] >> 11;
+                v[u] = z[row_of(code[u]) * ZP + (code[u] & 127)];
+                const bool other = !is_small(x[u]);
+                const u64 b = __builtin_amdgcn_ballot_w64(other);
+                if (b) {
+                    if (other) {
+                        far[others + (int)__builtin_amdgcn_mbcnt_hi((u32)(b >> 32), __builtin_amdgcn_mbcnt_lo((u32)b, 0))] = (unsigned short)code[u];
+                        x[u] = 0;
+                    }
+                    others += __builtin_popcountll(b);
+                    fence();
+                    if (others >= 64) {
+                        make_others(64);
+                        others -= 64;
+                        const unsigned short rest = far[64 + lane];
+                        fence();
+                        far[lane] = rest;
+                        fence();
+                    }
+                }
             }
+            if (BACKWARD)
+                small_g(v, x, value);
+            else
+                small_rest(v, x, value);
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (x[u] > 0) put(code[u], v[u], value[u]);
         }
-        if (others > 0) make(lane < others ? far[lane] : 0, lane < others, true);
-        fence();
-        for (int row = from; row < to; row += 16) {
-            const long long r = r0 + row;
-            if (r >= a.nb) break;
-            if (!BACKWARD) {
-                double f = 0.0;
-                for (int e = lists.begin[row] + sub; e < lists.end[row]; e += 16) f += (double)__builtin_bit_cast(float, cell[e]);
-                f = sum16(f);
-                if (sub == 0) a.part_f[tc * a.nb + r] = lists.f[row] + f;
-            } else {
-                const float* zr = z + row * ZP + sub * 8;
-                dme_store4(dz + r * a.lddz + c0 + sub * 8, *(const f32x4*)zr);
-                dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, *(const f32x4*)(zr + 4));
-            }
-        }
-        from = to;
         filled = 0;
         fence();
     };
 
 #pragma unroll 1
-    for (int row = tid >> 4; row < TR; row += 16) {
+    for (int it = 0; it < TR / STEP; ++it) {
+        const int row = it * STEP + (tid >> 4);
         const long long r = r0 + row;
         const bool real = r < a.nb;  // the same for all of a row's lanes
         float* zr = z + row * ZP + sub * 8;
@@ -757,7 +747,7 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
         }
         int v[8];
         next.get(a.rows.elem, v);
-        if (row + 16 < TR && r + 16 < a.nb) next.load(a.rows, r + 16, k0 + sub * 8, a.K);
+        if (it + 1 < TR / STEP && r + STEP < a.nb) next.load(a.rows, r + STEP, k0 + sub * 8, a.K);
         const f32x4 left = *(const f32x4*)zr, right = *(const f32x4*)(zr + 4);
         const float u[8] = {left[0], left[1], left[2], left[3], right[0], right[1], right[2], right[3]};
         bool listed[8];
@@ -765,53 +755,42 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
             int mine = 0;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                listed[q] = real && v[q] > 1 && (v[q] > NEAR || !(u[q] <= NEAR_Z));
+                listed[q] = real && v[q] > 1;
                 mine += listed[q];
             }
             const int upto = scan16(mine), n0 = __builtin_amdgcn_readlane(upto, 15), n1 = __builtin_amdgcn_readlane(upto, 31),
                       n2 = __builtin_amdgcn_readlane(upto, 47), n3 = __builtin_amdgcn_readlane(upto, 63), all = n0 + n1 + n2 + n3;
-            if (filled + all > LIST) empty(row);
-            const int g = lane >> 4;
+            if (filled + all > LIST) make();
+            const int g = lane >> 4, code = it << 9 | g << 7 | sub * 8;
             int at = filled + upto - mine + (g > 0 ? n0 : 0) + (g > 1 ? n1 : 0) + (g > 2 ? n2 : 0);
-            if (!BACKWARD) {
-                if (sub == 0) lists.begin[row] = (unsigned short)at;
-                if (sub == 15) lists.end[row] = (unsigned short)(at + mine);
-            }
             if (all)
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (listed[q]) cell[at++] = (u32)(row * DT + sub * 8 + q) | (u32)(v[q] < 0x3ffff ? v[q] : 0x3ffff) << 14;
+                for (int q = 0; q < 8; ++q) {
+                    cell[listed[q] ? at : LIST + lane] = (unsigned short)(code + q | (v[q] < 31 ? v[q] : 31) << 11);
+                    at += listed[q];
+                }
             filled += all;
         }
-        float zs[8];
-        int xs[8];
-        if (dirichlet)
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const bool here = real && v[q] > 0 && !listed[q];
-                zs[q] = here && v[q] > 1 ? u[q] : 0.f;  // R(z, 1) = 0 and G(z, 1) = 1 however large z is
-                xs[q] = here ? v[q] : 0;
-            }
+        float d[8];  // what takes the place of z; a listed cell waits as it is
         if (!BACKWARD) {
             const float m = max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(u[4], u[5]), fmaxf(u[6], u[7]))));
             const float base = m == -INFINITY ? 0.f : m;
             float s = 0.f, f = 0.f;
-            long long total = 0;
-            int counts = 0;
-            bool bad = false;
+            u64 total = 0;
+            int counts = 0, least = 0;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 s += exp_of(u[q], base);
-                bad |= v[q] < 0;
-                total += v[q];
+                least = v[q] < least ? v[q] : least;
+                total += (u32)v[q];
                 counts += v[q] > 0;
                 f += v[q] > 0 ? (u[q] - base) * (dirichlet ? 1.f : (float)v[q]) : 0.f;
+                d[q] = dirichlet && listed[q] ? u[q] : 0.f;
             }
-            if (dirichlet) f += small_rest<NEAR / 2 - 1>(zs, xs);
             s = sum16(s);
             const double all = sum16((double)f);
             const double w = sum16(dirichlet ? (double)counts : (double)total);
-            const double t = sum16(bad ? __builtin_nan("") : (double)total);
+            const double t = sum16(least < 0 ? __builtin_nan("") : (double)total);
             if (sub == 0 && real) {
                 a.part[tc * a.nb + r] = f32x2{m, s};
                 a.part_w[tc * a.nb + r] = w;
@@ -823,34 +802,55 @@ __global__ __launch_bounds__(256, 2) void dense_kernel(TileArgs a) {
             }
         } else {
             const float m = real ? a.largest_z[r] : 0.f, cf = real ? a.coef[r] : 0.f, weight = real ? a.weight[r] : 0.f;
-            float gs[8], d[8];
-            if (dirichlet) small_g<NEAR / 2 - 1>(zs, xs, gs);
+            if (dirichlet && sub < 3) lists.row[row][sub] = sub == 0 ? m : sub == 1 ? cf : weight;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 float e = exp_of(u[q], m) * cf;
-                if (v[q] > 0) e -= weight * (dirichlet ? gs[q] : (float)v[q]);
-                d[q] = !real ? 0.f : dirichlet && listed[q] ? u[q] : e;  // a listed cell waits as it is
+                if (v[q] > 0) e -= weight * (dirichlet ? 1.f : (float)v[q]);
+                d[q] = !real ? 0.f : dirichlet && listed[q] ? u[q] : e;
             }
-            const f32x4 d0 = f32x4{d[0], d[1], d[2], d[3]}, d1 = f32x4{d[4], d[5], d[6], d[7]};
-            *(f32x4*)zr = d0;
-            *(f32x4*)(zr + 4) = d1;
             if (!dirichlet && real) {
-                dme_store4(dz + r * a.lddz + c0 + sub * 8, d0);
-                dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, d1);
+                dme_store4(dz + r * a.lddz + c0 + sub * 8, f32x4{d[0], d[1], d[2], d[3]});
+                dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, f32x4{d[4], d[5], d[6], d[7]});
+            }
+        }
+        if (BACKWARD || dirichlet) {
+            *(f32x4*)zr = f32x4{d[0], d[1], d[2], d[3]};
+            *(f32x4*)(zr + 4) = f32x4{d[4], d[5], d[6], d[7]};
+        }
+    }
+    if (dirichlet) {
+        make();
+        if (others) make_others(others);
+        fence();
+        for (int row = tid >> 4; row < TR; row += STEP) {
+            const long long r = r0 + row;
+            if (r >= a.nb) break;
+            const f32x4 left = *(const f32x4*)(z + row * ZP + sub * 8), right = *(const f32x4*)(z + row * ZP + sub * 8 + 4);
+            if (!BACKWARD) {
+                const f32x4 both = left + right;
+                const double f = sum16((double)((both[0] + both[1]) + (both[2] + both[3])));
+                if (sub == 0) a.part_f[tc * a.nb + r] = lists.f[row] + f;
+            } else {
+                dme_store4(dz + r * a.lddz + c0 + sub * 8, left);
+                dme_store4(dz + r * a.lddz + c0 + sub * 8 + 4, right);
             }
         }
     }
-    if (dirichlet) empty(TR);
     if (!BACKWARD || !a.dbias) return;
     __syncthreads();
-    const int c = tid & 127, half = tid >> 7;
+    const int c = tid % DT, piece = tid / DT;
+    constexpr int PIECES = NT / DT;
     float sum = 0.f;
 #pragma unroll 4
-    for (int row = half * (TR / 2); row < (half + 1) * (TR / 2); ++row) sum += z[row * ZP + c];
+    for (int row = piece * (TR / PIECES); row < (piece + 1) * (TR / PIECES); ++row) sum += z[row * ZP + c];
     __syncthreads();
-    if (half) z[c] = sum;
+    if (piece) z[piece * ZP + c] = sum;
     __syncthreads();
-    if (!half && k0 + c < a.K) a.dbias[tr * a.K + k0 + c] = sum + z[c];
+    if (piece || k0 + c >= a.K) return;
+#pragma unroll
+    for (int q = 1; q < PIECES; ++q) sum += z[q * ZP + c];
+    a.dbias[tr * a.K + k0 + c] = sum;
 }
 
 struct RowArgs {
@@ -949,7 +949,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
             }
             const float z = a.entry_z[e];
             total += (double)x;
-            const bool small = dirichlet && x > 0 && is_small(z, x);
+            const bool small = dirichlet && x > 0 && is_small(x);
             if (x > 0) {
                 times += dirichlet ? 1.0 : (double)x;
                 f += ((double)z - top) * (dirichlet ? 1.0 : (double)x);
@@ -1399,13 +1399,11 @@ int launch_side(const TileArgs& a, int side, hipStream_t s) {
 
 template <class T, int TR, bool BACKWARD>
 int launch_dense(const TileArgs& a, hipStream_t s) {
-    typedef DmeTile<T, TR, DT, (TR == 16 ? 1 : 2), (TR == 16 ? 4 : 2)> Tile;
-    constexpr int bytes = Tile::LDS > TR * ZP * 4 + (int)sizeof(Lists) ? Tile::LDS : TR * ZP * 4 + (int)sizeof(Lists);
-    static_assert(2 * bytes <= 160 * 1024, "two workgroups a CU");
+    typedef Dense<T, TR> D;
     static std::atomic<bool> done[64];
-    const int rc = set_lds(done, dense_kernel<T, TR, BACKWARD>, bytes);
+    const int rc = set_lds(done, dense_kernel<T, TR, BACKWARD>, D::LDS);
     if (rc) return rc;
-    hipLaunchKernelGGL((dense_kernel<T, TR, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c)), dim3(256), bytes, s, a);
+    hipLaunchKernelGGL((dense_kernel<T, TR, BACKWARD>), dim3((unsigned)(a.tiles_r * a.tiles_c)), dim3(D::NT), D::LDS, s, a);
     return DME_OK;
 }
 
