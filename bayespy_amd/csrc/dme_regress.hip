@@ -185,6 +185,12 @@ __device__ __forceinline__ float sum16(float v) {
     v += dpp_f32<DME_DPP_HALF_MIRROR>(v);
     return v + dpp_f32<DME_DPP_MIRROR>(v);
 }
+__device__ __forceinline__ int sum16(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, DME_DPP_QUAD_XOR1, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, DME_DPP_QUAD_XOR2, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, DME_DPP_HALF_MIRROR, 0xf, 0xf, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, DME_DPP_MIRROR, 0xf, 0xf, false);
+}
 __device__ __forceinline__ double sum16(double v) {
     v += dme_dpp_f64<DME_DPP_QUAD_XOR1>(v);
     v += dme_dpp_f64<DME_DPP_QUAD_XOR2>(v);
@@ -615,12 +621,13 @@ struct Counts {
 
 // Dirichlet terms of a dense matrix: R(z, 1) = 0 and G(z, 1) = 1, and a wave that ran every cell's loop to the largest of its counts would
 // work for few lanes.  A wave's cells with counts above 1 are put on a list in LDS instead, their z left where it is, and taken 128 at a time; those
-// for the 64-bit functions go on to a second list and are taken 64 at a time or at the end (LISTS).
+// for the 64-bit functions go on to a second list and are taken 64 at a time or, the workgroup's few together, at the end (LISTS).
 constexpr int LIST = 512;            // cells that a wave makes at a time
 template <int WAVES>
 struct Lists {
     unsigned short cell[WAVES][LIST + 64];  // row of the wave 4 b | column 7 b | count 5 b (31: or more); 64 places for what is not listed
     unsigned short far[WAVES][128];
+    int others[WAVES];               // how many of those a wave has left
     union {
         double f[128];               // forward: of each row: what its sum has beside the listed cells
         float row[128][3];           // backward: of each row: m, coefficient, weight
@@ -657,17 +664,29 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
     const int tid = threadIdx.x, sub = tid & 15, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Counts next;
     if (r0 + (tid >> 4) < a.nb) next.load(a.rows, r0 + (tid >> 4), k0 + sub * 8, a.K);
+    float m_row = 0.f, cf_row = 0.f, weight_row = 0.f;  // of row `tid`
+    if (BACKWARD && tid < TR && r0 + tid < a.nb) {
+        m_row = a.largest_z[r0 + tid];
+        cf_row = a.coef[r0 + tid];
+        weight_row = a.weight[r0 + tid];
+    }
     {
         Tile t;
         t.clear();
         t.run(a.h, a.w, a.D, lds, r0, c0, 0, a.slices);
+        const bool inside = k0 + DT <= a.K;  // then no lane looks at its columns
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) {
             const int c = Tile::col_of(i);
-            const f32x4 b = bias_of(a, k0 + c);
+            const f32x4 b = inside && a.bias ? *(const f32x4_u*)(a.bias + k0 + c) : bias_of(a, k0 + c);
             const bool out = any_out(b);
 #pragma unroll
             for (int j = 0; j < Tile::NJ; ++j) *(f32x4*)(z + Tile::row_of(j) * ZP + c) = with_bias(t.acc[i][j], b, out);
+        }
+        if (BACKWARD && tid < TR) {
+            lists.row[tid][0] = m_row;
+            lists.row[tid][1] = cf_row;
+            lists.row[tid][2] = weight_row;
         }
     }
     __syncthreads();
@@ -675,21 +694,20 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
     T* dz = (T*)a.dz;
     unsigned short *cell = lists.cell[wave], *far = lists.far[wave];
     const auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };
-    const auto row_of = [&](int code) { return (code >> 9 & 3) * STEP + wave * 4 + (code >> 7 & 3); };
-    // the listed cell's value in place of its z
-    const auto put = [&](int code, float v, float value) {
-        const int row = row_of(code);
+    const auto row_of = [&](int code, int of) { return (code >> 9 & 3) * STEP + of * 4 + (code >> 7 & 3); };
+    // a listed cell's value in place of its z
+    const auto put = [&](int code, int row, float v, float value) {
         const float* of = lists.row[row];
         z[row * ZP + (code & 127)] = BACKWARD ? exp_of(v, of[0]) * of[1] - of[2] * value : value;
     };
     int filled = 0, others = 0;
-    const auto make_others = [&](int n) {
-        const int code = lane < n ? far[lane] : 0, row = row_of(code);
+    const auto make_other = [&](bool real, int code, int by) {
+        const int row = row_of(code, by);
         int x = code >> 11;
         if (x == 31) x = count_at(a.rows, r0 + row, k0 + (code & 127));
         const float v = z[row * ZP + (code & 127)];
         const float value = (float)(BACKWARD ? dirichlet_g((double)v, (double)x) : dirichlet_rest((double)v, (double)x));
-        if (lane < n) put(code, v, value);
+        if (real) put(code, row, v, value);
     };
     const auto make = [&] {
         constexpr int N = 2;
@@ -702,7 +720,7 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
                 const int at = e + u * 64 + lane;
                 code[u] = at < filled ? cell[at] : 0;
                 x[u] = code[u] >> 11;
-                v[u] = z[row_of(code[u]) * ZP + (code[u] & 127)];
+                v[u] = z[row_of(code[u], wave) * ZP + (code[u] & 127)];
                 const bool other = !is_small(x[u]);
                 const u64 b = __builtin_amdgcn_ballot_w64(other);
                 if (b) {
@@ -713,7 +731,7 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
                     others += __builtin_popcountll(b);
                     fence();
                     if (others >= 64) {
-                        make_others(64);
+                        make_other(true, far[lane], wave);
                         others -= 64;
                         const unsigned short rest = far[64 + lane];
                         fence();
@@ -728,7 +746,7 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
                 small_rest(v, x, value);
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (x[u] > 0) put(code[u], v[u], value[u]);
+                if (x[u] > 0) put(code[u], row_of(code[u], wave), v[u], value[u]);
         }
         filled = 0;
         fence();
@@ -776,21 +794,41 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
             const float m = max16(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(u[4], u[5]), fmaxf(u[6], u[7]))));
             const float base = m == -INFINITY ? 0.f : m;
             float s = 0.f, f = 0.f;
-            u64 total = 0;
-            int counts = 0, least = 0;
+            if (!__any(fabsf(base) > FAR)) {
+                const Reference e(base);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) s += e(u[q]);
+                s *= e.rest;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) s += exp_of(u[q], base);
+            }
+            int counts = 0;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                s += exp_of(u[q], base);
-                least = v[q] < least ? v[q] : least;
-                total += (u32)v[q];
                 counts += v[q] > 0;
                 f += v[q] > 0 ? (u[q] - base) * (dirichlet ? 1.f : (float)v[q]) : 0.f;
                 d[q] = dirichlet && listed[q] ? u[q] : 0.f;
             }
             s = sum16(s);
             const double all = sum16((double)f);
-            const double w = sum16(dirichlet ? (double)counts : (double)total);
-            const double t = sum16(least < 0 ? __builtin_nan("") : (double)total);
+            double t;
+            if (a.rows.elem == 2) {
+                int total = 0;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) total += v[q];
+                t = (double)sum16(total);
+            } else {
+                u64 total = 0;
+                int least = 0;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    total += (u32)v[q];
+                    least = v[q] < least ? v[q] : least;
+                }
+                t = sum16(least < 0 ? __builtin_nan("") : (double)total);
+            }
+            const double w = dirichlet ? (double)sum16(counts) : t;
             if (sub == 0 && real) {
                 a.part[tc * a.nb + r] = f32x2{m, s};
                 a.part_w[tc * a.nb + r] = w;
@@ -801,8 +839,7 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
                     a.part_f[tc * a.nb + r] = all;
             }
         } else {
-            const float m = real ? a.largest_z[r] : 0.f, cf = real ? a.coef[r] : 0.f, weight = real ? a.weight[r] : 0.f;
-            if (dirichlet && sub < 3) lists.row[row][sub] = sub == 0 ? m : sub == 1 ? cf : weight;
+            const float m = lists.row[row][0], cf = lists.row[row][1], weight = lists.row[row][2];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 float e = exp_of(u[q], m) * cf;
@@ -821,8 +858,24 @@ __global__ __launch_bounds__(TR == 16 ? 256 : 512, TR == 16 ? 2 : 4) void dense_
     }
     if (dirichlet) {
         make();
-        if (others) make_others(others);
-        fence();
+        if (lane == 0) lists.others[wave] = others;
+        __syncthreads();
+        for (int base = wave * 64;; base += NT) {
+            int at = base + lane, by = 0, all = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const int n = lists.others[w];
+                if (w < WAVES - 1 && base + lane >= all + n) {
+                    at = base + lane - all - n;
+                    by = w + 1;
+                }
+                all += n;
+            }
+            if (base >= all) break;
+            const bool in = base + lane < all;
+            make_other(in, in ? lists.far[by][at] : 0, in ? by : 0);
+        }
+        __syncthreads();
         for (int row = tid >> 4; row < TR; row += STEP) {
             const long long r = r0 + row;
             if (r >= a.nb) break;
