@@ -405,142 +405,112 @@ struct SmallArgs {
     long long out_batch, out_n, out_m;
 };
 
-// acc[i] += P[r][k] Q[c][k] over 64 k; this wave's 16 r, all c in four blocks.  P, Q: lines of SP values in LDS.
-__device__ __forceinline__ void small_product(f32x4 (&acc)[4], const float* P, const float* Q) {
+// Sixteen waves, each with 16 x 16 of the 64 x 64 values: a thread has one group of four of everything, so that all pieces of S are on their
+// way at once.
+constexpr int SMALL_THREADS = 1024;
+
+// acc += P[r][k] Q[c][k] over 64 k.  P, Q: lines of SP values in LDS.
+__device__ __forceinline__ void small_product(f32x4& acc, const float* P, const float* Q) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int k = 0; k < SMALL; k += 16) {
-        const u32q p = *(const u32q*)(P + (wave * 16 + c) * SP + k + g * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = dme_mma(*(const u32q*)(Q + (i * 16 + c) * SP + k + g * 4), p, acc[i], float());
-    }
+    for (int k = 0; k < SMALL; k += 16)
+        acc = dme_mma(*(const u32q*)(Q + ((wave & 3) * 16 + c) * SP + k + g * 4), *(const u32q*)(P + ((wave >> 2) * 16 + c) * SP + k + g * 4), acc, float());
 }
 
-// acc[i] += X[k][r] X[k][c] over 64 lines k
-__device__ __forceinline__ void small_square(f32x4 (&acc)[4], const float* X) {
+// acc += X[k][r] X[k][c] over 64 lines k
+__device__ __forceinline__ void small_square(f32x4& acc, const float* X) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int k = 0; k < SMALL; k += 4) {
         const float* line = X + (k + g) * SP + c;
-        const float p = line[wave * 16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(line[i * 16], p, acc[i], 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(line[(wave & 3) * 16], line[(wave >> 2) * 16], acc, 0, 0, 0);
     }
 }
 
-// this workgroup's piece of S
-__device__ __forceinline__ void small_leave(const f32x4 (&acc)[4], float* part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *(f32x4*)(part + (wave * 16 + c) * SMALL + i * 16 + g * 4) = acc[i];
-}
+// where this lane's four values are: row, first column
+__device__ __forceinline__ int small_row() { return (threadIdx.x >> 8) * 16 + (threadIdx.x & 15); }
+__device__ __forceinline__ int small_col() { return (threadIdx.x >> 6 & 3) * 16 + (threadIdx.x >> 4 & 3) * 4; }
 
 template <class T>
-__global__ __launch_bounds__(256) void small_begin_kernel(const T* G, long long sb, long long sn, long long sm, const double* norm, SmallArgs a) {
+__global__ __launch_bounds__(SMALL_THREADS) void small_begin_kernel(const T* G, long long sb, long long sn, long long sm, const double* norm, SmallArgs a) {
     __shared__ __attribute__((aligned(16))) float tile[SMALL * SP];
     __shared__ double sums[4];
-    double s = dme_wave_sum_f64(norm[blockIdx.y * NORM_BLOCKS + threadIdx.x]);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+    const int tid = threadIdx.x;
+    if (tid < NORM_BLOCKS) {
+        const double s = dme_wave_sum_f64(norm[blockIdx.y * NORM_BLOCKS + tid]);
+        if ((tid & 63) == 0) sums[tid >> 6] = s;
+    }
     __syncthreads();
-    s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const double s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     const double scale = s > 0.0 || s != s ? 1.0 / sqrt(s) : 0.0;
     const T* g = G + blockIdx.y * sb;
-    f32x4 acc[4] = {};
-    const int lo = threadIdx.x & 63, hi = threadIdx.x >> 6;
+    f32x4 acc = {};
+    const int lo = tid & 63, hi = tid >> 6;
     for (long long t = blockIdx.x; t < a.tiles; t += a.groups) {
         __syncthreads();
-        for (int q = hi; q < SMALL; q += 4) {  // neighbouring lanes along G's contiguous direction
-            const int y = sm == 1 ? q : lo, x = sm == 1 ? lo : q;
+#pragma unroll
+        for (int u = 0; u < SMALL; u += 16) {  // neighbouring lanes along G's contiguous direction
+            const int y = sm == 1 ? hi + u : lo, x = sm == 1 ? lo : hi + u;
             const long long r = t * SMALL + y;
             tile[y * SP + x] = r < a.n && x < a.m ? (float)((double)(float)g[r * sn + x * sm] * scale) : 0.f;
         }
         __syncthreads();
-        float* X = a.X + (blockIdx.y * a.tiles + t) * SMALL * SMALL;
-        for (int f = threadIdx.x; f < SMALL * SMALL / 4; f += 256) *(f32x4*)(X + f * 4) = *(const f32x4*)(tile + (f >> 4) * SP + (f & 15) * 4);
+        *(f32x4*)(a.X + (blockIdx.y * a.tiles + t) * SMALL * SMALL + tid * 4) = *(const f32x4*)(tile + (tid >> 4) * SP + (tid & 15) * 4);
         small_square(acc, tile);
     }
-    small_leave(acc, a.next + (blockIdx.y * a.groups + blockIdx.x) * SMALL * SMALL);
+    *(f32x4*)(a.next + (blockIdx.y * a.groups + blockIdx.x) * SMALL * SMALL + small_row() * SMALL + small_col()) = acc;
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void small_step_kernel(SmallArgs a) {
+__global__ __launch_bounds__(SMALL_THREADS) void small_step_kernel(SmallArgs a) {
     __shared__ __attribute__((aligned(16))) float S[SMALL * SP], B[SMALL * SP], X[SMALL * SP];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    float* mine = a.X + blockIdx.y * a.tiles * SMALL * SMALL;
-    f32x4 x[4];  // the first tile is on its way while S is added up
-#pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = *(const f32x4*)(mine + blockIdx.x * SMALL * SMALL + (q * 256 + tid) * 4);
+    const int tid = threadIdx.x, r = small_row(), k = small_col();
+    const int at = (tid >> 4) * SP + (tid & 15) * 4;  // of this thread's four values, counted along the lines
+    float* mine = a.X + blockIdx.y * a.tiles * SMALL * SMALL + tid * 4;
+    f32x4 x = *(const f32x4*)(mine + blockIdx.x * SMALL * SMALL);  // the first tile is on its way while S is added up
     {
-        f32x4 s[4] = {};
-        const float* part = a.part + blockIdx.y * a.groups * SMALL * SMALL;
-        for (int u = 0; u < a.groups; u += 4) {  // four pieces on their way at a time
-            f32x4 p[4][4];
+        const float* part = a.part + blockIdx.y * a.groups * SMALL * SMALL + tid * 4;
+        f32x4 p[SMALL_GROUPS], s = {};
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
+        for (int u = 0; u < SMALL_GROUPS; ++u) p[u] = *(const f32x4*)(part + (u < a.groups ? u : 0) * SMALL * SMALL);
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    p[v][q] = *(const f32x4*)(part + (u + v < a.groups ? u + v : u) * SMALL * SMALL + (q * 256 + tid) * 4);
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (u + v < a.groups) s[q] += p[v][q];
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int f = q * 256 + tid;
-            *(f32x4*)(S + (f >> 4) * SP + (f & 15) * 4) = s[q];
-        }
+        for (int u = 0; u < SMALL_GROUPS; ++u)
+            if (u < a.groups) s += p[u];
+        *(f32x4*)(S + at) = s;
     }
     __syncthreads();
-    f32x4 acc[4] = {};
-    small_product(acc, S, S);
-    const int r = wave * 16 + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = i * 16 + g * 4;
+    {
+        f32x4 acc = {};
+        small_product(acc, S, S);
         const f32x4 s = *(const f32x4*)(S + r * SP + k);
         f32x4 v;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = __builtin_fmaf(a.c, acc[i][q], a.b * s[q]) + (k + q == r ? a.a : 0.f);
+        for (int q = 0; q < 4; ++q) v[q] = __builtin_fmaf(a.c, acc[q], a.b * s[q]) + (k + q == r ? a.a : 0.f);
         *(f32x4*)(B + r * SP + k) = v;
     }
-    f32x4 next[4] = {};
+    f32x4 next = {};
     for (long long t = blockIdx.x; t < a.tiles; t += a.groups) {
-        float* at = mine + t * SMALL * SMALL;
-        __syncthreads();  // B is written, and X of the tile before read
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int f = q * 256 + tid;
-            if (t != blockIdx.x) x[q] = *(const f32x4*)(at + f * 4);
-            *(f32x4*)(X + (f >> 4) * SP + (f & 15) * 4) = x[q];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (t != blockIdx.x) x = *(const f32x4*)(mine + t * SMALL * SMALL);
+        __syncthreads();  // X of the tile before is read
+        *(f32x4*)(X + at) = x;
+        __syncthreads();  // and B is written
+        f32x4 acc = {};
         small_product(acc, X, B);  // B is symmetric
         if (a.out) {
             const long long line = t * SMALL + r;
             T* o = (T*)a.out + blockIdx.y * a.out_batch + line * a.out_n;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int k = i * 16 + g * 4 + q;
-                    if (line < a.n && k < a.m) o[k * a.out_m] = (T)acc[i][q];
-                }
+            for (int q = 0; q < 4; ++q)
+                if (line < a.n && k + q < a.m) o[(k + q) * a.out_m] = (T)acc[q];
             continue;
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            *(f32x4*)(X + r * SP + i * 16 + g * 4) = acc[i];
-            *(f32x4*)(at + r * SMALL + i * 16 + g * 4) = acc[i];
-        }
+        *(f32x4*)(X + r * SP + k) = acc;
         __syncthreads();
+        *(f32x4*)(mine + t * SMALL * SMALL) = *(const f32x4*)(X + at);
         small_square(next, X);
     }
-    if (!a.out) small_leave(next, a.next + (blockIdx.y * a.groups + blockIdx.x) * SMALL * SMALL);
+    if (!a.out) *(f32x4*)(a.next + (blockIdx.y * a.groups + blockIdx.x) * SMALL * SMALL + r * SMALL + k) = next;
 }
 
 inline long long up(long long v, long long to) { return (v + to - 1) / to * to; }
@@ -716,12 +686,12 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
         y.out_n = tall ? cols : 1;
         y.out_m = tall ? 1 : cols;
         const dim3 grid((unsigned)p.groups, (unsigned)batch);
-        hipLaunchKernelGGL(small_begin_kernel<T>, grid, dim3(256), 0, s, G, sb, tall ? rs : cs, tall ? cs : rs, part, y);
+        hipLaunchKernelGGL(small_begin_kernel<T>, grid, dim3(SMALL_THREADS), 0, s, G, sb, tall ? rs : cs, tall ? cs : rs, part, y);
         for (int i = 0; i < steps; ++i) {
             y.part = pieces[i & 1];
             y.next = pieces[(i & 1) ^ 1];
             y.out = i + 1 < steps ? nullptr : out;
-            hipLaunchKernelGGL(small_step_kernel<T>, grid, dim3(256), 0, s, y);
+            hipLaunchKernelGGL(small_step_kernel<T>, grid, dim3(SMALL_THREADS), 0, s, y);
         }
         DME_HIP_CHECK(hipGetLastError());
         return DME_OK;
