@@ -19,6 +19,7 @@
 #include <math.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "dme_products.h"
 
@@ -65,6 +66,19 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, lon
     if (threadIdx.x == 0) part[blockIdx.y * NORM_BLOCKS + blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
+typedef half f16x8 __attribute__((ext_vector_type(8)));
+
+// hi + lo of eight values, 16 bytes each
+__device__ __forceinline__ void split8(half* hi, half* lo, const float (&v)[8]) {
+    f16x8 h, l;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        h[q] = (half)v[q];
+        l[q] = (half)(v[q] - (float)h[q]);
+    }
+    *(f16x8*)hi = h;
+    *(f16x8*)lo = l;
+}
 // hi + lo of four values
 __device__ __forceinline__ void split4(half* hi, half* lo, f32x4 v) {
     f16x4 h, l;
@@ -85,10 +99,10 @@ __device__ __forceinline__ void split1(half* hi, half* lo, float v) {
 struct Matrices {
     half* X[2][2];  // [which of two][hi, lo]: [rows][ldx], read and written in turn
     float* Xf;      // fp32 matrices: X itself, scaled like its pair
-    float* S;       // [m][lds]
+    float* S;       // fp32 matrices: [m][lds], on and below the diagonal
     half* Sw[2];    // [hi, lo]: S without its diagonal; lo for fp32 matrices
     half* Bw[2];    // b S + c S S without its diagonal
-    float* Sd;      // [m]: the diagonals
+    float* Sd;      // [lds]: the diagonals
     float* Bd;
     float* part;    // [split][m][lds]: pieces of S
     long long stride_x, stride_s, stride_part;  // from matrix to matrix
@@ -141,7 +155,7 @@ struct StepArgs {
     int from;  // which of X is read
     T* out;    // the last step's result, or null
     long long out_batch;
-    int vector;  // its rows are aligned to four values
+    int vector;  // its rows are aligned to 16 bytes
     long long tiles_r, tiles_c, batch;
     int slices, per_split;
 };
@@ -174,9 +188,79 @@ __device__ __forceinline__ void triangle_tile(u32 block, u32 n, long long& tr, l
 template <int PARTS>
 __device__ __forceinline__ void put_s(const Matrices& x, long long so, long long mo, long long r, long long c, float v) {
     const long long at = so + r * x.lds + c;
-    x.S[at] = v;
+    if (PARTS == 2) x.S[at] = v;
     split1(x.Sw[0] + at, PARTS == 2 ? x.Sw[1] + at : nullptr, r == c ? 0.f : v * SCALE_S);
     if (r == c) x.Sd[mo + r] = v;
+}
+
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// How a wave's part of a tile, which the matrix instructions leave in groups of four values of 16 rows, goes through LDS so that its lanes
+// store 16 bytes beside each other.
+template <class Tile>
+struct Turn {
+    static constexpr int ROWS = 16, PITCH = Tile::WTC + 4;                   // 16 rows in 32 bits at a time
+    static constexpr int PER = Tile::WTC / 8, ITEMS = ROWS * PER, ITER = (ITEMS + 63) / 64;  // groups of eight values
+    static constexpr int HALVES = (Tile::WTR * (Tile::WTC + 8) > Tile::WTC * (Tile::WTR + 8) ? Tile::WTR * (Tile::WTC + 8) : Tile::WTC * (Tile::WTR + 8));
+    static constexpr int LDS = Tile::NW * (HALVES * 2 > ROWS * PITCH * 4 ? HALVES * 2 : ROWS * PITCH * 4);
+};
+
+// The wave's part v of the tile at (r0, c0) into a symmetric matrix of halves, and its mirror image for a tile beside the diagonal.  v is zero
+// outside the m x m values; the pitch's padding gets its zeros here.
+template <class Tile>
+__device__ __forceinline__ void store_symmetric(char* lds, half* M, long long ld, long long m, const f16x4 (&v)[Tile::NI][Tile::NJ], long long r0,
+                                                long long c0, bool mirror) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    half* mine = (half*)lds + wave * Turn<Tile>::HALVES;
+    const long long r1 = r0 + wave / (Tile::TC_ / Tile::WTC) * Tile::WTR, c1 = c0 + wave % (Tile::TC_ / Tile::WTC) * Tile::WTC;
+    {
+        constexpr int PITCH = Tile::WTC + 8, PER = Tile::WTC / 8, ITEMS = Tile::WTR * PER;
+#pragma unroll
+        for (int j = 0; j < Tile::NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < Tile::NI; ++i) *(f16x4*)(mine + (j * 16 + c) * PITCH + i * 16 + g * 4) = v[i][j];
+        wave_fence();
+#pragma unroll
+        for (int it = 0; it < (ITEMS + 63) / 64; ++it) {
+            const int f = it * 64 + lane;
+            if (ITEMS % 64 && f >= ITEMS) break;
+            const long long r = r1 + f / PER, k = c1 + f % PER * 8;
+            if (r < m && k < ld) *(u32q*)(M + r * ld + k) = *(const u32q*)(mine + f / PER * PITCH + f % PER * 8);
+        }
+        wave_fence();
+    }
+    if (mirror) {
+        constexpr int PITCH = Tile::WTR + 8, PER = Tile::WTR / 8, ITEMS = Tile::WTC * PER;
+#pragma unroll
+        for (int j = 0; j < Tile::NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < Tile::NI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) mine[(i * 16 + g * 4 + q) * PITCH + j * 16 + c] = v[i][j][q];
+        wave_fence();
+#pragma unroll
+        for (int it = 0; it < (ITEMS + 63) / 64; ++it) {
+            const int f = it * 64 + lane;
+            if (ITEMS % 64 && f >= ITEMS) break;
+            const long long r = c1 + f / PER, k = r1 + f % PER * 8;
+            if (r < m && k < ld) *(u32q*)(M + r * ld + k) = *(const u32q*)(mine + f / PER * PITCH + f % PER * 8);
+        }
+        wave_fence();
+    }
+}
+
+// the halves of a matrix of 32-bit values, part 0 or 1 of their pairs
+template <class Tile>
+__device__ __forceinline__ void halves(f16x4 (&h)[Tile::NI][Tile::NJ], const f32x4 (&v)[Tile::NI][Tile::NJ], int part) {
+#pragma unroll
+    for (int i = 0; i < Tile::NI; ++i)
+#pragma unroll
+        for (int j = 0; j < Tile::NJ; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const half hi = (half)v[i][j][q];
+                h[i][j][q] = part ? (half)(v[i][j][q] - (float)hi) : hi;
+            }
 }
 
 // S = X X' (X' X for a tall X), the tiles on and below the diagonal; what lies above is their mirror image.  Where the tiles are
@@ -186,7 +270,7 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArg
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DmeSquare<half, SIDE, TALL, TALL> Tile;
     const Matrices& x = a.mat;
-    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m, xo = blockIdx.y * x.stride_x;
+    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.lds, xo = blockIdx.y * x.stride_x;
     const DmeOperand op{nullptr, x.ldx * 2, x.m};
     long long tr, tc;
     triangle_tile(blockIdx.x, (u32)a.tiles_r, tr, tc);
@@ -196,25 +280,34 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArg
     Tile t;
     multiply<PARTS>(t, x.X[a.from], op, x.X[a.from], op, xo, xo, TALL ? x.rows : x.cols, lds, tr * SIDE, tc * SIDE, s0, s1);
     constexpr float UNIT = 1.f / (SCALE_X * SCALE_X);
+    const bool split = gridDim.z > 1;
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
         const long long r = tr * SIDE + Tile::row_of(j);
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) {
             const long long c = tc * SIDE + Tile::col_of(i);
-            if (r >= x.lds || c >= x.lds) continue;
-            const f32x4 v = t.acc[i][j] * UNIT;
-            if (gridDim.z > 1) {
-                if (r < x.m) *(f32x4*)(x.part + blockIdx.y * x.stride_part + blockIdx.z * x.stride_s + r * x.lds + c) = v;
+            f32x4& v = t.acc[i][j];
+            v *= UNIT;
+            const bool in = r < x.m && c < x.lds;
+            if (split) {
+                if (in) *(f32x4*)(x.part + blockIdx.y * x.stride_part + blockIdx.z * x.stride_s + r * x.lds + c) = v;
                 continue;
             }
+            if (PARTS == 2 && in) *(f32x4*)(x.S + so + r * x.lds + c) = v;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {  // the pitch's padding is zero, below the diagonal and above it
-                const bool in = r < x.m && c + q < x.m;
-                if (tr != tc && c + q < x.m) put_s<PARTS>(x, so, mo, c + q, r, in ? v[q] : 0.f);
-                if (r < x.m) put_s<PARTS>(x, so, mo, r, c + q, in ? v[q] : 0.f);
+            for (int q = 0; q < 4; ++q) {
+                if (in && c + q == r) x.Sd[mo + r] = v[q];
+                v[q] = r < x.m && c + q < x.m && c + q != r ? v[q] * SCALE_S : 0.f;
             }
         }
+    }
+    if (split) return;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+        f16x4 h[Tile::NI][Tile::NJ];
+        halves<Tile>(h, t.acc, part);
+        store_symmetric<Tile>(lds, x.Sw[part] + so, x.lds, x.m, h, tr * SIDE, tc * SIDE, tr != tc);
     }
 }
 
@@ -222,7 +315,7 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArg
 template <int PARTS>
 __global__ __launch_bounds__(256) void join_kernel(Matrices x, int splits) {
     __shared__ float turn[16][17];
-    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.lds;
     long long tr, tc;
     triangle_tile(blockIdx.x, (u32)((x.lds + 15) / 16), tr, tc);
     const int lo = threadIdx.x & 15, hi = threadIdx.x >> 4;
@@ -254,11 +347,29 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef DmeSquare<half, SIDE> Tile;
     const Matrices& x = a.mat;
-    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    const long long so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.lds;
     const DmeOperand op{nullptr, x.lds * 2, x.m};
     long long tr, tc;
     triangle_tile(blockIdx.x, (u32)a.tiles_r, tr, tc);
     Tile t;
+    // S[r][c ...]; edge: in a tile on the diagonal or at the end, where S above the diagonal is what lies below it
+    const auto own = [&](long long r, long long c, bool edge) {
+        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (edge && (r >= x.m || c >= x.lds)) return v;
+        if (PARTS == 1) {
+            const f16x4 h = *(const f16x4*)(x.Sw[0] + so + r * x.lds + c);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = (float)h[q] * (1.f / SCALE_S);
+        } else if (!edge) {
+            v = *(const f32x4*)(x.S + so + r * x.lds + c);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < x.m) v[q] = x.S[so + (c + q > r ? (c + q) * x.lds + r : r * x.lds + c + q)];
+        }
+        return v;
+    };
+    const bool edge = tr == tc || (tr + 1) * SIDE > x.m;  // tc <= tr
     // a small tile's own values are on their way while it is made
     constexpr bool EARLY = SIDE == 64;
     f32x4 early[EARLY ? Tile::NI : 1][EARLY ? Tile::NJ : 1];
@@ -266,123 +377,147 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
 #pragma unroll
         for (int j = 0; j < Tile::NJ; ++j)
 #pragma unroll
-            for (int i = 0; i < Tile::NI; ++i) {
-                const long long r = tr * SIDE + Tile::row_of(j), c = tc * SIDE + Tile::col_of(i);
-                early[i][j] = r < x.m && c < x.lds ? *(const f32x4*)(x.S + so + r * x.lds + c) : f32x4{0.f, 0.f, 0.f, 0.f};
-            }
+            for (int i = 0; i < Tile::NI; ++i) early[i][j] = own(tr * SIDE + Tile::row_of(j), tc * SIDE + Tile::col_of(i), edge);
     }
     multiply<PARTS>(t, x.Sw, op, x.Sw, op, so, so, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
     constexpr float UNIT = 1.f / (SCALE_S * SCALE_S);
+    const auto finish = [&](auto at_edge) {
+        constexpr bool EDGE = decltype(at_edge)::value;
 #pragma unroll
-    for (int j = 0; j < Tile::NJ; ++j) {
-        const long long r = tr * SIDE + Tile::row_of(j);
-        if (r >= x.lds) continue;
-        const bool real = r < x.m;  // the rows beyond are the padding above the diagonal
-        const float dr = real ? x.Sd[mo + r] : 0.f;
+        for (int j = 0; j < Tile::NJ; ++j) {
+            if (!EARLY) __builtin_amdgcn_sched_barrier(0);  // or all blocks' values are loaded first, and there are no registers for them
+            const long long r = tr * SIDE + Tile::row_of(j);
+            const float dr = !EDGE || r < x.m ? x.Sd[mo + r] : 0.f;
 #pragma unroll
-        for (int i = 0; i < Tile::NI; ++i) {
-            const long long c = tc * SIDE + Tile::col_of(i);
-            if (c >= x.lds) continue;
-            f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-            if constexpr (EARLY)
-                s = early[i][j];
-            else if (real)
-                s = *(const f32x4*)(x.S + so + r * x.lds + c);
-            f32x4 v;
+            for (int i = 0; i < Tile::NI; ++i) {
+                const long long c = tc * SIDE + Tile::col_of(i);
+                f32x4 s, &v = t.acc[i][j], dc = f32x4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (EARLY)
+                    s = early[i][j];
+                else
+                    s = own(r, c, EDGE);
+                if (!EDGE || c < x.lds) dc = *(const f32x4*)(x.Sd + mo + c);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const bool in = real && c + q < x.m, on = in && c + q == r;
-                const float dc = in ? x.Sd[mo + c + q] : 0.f;
-                const float ss = t.acc[i][j][q] * UNIT + (on ? dr * dr : (dr + dc) * s[q]);
-                const float poly = __builtin_fmaf(a.c, ss, a.b * s[q]);
-                if (on) x.Bd[mo + r] = poly;
-                v[q] = in && !on ? poly * SCALE_B : 0.f;
-                if (tr != tc && c + q < x.m) {
-                    const long long at = so + (c + q) * x.lds + r;
-                    split1(x.Bw[0] + at, PARTS == 2 ? x.Bw[1] + at : nullptr, v[q]);
+                for (int q = 0; q < 4; ++q) {
+                    const bool in = !EDGE || (r < x.m && c + q < x.m), on = EDGE && in && c + q == r;
+                    const float sq = on ? dr : s[q], ss = v[q] * UNIT + (on ? dr * dr : (dr + dc[q]) * sq);
+                    const float poly = __builtin_fmaf(a.c, ss, a.b * sq);
+                    if (on) x.Bd[mo + r] = poly;
+                    v[q] = in && !on ? poly * SCALE_B : 0.f;
                 }
             }
-            if (!real) continue;
-            if (PARTS == 2)
-                split4(x.Bw[0] + so + r * x.lds + c, x.Bw[1] + so + r * x.lds + c, v);
-            else
-                dme_store4(x.Bw[0] + so + r * x.lds + c, v);
         }
+    };
+    if (edge)
+        finish(std::true_type());
+    else
+        finish(std::false_type());
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+        f16x4 h[Tile::NI][Tile::NJ];
+        halves<Tile>(h, t.acc, part);
+        store_symmetric<Tile>(lds, x.Bw[part] + so, x.lds, x.m, h, tr * SIDE, tc * SIDE, tr != tc);
     }
 }
 
-// X <- a X + B X (a X + X B for a tall X)
-template <class T, int PARTS, int SIDE, bool TALL, int STAGES = 0>
-__global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void update_kernel(StepArgs<T> a) {
+// X <- a X + B X (a X + X B for a tall X).  EU: waves that a SIMD shall have room for.
+template <class T, int PARTS, class Tile, bool TALL, int EU>
+__global__ __launch_bounds__(Tile::NT, EU) void update_kernel(StepArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef DmeSquare<half, SIDE, false, !TALL, STAGES> Tile;
+    typedef Turn<Tile> Way;
     const Matrices& x = a.mat;
-    const long long xo = blockIdx.y * x.stride_x, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.m;
+    const long long xo = blockIdx.y * x.stride_x, so = blockIdx.y * x.stride_s, mo = blockIdx.y * x.lds;
     const DmeOperand b{nullptr, x.lds * 2, x.m}, y{nullptr, x.ldx * 2, TALL ? x.rows : x.cols};
     half* const* X = x.X[a.from];
     long long tr, tc;
     dme_tile_of(blockIdx.x, (u32)a.tiles_r, (u32)a.tiles_c, tr, tc);
-    Tile t;
-    // a small tile's own values are on their way while it is made
-    constexpr bool EARLY = SIDE == 64;
-    const auto own = [&](long long at) {
-        if (PARTS == 2) return *(const f32x4*)(x.Xf + xo + at);
-        const f16x4 h = *(const f16x4*)(X[0] + xo + at), l = *(const f16x4*)(X[1] + xo + at);
-        return f32x4{(float)h[0] + (float)l[0], (float)h[1] + (float)l[1], (float)h[2] + (float)l[2], (float)h[3] + (float)l[3]};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const long long r0 = tr * Tile::TR_, c0 = tc * Tile::TC_;
+    const long long r1 = r0 + wave / (Tile::TC_ / Tile::WTC) * Tile::WTR, c1 = c0 + wave % (Tile::TC_ / Tile::WTC) * Tile::WTC;
+    // X's own values, eight of a row for a lane, 16 rows of the wave at a time: the next ones on their way while these are made
+    struct Own {
+        u32q at[2];  // hi, lo; fp32 matrices: X itself
     };
-    f32x4 early[EARLY ? Tile::NI : 1][EARLY ? Tile::NJ : 1];
-    if constexpr (EARLY) {
+    const auto load = [&](int j, Own (&o)[Way::ITER]) {
 #pragma unroll
-        for (int j = 0; j < Tile::NJ; ++j)
-#pragma unroll
-            for (int i = 0; i < Tile::NI; ++i) {
-                const long long r = tr * SIDE + Tile::row_of(j), c = tc * SIDE + Tile::col_of(i);
-                early[i][j] = r < x.rows && c < x.ldx ? own(r * x.ldx + c) : f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-    }
+        for (int it = 0; it < Way::ITER; ++it) {
+            const int f = it * 64 + lane;
+            const long long r = r1 + j * 16 + f / Way::PER, c = c1 + f % Way::PER * 8, at = xo + r * x.ldx + c;
+            o[it].at[0] = o[it].at[1] = u32q{0, 0, 0, 0};
+            if (f >= Way::ITEMS || r >= x.rows || c >= x.ldx) continue;
+            o[it].at[0] = PARTS == 2 ? *(const u32q*)(x.Xf + at) : *(const u32q*)(X[0] + at);
+            o[it].at[1] = PARTS == 2 ? *(const u32q*)(x.Xf + at + 4) : *(const u32q*)(X[1] + at);
+        }
+    };
+    constexpr bool EARLY = Tile::NI * Tile::NJ <= 8;  // a small tile leaves registers for them while it is made
+    Own own[Way::ITER], next[Way::ITER];
+    Tile t;
+    if (EARLY) load(0, own);
     if (TALL)
-        multiply<PARTS>(t, X, y, x.Bw, b, xo, so, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+        multiply<PARTS>(t, X, y, x.Bw, b, xo, so, x.m, lds, r0, c0, 0, a.slices);
     else
-        multiply<PARTS>(t, x.Bw, b, X, y, so, xo, x.m, lds, tr * SIDE, tc * SIDE, 0, a.slices);
+        multiply<PARTS>(t, x.Bw, b, X, y, so, xo, x.m, lds, r0, c0, 0, a.slices);
+    if (!EARLY) load(0, own);
     constexpr float UNIT = 1.f / SCALE_B;  // X's scale stays
     half *hi = x.X[a.from ^ 1][0] + xo, *lo = x.X[a.from ^ 1][1] + xo;
+    float* mine = (float*)lds + wave * Way::ROWS * Way::PITCH;
 #pragma unroll
     for (int j = 0; j < Tile::NJ; ++j) {
-        const long long r = tr * SIDE + Tile::row_of(j);
-        if (r >= x.rows) continue;
-        const float dr = TALL ? 0.f : a.a + x.Bd[mo + r];
+        if (j + 1 < Tile::NJ) load(j + 1, next);
 #pragma unroll
-        for (int i = 0; i < Tile::NI; ++i) {
-            const long long c = tc * SIDE + Tile::col_of(i);
-            if (c >= x.ldx) continue;
-            const long long at = r * x.ldx + c;
-            f32x4 old;
-            if constexpr (EARLY)
-                old = early[i][j];
-            else
-                old = own(at);
-            f32x4 v;
+        for (int i = 0; i < Tile::NI; ++i) *(f32x4*)(mine + (lane & 15) * Way::PITCH + i * 16 + g * 4) = t.acc[i][j] * UNIT;
+        wave_fence();
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const bool in = c + q < x.cols;
-                const float d = TALL ? (in ? a.a + x.Bd[mo + c + q] : 0.f) : dr;
-                v[q] = in ? __builtin_fmaf(d, old[q], t.acc[i][j][q] * UNIT) : 0.f;
+        for (int it = 0; it < Way::ITER; ++it) {
+            const int f = it * 64 + lane, row = f / Way::PER, col = f % Way::PER * 8;
+            const long long r = r1 + j * 16 + row, c = c1 + col, at = r * x.ldx + c;
+            if (f >= Way::ITEMS || r >= x.rows || c >= x.ldx) continue;
+            const f32x4 left = *(const f32x4*)(mine + row * Way::PITCH + col), right = *(const f32x4*)(mine + row * Way::PITCH + col + 4);
+            const f16x8 h = __builtin_bit_cast(f16x8, own[it].at[0]), l = __builtin_bit_cast(f16x8, own[it].at[1]);
+            const f32x4 o0 = __builtin_bit_cast(f32x4, own[it].at[0]), o1 = __builtin_bit_cast(f32x4, own[it].at[1]);
+            f32x4 d0, d1;
+            if (TALL) {  // c < ldx = lds
+                d0 = *(const f32x4*)(x.Bd + mo + c);
+                d1 = *(const f32x4*)(x.Bd + mo + c + 4);
+            } else {
+                const float d = x.Bd[mo + r];
+                d0 = d1 = f32x4{d, d, d, d};
+            }
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float old = PARTS == 2 ? (q < 4 ? o0[q & 3] : o1[q & 3]) : (float)h[q] + (float)l[q];
+                const float d = a.a + (q < 4 ? d0[q & 3] : d1[q & 3]), product = q < 4 ? left[q & 3] : right[q & 3];
+                v[q] = c + q < x.cols ? __builtin_fmaf(d, old, product) : 0.f;
             }
             if (!a.out) {
-                split4(hi + at, lo + at, v);
-                if (PARTS == 2) *(f32x4*)(x.Xf + xo + at) = v;
-            } else if (c < x.cols) {  // the result has no padding
-                v *= 1.f / SCALE_X;
-                T* o = a.out + blockIdx.y * a.out_batch + r * x.cols + c;
-                if (a.vector) {
-                    dme_store4(o, v);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (c + q < x.cols) o[q] = (T)v[q];
+                split8(hi + at, lo + at, v);
+                if (PARTS == 2) {
+                    *(f32x4*)(x.Xf + xo + at) = f32x4{v[0], v[1], v[2], v[3]};
+                    *(f32x4*)(x.Xf + xo + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
                 }
+                continue;
+            }
+            T* to = a.out + blockIdx.y * a.out_batch + r * x.cols + c;  // the result has no padding
+            if (a.vector) {
+                constexpr int VEC = 16 / sizeof(T);
+                typedef T tv __attribute__((ext_vector_type(VEC)));
+#pragma unroll
+                for (int q = 0; q < 8; q += VEC) {
+                    tv w;
+#pragma unroll
+                    for (int u = 0; u < VEC; ++u) w[u] = (T)(v[q + u] * (1.f / SCALE_X));
+                    if (c + q < x.cols) *(tv*)(to + q) = w;
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (c + q < x.cols) to[q] = (T)(v[q] * (1.f / SCALE_X));
             }
         }
+        wave_fence();
+#pragma unroll
+        for (int it = 0; it < Way::ITER; ++it) own[it] = next[it];
     }
 }
 
@@ -521,6 +656,7 @@ struct StepPlan {
     int groups;
     long long m, n, ldx, lds;
     DmeCut square, poly, update;
+    bool slab;        // the update by slabs of 64 lines
     long long norm, X[2][2], Xf, S, Sw[2], Bw[2], Sd, Bd, part, bytes;
 };
 
@@ -536,8 +672,8 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     p.square = dme_cut(p.m, p.m, slices(p.n), 2, true, 0.0, true, batch);
     p.poly = dme_cut(p.m, p.m, slices(p.m), 2, false, 0.0, true, batch);
     p.update = dme_cut(rows, cols, slices(p.m), 2, false, 0.0, false, batch);
-    // few slices: the update is bound by its passes over X, which small tiles overlap (50000 x 256: 50 us with 256, 41 with 64)
-    if (slices(p.m) <= 8) p.update.side = 64;
+    // a slab of X with all its singular values is one tile, and X is read once: where there are slabs enough for the card
+    p.slab = p.m <= 256 && batch * ((p.n + 63) / 64) >= 256;
     long long at = 0;
     const auto take = [&](long long bytes) {
         const long long here = at;
@@ -556,28 +692,29 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     }
     for (int i = 0; i < 4; ++i) p.X[i / 2][i % 2] = take(batch * rows * p.ldx * 2);
     if (parts == 2) p.Xf = take(batch * rows * p.ldx * 4);
-    p.S = take(batch * p.m * p.lds * 4);
+    if (parts == 2) p.S = take(batch * p.m * p.lds * 4);
     for (int i = 0; i < parts; ++i) {
         p.Sw[i] = take(batch * p.m * p.lds * 2);
         p.Bw[i] = take(batch * p.m * p.lds * 2);
     }
-    p.Sd = take(batch * p.m * 4);
-    p.Bd = take(batch * p.m * 4);
+    p.Sd = take(batch * p.lds * 4);
+    p.Bd = take(batch * p.lds * 4);
     if (p.square.splits > 1) p.part = take(batch * p.square.splits * p.m * p.lds * 4);
     p.bytes = at;
     return p;
 }
 
-template <int SIDE, int STAGES = 0, class F, class A>
+template <class Tile, class F, class A>
 int launch(F kernel, std::atomic<bool>* done, const A& a, long long tiles, int splits, hipStream_t s) {
-    constexpr int bytes = DmeSquare<half, SIDE, false, false, STAGES>::LDS;
+    constexpr int bytes = Tile::LDS > Turn<Tile>::LDS ? Tile::LDS : Turn<Tile>::LDS;
+    static_assert(bytes <= 160 * 1024, "more than a CU has");
     int dev = 0;
     DME_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
         DME_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)splits), dim3(SIDE >= 192 ? 512 : 256), bytes, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)a.batch, (unsigned)splits), dim3(Tile::NT), bytes, s, a);
     return DME_OK;
 }
 
@@ -587,7 +724,7 @@ int square(StepArgs<T> a, const DmeCut& cut, hipStream_t s) {
     a.tiles_r = (a.mat.m + SIDE - 1) / SIDE;
     a.slices = (int)(((TALL ? a.mat.rows : a.mat.cols) * 2 + DME_SLICE - 1) / DME_SLICE);
     a.per_split = (a.slices + cut.splits - 1) / cut.splits;
-    return launch<SIDE>(square_kernel<T, PARTS, SIDE, TALL>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, cut.splits, s);
+    return launch<DmeSquare<half, SIDE>>(square_kernel<T, PARTS, SIDE, TALL>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, cut.splits, s);
 }
 
 template <class T, int PARTS, int SIDE>
@@ -595,20 +732,24 @@ int poly(StepArgs<T> a, hipStream_t s) {
     static std::atomic<bool> done[64];
     a.tiles_r = (a.mat.m + SIDE - 1) / SIDE;
     a.slices = (int)((a.mat.m * 2 + DME_SLICE - 1) / DME_SLICE);
-    return launch<SIDE>(poly_kernel<T, PARTS, SIDE>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, 1, s);
+    return launch<DmeSquare<half, SIDE>>(poly_kernel<T, PARTS, SIDE>, done, a, a.tiles_r * (a.tiles_r + 1) / 2, 1, s);
+}
+
+template <class T, int PARTS, class Tile, bool TALL, int EU>
+int update_by(StepArgs<T> a, hipStream_t s) {
+    static std::atomic<bool> done[64];
+    a.tiles_r = (a.mat.rows + Tile::TR_ - 1) / Tile::TR_;
+    a.tiles_c = (a.mat.cols + Tile::TC_ - 1) / Tile::TC_;
+    a.slices = (int)((a.mat.m * 2 + DME_SLICE - 1) / DME_SLICE);
+    return launch<Tile>(update_kernel<T, PARTS, Tile, TALL, EU>, done, a, a.tiles_r * a.tiles_c, 1, s);
 }
 
 template <class T, int PARTS, int SIDE, bool TALL>
 int update(StepArgs<T> a, hipStream_t s) {
-    static std::atomic<bool> done[64], done2[64];
-    a.tiles_r = (a.mat.rows + SIDE - 1) / SIDE;
-    a.tiles_c = (a.mat.cols + SIDE - 1) / SIDE;
-    a.slices = (int)((a.mat.m * 2 + DME_SLICE - 1) / DME_SLICE);
     // small tiles: a deep pipeline where a CU has one or two of them, two buffers where it can hold five
     if constexpr (SIDE == 64)
-        if (a.tiles_r * a.tiles_c * a.batch > 512)
-            return launch<SIDE, 2>(update_kernel<T, PARTS, SIDE, TALL, 2>, done2, a, a.tiles_r * a.tiles_c, 1, s);
-    return launch<SIDE>(update_kernel<T, PARTS, SIDE, TALL>, done, a, a.tiles_r * a.tiles_c, 1, s);
+        if ((a.mat.rows + 63) / 64 * ((a.mat.cols + 63) / 64) * a.batch > 512) return update_by<T, PARTS, DmeSquare<half, SIDE, false, !TALL, 2>, TALL, 1>(a, s);
+    return update_by<T, PARTS, DmeSquare<half, SIDE, false, !TALL>, TALL, 1>(a, s);
 }
 
 template <class T, int PARTS, bool TALL>
@@ -627,6 +768,14 @@ int one_step(const StepArgs<T>& k, const StepPlan& p, hipStream_t s) {
          : p.poly.side == 128 ? poly<T, PARTS, 128>(k, s)
                               : poly<T, PARTS, 64>(k, s);
     if (rc) return rc;
+    if (p.slab) {
+        if constexpr (TALL)
+            return p.m <= 128 ? update_by<T, PARTS, DmeTile<half, 64, 128, 4, 2, false, false, 2>, true, 4>(k, s)
+                              : update_by<T, PARTS, DmeTile<half, 64, 256, 4, 2, false, false, 2>, true, 4>(k, s);
+        else
+            return p.m <= 128 ? update_by<T, PARTS, DmeTile<half, 128, 64, 8, 1, false, true, 2>, false, 4>(k, s)
+                              : update_by<T, PARTS, DmeTile<half, 256, 64, 8, 1, false, true, 2>, false, 4>(k, s);
+    }
     return p.update.side == 256   ? update<T, PARTS, 256, TALL>(k, s)
            : p.update.side == 192 ? update<T, PARTS, 192, TALL>(k, s)
            : p.update.side == 128 ? update<T, PARTS, 128, TALL>(k, s)
@@ -661,7 +810,7 @@ int run(const T* G, long long sb, long long rs, long long cs, long long batch, l
     k.b = (float)b;
     k.c = (float)c;
     k.out_batch = rows * cols;
-    k.vector = cols % 4 == 0 && (uintptr_t)out % 16 == 0;
+    k.vector = cols * sizeof(T) % 16 == 0 && (uintptr_t)out % 16 == 0;
     k.batch = batch;
     double* part = (double*)(ws + p.norm);
     // the norm is read along G's contiguous direction, as one line where G has no gaps

@@ -75,7 +75,7 @@ static __device__ __attribute__((aligned(256))) u32 dme_zeros[64];
 // group ^ f(k), f spreading them over the banks.
 template <class T, int TR, int TC, int WR, int WC, bool PK = false, bool QK = false, int STAGES_ = 0>
 struct DmeTile {
-    static constexpr int NW = WR * WC, NT = NW * 64;
+    static constexpr int TR_ = TR, TC_ = TC, NW = WR * WC, NT = NW * 64;
     static constexpr int WTR = TR / WR, WTC = TC / WC;  // a wave's part
     static constexpr int NJ = WTR / 16, NI = WTC / 16;  // its 16 x 16 blocks
     static constexpr int STAGE = (TR + TC) * DME_SLICE;  // bytes of one buffer
