@@ -335,7 +335,7 @@ inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool
             if (best.side == 0 || us < best.us) best = DmeCut{side, (int)s, us};
         };
         for (int s = 1; s <= (split ? 64 : 1); s *= 2) consider(s);
-        if (split && tiles < 256) consider(256 / tiles < 64 ? 256 / tiles : 64);  // a tile for every CU
+        if (split && tiles > 0 && tiles < 256) consider(256 / tiles < 64 ? 256 / tiles : 64);  // a tile for every CU
     }
     return best;
 }

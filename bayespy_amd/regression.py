@@ -120,28 +120,34 @@ def _pitch(t, name):
     return t.stride(0)
 
 
+def _operand(t, name, device):
+    """(rows, columns, pointer, pitch) of features or weights."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D float32 or bfloat16 tensor")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    n, d = t.shape
+    return n, d, t.data_ptr(), max(d, 1) if t.is_contiguous() else _pitch(t, name)
+
+
 def _call(features, weights, rows, bias, likelihood):
     """Checks what log_loss and log_loss_gradient share; returns the arguments up to the likelihood."""
     if not isinstance(rows, CountRows):
         raise ValueError("rows must be a CountRows")
     if likelihood not in _LIKELIHOODS:
         raise ValueError(f"likelihood must be one of {', '.join(_LIKELIHOODS)}")
-    for t, name in ((features, "features"), (weights, "weights")):
-        if not torch.is_tensor(t) or t.dtype not in _TYPES or t.dim() != 2:
-            raise ValueError(f"{name} must be a 2-D float32 or bfloat16 tensor")
-        if t.device != rows.device:
-            raise ValueError(f"{name} must be on {rows.device}")
+    device = rows.device  # a GPU: CountRows takes no other
+    N, D, h, ldh = _operand(features, "features", device)
+    K, width, w, ldw = _operand(weights, "weights", device)
     if features.dtype != weights.dtype:
         raise ValueError("features and weights differ in type")
-    N, D = features.shape
-    if N != rows.N or weights.shape[0] != rows.K or weights.shape[1] != D or D < 1:
+    if N != rows.N or K != rows.K or width != D or D < 1:
         raise ValueError(f"features {tuple(features.shape)} and weights {tuple(weights.shape)} do not fit {rows.N} rows of {rows.K} columns")
     if bias is not None:
-        _flat(bias, torch.float32, "bias", rows.device)
-        if bias.numel() != rows.K:
-            raise ValueError(f"bias must have {rows.K} values")
-    require_gpu(rows.device)
-    return (features.data_ptr(), _pitch(features, "features"), weights.data_ptr(), _pitch(weights, "weights")), (N, rows.K, D)
+        _flat(bias, torch.float32, "bias", device)
+        if bias.numel() != K:
+            raise ValueError(f"bias must have {K} values")
+    return (h, ldh, w, ldw), (N, K, D)
 
 
 _NEEDS = {}  # scratch bytes by what they depend on: sizes, pitches, alignment

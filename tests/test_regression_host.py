@@ -54,6 +54,7 @@ def test_step_refused_before_any_launch():
     L = _lib.lib()
     need = L.dme_orthogonal_step_workspace_bytes(0, 1, 300, 200)
     assert need > 0 and L.dme_orthogonal_step_workspace_bytes(1, 3, 300, 200) > 0
+    assert L.dme_orthogonal_step_workspace_bytes(0, 0, 300, 200) >= 0  # no matrices
     for bad in ((2, 1, 3, 3), (0, -1, 3, 3), (0, 1, 0, 3), (0, 1, 3, 0), (0, 1, 1 << 17, 1 << 17), (0, 65536, 3, 3)):
         assert L.dme_orthogonal_step_workspace_bytes(*bad) == -1
 
