@@ -25,6 +25,7 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr long long ROW_BLOCK = 16384;             // rows worked on at a time
 // ... and less of them where K is vast: a launch has fewer than 2^32 threads, and tiles of 64 take a thread for 16 values of z
 constexpr long long MOST_CELLS = 1ll << 35;
+constexpr long long FEW_ROWS = 128;                // up to here a workgroup a row: too few to fill the card with 16 lanes each
 // of d loss / d z held at a time: about the memory-side cache, so that the two products read it from there, and pieces still
 // large enough to fill the card (N = 8192, K = 50000, D = 1024: 3508 us with 512 MB, 3400 with 256, 3419 with 128, 3582 with 64;
 // N = 4099, D = 128: 707, 653, 724, 790)
@@ -921,7 +922,7 @@ struct RowArgs {
     float* coef;
     float* weight;
     float* entry_g;        // CSR: [nnz], LABELS: [nb]: weight * G(z, x)
-    u32* largest;          // the largest |entry_g| so far, as the bits of a float
+    float* most;           // [workgroup]: its largest finite |entry_g|
 };
 
 // The row's pieces become l, the loss, and what the gradient needs of them, in 64 bits.  CSR rows are checked here: columns
@@ -933,6 +934,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     constexpr int ROWS = 256 / LANES;
     __shared__ float m_seen[LANES][ROWS];
     __shared__ double s_seen[LANES][ROWS], sums[3][4];
+    __shared__ float most_seen[4];
     const long long first = (long long)blockIdx.x * ROWS;
     {
         const int row = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
@@ -1044,24 +1046,24 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         total = (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]);
         times = (sums[2][0] + sums[2][1]) + (sums[2][2] + sums[2][3]);
     }
-    if (a.largest_z && a.kind != DENSE) {  // one atomic a wave
+    // the row's own terms take a thousand instructions in 64 bits: one wave makes the loss of all rows here, one the gradient's coefficients
+    const int part = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (a.largest_z && a.kind != DENSE) {  // no atomics: a thousand of them to one address took 10 us
         most = max16(most);
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
-        if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(a.largest, __builtin_bit_cast(u32, most));
+        if (lane == 0) most_seen[part] = most;
     }
-    // the row's own terms take a thousand instructions in 64 bits: one wave makes the loss of all rows here, one the gradient's coefficients
-    const int part = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    if constexpr (LANES == 16) {
-        if (sub == 0) {
-            s_seen[0][row] = s;
-            s_seen[1][row] = f;
-            s_seen[2][row] = total;
-            s_seen[3][row] = times;
-            m_seen[0][row] = m;
-        }
-        __syncthreads();
+    if (LANES == 16 && sub == 0) {
+        s_seen[0][row] = s;
+        s_seen[1][row] = f;
+        s_seen[2][row] = total;
+        s_seen[3][row] = times;
+        m_seen[0][row] = m;
     }
+    __syncthreads();
+    if (a.largest_z && a.kind != DENSE && threadIdx.x == 0)
+        a.most[blockIdx.x] = fmaxf(fmaxf(most_seen[0], most_seen[1]), fmaxf(most_seen[2], most_seen[3]));
     if (lane >= ROWS || first + lane >= a.nb) return;
     if constexpr (LANES == 16) {
         s = s_seen[0][lane];
@@ -1099,13 +1101,25 @@ struct PatchArgs {
     void* dz;
     long long lddz;
     long long* fixed;  // [K] or null
-    const u32* largest;
+    const float* most; // [mosts]
+    int mosts;
     int headroom;      // bits that the sum of all entries may need above one entry
 };
 
-// The exponent of the fixed-point sums of entry_g: the largest one takes 62 - headroom bits, whatever its size.
-__device__ __forceinline__ int fixed_shift(const u32* largest, int headroom) {
-    const float v = __builtin_bit_cast(float, *largest);
+// The exponent of the fixed-point sums of entry_g: the largest one takes 62 - headroom bits, whatever its size.  Every thread of the
+// workgroup calls this.
+template <int WAVES>
+__device__ __forceinline__ int fixed_shift(const float* most, int mosts, int headroom) {
+    __shared__ float seen[WAVES];
+    float v = 0.f;
+    for (int i = threadIdx.x; i < mosts; i += WAVES * 64) v = fmaxf(v, most[i]);
+    v = max16(v);
+    v = fmaxf(v, __shfl_xor(v, 16));
+    v = fmaxf(v, __shfl_xor(v, 32));
+    if ((threadIdx.x & 63) == 0) seen[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v = fmaxf(v, seen[w]);
     return 62 - headroom - (v > 0.f ? ilogbf(v) + 1 : 0);
 }
 
@@ -1119,18 +1133,18 @@ __global__ __launch_bounds__(512) void patch_kernel(PatchArgs a) {
     __shared__ int keys[SLOTS];
     __shared__ u64 sums[SLOTS];
     const bool add = a.fixed != nullptr;
+    int shift = 0;
     if (add) {
         for (int i = threadIdx.x; i < SLOTS; i += 512) {
             keys[i] = -1;
             sums[i] = 0;
         }
-        __syncthreads();
+        shift = fixed_shift<8>(a.most, a.mosts, a.headroom);  // passes a barrier
     }
     const int sub = threadIdx.x % LANES;
     const long long r = (long long)blockIdx.x * (512 / LANES) + threadIdx.x / LANES;
     if (r < a.nb) {
         const float m = a.largest_z[r], cf = a.coef[r];
-        const int shift = add ? fixed_shift(a.largest, a.headroom) : 0;
         const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
         for (long long e = p0 + sub; e < p1; e += LANES) {
             const long long k = KIND == CSR ? (long long)a.rows.col[e] : a.rows.labels[r];
@@ -1268,8 +1282,8 @@ struct BiasArgs {
     const float* part;
     long long tiles, K;
     const long long* fixed;
-    const u32* largest;
-    int headroom, add;
+    const float* most;
+    int mosts, headroom, add;
     float* dbias;
     u32 blocks;
 };
@@ -1287,11 +1301,12 @@ __device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*
             for (int u = 0; u < 4; ++u) v += (double)p[u];
         }
     sums[wave][lane] = v;
+    const int shift = a.fixed ? fixed_shift<4>(a.most, a.mosts, a.headroom) : 0;
     __syncthreads();
     if (wave != 0 || k >= a.K) return;
     v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
     if (a.add) v += (double)a.dbias[k];
-    if (a.fixed) v -= ldexp((double)a.fixed[k], -fixed_shift(a.largest, a.headroom));
+    if (a.fixed) v -= ldexp((double)a.fixed[k], -shift);
     a.dbias[k] = (float)v;
 }
 
@@ -1329,8 +1344,8 @@ struct Plan {
     long long ldpart;
     int headroom;
     // places in the workspace
-    long long largest, fixed, h, w, part, part_f, part_w, part_t, entry_z, entry_g, largest_z, coef, weight, dbias, dz, pw, ph, bytes;
-    long long zero_words;     // from the beginning: the largest entry and the fixed-point sums
+    long long most, fixed, h, w, part, part_f, part_w, part_t, entry_z, entry_g, largest_z, coef, weight, dbias, dz, pw, ph, bytes;
+    long long zero_words;     // from the beginning: the fixed-point sums
 };
 
 inline long long few_lds(long long bytes) { return 16 * (up(bytes, 64) + 64); }
@@ -1363,9 +1378,9 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         return here;
     };
     if (gradient && rows->kind != DENSE) {
-        p.largest = take(256);
         p.fixed = take(K * 8);
         p.zero_words = at / 4;
+        p.most = take((p.nb <= FEW_ROWS ? p.nb : FEW_ROWS + p.nb / 16) * 4);
     }
     if (p.pack_h) p.h = take(p.nb * p.dpad * p.size);
     if (p.pack_w) p.w = take(K * p.dpad * p.size);
@@ -1544,7 +1559,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         pack((const char*)c.W, c.ldw * size, c.K, c.D * size, ws + p.w, p.dpad * size, s);
         w = DmeOperand{ws + p.w, p.dpad * size, c.K};
     }
-    u32* largest = (u32*)(ws + p.largest);
+    float* most = (float*)(ws + p.most);
     long long* fixed = gradient && kind != DENSE && c.dbias ? (long long*)(ws + p.fixed) : nullptr;
     for (long long n0 = 0; n0 < c.N; n0 += p.nb) {
         const long long nb = c.N - n0 < p.nb ? c.N - n0 : p.nb;
@@ -1614,12 +1629,13 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             ra.coef = (float*)(ws + p.coef);
             ra.weight = (float*)(ws + p.weight);
             ra.entry_g = (float*)(ws + p.entry_g);
-            ra.largest = largest;
+            ra.most = most;
         }
-        if (nb <= 128)  // too few rows to fill the card with 16 lanes each
-            hipLaunchKernelGGL(row_kernel<256>, dim3((unsigned)nb), dim3(256), 0, s, ra);
+        const unsigned groups = (unsigned)(nb <= FEW_ROWS ? nb : (nb + 15) / 16);
+        if (nb <= FEW_ROWS)
+            hipLaunchKernelGGL(row_kernel<256>, dim3(groups), dim3(256), 0, s, ra);
         else
-            hipLaunchKernelGGL(row_kernel<16>, dim3((unsigned)((nb + 15) / 16)), dim3(256), 0, s, ra);
+            hipLaunchKernelGGL(row_kernel<16>, dim3(groups), dim3(256), 0, s, ra);
         if (!gradient) continue;
         a.largest_z = ra.largest_z;
         a.coef = ra.coef;
@@ -1635,7 +1651,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             rc = tiles_of_z<T, true>(a, kind, p.side, s);
             if (rc) return rc;
             if (kind != DENSE) {
-                PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.largest_z, ra.coef, a.dz, a.lddz, fixed, largest, p.headroom};
+                PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.largest_z, ra.coef, a.dz, a.lddz, fixed, most, (int)groups, p.headroom};
                 if (kind == CSR)
                     hipLaunchKernelGGL((patch_kernel<T, CSR, 16>), dim3((unsigned)((nb + 31) / 32)), dim3(512), 0, s, pa);
                 else
@@ -1682,7 +1698,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         if (p.pieces_w && n0 + nb == c.N) jw = join_args(ws + p.pw, p.ldpart, c.K * p.ldpart, p.cut_w.splits_w, c.K, c.D, c.dW);
         if (p.pieces_h) jh = join_args(ws + p.ph, p.ldpart, p.nb * p.ldpart, p.cut_h.splits_h, nb, c.D, (T*)c.dH + n0 * c.D);
         if (c.dbias)
-            bias = BiasArgs{a.dbias, a.tiles_r, c.K, fixed, largest, p.headroom, (int)(n0 > 0), c.dbias, (u32)((c.K + 63) / 64)};
+            bias = BiasArgs{a.dbias, a.tiles_r, c.K, fixed, most, (int)groups, p.headroom, (int)(n0 > 0), c.dbias, (u32)((c.K + 63) / 64)};
         const u32 blocks = jw.blocks + jh.blocks + bias.blocks;
         if (blocks) hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks), dim3(256), 0, s, jw, jh, bias);
     }
