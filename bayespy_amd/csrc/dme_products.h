@@ -278,12 +278,32 @@ __device__ __forceinline__ void dme_tile_of(u32 block, u32 tiles_r, u32 tiles_c,
     tc = t / high;
 }
 
-// dst [rows][ldd] = src [rows][cols], zero beyond cols, all counted in values of V (as many bytes as every row's beginning and length
-// allow).  A wave takes a row.
+// dst (rows of `width` bytes) = src (rows of `bytes` bytes, `pitch` apart), zero in what is more.
+struct DmePack {
+    const char* src;
+    long long pitch, rows, bytes;
+    char* dst;
+    long long width;
+};
+
+// Two of them, in values of V (as many bytes as every row's beginning and length allow).  A wave takes a row.
 template <class V>
-__global__ __launch_bounds__(256) void dme_pack_kernel(const V* src, long long lds_, long long rows, long long cols, V* dst, long long ldd) {
-    for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (long long)gridDim.x * 4)
-        for (long long c = threadIdx.x & 63; c < ldd; c += 64) dst[r * ldd + c] = c < cols ? src[r * lds_ + c] : V(0);
+__global__ __launch_bounds__(256) void dme_pack_kernel(DmePack a, DmePack b) {
+    constexpr long long SIZE = sizeof(V);
+    for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows + b.rows; r += (long long)gridDim.x * 4) {
+        const bool first = r < a.rows;
+        const long long line = first ? r : r - a.rows, bytes = first ? a.bytes : b.bytes, width = first ? a.width : b.width;
+        const char* src = first ? a.src + line * a.pitch : b.src + line * b.pitch;
+        char* dst = first ? a.dst + line * a.width : b.dst + line * b.width;
+        for (long long c = (threadIdx.x & 63) * SIZE; c < width; c += 256 * SIZE) {
+            V v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = c + u * 64 * SIZE < bytes ? *(const V*)(src + c + u * 64 * SIZE) : V(0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (c + u * 64 * SIZE < width) *(V*)(dst + c + u * 64 * SIZE) = v[u];
+        }
+    }
 }
 
 inline int dme_blocks(long long work, long long per, long long most) {

@@ -1321,10 +1321,6 @@ __global__ __launch_bounds__(256) void finish_kernel(JoinArgs w, JoinArgs h, Bia
     add_bias(b, block - h.blocks, sums);
 }
 
-__global__ void zero_kernel(u32* p, long long words) {
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += (long long)gridDim.x * blockDim.x) p[i] = 0;
-}
-
 inline long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 // Everything a call decides before its first launch.
@@ -1520,17 +1516,18 @@ JoinArgs join_args(const void* part, long long ldpart, long long split_stride, i
     return a;
 }
 
-// dst (rows of `width` bytes) = src (rows of `bytes` bytes, `pitch` apart), zero in what is more
-void pack(const char* src, long long pitch, long long rows, long long bytes, char* dst, long long width, hipStream_t s) {
-    const dim3 grid(dme_blocks(rows, 4, 16384)), block(256);
-    const uintptr_t all = (uintptr_t)src | (uintptr_t)(rows > 1 ? pitch : 0) | (uintptr_t)bytes;  // width: a multiple of 16
+// both in one launch; either may have no rows
+void pack(const DmePack& a, const DmePack& b, hipStream_t s) {
+    const dim3 grid(dme_blocks(a.rows + b.rows, 4, 16384)), block(256);
+    uintptr_t all = 0;  // widths are multiples of 16
+    for (const DmePack* p : {&a, &b})
+        if (p->rows > 0) all |= (uintptr_t)p->src | (uintptr_t)(p->rows > 1 ? p->pitch : 0) | (uintptr_t)p->bytes | (uintptr_t)p->width;
     if (all % 8 == 0)
-        hipLaunchKernelGGL(dme_pack_kernel<u64>, grid, block, 0, s, (const u64*)src, pitch / 8, rows, bytes / 8, (u64*)dst, width / 8);
+        hipLaunchKernelGGL(dme_pack_kernel<u64>, grid, block, 0, s, a, b);
     else if (all % 4 == 0)
-        hipLaunchKernelGGL(dme_pack_kernel<u32>, grid, block, 0, s, (const u32*)src, pitch / 4, rows, bytes / 4, (u32*)dst, width / 4);
+        hipLaunchKernelGGL(dme_pack_kernel<u32>, grid, block, 0, s, a, b);
     else
-        hipLaunchKernelGGL(dme_pack_kernel<unsigned short>, grid, block, 0, s, (const unsigned short*)src, pitch / 2, rows, bytes / 2,
-                           (unsigned short*)dst, width / 2);
+        hipLaunchKernelGGL(dme_pack_kernel<unsigned short>, grid, block, 0, s, a, b);
 }
 
 struct Call {
@@ -1555,8 +1552,9 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
     const int size = p.size, kind = c.rows->kind;
     char* ws = c.ws;
     DmeOperand w{(const char*)c.W, c.ldw * size, c.K};
+    DmePack pack_w{};
     if (p.pack_w) {
-        pack((const char*)c.W, c.ldw * size, c.K, c.D * size, ws + p.w, p.dpad * size, s);
+        pack_w = DmePack{w.at, w.ld, c.K, c.D * size, ws + p.w, p.dpad * size};
         w = DmeOperand{ws + p.w, p.dpad * size, c.K};
     }
     float* most = (float*)(ws + p.most);
@@ -1564,10 +1562,13 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
     for (long long n0 = 0; n0 < c.N; n0 += p.nb) {
         const long long nb = c.N - n0 < p.nb ? c.N - n0 : p.nb;
         DmeOperand h{(const char*)c.H + n0 * c.ldh * size, c.ldh * size, nb};
+        DmePack pack_h{};
         if (p.pack_h) {
-            pack(h.at, c.ldh * size, nb, c.D * size, ws + p.h, p.dpad * size, s);
+            pack_h = DmePack{h.at, h.ld, nb, c.D * size, ws + p.h, p.dpad * size};
             h = DmeOperand{ws + p.h, p.dpad * size, nb};
         }
+        if (pack_h.rows + pack_w.rows > 0) pack(pack_h, pack_w, s);
+        pack_w.rows = 0;  // once
         TileArgs a{};
         a.h = h;
         a.w = w;
@@ -1761,9 +1762,7 @@ extern "C" int dme_log_loss_gradient(const void* H, int64_t ldh, const void* W, 
     const long long size = type == DME_TYPE_BF16 ? 2 : 4;
     DME_REQUIRE((uintptr_t)dW % 16 == 0 && (uintptr_t)dH % 16 == 0, "gradients must be aligned to 16 bytes");
     if (N == 0) {  // a sum over no rows
-        hipLaunchKernelGGL(dme_pack_kernel<unsigned short>, dim3(dme_blocks(K, 4, 16384)), dim3(256), 0, (hipStream_t)stream, (const unsigned short*)nullptr, 0,
-                           K, 0, (unsigned short*)dW, D * size / 2);
-        if (dbias) hipLaunchKernelGGL(zero_kernel, dim3(dme_blocks(K, 1024, 4096)), dim3(256), 0, (hipStream_t)stream, (u32*)dbias, K);
+        pack(DmePack{nullptr, 0, K, 0, (char*)dW, D * size}, DmePack{nullptr, 0, dbias ? 1 : 0, 0, (char*)dbias, K * 4}, (hipStream_t)stream);
         DME_HIP_CHECK(hipGetLastError());
         return DME_OK;
     }
