@@ -44,10 +44,15 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* G, long long sb, lon
     if (lines == 1 && step == 1 && (uintptr_t)g % 16 == 0) {  // contiguous: 16 bytes a lane
         const long long n = length / VEC;
         const tv* v = (const tv*)g;
-        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += NORM_BLOCKS * 256) {
-            const tv x = v[i];
+        constexpr int DEEP = 4;  // loads on their way at a time
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += DEEP * NORM_BLOCKS * 256) {
+            tv x[DEEP];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) s += (double)(float)x[q] * (double)(float)x[q];
+            for (int u = 0; u < DEEP; ++u) x[u] = i + u * NORM_BLOCKS * 256 < n ? v[i + u * NORM_BLOCKS * 256] : tv{};
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u)
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) s += (double)(float)x[u][q] * (double)(float)x[u][q];
         }
         const long long i = n * VEC + threadIdx.x;
         if (blockIdx.x == 0 && i < length) s += (double)(float)g[i] * (double)(float)g[i];

@@ -333,8 +333,9 @@ constexpr DmeKind DME_KINDS[] = {{256, 1, 1200e6, 141e6}, {192, 1, 1000e6, 135e6
 inline double dme_slice_us(const DmeKind& kind, int size) {
     return (double)kind.side * kind.side * (DME_SLICE / size) * 2.0 * 256.0 * kind.per_cu / (size == 4 ? kind.f32 : kind.bf16);
 }
-// ... and of that while they are not, in its share
-constexpr double DME_ALONE = 0.6;
+// ... and of a piece of k while they are not, in its share.  (Whole products gain less: told the same of those, 2048 x 2048 steps took smaller
+// tiles and 500 us instead of 447.)
+constexpr double DME_ALONE = 0.75;
 // us of writing and adding up pieces of 32-bit sums
 inline double dme_join_us(int splits, double values) { return splits > 1 ? 4.0 + splits * values * 8.0 / 4e6 : 0.0; }
 
@@ -349,7 +350,7 @@ inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool
         const auto consider = [&](long long s) {
             if (s > 1 && slices / s < 2) return;
             const double rounds = (double)((tiles * s + slots - 1) / slots);
-            const double each = tiles * s <= 256 && per_cu > 1 ? DME_ALONE * slice : slice;
+            const double each = s > 1 && tiles * s <= 256 && per_cu > 1 ? DME_ALONE * slice : slice;
             const double us = rounds * ((double)((slices + s - 1) / s + 2) * each + extra_per_tile_us * side * side / 65536.0 * per_cu) +
                               dme_join_us((int)s, (double)batch * R * C);
             if (best.side == 0 || us < best.us) best = DmeCut{side, (int)s, us};
