@@ -1,12 +1,12 @@
 // dme_products.h — the tile product that the regression operators are made of: out[r][c] = sum_k P[r][k] Q[c][k],
-// both operands with k contiguous, on the matrix cores, 32-bit sums.
+// on the matrix cores, 32-bit sums.
 //
 // A workgroup of NW = WR x WC waves makes a tile of TR x TC outputs.  k goes by slices of 128 bytes (64 bf16 / fp16,
 // 32 fp32 values): a slice of the tile's TR + TC rows is copied from memory straight into LDS (16 bytes a lane, no
 // registers in between), two buffers (four for small tiles, whose products are short beside the memory's answer), so that the
 // copies of later slices fly while slice s is multiplied.  A row's eight
 // 16-byte chunks are stored at chunk ^ (row & 7): lanes of a wave that read the same chunk of 8 neighbouring rows then
-// touch all banks once.  Q is the matrix instruction's first operand, so a lane ends up with ONE r (lane & 15) and four
+// touch all banks once.  Both operands may also lie the other way round ("k-major", see DmeTile).  Q is the matrix instruction's first operand, so a lane ends up with ONE r (lane & 15) and four
 // neighbouring c: rows are reduced and stored in vectors.
 #pragma once
 #include "dme_common.h"
