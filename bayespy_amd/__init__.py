@@ -6,6 +6,7 @@ maxsklar/BayesPy behind the reference's own Python surface:
     bayespy_amd.dirichletMultinomialEstimation   drop-in module (same names and signatures)
     bayespy_amd.findDirichletPrior               the CLI (same options, stdin and stdout format)
     bayespy_amd.device                           device-resident statistics / solver objects
+    bayespy_amd.regression                       count rows under a linear predictor: loss, gradient, step
     bayespy_amd.parallel                         row-sharded multi-GPU estimation (RCCL)
 
 All computation is in libdme_hip.so (bayespy_amd/csrc, C ABI in include/dme_hip.h).
