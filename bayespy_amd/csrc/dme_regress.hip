@@ -15,6 +15,7 @@
 // and e^(z - l) = e^(z - m) / s.
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "dme_products.h"
@@ -23,6 +24,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr long long ROW_BLOCK = 16384;             // rows worked on at a time
+constexpr long long LOSS_BLOCK = 65536;            // ... where no gradient is wanted, which keeps 8 to 32 bytes a row and tile
 // ... and less of them where K is vast: a launch has fewer than 2^32 threads, and tiles of 64 take a thread for 16 values of z
 constexpr long long MOST_CELLS = 1ll << 35;
 constexpr long long FEW_ROWS = 128;                // up to here a workgroup a row: too few to fill the card with 16 lanes each
@@ -1366,7 +1368,7 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     p.pack_h = loose(H, ldh);
     p.pack_w = loose(W, ldw);
     p.dpad = up(D, 16 / p.size);
-    p.nb = N < 1 ? 1 : N < ROW_BLOCK ? N : ROW_BLOCK;
+    p.nb = std::min(std::max(N, 1ll), gradient ? ROW_BLOCK : LOSS_BLOCK);
     while (p.nb * K > MOST_CELLS) p.nb = (p.nb + 1) / 2;
     const long long slices = (D * p.size + DME_SLICE - 1) / DME_SLICE;
     const int cut = dme_cut(p.nb, K, slices, p.size, false, 4.0).side;
