@@ -238,8 +238,6 @@ struct TileArgs {
     double* part_w;    // DENSE: [tile][nb]: how often that z goes into it: sum x (multinomial), number of counts (Dirichlet)
     double* part_t;    // DENSE: [tile][nb]: sum x, NaN where a count is negative
     float* entry_z;    // CSR: [nnz], LABELS: [nb]: z at the counts
-    u32* clear;        // cleared on the way
-    long long clear_words;
     int likelihood;
     // backward
     const float* largest_z;  // [nb]: m
@@ -352,12 +350,9 @@ __device__ __forceinline__ void entries_of(const TileArgs& a, long long r, int f
     }
 }
 
-// What workgroups beyond the tiles do in the forward launch: a wave makes a row's z at its counts, and together they clear the words
-// that the gradient adds into later.
+// What workgroups beyond the tiles do in the forward launch: a wave makes a row's z at its counts.
 template <class T, int KIND, int WAVES>
 __device__ __forceinline__ void beyond_tiles(const TileArgs& a, u32 block) {
-    const u32 blocks = (u32)((a.nb + WAVES - 1) / WAVES);
-    for (long long i = (long long)block * WAVES * 64 + threadIdx.x; i < a.clear_words; i += (long long)blocks * WAVES * 64) a.clear[i] = 0;
     const long long r = (long long)block * WAVES + (threadIdx.x >> 6);
     if (r < a.nb) entries_of<T, KIND>(a, r, 0, 1);
 }
@@ -378,7 +373,6 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
     __shared__ f32x2 seen[4][16];
     if (blockIdx.x >= a.tiles_c) {
         const u32 r = blockIdx.x - (u32)a.tiles_c;
-        for (long long i = (long long)r * 256 + threadIdx.x; i < a.clear_words; i += a.nb * 256) a.clear[i] = 0;
         entries_of<T, KIND>(a, r, threadIdx.x >> 6, 4);
         return;
     }
@@ -1110,10 +1104,13 @@ struct PatchArgs {
     const float* coef;
     void* dz;
     long long lddz;
-    long long* fixed;  // [K] or null
-    const float* most; // [mosts]
+    // the counts' column sums for dbias, in the first piece's launch
+    u32 blocks, ranges;  // workgroups for them (0: none), ranges of columns
+    long long group;     // rows of a group
+    long long* sums;     // [group of rows][K]
+    const float* most;   // [mosts]
     int mosts;
-    int headroom;      // bits that the sum of all entries may need above one entry
+    int headroom;        // bits that the sum of all entries may need above one entry
 };
 
 // The exponent of the fixed-point sums of entry_g: the largest one takes 62 - headroom bits, whatever its size.  Every thread of the
@@ -1133,53 +1130,56 @@ __device__ __forceinline__ int fixed_shift(const float* most, int mosts, int hea
     return 62 - headroom - (v > 0.f ? ilogbf(v) + 1 : 0);
 }
 
-// d loss / d z at the counts: the tiles' value made again, minus G, in its place.  What dbias needs of G is added up in fixed
-// point, 64 bits wide: sums of whole numbers do not depend on their order.  A workgroup adds its entries up by column in LDS first:
-// word frequencies send thousands of entries to one address, where memory takes one at a time (4099 rows, 144 000 entries in two pieces: 88 us
-// with an atomic each, 2 x 19 so, 2 x 6 without dbias).  LANES lanes a row.
+// What dbias needs of the counts, entry_g added up by column: a workgroup takes a group of rows and a range of columns, looks through all
+// entries of those rows and adds up the range's in LDS, in fixed point, 64 bits wide: sums of whole numbers do not depend on their order.
+// Word frequencies leave few entries of a column together: with atomics in memory, after a hash table in LDS had joined those of 32 rows, 100 000
+// of 144 000 were left, and took 25 us; so it is 7, beside the other workgroups.  Groups are of 256 rows (each leaves K sums), smaller ones where
+// there would be few workgroups (1024 rows, 10 007 columns: 12 us with 256, 7 with 16).
+constexpr int RANGE = 8192;          // columns
+template <int KIND>
+__device__ __forceinline__ void sum_counts(const PatchArgs& a, char* lds) {
+    u64* sums = (u64*)lds;
+    const long long group = blockIdx.x / a.ranges, c0 = (long long)(blockIdx.x % a.ranges) * RANGE;
+    const int width = (int)(a.K - c0 < RANGE ? a.K - c0 : RANGE);
+    for (int i = threadIdx.x; i < width; i += 512) sums[i] = 0;
+    const int shift = fixed_shift<8>(a.most, a.mosts, a.headroom);  // passes a barrier
+    const long long r0 = group * a.group, r1 = r0 + a.group < a.nb ? r0 + a.group : a.nb;
+    const long long p0 = KIND == CSR ? row_begin(a.rows, r0) : r0, p1 = KIND == CSR ? row_begin(a.rows, r1) : r1;
+    constexpr int DEEP = KIND == CSR ? 4 : 1;
+    for (long long e = p0 + threadIdx.x; e < p1; e += DEEP * 512) {
+        long long k[DEEP];
+        float g[DEEP];
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) {
+            const bool in = e + u * 512 < p1;
+            k[u] = !in ? -1 : KIND == CSR ? (long long)a.rows.col[e + u * 512] - c0 : a.rows.labels[e + u * 512] - c0;
+            g[u] = in ? a.entry_g[e + u * 512] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u)
+            if (k[u] >= 0 && k[u] < width && __builtin_isfinite(g[u])) atomicAdd(&sums[k[u]], (u64)llrint(ldexp((double)g[u], shift)));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < width; i += 512) a.sums[group * a.K + c0 + i] = (long long)sums[i];
+}
+
+// d loss / d z at the counts: the tiles' value made again, minus G, in its place.  LANES lanes a row.  Bound by latency: 4099 rows with 144 000
+// entries take 6 us a piece.
 template <class T, int KIND, int LANES>
 __global__ __launch_bounds__(512) void patch_kernel(PatchArgs a) {
-    constexpr int SLOTS = 2048;
-    __shared__ int keys[SLOTS];
-    __shared__ u64 sums[SLOTS];
-    const bool add = a.fixed != nullptr;
-    int shift = 0;
-    if (add) {
-        for (int i = threadIdx.x; i < SLOTS; i += 512) {
-            keys[i] = -1;
-            sums[i] = 0;
-        }
-        shift = fixed_shift<8>(a.most, a.mosts, a.headroom);  // passes a barrier
-    }
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if (blockIdx.x < a.blocks) return sum_counts<KIND>(a, lds);
     const int sub = threadIdx.x % LANES;
-    const long long r = (long long)blockIdx.x * (512 / LANES) + threadIdx.x / LANES;
-    if (r < a.nb) {
-        const float m = a.largest_z[r], cf = a.coef[r];
-        const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
-        for (long long e = p0 + sub; e < p1; e += LANES) {
-            const long long k = KIND == CSR ? (long long)a.rows.col[e] : a.rows.labels[r];
-            const long long c = k - a.column;
-            if (c < 0 || c >= a.width || k >= a.K) continue;
-            const float g = a.entry_g[e];
-            ((T*)a.dz)[r * a.lddz + c] = (T)(exp_of(a.entry_z[e], m) * cf - g);
-            if (!add || !__builtin_isfinite(g)) continue;
-            const u64 v = (u64)llrint(ldexp((double)g, shift));
-            u32 slot = ((u32)k * 2654435761u) >> 21;
-            bool done = false;
-            for (int probe = 0; probe < 8 && !done; ++probe, slot = (slot + 1) % SLOTS) {
-                const int was = atomicCAS(&keys[slot], -1, (int)k);
-                if (was == -1 || was == (int)k) {
-                    atomicAdd(&sums[slot], v);
-                    done = true;
-                }
-            }
-            if (!done) atomicAdd((u64*)(a.fixed + k), v);
-        }
+    const long long r = (long long)(blockIdx.x - a.blocks) * (512 / LANES) + threadIdx.x / LANES;
+    if (r >= a.nb) return;
+    const float m = a.largest_z[r], cf = a.coef[r];
+    const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
+    for (long long e = p0 + sub; e < p1; e += LANES) {
+        const long long k = KIND == CSR ? (long long)a.rows.col[e] : a.rows.labels[r];
+        const long long c = k - a.column;
+        if (c < 0 || c >= a.width || k >= a.K) continue;
+        ((T*)a.dz)[r * a.lddz + c] = (T)(exp_of(a.entry_z[e], m) * cf - a.entry_g[e]);
     }
-    if (!add) return;
-    __syncthreads();
-    for (int i = threadIdx.x; i < SLOTS; i += 512)
-        if (keys[i] >= 0 && sums[i] != 0) atomicAdd((u64*)(a.fixed + keys[i]), sums[i]);
 }
 
 struct ProductArgs {
@@ -1288,19 +1288,20 @@ __device__ __forceinline__ void join(const JoinArgs& a, u32 block) {
     }
 }
 
-// dbias [K] (+)= the row tiles' sums, minus the counts' (fixed, null for dense rows).  64 columns a workgroup, a quarter of the
+// dbias [K] (+)= the row tiles' sums, minus the counts'.  64 columns a workgroup, a quarter of the
 // tiles a wave, the quarters added in their order.
 struct BiasArgs {
     const float* part;
     long long tiles, K;
-    const long long* fixed;
+    const long long* sums;  // [groups][K], or null: dense rows
+    long long groups;
     const float* most;
     int mosts, headroom, add;
     float* dbias;
     u32 blocks;
 };
 
-__device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*sums)[64]) {
+__device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*sums)[64], long long (*counts)[64]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long k = (long long)block * 64 + lane;
     double v = 0.0;
@@ -1313,12 +1314,24 @@ __device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*
             for (int u = 0; u < 4; ++u) v += (double)p[u];
         }
     sums[wave][lane] = v;
-    const int shift = a.fixed ? fixed_shift<4>(a.most, a.mosts, a.headroom) : 0;
+    long long whole = 0;
+    int shift = 0;
+    if (a.sums) {
+        shift = fixed_shift<4>(a.most, a.mosts, a.headroom);
+        if (k < a.K)
+            for (long long t = wave; t < a.groups; t += 16) {
+                long long p[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) p[u] = t + u * 4 < a.groups ? a.sums[(t + u * 4) * a.K + k] : 0;
+                whole += (p[0] + p[1]) + (p[2] + p[3]);
+            }
+        counts[wave][lane] = whole;
+    }
     __syncthreads();
     if (wave != 0 || k >= a.K) return;
     v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
     if (a.add) v += (double)a.dbias[k];
-    if (a.fixed) v -= ldexp((double)a.fixed[k], -shift);
+    if (a.sums) v -= ldexp((double)((counts[0][lane] + counts[1][lane]) + (counts[2][lane] + counts[3][lane])), -shift);
     a.dbias[k] = (float)v;
 }
 
@@ -1326,11 +1339,12 @@ __device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*
 template <class T>
 __global__ __launch_bounds__(256) void finish_kernel(JoinArgs w, JoinArgs h, BiasArgs b) {
     __shared__ double sums[4][64];
+    __shared__ long long counts[4][64];
     u32 block = blockIdx.x;
     if (block < w.blocks) return join<T>(w, block);
     block -= w.blocks;
     if (block < h.blocks) return join<T>(h, block);
-    add_bias(b, block - h.blocks, sums);
+    add_bias(b, block - h.blocks, sums, counts);
 }
 
 inline long long up(long long v, long long to) { return (v + to - 1) / to * to; }
@@ -1351,9 +1365,9 @@ struct Plan {
     bool pieces_w, pieces_h;  // the products leave 32-bit pieces
     long long ldpart;
     int headroom;
+    long long group;          // rows of a group of the counts' column sums
     // places in the workspace
-    long long most, fixed, h, w, part, part_f, part_w, part_t, entry_z, entry_g, largest_z, coef, weight, dbias, dz, pw, ph, bytes;
-    long long zero_words;     // from the beginning: the fixed-point sums
+    long long most, sums, h, w, part, part_f, part_w, part_t, entry_z, entry_g, largest_z, coef, weight, dbias, dz, pw, ph, bytes;
 };
 
 inline long long few_lds(long long bytes) { return 16 * (up(bytes, 64) + 64); }
@@ -1361,6 +1375,7 @@ inline long long few_lds(long long bytes) { return 16 * (up(bytes, 64) + 64); }
 Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int type, long long N, long long K, long long D,
                const dme_count_rows_t* rows, bool gradient) {
     Plan p{};
+    p.group = 16;
     p.size = type == DME_TYPE_BF16 ? 2 : 4;
     const auto loose = [&](const void* at, long long ld) {
         return ((uintptr_t)at | (uintptr_t)(ld * p.size) | (uintptr_t)(D * p.size)) % 16 != 0;
@@ -1386,8 +1401,9 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         return here;
     };
     if (gradient && rows->kind != DENSE) {
-        p.fixed = take(K * 8);
-        p.zero_words = at / 4;
+        const long long ranges = (K + RANGE - 1) / RANGE;
+        for (; p.group < 256 && (p.nb + p.group - 1) / p.group * ranges > 128;) p.group *= 2;
+        p.sums = take((p.nb + p.group - 1) / p.group * K * 8);
         p.most = take((p.nb <= FEW_ROWS ? p.nb : FEW_ROWS + p.nb / 16) * 4);
     }
     if (p.pack_h) p.h = take(p.nb * p.dpad * p.size);
@@ -1521,6 +1537,16 @@ int products(const ProductArgs& w, const ProductArgs& h, const DmePair& cut, boo
     return launch_products<T, 64>(w, h, cut, do_w, do_h, s);
 }
 
+template <class T, int KIND, int LANES>
+int launch_patch(const PatchArgs& a, unsigned lds, hipStream_t s) {
+    static std::atomic<bool> done[64];
+    const int rc = set_lds(done, patch_kernel<T, KIND, LANES>, RANGE * 8);
+    if (rc) return rc;
+    constexpr int rows = 512 / LANES;
+    hipLaunchKernelGGL((patch_kernel<T, KIND, LANES>), dim3(a.blocks + (unsigned)((a.nb + rows - 1) / rows)), dim3(512), lds, s, a);
+    return DME_OK;
+}
+
 JoinArgs join_args(const void* part, long long ldpart, long long split_stride, int splits, long long R, long long C, void* out) {
     const bool whole = ldpart == C;
     JoinArgs a{(const float*)part, ldpart, split_stride, splits, whole ? 1 : R, whole ? R * C : C, out, (int)(C % 4 == 0), 0};
@@ -1570,7 +1596,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         w = DmeOperand{ws + p.w, p.dpad * size, c.K};
     }
     float* most = (float*)(ws + p.most);
-    long long* fixed = gradient && kind != DENSE && c.dbias ? (long long*)(ws + p.fixed) : nullptr;
+    long long* sums = gradient && kind != DENSE && c.dbias ? (long long*)(ws + p.sums) : nullptr;
     for (long long n0 = 0; n0 < c.N; n0 += p.nb) {
         const long long nb = c.N - n0 < p.nb ? c.N - n0 : p.nb;
         DmeOperand h{(const char*)c.H + n0 * c.ldh * size, c.ldh * size, nb};
@@ -1610,8 +1636,6 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         a.part_w = (double*)(ws + p.part_w);
         a.part_t = (double*)(ws + p.part_t);
         a.entry_z = (float*)(ws + p.entry_z);
-        a.clear = (u32*)ws;  // each block of rows has fixed-point sums of its own: their scale is the block's
-        a.clear_words = p.zero_words;
         int rc = DME_OK;
         if (p.few) {
             const unsigned blocks = (unsigned)(p.tiles + nb), bytes = (unsigned)few_lds(c.D * size);
@@ -1664,11 +1688,20 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             rc = tiles_of_z<T, true>(a, kind, p.side, s);
             if (rc) return rc;
             if (kind != DENSE) {
-                PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.largest_z, ra.coef, a.dz, a.lddz, fixed, most, (int)groups, p.headroom};
-                if (kind == CSR)
-                    hipLaunchKernelGGL((patch_kernel<T, CSR, 16>), dim3((unsigned)((nb + 31) / 32)), dim3(512), 0, s, pa);
-                else
-                    hipLaunchKernelGGL((patch_kernel<T, LABELS, 1>), dim3((unsigned)((nb + 511) / 512)), dim3(512), 0, s, pa);
+                PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.largest_z, ra.coef, a.dz, a.lddz};
+                unsigned lds = 0;
+                if (sums && k0 == 0) {
+                    pa.ranges = (u32)((c.K + RANGE - 1) / RANGE);
+                    pa.blocks = (u32)((nb + p.group - 1) / p.group) * pa.ranges;
+                    pa.group = p.group;
+                    pa.sums = sums;
+                    pa.most = most;
+                    pa.mosts = (int)groups;
+                    pa.headroom = p.headroom;
+                    lds = (unsigned)std::min(c.K, (long long)RANGE) * 8;
+                }
+                rc = kind == CSR ? launch_patch<T, CSR, 16>(pa, lds, s) : launch_patch<T, LABELS, 1>(pa, lds, s);
+                if (rc) return rc;
             }
             const char* dz = (const char*)a.dz;
             ProductArgs mw{}, mh{};
@@ -1711,7 +1744,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         if (p.pieces_w && n0 + nb == c.N) jw = join_args(ws + p.pw, p.ldpart, c.K * p.ldpart, p.cut_w.splits_w, c.K, c.D, c.dW);
         if (p.pieces_h) jh = join_args(ws + p.ph, p.ldpart, p.nb * p.ldpart, p.cut_h.splits_h, nb, c.D, (T*)c.dH + n0 * c.D);
         if (c.dbias)
-            bias = BiasArgs{a.dbias, a.tiles_r, c.K, fixed, most, (int)groups, p.headroom, (int)(n0 > 0), c.dbias, (u32)((c.K + 63) / 64)};
+            bias = BiasArgs{a.dbias, a.tiles_r, c.K, sums, (nb + p.group - 1) / p.group, most, (int)groups, p.headroom, (int)(n0 > 0), c.dbias, (u32)((c.K + 63) / 64)};
         const u32 blocks = jw.blocks + jh.blocks + bias.blocks;
         if (blocks) hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks), dim3(256), 0, s, jw, jh, bias);
     }

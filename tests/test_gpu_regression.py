@@ -457,6 +457,35 @@ def test_more_rows_than_a_block():
         near(db, want["db"], "dbias")
 
 
+def test_more_rows_than_a_block_of_losses():
+    from bayespy_amd import regression
+    n, k, d = 65536 + 37, 20, 4
+    h, w, b, x, g = make(n, k, d, torch.float32, 8)
+    want = oracle(h, w, b, x, g, "dirichlet", torch.float32)
+    for kind in ("csr", "dense16"):
+        near(regression.log_loss(h, w, as_rows(x, kind), bias=b, likelihood="dirichlet"), want["loss"], "loss")
+
+
+def test_dense_counts_of_every_size():
+    """Lists that fill up, counts at the borders of their forms (1, 2, 15 to 17, 30 to 32), z far out to both sides."""
+    from bayespy_amd import regression
+    r = np.random.default_rng(2)
+    for n, k, d in ((9, 300, 8), (140, 517, 16)):
+        h, w, b, _, g = make(n, k, d, torch.float32, 3)
+        b = torch.from_numpy(r.choice([-30.0, -3.0, 0.0, 3.0, 25.0], size=k)).float().cuda()
+        x = torch.from_numpy(r.choice([1, 2, 3, 15, 16, 17, 30, 31, 32, 100000], size=(n, k)).astype(np.int32))
+        x[1] = 17   # a row for the 64-bit functions alone
+        x[2] = 16
+        x[3] = 0
+        want = oracle(h, w, b, x, g, "dirichlet", torch.float32)
+        for kind in ("dense32", "csr"):
+            loss, dh, dw, db = regression.log_loss_gradient(h, w, as_rows(x, kind), bias=b, likelihood="dirichlet", row_weights=g)
+            near(loss, want["loss"], "loss")
+            near(dh, want["dh"], "dfeatures")
+            near(dw, want["dw"], "dweights")
+            near(db, want["db"], "dbias")
+
+
 def test_more_columns_than_a_piece():
     """d loss / d z of 1500 x 60000 in fp32 is 360 MB: two pieces."""
     from bayespy_amd import regression
