@@ -214,6 +214,33 @@ def test_orthogonal_step_larger(shape, dtype):
     assert off <= step_tolerance(want, TYPES[dtype], 5, *shape)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(17000, 200), (200, 17001), (17000, 100), (99, 17003), (64, 300, 130), (64, 129, 300), (1500, 1400), (2600, 2500), (4100, 4200)])
+def test_orthogonal_step_of_every_tile(shape, dtype):
+    """Slabs and every tile side, with ragged ends; in 64 bits on the GPU.  The result is rounded to its type, which is off by at most
+    eps / 2 of each value, so of every part of the matrix; the steps before may add as much again (bf16), or `one` times the 2^-21 that
+    pairs of halves drop at each step, amplified (fp32, see step_tolerance)."""
+    from bayespy_amd import regression
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    g = torch.randn(shape, generator=gen, device="cuda").to(TYPES[dtype])
+    got = regression.orthogonal_step(g).double()
+    a, b, c = COEFFICIENTS
+    y = g.double().reshape(-1, *shape[-2:])
+    y = y / torch.linalg.vector_norm(y, dim=(1, 2), keepdim=True)
+    tall = shape[-2] > shape[-1]
+    for _ in range(5):
+        t = y.transpose(1, 2).contiguous()
+        s = t @ y if tall else y @ t
+        q = b * s + c * (s @ s)
+        y = a * y + (y @ q if tall else q @ y)
+    one = 3.4445 + 4 * 4.775 * 1.44 + 8 * 2.0315 * 2.07
+    u = torch.finfo(TYPES[dtype]).eps / 2
+    tol = 2 * u if dtype == "bf16" else u + one * 2.0**-21 * (1 + 3.4445 + 3.4445**2)
+    off = got.reshape(y.shape) - y
+    for part in (np.s_[:], np.s_[:, -16:], np.s_[:, :, -16:], np.s_[:, :16], np.s_[:, :, :16], np.s_[-1:]):
+        assert float(torch.linalg.vector_norm(off[part])) <= tol * float(torch.linalg.vector_norm(y[part])), part
+
+
 def test_orthogonal_step_precision():
     """Rounded once from 64 bits bf16 is off by 2^-8 / sqrt(3) / 1.4 of the norm (a uniform rounding error, values spread over a
     power of two); the products in fp16 may add as much again.  fp32: no further off than the same steps in 32-bit arithmetic are, which is
@@ -442,6 +469,22 @@ def test_few_rows_of_many_features(d):
         h, w, b, x, g = make(3, 200, d, TYPES[dtype], 2)
         want = oracle(h, w, b, x, g, "multinomial", TYPES[dtype])
         near(regression.log_loss(h, w, as_rows(x, "csr"), bias=b), want["loss"], "loss")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_large_tiles(dtype):
+    """Enough work for tiles of 256, with ragged ends and a pitch."""
+    from bayespy_amd import regression
+    n, k, d = 4100, 6001, 72
+    h, w, b, x, g = make(n, k, d, TYPES[dtype], 12, density=0.003)
+    want = oracle(h, w, b, x, g, "multinomial", TYPES[dtype])
+    wide = torch.zeros(k, d + 8, dtype=TYPES[dtype], device="cuda")
+    wide[:, :d] = w
+    loss, dh, dw, db = regression.log_loss_gradient(h, wide[:, :d], as_rows(x, "csr"), bias=b, row_weights=g)
+    near(loss, want["loss"], "loss")
+    near(dh, want["dh"], "dfeatures")
+    near(dw, want["dw"], "dweights")
+    near(db, want["db"], "dbias")
 
 
 def test_more_rows_than_a_block():
