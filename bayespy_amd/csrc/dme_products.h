@@ -205,27 +205,32 @@ struct DmeTile {
             }
         };
         const int wr = wave / WC * NJ, wc = wave % WC * NI;
-        auto multiply = [&](const char* at) {
+        auto half = [&](const char* at, int h) {
+            u32q x[NJ], y[NI];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32q x[NJ], y[NI];
+            for (int j = 0; j < NJ; ++j) x[j] = fragment<TR, PK>(at, wr + j, h);
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) x[j] = fragment<TR, PK>(at, wr + j, h);
+            for (int i = 0; i < NI; ++i) y[i] = fragment<TC, QK>(at + TR * DME_SLICE, wc + i, h);
 #pragma unroll
-                for (int i = 0; i < NI; ++i) y[i] = fragment<TC, QK>(at + TR * DME_SLICE, wc + i, h);
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int i = 0; i < NI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc[i][j] = dme_mma(y[i], x[j], acc[i][j], T());
-            }
+                for (int j = 0; j < NJ; ++j) acc[i][j] = dme_mma(y[i], x[j], acc[i][j], T());
         };
-        const int n = (s1 - s0) * PARTS;
+        auto multiply = [&](const char* at) {
+            half(at, 0);
+            half(at, 1);
+        };
+        // 32 bits: the last slice by itself, whose second half may lie beyond K (1024 x 10007 x 100: three and a half slices instead of four, 144 ->
+        // 141 us).  In 16 bits a half is few instructions, and the longer code costs more (4099 x 50000 x 128: 504 -> 515).
+        constexpr bool APART = SIZE == 4;
+        const int n = (s1 - s0) * PARTS, body = APART ? n - 1 : n;
+        const bool whole = !APART || K * SIZE > (long long)s1 * DME_SLICE - DME_SLICE / 2;
         if constexpr (STAGES == 2) {
             copy(0);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            for (int u = 0; u < n; ++u) {
-                if (u + 1 < n) copy((u + 1) & 1);
+            for (int u = 0; u < body; ++u) {
+                if (APART || u + 1 < n) copy((u + 1) & 1);
                 multiply(lds + (u & 1) * STAGE);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // slice u + 1 is in LDS ...
                 __syncthreads();                                  // ... and everybody has read slice u
@@ -238,7 +243,7 @@ struct DmeTile {
 #pragma unroll
             for (int u = 0; u < STAGES - 1; ++u)
                 if (u < n) copy(u);
-            for (int u = 0; u < n; ++u) {
+            for (int u = 0; u < body; ++u) {
                 if (u + AHEAD < n)
                     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OUT) : "memory");
                 else
@@ -247,6 +252,12 @@ struct DmeTile {
                 if (u + STAGES - 1 < n) copy((u + STAGES - 1) % STAGES);
                 multiply(lds + u % STAGES * STAGE);
             }
+            if (APART) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+        if (APART) {
+            half(lds + body % STAGES * STAGE, 0);
+            if (whole) half(lds + body % STAGES * STAGE, 1);
             __syncthreads();
         }
     }
