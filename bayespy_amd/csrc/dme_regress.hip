@@ -225,6 +225,7 @@ __device__ __forceinline__ int count_at(const Rows& rows, long long r, long long
 struct TileArgs {
     DmeOperand h, w;
     long long D;
+    int row_bytes;     // of an operand's row that may be read: whole chunks of 16 where it is packed or lies so
     long long tiles_r, tiles_c;
     int slices;
     const float* bias;
@@ -306,14 +307,59 @@ __device__ __forceinline__ float dot_step(const u32q& h, const u32q& w, float s,
     return s;
 }
 
+// The `full`-th 16 bytes of a row, of which only what is left of `bytes` belongs to it: the others are 0.
+template <class T>
+__device__ __forceinline__ u32q row_end(const char* row, int bytes) {
+    constexpr int VEC = 16 / sizeof(T);
+    typedef T tv __attribute__((ext_vector_type(VEC)));
+    const int first = bytes / 16 * 16;
+    tv v{};
+#pragma unroll
+    for (int q = 0; q < VEC; ++q)
+        if (first + q * (int)sizeof(T) < bytes) v[q] = *(const T*)(row + first + q * sizeof(T));
+    return __builtin_bit_cast(u32q, v);
+}
+// 16 bytes of a row, aligned to its values alone if LOOSE.  16-bit values: words of four bytes (17 to 20 bytes in all, each word with bytes of the row in
+// it), shifted together where they are used; 16-byte loads from odd places took twice as long.
+template <class T, bool LOOSE>
+struct Chunk {
+    typedef u32q u32q_4 __attribute__((aligned(4)));
+    u32q v;
+    u32 more;
+    __device__ __forceinline__ void load(const char* at) {
+        if constexpr (!LOOSE) {
+            v = *(const u32q*)at;
+        } else if constexpr (sizeof(T) == 4) {
+            v = *(const u32q_4*)at;
+        } else {
+            const u32 shift = (u32)(uintptr_t)at & 2;
+            v = *(const u32q_4*)(at - shift);
+            more = *(const u32*)(at - shift + (shift ? 16 : 12));
+        }
+    }
+    __device__ __forceinline__ u32q get(u32 shift) const {  // address & 2
+        if constexpr (!LOOSE || sizeof(T) == 4) return v;
+        u32q o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = __builtin_amdgcn_alignbyte(q < 3 ? v[(q + 1) & 3] : more, v[q], shift);
+        return o;
+    }
+};
+template <class T, bool LOOSE>
+__device__ __forceinline__ u32q chunk_at(const char* at) {
+    Chunk<T, LOOSE> c;
+    c.load(at);
+    return c.get((u32)(uintptr_t)at & 2);
+}
+
 // z at a row's counts: a scalar product for each, 16 lanes an entry, 16 entries of a wave in flight.  There are few of them beside
 // the N K values of z that the tiles make (and drop), so they are made once more here instead of being looked for in every tile.
 // One wave takes batches `first`, `first + step`, ... of 16 entries.
-template <class T, int KIND>
+template <class T, int KIND, bool LOOSE = false>
 __device__ __forceinline__ void entries_of(const TileArgs& a, long long r, int first, int step) {
     const int lane = threadIdx.x & 63, sub = lane & 15, group = lane >> 4;
-    const int chunks = (int)((a.D * (long long)sizeof(T) + 15) / 16);
-    const u32q* h = (const u32q*)(a.h.at + r * a.h.ld);
+    const int full = a.row_bytes / 16;
+    const char* h = a.h.at + r * a.h.ld;
     const long long p0 = KIND == CSR ? row_begin(a.rows, r) : r, p1 = KIND == CSR ? row_begin(a.rows, r + 1) : r + 1;
     for (long long e0 = p0 + first * 16; e0 < p1; e0 += step * 16) {
         int col = -1;
@@ -323,21 +369,26 @@ __device__ __forceinline__ void entries_of(const TileArgs& a, long long r, int f
         }
         constexpr int DEEP = KIND == CSR ? 4 : 1;
         int k[DEEP];
-        const u32q* w[DEEP];
+        const char* w[DEEP];
         float s[DEEP];
 #pragma unroll
         for (int u = 0; u < DEEP; ++u) {
             k[u] = __shfl(col, u * 4 + group);
-            w[u] = (const u32q*)(a.w.at + (k[u] < 0 ? 0 : k[u]) * a.w.ld);  // row 0 in place of none: read, not used
+            w[u] = a.w.at + (k[u] < 0 ? 0 : k[u]) * a.w.ld;  // row 0 in place of none: read, not used
             s[u] = 0.f;
         }
-        for (int q = sub; q < chunks; q += 16) {
-            const u32q x = h[q];
+        for (int q = sub; q < full; q += 16) {
+            const u32q x = chunk_at<T, LOOSE>(h + q * 16);
             u32q y[DEEP];
 #pragma unroll
-            for (int u = 0; u < DEEP; ++u) y[u] = w[u][q];
+            for (int u = 0; u < DEEP; ++u) y[u] = chunk_at<T, LOOSE>(w[u] + q * 16);
 #pragma unroll
             for (int u = 0; u < DEEP; ++u) s[u] = dot_step(x, y[u], s[u], T());
+        }
+        if (LOOSE && a.row_bytes % 16 && sub == 0) {
+            const u32q x = row_end<T>(h, a.row_bytes);
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u) s[u] = dot_step(x, row_end<T>(w[u], a.row_bytes), s[u], T());
         }
 #pragma unroll
         for (int u = 0; u < DEEP; ++u) {
@@ -366,46 +417,59 @@ __device__ __forceinline__ f32x2 merge(f32x2 v, f32x2 o) {
 // go from memory straight into the matrix instructions' registers, WIDE loads of 16 bytes a lane ahead, and the rows wait in LDS.
 // Nothing is shared between waves but the rows, so many small workgroups keep ~200 KB a CU in flight.  Workgroups beyond the
 // columns make the rows' z at their counts, so that a call has two launches.  Bound by memory: 1 x 50000 x 512 in bf16 reads 51 MB in
-// 12.5 us (4.1 TB/s).
-template <class T, int KIND>
+// 12.5 us (4.1 TB/s).  LOOSE: rows that are not whole chunks of 16 bytes are read as they lie.
+template <class T, int KIND, bool LOOSE>
 __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ f32x2 seen[4][16];
     if (blockIdx.x >= a.tiles_c) {
         const u32 r = blockIdx.x - (u32)a.tiles_c;
-        entries_of<T, KIND>(a, r, threadIdx.x >> 6, 4);
+        entries_of<T, KIND, LOOSE>(a, r, threadIdx.x >> 6, 4);
         return;
     }
     constexpr int WIDE = 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const int chunks = (int)((a.D * (long long)sizeof(T) + 15) / 16), rounds = (chunks + 3) / 4;  // a round: 64 bytes of each row
+    const int full = a.row_bytes / 16, chunks = (a.row_bytes + 15) / 16, rounds = (chunks + 3) / 4;  // a round: 64 bytes of each row
     const long long k0 = (long long)blockIdx.x * 64 + wave * 16;
     const long long k = k0 + c < a.K ? k0 + c : a.K - 1;
-    const u32q* w = (const u32q*)(a.w.at + k * a.w.ld);
+    const char* w = a.w.at + k * a.w.ld;
     const u32q none = u32q{0, 0, 0, 0};
-    u32q y[2][WIDE];
-    auto load = [&](u32q* to, int round) {
+    const u32 shift = (u32)(uintptr_t)w & 2;
+    Chunk<T, LOOSE> y[2][WIDE];
+    u32q end = none;
+    if (LOOSE && full < chunks && g == (full & 3)) end = row_end<T>(w, a.row_bytes);
+    auto load = [&](Chunk<T, LOOSE>* to, int round) {
 #pragma unroll
         for (int u = 0; u < WIDE; ++u) {
             const int at = (round + u) * 4 + g;
-            to[u] = at < chunks ? w[at] : none;
+            to[u].v = none;
+            to[u].more = 0;
+            if (at < full) to[u].load(w + at * 16);
         }
     };
     load(y[0], 0);
     const int pitch = (rounds * 4 + 4) * 16;  // bytes; the four chunks more spread the rows over the banks
     for (int i = tid; i < 16 * rounds * 4; i += 256) {
         const int r = i / (rounds * 4), at = i - r * (rounds * 4);
+        const char* from = a.h.at + r * a.h.ld;
         u32q v = none;
-        if (r < a.nb && at < chunks) v = *(const u32q*)(a.h.at + r * a.h.ld + at * 16);
+        if (r < a.nb && at < full)
+            v = chunk_at<T, LOOSE>(from + at * 16);
+        else if (LOOSE && r < a.nb && at < chunks)
+            v = row_end<T>(from, a.row_bytes);
         *(u32q*)(lds + r * pitch + at * 16) = v;
     }
     __syncthreads();
     f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     const char* h = lds + c * pitch + g * 16;
-    auto multiply = [&](const u32q* with, int round) {
+    auto multiply = [&](const Chunk<T, LOOSE>* with, int round) {
 #pragma unroll
         for (int u = 0; u < WIDE; ++u)
-            if (round + u < rounds) acc[u & 1] = dme_mma(with[u], *(const u32q*)(h + (round + u) * 64), acc[u & 1], T());
+            if (round + u < rounds) {
+                u32q v = with[u].get(shift);
+                if (LOOSE && (round + u) * 4 + g == full) v = end;
+                acc[u & 1] = dme_mma(v, *(const u32q*)(h + (round + u) * 64), acc[u & 1], T());
+            }
     };
     for (int round = 0; round < rounds; round += 2 * WIDE) {
         load(y[1], round + WIDE);
@@ -1380,8 +1444,6 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     const auto loose = [&](const void* at, long long ld) {
         return ((uintptr_t)at | (uintptr_t)(ld * p.size) | (uintptr_t)(D * p.size)) % 16 != 0;
     };
-    p.pack_h = loose(H, ldh);
-    p.pack_w = loose(W, ldw);
     p.dpad = up(D, 16 / p.size);
     p.nb = std::min(std::max(N, 1ll), gradient ? ROW_BLOCK : LOSS_BLOCK);
     while (p.nb * K > MOST_CELLS) p.nb = (p.nb + 1) / 2;
@@ -1394,6 +1456,10 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     // up to 16 rows, while they fit into the LDS that needs no attribute
     p.few = p.side == 16 && rows->kind != DENSE && few_lds(D * p.size) <= 61440;
     p.tiles = p.few ? (K + 63) / 64 : tiles;
+    // few rows' losses read every weight once: from anywhere, where a copy would be two passes more
+    // (1 x 50000 x 511 in bf16: 36 us with it, 26 without; 7 x 20011 x 201 in fp32: 23, 17)
+    p.pack_h = loose(H, ldh) && (gradient || !p.few);
+    p.pack_w = loose(W, ldw) && (gradient || !p.few);
     long long at = 0;
     const auto take = [&](long long bytes) {
         const long long here = at;
@@ -1614,6 +1680,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         a.tiles_r = (nb + p.tile_rows - 1) / p.tile_rows;
         a.tiles_c = p.tiles;
         a.slices = (int)((c.D * size + DME_SLICE - 1) / DME_SLICE);
+        a.row_bytes = (int)((p.pack_h ? p.dpad : c.D) * size);  // rows that are not whole chunks: both operands are packed, or neither
         a.bias = c.bias;
         a.nb = nb;
         a.K = c.K;
@@ -1639,10 +1706,15 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         int rc = DME_OK;
         if (p.few) {
             const unsigned blocks = (unsigned)(p.tiles + nb), bytes = (unsigned)few_lds(c.D * size);
-            if (kind == CSR)
-                hipLaunchKernelGGL((few_kernel<T, CSR>), dim3(blocks), dim3(256), bytes, s, a);
+            const bool loose = a.row_bytes % 16 || ((uintptr_t)h.at | (uintptr_t)h.ld | (uintptr_t)w.at | (uintptr_t)w.ld) % 16;
+            if (kind == CSR && loose)
+                hipLaunchKernelGGL((few_kernel<T, CSR, true>), dim3(blocks), dim3(256), bytes, s, a);
+            else if (kind == CSR)
+                hipLaunchKernelGGL((few_kernel<T, CSR, false>), dim3(blocks), dim3(256), bytes, s, a);
+            else if (loose)
+                hipLaunchKernelGGL((few_kernel<T, LABELS, true>), dim3(blocks), dim3(256), bytes, s, a);
             else
-                hipLaunchKernelGGL((few_kernel<T, LABELS>), dim3(blocks), dim3(256), bytes, s, a);
+                hipLaunchKernelGGL((few_kernel<T, LABELS, false>), dim3(blocks), dim3(256), bytes, s, a);
         } else {
             rc = tiles_of_z<T, false>(a, kind, p.side, s);
         }

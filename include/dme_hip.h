@@ -581,7 +581,7 @@ int dme_synth_dirmult(void* X /*[dev]*/, int elem_bytes, int64_t N, int64_t K, i
  * what each entry of the rows needs).
  *
  *   H [dev][N][ldh], W [dev][K][ldw]: bf16 or fp32 (type), values contiguous within a row, any pitch
- *     and alignment (rows that are not whole 16-byte groups cost a copy of the operand).
+ *     and alignment (rows that are not whole 16-byte groups cost a copy of the operands, but for losses of up to 16 rows).
  *   K up to 2^29, D up to 2^20.
  *   bias [dev][K] fp32 or NULL.  -inf takes a column out: its probability is 0, a count in it costs +inf.  Its weights do not
  *     enter the loss, whatever they hold; dH has 0 times them.
