@@ -415,22 +415,22 @@ __device__ __forceinline__ f32x2 merge(f32x2 v, f32x2 o) {
 
 // The forward pass for up to 16 rows: a read of the weights and little else.  A wave makes 16 columns for all rows; its weights
 // go from memory straight into the matrix instructions' registers, WIDE loads of 16 bytes a lane ahead, and the rows wait in LDS.
-// Nothing is shared between waves but the rows, so many small workgroups keep ~200 KB a CU in flight.  Workgroups beyond the
-// columns make the rows' z at their counts, so that a call has two launches.  Bound by memory: 1 x 50000 x 512 in bf16 reads 51 MB in
+// Nothing is shared between waves but the rows, so many small workgroups keep ~200 KB a CU in flight.  Workgroups before the
+// columns' make the rows' z at their counts, so that a call has two launches.  Bound by memory: 1 x 50000 x 512 in bf16 reads 51 MB in
 // 12.5 us (4.1 TB/s).  LOOSE: rows that are not whole chunks of 16 bytes are read as they lie.
 template <class T, int KIND, bool LOOSE>
 __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ f32x2 seen[4][16];
-    if (blockIdx.x >= a.tiles_c) {
-        const u32 r = blockIdx.x - (u32)a.tiles_c;
-        entries_of<T, KIND, LOOSE>(a, r, threadIdx.x >> 6, 4);
+    if (blockIdx.x < a.nb) {  // first, since they wait the longest
+        entries_of<T, KIND, LOOSE>(a, blockIdx.x, threadIdx.x >> 6, 4);
         return;
     }
+    const u32 block = blockIdx.x - (u32)a.nb;
     constexpr int WIDE = 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const int full = a.row_bytes / 16, chunks = (a.row_bytes + 15) / 16, rounds = (chunks + 3) / 4;  // a round: 64 bytes of each row
-    const long long k0 = (long long)blockIdx.x * 64 + wave * 16;
+    const long long k0 = (long long)block * 64 + wave * 16;
     const long long k = k0 + c < a.K ? k0 + c : a.K - 1;
     const char* w = a.w.at + k * a.w.ld;
     const u32q none = u32q{0, 0, 0, 0};
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
     s += __shfl_xor(s, 32);
     if (g == 0) seen[wave][c] = f32x2{m, s};
     __syncthreads();
-    if (tid < 16 && tid < a.nb) a.part[blockIdx.x * a.nb + tid] = merge(merge(seen[0][tid], seen[1][tid]), merge(seen[2][tid], seen[3][tid]));
+    if (tid < 16 && tid < a.nb) a.part[block * a.nb + tid] = merge(merge(seen[0][tid], seen[1][tid]), merge(seen[2][tid], seen[3][tid]));
 }
 
 // Tiles of z, reduced where the matrix instructions left them: a lane has NJ rows and 4 NI columns of each.
