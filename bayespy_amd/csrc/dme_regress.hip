@@ -280,8 +280,10 @@ __device__ __forceinline__ f32x4 with_bias(f32x4 v, f32x4 b, bool out) {
 __device__ __forceinline__ float exp_of(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * LOG2E); }
 
 // The same for many z of one m, one operation less: 2^(z log2 e - r) e^rest with r = m log2 e rounded to 32 bits and what that drops.
-// Not for |m| > FAR, where r's rounding is no small number.
-constexpr float FAR = 1e30f;
+// Not for |m| > FAR, where r's rounding is no small number: it is below 2^-24 |r|, so up to FAR 2^(z log2 e - r) is within a factor 2^(1/8) of
+// e^(z - m); at 1e10 it is hundreds, and of 2^rounding and 2^-rounding one is infinite and the other 0.  m is a tile's largest z here and a row's
+// there: a run of masked columns is enough to be beyond.
+constexpr float FAR = 1e6f;
 struct Reference {
     float r, rest;
     __device__ __forceinline__ explicit Reference(float m) {
