@@ -991,7 +991,6 @@ struct RowArgs {
     float* coef;
     float* weight;
     float* entry_g;        // CSR: [nnz], LABELS: [nb]: weight * G(z, x)
-    float* most;           // [workgroup]: its largest finite |entry_g|
 };
 
 // The row's pieces become l, the loss, and what the gradient needs of them, in 64 bits.  Bound by latency: 4099 rows of 196 pieces and
@@ -1004,7 +1003,6 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     constexpr int ROWS = 256 / LANES;
     __shared__ float m_seen[LANES][ROWS];
     __shared__ double s_seen[LANES][ROWS], sums[3][4];
-    __shared__ float most_seen[4];
     const long long first = (long long)blockIdx.x * ROWS;
     {
         const int row = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
@@ -1051,7 +1049,6 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     const bool dirichlet = a.likelihood == DME_LIKELIHOOD_DIRICHLET;
     const double top = (double)m;
     const float weight = a.weights ? a.weights[rr] : 1.f;
-    float most = 0.f;
     double f = 0.0, total = 0.0, times = 0.0;
     if (a.kind == DENSE) {
         for (int tile = sub; tile < a.tiles; tile += LANES) {
@@ -1080,11 +1077,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
                 f += ((double)z - top) * (dirichlet ? 1.0 : (double)x);
                 if (dirichlet) f += small ? (double)small_rest(z, x) : dirichlet_rest((double)z, (double)x);
             }
-            if (a.largest_z && real) {
-                const float v = weight * (small ? small_g(z, x) : (float)g_of(a.likelihood, (double)z, (double)x));
-                a.entry_g[e] = v;
-                if (__builtin_isfinite(v)) most = fmaxf(most, fabsf(v));
-            }
+            if (a.largest_z && real) a.entry_g[e] = weight * (small ? small_g(z, x) : (float)g_of(a.likelihood, (double)z, (double)x));
         }
         if (bad) total = __builtin_nan("");
     } else if (sub == 0) {  // F(z, 1) = z, G(z, 1) = 1 in both likelihoods
@@ -1093,10 +1086,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         total = k < 0 ? 0.0 : in ? 1.0 : __builtin_nan("");
         f = in ? (double)a.entry_z[rr] - top : 0.0;
         times = in ? 1.0 : 0.0;
-        if (a.largest_z && real) {
-            a.entry_g[r] = weight;
-            most = k >= 0 && __builtin_isfinite(weight) ? fabsf(weight) : 0.f;
-        }
+        if (a.largest_z && real) a.entry_g[r] = weight;
     }
     if constexpr (LANES == 16) {
         f = sum16(f);
@@ -1118,12 +1108,6 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     }
     // the row's own terms take a thousand instructions in 64 bits: one wave makes the loss of all rows here, one the gradient's coefficients
     const int part = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    if (a.largest_z && a.kind != DENSE) {  // no atomics: a thousand of them to one address took 10 us
-        most = max16(most);
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        if (lane == 0) most_seen[part] = most;
-    }
     if (LANES == 16 && sub == 0) {
         s_seen[0][row] = s;
         s_seen[1][row] = f;
@@ -1132,8 +1116,6 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         m_seen[0][row] = m;
     }
     __syncthreads();
-    if (a.largest_z && a.kind != DENSE && threadIdx.x == 0)
-        a.most[blockIdx.x] = fmaxf(fmaxf(most_seen[0], most_seen[1]), fmaxf(most_seen[2], most_seen[3]));
     if (lane >= ROWS || first + lane >= a.nb) return;
     if constexpr (LANES == 16) {
         s = s_seen[0][lane];
@@ -1173,60 +1155,76 @@ struct PatchArgs {
     // the counts' column sums for dbias, in the first piece's launch
     u32 blocks, ranges;  // workgroups for them (0: none), ranges of columns
     long long group;     // rows of a group
-    long long* sums;     // [group of rows][K]
-    const float* most;   // [mosts]
-    int mosts;
-    int headroom;        // bits that the sum of all entries may need above one entry
+    double* sums;        // [group of rows][K]
 };
-
-// The exponent of the fixed-point sums of entry_g: the largest one takes 62 - headroom bits, whatever its size.  Every thread of the
-// workgroup calls this.
-template <int WAVES>
-__device__ __forceinline__ int fixed_shift(const float* most, int mosts, int headroom) {
-    __shared__ float seen[WAVES];
-    float v = 0.f;
-    for (int i = threadIdx.x; i < mosts; i += WAVES * 64) v = fmaxf(v, most[i]);
-    v = max16(v);
-    v = fmaxf(v, __shfl_xor(v, 16));
-    v = fmaxf(v, __shfl_xor(v, 32));
-    if ((threadIdx.x & 63) == 0) seen[threadIdx.x >> 6] = v;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) v = fmaxf(v, seen[w]);
-    return 62 - headroom - (v > 0.f ? ilogbf(v) + 1 : 0);
-}
 
 // What dbias needs of the counts, entry_g added up by column: a workgroup takes a group of rows and a range of columns, looks through all
 // entries of those rows and adds up the range's in LDS, in fixed point, 64 bits wide: sums of whole numbers do not depend on their order.
+// Each column has a point of its own, set by its largest entry of the group, which a first look finds: rows of next to no weight have columns of their own
+// beside rows of much, and their entries would be lost behind one point for all.  The largest takes 54 bits, which leaves 8 for a group's sum (a row has a
+// column once) and holds the 24 bits of entries down to 2^-30 of it whole.  A column with an entry that has left 32 bits is NaN.
 // Word frequencies leave few entries of a column together: with atomics in memory, after a hash table in LDS had joined those of 32 rows, 100 000
-// of 144 000 were left, and took 25 us; so it is 7, beside the other workgroups.  Groups are of 256 rows (each leaves K sums), smaller ones where
-// there would be few workgroups (1024 rows, 10 007 columns: 12 us with 256, 7 with 16).
+// of 144 000 were left, and took 25 us; so it is 10, beside the other workgroups.  Groups are of up to 256 rows (each leaves K sums), smaller ones
+// where there would be fewer workgroups than CUs (the launch at 4099 rows, 50 000 columns: 24 us with 119 workgroups for groups of 256, 18 with 231 for
+// groups of 128, 16 with a thread's first entries kept).
 constexpr int RANGE = 8192;          // columns
+constexpr int RANGE_BYTES = 8 + 2;   // of LDS for each: its sum and its point
+constexpr int MOST_GROUP = 256;      // rows
 template <int KIND>
 __device__ __forceinline__ void sum_counts(const PatchArgs& a, char* lds) {
-    u64* sums = (u64*)lds;
+    constexpr short LOST = 0x7fff;
     const long long group = blockIdx.x / a.ranges, c0 = (long long)(blockIdx.x % a.ranges) * RANGE;
     const int width = (int)(a.K - c0 < RANGE ? a.K - c0 : RANGE);
-    for (int i = threadIdx.x; i < width; i += 512) sums[i] = 0;
-    const int shift = fixed_shift<8>(a.most, a.mosts, a.headroom);  // passes a barrier
+    u64* sums = (u64*)lds;
+    short* point = (short*)(lds + (a.K < RANGE ? a.K : RANGE) * 8);
     const long long r0 = group * a.group, r1 = r0 + a.group < a.nb ? r0 + a.group : a.nb;
     const long long p0 = KIND == CSR ? row_begin(a.rows, r0) : r0, p1 = KIND == CSR ? row_begin(a.rows, r1) : r1;
-    constexpr int DEEP = KIND == CSR ? 4 : 1;
-    for (long long e = p0 + threadIdx.x; e < p1; e += DEEP * 512) {
-        long long k[DEEP];
-        float g[DEEP];
+    // DEEP entries of a thread at a time; the first ones stay for the second look
+    constexpr int DEEP = KIND == CSR ? 8 : 1;
+    const auto load = [&](long long e, int (&k)[DEEP], float (&g)[DEEP]) {
 #pragma unroll
         for (int u = 0; u < DEEP; ++u) {
-            const bool in = e + u * 512 < p1;
-            k[u] = !in ? -1 : KIND == CSR ? (long long)a.rows.col[e + u * 512] - c0 : a.rows.labels[e + u * 512] - c0;
-            g[u] = in ? a.entry_g[e + u * 512] : 0.f;
+            k[u] = -1;
+            g[u] = 0.f;
+            if (e + u * 512 < p1) {
+                const u64 c = (u64)(KIND == CSR ? (long long)a.rows.col[e + u * 512] : a.rows.labels[e + u * 512]) - (u64)c0;
+                k[u] = c < (u64)width ? (int)c : -1;
+                g[u] = a.entry_g[e + u * 512];
+            }
         }
+    };
+    int k0[DEEP];
+    float g0[DEEP];
+    load(p0 + threadIdx.x, k0, g0);
+    const auto each = [&](auto take) {
 #pragma unroll
         for (int u = 0; u < DEEP; ++u)
-            if (k[u] >= 0 && k[u] < width && __builtin_isfinite(g[u])) atomicAdd(&sums[k[u]], (u64)llrint(ldexp((double)g[u], shift)));
+            if (k0[u] >= 0) take(k0[u], g0[u]);
+        for (long long e = p0 + threadIdx.x + DEEP * 512; e < p1; e += DEEP * 512) {
+            int k[DEEP];
+            float g[DEEP];
+            load(e, k, g);
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u)
+                if (k[u] >= 0) take(k[u], g[u]);
+        }
+    };
+    for (int i = threadIdx.x; i < width; i += 512) sums[i] = 0;
+    __syncthreads();
+    each([&](int k, float g) { atomicMax((u32*)(sums + k), __builtin_bit_cast(u32, fabsf(g))); });  // ordered like the values
+    __syncthreads();
+    for (int i = threadIdx.x; i < width; i += 512) {
+        const float most = __builtin_bit_cast(float, (u32)sums[i]);
+        point[i] = !__builtin_isfinite(most) ? LOST : (short)(most > 0.f ? 53 - ilogbf(most) : 0);
+        sums[i] = 0;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < width; i += 512) a.sums[group * a.K + c0 + i] = (long long)sums[i];
+    each([&](int k, float g) {
+        if (point[k] != LOST) atomicAdd(sums + k, (u64)llrint(ldexp((double)g, point[k])));
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < width; i += 512)
+        a.sums[group * a.K + c0 + i] = point[i] == LOST ? __builtin_nan("") : ldexp((double)(long long)sums[i], -point[i]);
 }
 
 // d loss / d z at the counts: the tiles' value made again, minus G, in its place.  LANES lanes a row.  Bound by latency: 4099 rows with 144 000
@@ -1359,19 +1357,18 @@ __device__ __forceinline__ void join(const JoinArgs& a, u32 block) {
 struct BiasArgs {
     const float* part;
     long long tiles, K;
-    const long long* sums;  // [groups][K], or null: dense rows
+    const double* sums;  // [groups][K], or null: dense rows
     long long groups;
-    const float* most;
-    int mosts, headroom, add;
+    int add;
     float* dbias;
     u32 blocks;
 };
 
-__device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*sums)[64], long long (*counts)[64]) {
+__device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*sums)[64]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long k = (long long)block * 64 + lane;
     double v = 0.0;
-    if (k < a.K)
+    if (k < a.K) {
         for (long long t = wave; t < a.tiles; t += 16) {
             float p[4];
 #pragma unroll
@@ -1379,25 +1376,20 @@ __device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*
 #pragma unroll
             for (int u = 0; u < 4; ++u) v += (double)p[u];
         }
-    sums[wave][lane] = v;
-    long long whole = 0;
-    int shift = 0;
-    if (a.sums) {
-        shift = fixed_shift<4>(a.most, a.mosts, a.headroom);
-        if (k < a.K)
+        if (a.sums)
             for (long long t = wave; t < a.groups; t += 16) {
-                long long p[4];
+                double p[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) p[u] = t + u * 4 < a.groups ? a.sums[(t + u * 4) * a.K + k] : 0;
-                whole += (p[0] + p[1]) + (p[2] + p[3]);
+                for (int u = 0; u < 4; ++u) p[u] = t + u * 4 < a.groups ? a.sums[(t + u * 4) * a.K + k] : 0.0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v -= p[u];
             }
-        counts[wave][lane] = whole;
     }
+    sums[wave][lane] = v;
     __syncthreads();
     if (wave != 0 || k >= a.K) return;
     v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
     if (a.add) v += (double)a.dbias[k];
-    if (a.sums) v -= ldexp((double)((counts[0][lane] + counts[1][lane]) + (counts[2][lane] + counts[3][lane])), -shift);
     a.dbias[k] = (float)v;
 }
 
@@ -1405,12 +1397,11 @@ __device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*
 template <class T>
 __global__ __launch_bounds__(256) void finish_kernel(JoinArgs w, JoinArgs h, BiasArgs b) {
     __shared__ double sums[4][64];
-    __shared__ long long counts[4][64];
     u32 block = blockIdx.x;
     if (block < w.blocks) return join<T>(w, block);
     block -= w.blocks;
     if (block < h.blocks) return join<T>(h, block);
-    add_bias(b, block - h.blocks, sums, counts);
+    add_bias(b, block - h.blocks, sums);
 }
 
 inline long long up(long long v, long long to) { return (v + to - 1) / to * to; }
@@ -1430,10 +1421,9 @@ struct Plan {
     DmePair cut_w, cut_h;     // how they are cut: one cut for both, or each its own
     bool pieces_w, pieces_h;  // the products leave 32-bit pieces
     long long ldpart;
-    int headroom;
     long long group;          // rows of a group of the counts' column sums
     // places in the workspace
-    long long most, sums, h, w, part, part_f, part_w, part_t, entry_z, entry_g, largest_z, coef, weight, dbias, dz, pw, ph, bytes;
+    long long sums, h, w, part, part_f, part_w, part_t, entry_z, entry_g, largest_z, coef, weight, dbias, dz, pw, ph, bytes;
 };
 
 inline long long few_lds(long long bytes) { return 16 * (up(bytes, 64) + 64); }
@@ -1470,9 +1460,8 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     };
     if (gradient && rows->kind != DENSE) {
         const long long ranges = (K + RANGE - 1) / RANGE;
-        for (; p.group < 256 && (p.nb + p.group - 1) / p.group * ranges > 128;) p.group *= 2;
+        for (; p.group < MOST_GROUP && (p.nb + p.group - 1) / p.group * ranges > 256;) p.group *= 2;
         p.sums = take((p.nb + p.group - 1) / p.group * K * 8);
-        p.most = take((p.nb <= FEW_ROWS ? p.nb : FEW_ROWS + p.nb / 16) * 4);
     }
     if (p.pack_h) p.h = take(p.nb * p.dpad * p.size);
     if (p.pack_w) p.w = take(K * p.dpad * p.size);
@@ -1488,7 +1477,6 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
     }
     if (gradient) {
         if (rows->kind != DENSE) p.entry_g = take((rows->kind == CSR ? rows->nnz : p.nb) * 4);
-        for (p.headroom = 1; (rows->kind == CSR ? rows->nnz : N) >> p.headroom; ++p.headroom) {}
         p.largest_z = take(p.nb * 4);
         p.coef = take(p.nb * 4);
         p.weight = take(p.nb * 4);
@@ -1608,7 +1596,7 @@ int products(const ProductArgs& w, const ProductArgs& h, const DmePair& cut, boo
 template <class T, int KIND, int LANES>
 int launch_patch(const PatchArgs& a, unsigned lds, hipStream_t s) {
     static std::atomic<bool> done[64];
-    const int rc = set_lds(done, patch_kernel<T, KIND, LANES>, RANGE * 8);
+    const int rc = set_lds(done, patch_kernel<T, KIND, LANES>, RANGE * RANGE_BYTES);
     if (rc) return rc;
     constexpr int rows = 512 / LANES;
     hipLaunchKernelGGL((patch_kernel<T, KIND, LANES>), dim3(a.blocks + (unsigned)((a.nb + rows - 1) / rows)), dim3(512), lds, s, a);
@@ -1663,8 +1651,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         pack_w = DmePack{w.at, w.ld, c.K, c.D * size, ws + p.w, p.dpad * size};
         w = DmeOperand{ws + p.w, p.dpad * size, c.K};
     }
-    float* most = (float*)(ws + p.most);
-    long long* sums = gradient && kind != DENSE && c.dbias ? (long long*)(ws + p.sums) : nullptr;
+    double* sums = gradient && kind != DENSE && c.dbias ? (double*)(ws + p.sums) : nullptr;
     for (long long n0 = 0; n0 < c.N; n0 += p.nb) {
         const long long nb = c.N - n0 < p.nb ? c.N - n0 : p.nb;
         DmeOperand h{(const char*)c.H + n0 * c.ldh * size, c.ldh * size, nb};
@@ -1740,7 +1727,6 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
             ra.coef = (float*)(ws + p.coef);
             ra.weight = (float*)(ws + p.weight);
             ra.entry_g = (float*)(ws + p.entry_g);
-            ra.most = most;
         }
         const unsigned groups = (unsigned)(nb <= FEW_ROWS ? nb : (nb + 15) / 16);
         if (nb <= FEW_ROWS)
@@ -1769,10 +1755,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
                     pa.blocks = (u32)((nb + p.group - 1) / p.group) * pa.ranges;
                     pa.group = p.group;
                     pa.sums = sums;
-                    pa.most = most;
-                    pa.mosts = (int)groups;
-                    pa.headroom = p.headroom;
-                    lds = (unsigned)std::min(c.K, (long long)RANGE) * 8;
+                    lds = (unsigned)std::min(c.K, (long long)RANGE) * RANGE_BYTES;
                 }
                 rc = kind == CSR ? launch_patch<T, CSR, 16>(pa, lds, s) : launch_patch<T, LABELS, 1>(pa, lds, s);
                 if (rc) return rc;
@@ -1818,7 +1801,7 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
         if (p.pieces_w && n0 + nb == c.N) jw = join_args(ws + p.pw, p.ldpart, c.K * p.ldpart, p.cut_w.splits_w, c.K, c.D, c.dW);
         if (p.pieces_h) jh = join_args(ws + p.ph, p.ldpart, p.nb * p.ldpart, p.cut_h.splits_h, nb, c.D, (T*)c.dH + n0 * c.D);
         if (c.dbias)
-            bias = BiasArgs{a.dbias, a.tiles_r, c.K, sums, (nb + p.group - 1) / p.group, most, (int)groups, p.headroom, (int)(n0 > 0), c.dbias, (u32)((c.K + 63) / 64)};
+            bias = BiasArgs{a.dbias, a.tiles_r, c.K, sums, (nb + p.group - 1) / p.group, (int)(n0 > 0), c.dbias, (u32)((c.K + 63) / 64)};
         const u32 blocks = jw.blocks + jh.blocks + bias.blocks;
         if (blocks) hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks), dim3(256), 0, s, jw, jh, bias);
     }

@@ -180,3 +180,35 @@ def test_two_masks_beside_each_other(n):
     for kind in ("csr", "dense"):
         for likelihood in ("multinomial", "dirichlet"):
             all_of_it(h, w, b, x, weight, kind, likelihood, torch.bfloat16)
+
+
+@pytest.mark.parametrize("kind", ["labels", "csr", "dense"])
+@pytest.mark.parametrize("n", [12, 60, 700])
+def test_bias_gradient_of_light_rows(n, kind):
+    """Rows of a responsibility near 1 and rows of next to none, each with columns of its own: the light rows' columns have the gradient of
+    those rows, relative to its own size.  (The heavy rows' p is 0 in 32 bits there, and the light rows' in theirs.)"""
+    k, d = 9001, 8
+    r = np.random.default_rng(n)
+    heavy = torch.arange(n, device="cuda") % 2 == 0
+    h = torch.zeros(n, d, device="cuda")
+    h[:, 0] = torch.where(heavy, 100.0, -100.0)
+    w = torch.zeros(k, d, device="cuda")
+    w[:, 0] = torch.where(torch.arange(k, device="cuda") < k // 2, 2.0, -2.0)
+    b = torch.from_numpy(r.integers(-8, 9, size=k) / 4).float().cuda()
+    x = np.zeros((n, k), dtype=np.int32)
+    labels = np.zeros(n, dtype=np.int64)
+    for i in range(n):
+        at = (0 if i % 2 == 0 else k // 2) + r.choice(k // 2, size=9, replace=False)
+        labels[i] = at[0]
+        if kind == "labels":
+            x[i, at[0]] = 1
+        else:
+            x[i, at] = r.choice([1, 2, 3, 1000000], size=9) if i % 2 == 0 else r.choice([1, 2, 3], size=9)
+    x, labels = torch.from_numpy(x).cuda(), torch.from_numpy(labels).cuda()
+    for light in (1e-6, 1e-13, 1e-25):
+        weight = torch.where(heavy, 1.0, light)
+        want = exact(h, w, b, x, weight, "multinomial", torch.float32)
+        from bayespy_amd import regression
+        got = regression.log_loss_gradient(h, w, rows_of(x, kind, labels), bias=b, row_weights=weight)[3]
+        near(got[:k // 2], [v[:k // 2] for v in want["dbias"]], "dbias of the heavy rows' columns")
+        near(got[k // 2:], [v[k // 2:] for v in want["dbias"]], "dbias of the light rows' columns, weight %g" % light)
