@@ -1458,29 +1458,32 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         at += up(bytes, 256);
         return here;
     };
-    if (gradient && rows->kind != DENSE) {
-        const long long ranges = (K + RANGE - 1) / RANGE;
-        for (; p.group < MOST_GROUP && (p.nb + p.group - 1) / p.group * ranges > 256;) p.group *= 2;
-        p.sums = take((p.nb + p.group - 1) / p.group * K * 8);
-    }
     if (p.pack_h) p.h = take(p.nb * p.dpad * p.size);
     if (p.pack_w) p.w = take(K * p.dpad * p.size);
+    const long long forward = at;
     p.part = take(p.tiles * p.nb * 8);
-    if (rows->kind == CSR) {
-        p.entry_z = take(rows->nnz * 4);
-    } else if (rows->kind == DENSE) {
+    if (rows->kind == DENSE) {
         p.part_f = take(p.tiles * p.nb * 8);
         p.part_w = take(p.tiles * p.nb * 8);
         p.part_t = take(p.tiles * p.nb * 8);
-    } else {
-        p.entry_z = take(p.nb * 4);
     }
+    if (gradient) {  // the sums for dbias lie where the forward pass's pieces were: row_kernel, the launch before theirs, is the last to read those
+        const long long end = at;
+        at = forward;
+        if (rows->kind != DENSE) {
+            const long long ranges = (K + RANGE - 1) / RANGE;
+            for (; p.group < MOST_GROUP && (p.nb + p.group - 1) / p.group * ranges > 256;) p.group *= 2;
+            p.sums = take((p.nb + p.group - 1) / p.group * K * 8);
+        }
+        p.dbias = take((p.nb + p.tile_rows - 1) / p.tile_rows * K * 4);
+        at = std::max(at, end);
+    }
+    if (rows->kind != DENSE) p.entry_z = take((rows->kind == CSR ? rows->nnz : p.nb) * 4);
     if (gradient) {
         if (rows->kind != DENSE) p.entry_g = take((rows->kind == CSR ? rows->nnz : p.nb) * 4);
         p.largest_z = take(p.nb * 4);
         p.coef = take(p.nb * 4);
         p.weight = take(p.nb * 4);
-        p.dbias = take((p.nb + p.tile_rows - 1) / p.tile_rows * K * 4);
         long long c = PIECE_BYTES / (p.nb * p.size) / p.tile_cols;
         if (c < 1) c = 1;
         if (c > tiles) c = tiles;

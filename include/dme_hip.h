@@ -576,9 +576,16 @@ int dme_synth_dirmult(void* X /*[dev]*/, int elem_bytes, int64_t N, int64_t K, i
  * With T = sum_k x_k, l = log sum_k exp(z_k):
  *   multinomial   loss = T l - sum_k x_k z_k                          (softmax; the multinomial coefficient left out)
  *   Dirichlet     loss = lgamma(e^l + T) - lgamma(e^l) - sum_k [lgamma(e^z_k + x_k) - lgamma(e^z_k)]
- * z is never stored whole: the loss takes one pass over the columns, the gradient makes z again in pieces of the
- * columns (256 MB of d loss / d z at a time, at most 16384 rows at a time; beside it dW and dH in 32 bits where a sum is split, and
- * what each entry of the rows needs).
+ * z is never stored whole: the loss takes one pass over the columns, the gradient makes z again in pieces of the columns.
+ * Scratch (dme_log_loss_workspace_bytes) for R rows, N of them or 65536, in a gradient 16384 (fewer where K passes 2^19, 2^21):
+ *   what the tiles leave: 8 R bytes for every 64 (up to 16 rows, small shapes), 128 or 256 columns; dense rows 32 R for every 128
+ *   z at the counts: 4 bytes for each CSR entry or row of labels, in a gradient 8
+ *   copies of H's R rows and of W, where they are not whole 16-byte groups
+ * and in a gradient
+ *   d loss / d z: 256 MB or one tile's columns of R rows, whichever is more
+ *   dW and dH in 32 bits, once for each piece that a sum is split into
+ *   dbias's sums, in the place of what the tiles left and as far as they are more: of each column 4 bytes for every 16 to 256 rows and, unless rows
+ *   are dense, 8 for every 16 to 256.  (Their place is kept without dbias too.)
  *
  *   H [dev][N][ldh], W [dev][K][ldw]: bf16 or fp32 (type), values contiguous within a row, any pitch
  *     and alignment (rows that are not whole 16-byte groups cost a copy of the operands, but for losses of up to 16 rows).
