@@ -330,15 +330,16 @@ __global__ __launch_bounds__(256) void join_kernel(Matrices x, int splits) {
     float v = 0.f;
     if (r < x.m && c < x.m) {
         const float* at = x.part + blockIdx.y * x.stride_part + (r > c ? r * x.lds + c : c * x.lds + r);  // above the diagonal: the same sum
-        int s = 0;
-        for (; s + 8 <= splits; s += 8) {
+        const auto eight = [&](int s, auto last) {  // loads without branches: all on their way at once
             float p[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) p[u] = at[(s + u) * x.stride_s];
+            for (int u = 0; u < 8; ++u) p[u] = at[(!last || s + u < splits ? s + u : s) * x.stride_s];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v += p[u];
-        }
-        for (; s < splits; ++s) v += at[s * x.stride_s];
+            for (int u = 0; u < 8; ++u) v += !last || s + u < splits ? p[u] : 0.f;
+        };
+        int s = 0;
+        for (; s + 8 <= splits; s += 8) eight(s, std::false_type());
+        if (s < splits) eight(s, std::true_type());
     }
     turn[hi][lo] = v;
     if (r < x.m && c < x.lds) put_s<PARTS>(x, so, mo, r, c, v);
@@ -676,11 +677,11 @@ StepPlan plan_of(int type, long long batch, long long rows, long long cols) {
     p.n = rows < cols ? cols : rows;
     p.ldx = up(cols, 8);
     p.lds = up(p.m, 8);
-    // three products of halves cost three times the slices
-    const auto slices = [&](long long k) { return (k * 2 + DME_SLICE - 1) / DME_SLICE * (parts == 2 ? 3 : 1); };
-    p.square = dme_cut(p.m, p.m, slices(p.n), 2, true, 0.0, true, batch);
-    p.poly = dme_cut(p.m, p.m, slices(p.m), 2, false, 0.0, true, batch);
-    p.update = dme_cut(rows, cols, slices(p.m), 2, false, 0.0, false, batch);
+    const int products = parts == 2 ? 3 : 1;
+    const auto slices = [](long long k) { return (k * 2 + DME_SLICE - 1) / DME_SLICE; };
+    p.square = dme_cut(p.m, p.m, slices(p.n), 2, true, 0.0, true, batch, products);
+    p.poly = dme_cut(p.m, p.m, slices(p.m), 2, false, 0.0, true, batch, products);
+    p.update = dme_cut(rows, cols, slices(p.m), 2, false, 0.0, false, batch, products);
     // a slab of X with all its singular values is one tile, and X is read once: where there are slabs enough for the card
     p.slab = p.m <= 256 && batch * ((p.n + 63) / 64) >= 256;
     long long at = 0;

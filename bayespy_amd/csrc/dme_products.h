@@ -350,8 +350,15 @@ constexpr double DME_ALONE = 0.75;
 // us of writing and adding up pieces of 32-bit sums
 inline double dme_join_us(int splits, double values) { return splits > 1 ? 4.0 + splits * values * 8.0 / 4e6 : 0.0; }
 
+// into how many pieces `slices` slices go when they are cut into `splits` of the same length, rounded up: the others would have none
+inline int dme_pieces(long long slices, long long splits) {
+    const long long each = (slices + splits - 1) / splits;
+    return each > 0 ? (int)((slices + each - 1) / each) : 1;
+}
+
+// `products`: how many a slice costs (the sum of as many products is made)
 inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool split, double extra_per_tile_us = 0.0, bool symmetric = false,
-                      long long batch = 1) {
+                      long long batch = 1, int products = 1) {
     DmeCut best{0, 1, 0.0};
     for (const DmeKind& kind : DME_KINDS) {
         const int side = kind.side, per_cu = kind.per_cu;
@@ -359,10 +366,11 @@ inline DmeCut dme_cut(long long R, long long C, long long slices, int size, bool
         const long long tiles = batch * (symmetric ? along * (along + 1) / 2 : along * ((C + side - 1) / side));
         const double slice = dme_slice_us(kind, size);
         const auto consider = [&](long long s) {
-            if (s > 1 && slices / s < 2) return;
+            if (s > 1 && slices * products / s < 2) return;
+            s = dme_pieces(slices, s);
             const double rounds = (double)((tiles * s + slots - 1) / slots);
             const double each = s > 1 && tiles * s <= 256 && per_cu > 1 ? DME_ALONE * slice : slice;
-            const double us = rounds * ((double)((slices + s - 1) / s + 2) * each + extra_per_tile_us * side * side / 65536.0 * per_cu) +
+            const double us = rounds * ((double)((slices + s - 1) / s * products + 2) * each + extra_per_tile_us * side * side / 65536.0 * per_cu) +
                               dme_join_us((int)s, (double)batch * R * C);
             if (best.side == 0 || us < best.us) best = DmeCut{side, (int)s, us};
         };
@@ -384,8 +392,9 @@ inline DmePair dme_pair(long long Rw, long long sw, long long Rh, long long sh, 
     for (const DmeKind& kind : DME_KINDS) {
         const long long side = kind.side, across = (C + side - 1) / side, tw = (Rw + side - 1) / side * across, th = (Rh + side - 1) / side * across;
         const double slots = 256.0 * kind.per_cu, slice = dme_slice_us(kind, size);
-        for (int a = 1; a <= 64 && (a == 1 || sw / a >= 2); a *= 2)
-            for (int b = 1; b <= 64 && (b == 1 || sh / b >= 2); b *= 2) {
+        for (int cuts_w = 1; cuts_w <= 64 && (cuts_w == 1 || sw / cuts_w >= 2); cuts_w *= 2)
+            for (int cuts_h = 1; cuts_h <= 64 && (cuts_h == 1 || sh / cuts_h >= 2); cuts_h *= 2) {
+                const int a = dme_pieces(sw, cuts_w), b = dme_pieces(sh, cuts_h);
                 const double lw = (double)((sw + a - 1) / a + 2), lh = (double)((sh + b - 1) / b + 2);
                 const double whole = ((double)tw * a * lw + (double)th * b * lh) / slots, last = lw < lh ? lw : lh, longest = lw < lh ? lh : lw;
                 double us = whole + 0.5 * last;

@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "dme_products.h"
 
@@ -1332,15 +1333,16 @@ __device__ __forceinline__ void join(const JoinArgs& a, u32 block) {
         if (c >= a.length) continue;
         const float* at = a.part + line * a.ldpart + c;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-        int s = 0;
-        for (; s + 4 <= a.splits; s += 4) {
+        const auto four = [&](int s, auto last) {  // loads without branches: all on their way at once
             f32x4 p[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) p[u] = *(const f32x4*)(at + (s + u) * a.split_stride);
+            for (int u = 0; u < 4; ++u) p[u] = *(const f32x4*)(at + (!last || s + u < a.splits ? s + u : s) * a.split_stride);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v += p[u];
-        }
-        for (; s < a.splits; ++s) v += *(const f32x4*)(at + s * a.split_stride);
+            for (int u = 0; u < 4; ++u) v += !last || s + u < a.splits ? p[u] : f32x4{0.f, 0.f, 0.f, 0.f};
+        };
+        int s = 0;
+        for (; s + 4 <= a.splits; s += 4) four(s, std::false_type());
+        if (s < a.splits) four(s, std::true_type());
         T* o = (T*)a.out + line * a.length + c;
         if (a.vector) {
             dme_store4(o, v);

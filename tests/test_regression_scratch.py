@@ -29,3 +29,27 @@ def test_dense_rows_leave_more_than_dbias_needs():
     gradient = _bytes(n, k, d, 1, kind=2)
     dz = n * k * 2
     assert forward + dz <= gradient <= forward + dz + 64 * (n + k) * d * 4 + n * 32 + 4096
+
+
+def test_no_empty_pieces_of_a_step_s_square():
+    """Every piece that k is cut into has slices (64 halves each) of its own.  The rest of what a step of matrices beyond 64 singular values takes is
+    its pairs, S and B, so the pieces' number follows from the bytes."""
+    from bayespy_amd import _lib
+    up = lambda v, to: (v + to - 1) // to * to  # noqa: E731
+    several = 0
+    for type_ in (0, 1):
+        for m, n in ((250, 2000), (2000, 250), (100, 8300), (129, 129), (300, 5000), (512, 4097), (70, 20000), (250, 8321), (1000, 1030)):
+            rows, cols = m, n
+            ldx, small = up(cols, 8), min(m, n)
+            lds, parts = up(small, 8), 2 if type_ == 0 else 1
+            sizes = [256 * 8] + [rows * ldx * 2] * 4 + [small * lds * 2] * 2 * parts + [lds * 4] * 2
+            if type_ == 0:
+                sizes += [rows * ldx * 4, small * lds * 4]
+            left = _lib.lib().dme_orthogonal_step_workspace_bytes(type_, 1, rows, cols) - sum(up(s, 256) for s in sizes)
+            slices = -(-max(m, n) * 2 // 128)
+            pieces = left // (small * lds * 4)
+            assert left == up(pieces * small * lds * 4, 256)
+            if pieces:
+                several += 1
+                assert -(-slices // -(-slices // pieces)) == pieces, (type_, m, n, slices, pieces)
+    assert several > 6
