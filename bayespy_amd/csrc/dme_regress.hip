@@ -1155,6 +1155,7 @@ struct PatchArgs {
     long long lddz;
     // the counts' column sums for dbias, in the first piece's launch
     u32 blocks, ranges;  // workgroups for them (0: none), ranges of columns
+    int range;           // columns of a range
     long long group;     // rows of a group
     double* sums;        // [group of rows][K]
 };
@@ -1165,19 +1166,21 @@ struct PatchArgs {
 // beside rows of much, and their entries would be lost behind one point for all.  The largest takes 54 bits, which leaves 8 for a group's sum (a row has a
 // column once) and holds the 24 bits of entries down to 2^-30 of it whole.  A column with an entry that has left 32 bits is NaN.
 // Word frequencies leave few entries of a column together: with atomics in memory, after a hash table in LDS had joined those of 32 rows, 100 000
-// of 144 000 were left, and took 25 us; so it is 10, beside the other workgroups.  Groups are of up to 256 rows (each leaves K sums), smaller ones
-// where there would be fewer workgroups than CUs (the launch at 4099 rows, 50 000 columns: 24 us with 119 workgroups for groups of 256, 18 with 231 for
-// groups of 128, 16 with a thread's first entries kept).
-constexpr int RANGE = 8192;          // columns
+// of 144 000 were left, and took 25 us; so it is 10, beside the other workgroups.  A group has up to 256 rows, since each leaves K sums, and as many
+// entries as the threads hold in two looks, since every range's workgroup looks through all of them (the launch at 4099 rows, 50 000 columns: 24 us with
+// groups of 256, 16 with 128).  Ranges are wide and groups large unless too many CUs would be without a workgroup (1024 rows, 10 007 columns: 9 us in
+// 32 workgroups, 6 in 160); labels are looked through at once, whatever the group (4000 rows, 1000 columns: 76 us a gradient with 16, 70 with 256).
+constexpr int RANGE = 8192, LEAST_RANGE = 1024;  // columns
 constexpr int RANGE_BYTES = 8 + 2;   // of LDS for each: its sum and its point
 constexpr int MOST_GROUP = 256;      // rows
+constexpr int GROUP_ENTRIES = 8192;  // twice what the threads hold at a time
 template <int KIND>
 __device__ __forceinline__ void sum_counts(const PatchArgs& a, char* lds) {
     constexpr short LOST = 0x7fff;
-    const long long group = blockIdx.x / a.ranges, c0 = (long long)(blockIdx.x % a.ranges) * RANGE;
-    const int width = (int)(a.K - c0 < RANGE ? a.K - c0 : RANGE);
+    const long long group = blockIdx.x / a.ranges, c0 = (long long)(blockIdx.x % a.ranges) * a.range;
+    const int width = (int)(a.K - c0 < a.range ? a.K - c0 : a.range);
     u64* sums = (u64*)lds;
-    short* point = (short*)(lds + (a.K < RANGE ? a.K : RANGE) * 8);
+    short* point = (short*)(lds + a.range * 8);
     const long long r0 = group * a.group, r1 = r0 + a.group < a.nb ? r0 + a.group : a.nb;
     const long long p0 = KIND == CSR ? row_begin(a.rows, r0) : r0, p1 = KIND == CSR ? row_begin(a.rows, r1) : r1;
     // DEEP entries of a thread at a time; the first ones stay for the second look
@@ -1473,8 +1476,9 @@ Plan make_plan(const void* H, long long ldh, const void* W, long long ldw, int t
         const long long end = at;
         at = forward;
         if (rows->kind != DENSE) {
-            const long long ranges = (K + RANGE - 1) / RANGE;
-            for (; p.group < MOST_GROUP && (p.nb + p.group - 1) / p.group * ranges > 256;) p.group *= 2;
+            const double entries = rows->kind == CSR ? (double)rows->nnz / (double)std::max(N, 1ll) : 1.0;  // of a row
+            const auto workgroups = [&](long long group) { return (p.nb + group - 1) / group * ((K + LEAST_RANGE - 1) / LEAST_RANGE); };
+            while (p.group < MOST_GROUP && 2 * p.group * entries <= GROUP_ENTRIES && (rows->kind == LABELS || workgroups(2 * p.group) >= 128)) p.group *= 2;
             p.sums = take((p.nb + p.group - 1) / p.group * K * 8);
         }
         p.dbias = take((p.nb + p.tile_rows - 1) / p.tile_rows * K * 4);
@@ -1756,11 +1760,14 @@ int work(const Call& c, const Plan& p, bool gradient, hipStream_t s) {
                 PatchArgs pa{nb, c.K, k0, width, rows, a.entry_z, ra.entry_g, ra.largest_z, ra.coef, a.dz, a.lddz};
                 unsigned lds = 0;
                 if (sums && k0 == 0) {
-                    pa.ranges = (u32)((c.K + RANGE - 1) / RANGE);
-                    pa.blocks = (u32)((nb + p.group - 1) / p.group) * pa.ranges;
+                    const long long row_groups = (nb + p.group - 1) / p.group;
+                    pa.range = RANGE;
+                    while (pa.range > LEAST_RANGE && row_groups * ((c.K + pa.range - 1) / pa.range) < 256) pa.range /= 2;
+                    pa.ranges = (u32)((c.K + pa.range - 1) / pa.range);
+                    pa.blocks = (u32)row_groups * pa.ranges;
                     pa.group = p.group;
                     pa.sums = sums;
-                    lds = (unsigned)std::min(c.K, (long long)RANGE) * RANGE_BYTES;
+                    lds = (unsigned)pa.range * RANGE_BYTES;
                 }
                 rc = kind == CSR ? launch_patch<T, CSR, 16>(pa, lds, s) : launch_patch<T, LABELS, 1>(pa, lds, s);
                 if (rc) return rc;
