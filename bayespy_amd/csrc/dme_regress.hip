@@ -1135,7 +1135,9 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         } else {
             loss += total * over;
         }
-        a.loss[at] = total == 0.0 ? 0.f : (float)loss;
+        // both likelihoods are of a sequence of draws, never above 1: what is below 0 is the rounding of z, which was summed in two orders
+        // (the tiles' and entries_of's), or of s
+        a.loss[at] = total == 0.0 || loss < 0.0 ? 0.f : (float)loss;
     } else if (part == 1 && a.largest_z) {
         const float w = a.weights ? a.weights[at] : 1.f;
         a.largest_z[at] = total == 0.0 ? INFINITY : m;

@@ -594,7 +594,8 @@ int dme_synth_dirmult(void* X /*[dev]*/, int elem_bytes, int64_t N, int64_t K, i
  *     enter the loss, whatever they hold; dH has 0 times them.
  *   rows: what the counts are (a host struct of device pointers), see below.
  *   row_weights [dev][N] fp32 or NULL (ones): the gradient is that of sum_i row_weights[i] loss[i].
- *   loss [dev][N] fp32, unweighted.  A row without counts has loss 0 and gradient 0; its features must be finite like all others.
+ *   loss [dev][N] fp32, unweighted, never below 0.  A row without counts has loss 0 and gradient 0; its features must be finite like all others.
+ *     z at the counts is summed in an order of its own: what a loss near 0 is off by is the 32-bit rounding of z, not of the loss.
  *   dH [dev][N][D], dW [dev][K][D] in H's type, dbias [dev][K] fp32 or NULL: overwritten, aligned to 16 bytes.
  * Sums, l and the row terms are held in 32 bits or more; d loss / d z is rounded once to H's type
  * before its products with W and H (dbias is summed before that rounding).  Results do not depend on timing:

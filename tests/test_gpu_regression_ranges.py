@@ -212,3 +212,27 @@ def test_bias_gradient_of_light_rows(n, kind):
         got = regression.log_loss_gradient(h, w, rows_of(x, kind, labels), bias=b, row_weights=weight)[3]
         near(got[:k // 2], [v[:k // 2] for v in want["dbias"]], "dbias of the heavy rows' columns")
         near(got[k // 2:], [v[k // 2:] for v in want["dbias"]], "dbias of the light rows' columns, weight %g" % light)
+
+
+@pytest.mark.parametrize("kind", ["labels", "csr", "dense"])
+@pytest.mark.parametrize("n", [9, 500])
+def test_losses_of_sure_rows_are_not_negative(n, kind):
+    """The label's z is far above all others: the loss is 0, up to the rounding of z (d + 2 roundings of 2^-23 of sum |h w| for each of its two
+    sums), and not below it."""
+    from bayespy_amd import regression
+    k, d = 700, 300
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    h = torch.randn(n, d, generator=gen, device="cuda")
+    w = torch.randn(k, d, generator=gen, device="cuda") * 0.01
+    labels = torch.arange(n, device="cuda") % k
+    w[labels[:k]] += h[:k] * 0.2
+    x = torch.zeros(n, k, dtype=torch.int32, device="cuda")
+    x[torch.arange(n, device="cuda"), labels] = 1 if kind == "labels" else 3
+    for t in (torch.float32, torch.bfloat16):
+        hh, ww = h.to(t), w.to(t)
+        off = 2 * (d + 2) * 2.0**-23 * (hh.double().abs() @ ww.double().abs().t()).max(dim=1).values + 2.0**-18
+        for likelihood in ("multinomial", "dirichlet"):
+            loss = regression.log_loss(hh, ww, rows_of(x, kind, labels), likelihood=likelihood)
+            want = exact(hh, ww, torch.zeros(k, device="cuda"), x, torch.ones(n, device="cuda"), likelihood, t)["loss"][0]
+            assert float(want.max()) < 1e-3 and bool((loss >= 0).all())
+            assert bool(((loss.double() - want).abs() <= 2 * x.sum(1) * off).all())
