@@ -1,7 +1,9 @@
 // dme_orth.hip — the orthogonalised step (include/dme_hip.h, dme_orthogonal_step): X = G / |G|, then `steps` times
 // X <- a X + (b S + c S S) X with S = X X'.  The polynomial p(x) = a x + b x^3 + c x^5 acts on X's singular values and
 // leaves its singular vectors alone (Carlson et al. 2015 take this step's limit as the steepest descent of log-sum-exp
-// losses; the quintic iteration is Bjorck and Bowie's, 1971).
+// losses; the quintic iteration is Bjorck and Bowie's, 1971; the coefficients that bayespy_amd/regression.py begins with, 3.4445, -4.7750 and 2.0315,
+// are those that Jordan et al. 2024 publish for the Muon optimiser: steep at 0; five steps take singular values
+// from 0.005 of |G| on to between 0.68 and 1.16).
 //
 // S is the square of the smaller side: X X' for a wide X, X' X for a tall one (then X <- a X + X (b S + c S S)); X keeps G's
 // orientation.
@@ -115,7 +117,7 @@ struct Matrices {
     long long rows, cols, ldx, m, lds;
 };
 
-// X = G / |G|, zero in the padding of its pitch.  One read of G, one write of the pairs: 50000 x 256 in bf16 takes 19 us (4.0 TB/s).
+// X = G / |G|, zero in the padding of its pitch.  One read of G, one write of the pairs: 50000 x 256 in bf16 takes 18 us (4.2 TB/s).
 template <class T, int PARTS>
 __global__ __launch_bounds__(256) void begin_kernel(const T* G, long long sb, long long rs, long long cs, const double* part, Matrices a) {
     __shared__ float tile[64][65];
@@ -270,7 +272,7 @@ __device__ __forceinline__ void halves(f16x4 (&h)[Tile::NI][Tile::NJ], const f32
 }
 
 // S = X X' (X' X for a tall X), the tiles on and below the diagonal; what lies above is their mirror image.  Where the tiles are
-// too few for the card, k is split and join_kernel adds the pieces.  4096 x 4096 (253 tiles of 192, one to a CU) takes 77 us (920 TFLOP/s of
+// too few for the card, k is split and join_kernel adds the pieces.  4096 x 4096 (253 tiles of 192, one to a CU) takes 73 us (940 TFLOP/s of
 // the half that is made); 50000 x 256 (10 tiles in 25 pieces) 18 us and the join 5, bound by how fast one workgroup a CU takes its slices.
 template <class T, int PARTS, int SIDE, bool TALL>
 __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void square_kernel(StepArgs<T> a) {
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(256) void join_kernel(Matrices x, int splits) {
     if (rr < x.m && cc < x.lds) put_s<PARTS>(x, so, mo, rr, cc, turn[lo][hi]);
 }
 
-// (4096 x 4096: 84 us.)  B = b S + c S S.  With S = d + O (diagonal, rest): (S S)[r][c] = (O O)[r][c] + (d_r + d_c) O[r][c], + d_r^2 where r = c.
+// (4096 x 4096: 80 us.)  B = b S + c S S.  With S = d + O (diagonal, rest): (S S)[r][c] = (O O)[r][c] + (d_r + d_c) O[r][c], + d_r^2 where r = c.
 template <class T, int PARTS, int SIDE>
 __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -428,9 +430,9 @@ __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void poly_kernel(StepArgs<
     }
 }
 
-// X <- a X + B X (a X + X B for a tall X).  EU: waves that a SIMD shall have room for.  4096 x 4096 takes 128 us, 96 of them the matrix
+// X <- a X + B X (a X + X B for a tall X).  EU: waves that a SIMD shall have room for.  4096 x 4096 takes 122 us, 96 of them the matrix
 // instructions' and most of the rest 134 MB of X read and written behind them (155 before the values went through LDS).  50000 x 256
-// is bound by memory: slabs of 64 lines read X once and take 28 us for 102 MB (3.7 TB/s; tiles of 64 x 64 took 43).
+// is bound by memory: slabs of 64 lines read X once and take 26 us for 102 MB (3.9 TB/s; tiles of 64 x 64 took 43).
 template <class T, int PARTS, class Tile, bool TALL, int EU>
 __global__ __launch_bounds__(Tile::NT, EU) void update_kernel(StepArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];

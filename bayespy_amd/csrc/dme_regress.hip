@@ -420,7 +420,7 @@ __device__ __forceinline__ f32x2 merge(f32x2 v, f32x2 o) {
 // go from memory straight into the matrix instructions' registers, WIDE loads of 16 bytes a lane ahead, and the rows wait in LDS.
 // Nothing is shared between waves but the rows, so many small workgroups keep ~200 KB a CU in flight.  Workgroups before the
 // columns' make the rows' z at their counts, so that a call has two launches.  Bound by memory: 1 x 50000 x 512 in bf16 reads 51 MB in
-// 12.5 us (4.1 TB/s).  LOOSE: rows that are not whole chunks of 16 bytes are read as they lie.
+// 12.6 us (4.1 TB/s, call after call of the same weights, which the memory-side cache holds).  LOOSE: rows that are not whole chunks of 16 bytes are read as they lie.
 template <class T, int KIND, bool LOOSE>
 __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -499,9 +499,9 @@ __global__ __launch_bounds__(256) void few_kernel(TileArgs a) {
 //   forward   the largest z of each row and the sum of e^(z - that)
 //   backward  e^(z - m) coef, rounded to T (the gradient's one rounding before its products), and the columns' sums
 //             of the unrounded values.  The counts are not looked at: patch_kernel puts them in.
-// 256 a side where there is work for every CU: 4096 x 50000 x 512 in bf16 takes 218 us forward (960 TFLOP/s; 128 a side 320), which is
+// 256 a side where there is work for every CU: 4096 x 50000 x 512 in bf16 takes 221 us forward (950 TFLOP/s; 128 a side 320), which is
 // the matrix instructions' time and a pass over the tile's 65536 exponentials beside it.  At D = 128 the passes count as much as the products:
-// 4099 x 50000 forward 147 us, backward 168 us for 410 MB of d loss / d z.  A workgroup that stayed for tile after tile, the next one's first
+// 4099 x 50000 forward 139 us, backward 158 us for 410 MB of d loss / d z.  A workgroup that stayed for tile after tile, the next one's first
 // slice on its way under the epilogue, was 1% faster forward and 4% slower backward, where it had no registers left.
 template <class T, int TR, int TC, int WR, int WC, int KIND, bool BACKWARD, int STAGES = 0>
 __global__ __launch_bounds__(WR * WC * 64) void tile_kernel(TileArgs a) {
@@ -1305,7 +1305,7 @@ __device__ __forceinline__ void product(const ProductArgs& a, u32 block, char* l
 // Both products of a piece of d loss / d z: dW = dz' H and dH = dz W, in one launch or (no workgroups for the other) one alone.  Their
 // tiles are many and few, short and long; together they leave fewer CUs idle than one after the other.  The longer ones begin.
 // At D = 128 both are bound by their reads of dz: 4099 x 50000 takes 161 us for twice 410 MB (5.1 TB/s, most of it from the memory-side
-// cache); at D = 1024 by the matrix instructions: 8192 x 50000 takes 1560 us (1080 TFLOP/s).
+// cache); at D = 1024 by the matrix instructions: 8192 x 50000 takes 1550 us (1080 TFLOP/s).
 template <class T, int SIDE, int STAGES>
 __global__ __launch_bounds__(SIDE >= 192 ? 512 : 256) void products_kernel(ProductArgs w, ProductArgs h, u32 blocks_w, u32 blocks_h, int h_first) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -1400,7 +1400,7 @@ __device__ __forceinline__ void add_bias(const BiasArgs& a, u32 block, double (*
     a.dbias[k] = (float)v;
 }
 
-// What is left when the products are through, in one launch (9 us at 4099 x 50000 x 128, 20 MB of pieces): the pieces of dH and dW, and dbias (0 workgroups: not this time).
+// What is left when the products are through, in one launch (10 us at 4099 x 50000 x 128, 20 MB of pieces): the pieces of dH and dW, and dbias (0 workgroups: not this time).
 template <class T>
 __global__ __launch_bounds__(256) void finish_kernel(JoinArgs w, JoinArgs h, BiasArgs b) {
     __shared__ double sums[4][64];

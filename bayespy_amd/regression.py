@@ -220,9 +220,10 @@ def log_loss_gradient(features, weights, rows, bias=None, likelihood="multinomia
 
 def orthogonal_step(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315)):
     """The update matrix with its singular values brought near one: X = update / |update|, then `steps` times
-    X <- a X + (b S + c S S) X with S = X X'.  update: float32 or bfloat16, [rows, cols] or a batch [B, rows, cols], any
-    strides; the result is contiguous and of the same type, and has no graph (refused where autograd would record one).  A zero matrix gives zeros.  The step from the gradient alone
-    that stands beside device.predicted_step, which needs a Hessian."""
+    X <- a X + (b S + c S S) X with S = X X'.  The coefficients are those of Jordan et al. 2024 (Muon): five steps take singular values
+    from 0.005 of |update| on to between 0.68 and 1.16.  update: float32 or bfloat16, [rows, cols] or a batch [B, rows, cols], any
+    strides; the result is contiguous and of the same type, and has no graph (refused where autograd would record one).  A zero matrix
+    gives zeros.  The step from the gradient alone that stands beside device.predicted_step, which needs a Hessian."""
     if not torch.is_tensor(update) or update.dtype not in _TYPES or update.dim() not in (2, 3):
         raise ValueError("update must be a float32 or bfloat16 matrix or a batch of them")
     if update.shape[-1] < 1 or update.shape[-2] < 1:

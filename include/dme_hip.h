@@ -598,7 +598,7 @@ int dme_synth_dirmult(void* X /*[dev]*/, int elem_bytes, int64_t N, int64_t K, i
  *     z at the counts is summed in an order of its own: what a loss near 0 is off by is the 32-bit rounding of z, not of the loss.
  *   dH [dev][N][D], dW [dev][K][D] in H's type, dbias [dev][K] fp32 or NULL: overwritten, aligned to 16 bytes.
  * Sums, l and the row terms are held in 32 bits or more; d loss / d z is rounded once to H's type
- * before its products with W and H (dbias is summed before that rounding).  Results do not depend on timing:
+ * before its products with W and H (dbias is summed before that rounding; a column where row_weights times a count's G leaves 32 bits is NaN in it).  Results do not depend on timing:
  * the same call gives the same bits.
  * Rows: DME_ROWS_LABELS  labels int64 [N]: one count in column labels[i]; negative: no count.
  *       DME_ROWS_CSR     rowptr int64 [N+1], colidx int32 [nnz] strictly ascending within a row, vals int32 [nnz] >= 0.
@@ -643,7 +643,8 @@ int dme_log_loss_gradient(const void* H /*[dev]*/, int64_t ldh, const void* W /*
  * X = G / |G|_F, then `steps` times X <- a X + b X X'X + c X X'X X'X (products over the smaller side);
  * out [dev][batch][rows][cols], contiguous, in G's type.  A zero matrix stays zero.  Products run on fp16
  * operands with 32-bit sums: one for bf16 matrices, whose X is kept as a pair of fp16 values (22 bits); three, of pairs, for fp32
- * matrices, whose X is kept in 32 bits (min(rows, cols) <= 64: fp32 products throughout).  The coefficients
+ * matrices, whose X is kept in 32 bits.  Where the smaller side is at most 64 and the larger at most 4096, either type: X in 32 bits, fp32 products.
+ * The coefficients
  * must keep singular values that begin in [0, 1] below 3.  The smaller side is at most 2^16, the larger one 2^28.  The step that dme_predicted_step takes from a Hessian is taken
  * here from the gradient alone: log-sum-exp losses are smooth in the spectral norm.
  * ------------------------------------------------------------------------------------------- */
