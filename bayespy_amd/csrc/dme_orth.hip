@@ -332,16 +332,20 @@ __global__ __launch_bounds__(256) void join_kernel(Matrices x, int splits) {
     float v = 0.f;
     if (r < x.m && c < x.m) {
         const float* at = x.part + blockIdx.y * x.stride_part + (r > c ? r * x.lds + c : c * x.lds + r);  // above the diagonal: the same sum
-        const auto eight = [&](int s, auto last) {  // loads without branches: all on their way at once
-            float p[8];
+        const auto some = [&](int s, auto count, bool last) {  // loads without branches: all on their way at once
+            constexpr int N = decltype(count)::value;
+            float p[N];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) p[u] = at[(!last || s + u < splits ? s + u : s) * x.stride_s];
+            for (int u = 0; u < N; ++u) p[u] = at[(!last || s + u < splits ? s + u : s) * x.stride_s];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v += !last || s + u < splits ? p[u] : 0.f;
+            for (int u = 0; u < N; ++u) v += !last || s + u < splits ? p[u] : 0.f;
         };
         int s = 0;
-        for (; s + 8 <= splits; s += 8) eight(s, std::false_type());
-        if (s < splits) eight(s, std::true_type());
+        for (; s + 8 <= splits; s += 8) some(s, std::integral_constant<int, 8>(), false);
+        if (splits - s > 2)
+            some(s, std::integral_constant<int, 8>(), true);
+        else if (splits - s > 0)
+            some(s, std::integral_constant<int, 2>(), true);
     }
     turn[hi][lo] = v;
     if (r < x.m && c < x.lds) put_s<PARTS>(x, so, mo, r, c, v);
