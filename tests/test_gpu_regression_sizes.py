@@ -108,3 +108,37 @@ def test_a_bias_gradient_that_leaves_32_bits():
     g[0] = 3e38
     db = regression.log_loss_gradient(h, w, as_rows(x, "csr"), bias=b, row_weights=g)[3]
     assert bool(torch.isnan(db[5])) and bool(torch.isfinite(db[300:]).all())
+
+
+@pytest.mark.parametrize("kind", ["csr", "labels"])
+def test_bias_gradient_of_a_wide_vocabulary(kind):
+    """Column sums by ranges of every width, up to the widest.  Weights of 0: z is the bias, p the same for all rows, and the gradient
+    p sum_i g_i T_i - sum_i g_i x_ik.  p is off by 2^-22 (|b - l| + 4) + 2^-17 (its sum), each sum over n rows by n 2^-23 of its terms."""
+    from bayespy_amd import regression
+    from bayespy_amd.regression import CountRows
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    n = 3000
+    for k in (1023, 5000, 70001, 300007):
+        b = torch.randn(k, generator=gen, device="cuda")
+        g = torch.rand(n, generator=gen, device="cuda")
+        each = 1 if kind == "labels" else 40
+        col = (torch.rand(n, each, generator=gen, device="cuda").pow(3) * k).long().clamp(max=k - 1)
+        val = torch.randint(1, 50, (n, each), generator=gen, device="cuda") if kind == "csr" else torch.ones_like(col)
+        if kind == "labels":
+            rows = CountRows.from_labels(col[:, 0].contiguous(), k)
+        else:
+            col = col.sort(dim=1).values
+            val[:, 1:] *= col[:, 1:] != col[:, :-1]  # a column once
+            at = (val > 0).nonzero(as_tuple=True)
+            rowptr = torch.zeros(n + 1, dtype=torch.int64, device="cuda")
+            rowptr[1:] = (val > 0).sum(1).cumsum(0)
+            rows = CountRows.from_csr(rowptr, col[at].int(), val[at].int(), k).check()
+        h, w = torch.randn(n, 4, generator=gen, device="cuda"), torch.zeros(k, 4, device="cuda")
+        got = regression.log_loss_gradient(h, w, rows, bias=b, row_weights=g)[3].double()
+        total, counts = val.sum(1).double(), torch.zeros(k, dtype=torch.float64, device="cuda")
+        counts.index_add_(0, col.reshape(-1), (val * g.double()[:, None]).reshape(-1))
+        z = b.double()
+        l = torch.logsumexp(z, 0)
+        first = torch.exp(z - l) * (g.double() * total).sum()
+        tol = first * (2.0**-22 * ((z - l).abs() + 4) + 2.0**-17 + n * 2.0**-23) + (n + 1) * 2.0**-23 * counts + 2.0**-24 * (first + counts)
+        assert bool(((got - (first - counts)).abs() <= tol).all()), k
